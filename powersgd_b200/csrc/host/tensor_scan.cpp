@@ -182,9 +182,72 @@ PyObject* step_fits(PyObject*, PyObject* args) {
   });
 }
 
+// adam_items(params, state, names, first_block): the list of an AdamW step (PsgdAdamTensor, csrc/adamw.cu), see ops/scan.py.
+struct AdamItem {
+  uint64_t p, g, m, v, m_scale, v_scale, step;
+  int64_t n;
+  uint32_t block0, chunk_end;
+};
+PyObject* adam_items(PyObject*, PyObject* args) {
+  return guarded([&]() -> PyObject* {
+    PyObject *list, *state, *names;
+    long long block;
+    if (!PyArg_ParseTuple(args, "OOOL", &list, &state, &names, &block)) return nullptr;
+    Sequence params(list), keys(names);
+    if (!params.fast || !keys.fast || !PyDict_Check(state)) Py_RETURN_NONE;
+    const bool narrow = keys.size() == 5;   // step, two moments, their scales
+    if (!narrow && keys.size() != 3) Py_RETURN_NONE;
+    std::vector<AdamItem> items;
+    items.reserve(params.size());
+    int device = -1;
+    at::ScalarType type = at::kFloat;
+    for (Py_ssize_t i = 0; i < params.size(); ++i) {
+      const at::Tensor* p = plain(params[i]);
+      if (p == nullptr) Py_RETURN_NONE;
+      const int64_t n = p->numel(), blocks = (n + 255) / 256;
+      const long long block0 = block;
+      block += blocks;
+      const at::Tensor& g = p->grad();
+      if (!g.defined()) continue;
+      if (items.empty()) {
+        device = p->get_device();
+        type = p->scalar_type();
+      }
+      if (!p->is_cuda() || p->get_device() != device || p->scalar_type() != type || !p->is_non_overlapping_and_dense()) Py_RETURN_NONE;
+      if (g.layout() != at::kStrided || !g.unsafeGetTensorImpl()->has_storage() || at::isTensorSubclassLike(g)) Py_RETURN_NONE;
+      if (g.scalar_type() != type || !g.is_cuda() || g.get_device() != device || !same_layout(g, *p)) Py_RETURN_NONE;
+      PyObject* own = PyDict_GetItemWithError(state, params[i]);
+      if (own == nullptr || !PyDict_Check(own)) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+      }
+      const at::Tensor* t[5] = {nullptr, nullptr, nullptr, nullptr, nullptr};
+      for (Py_ssize_t j = 0; j < keys.size(); ++j) {
+        PyObject* value = PyDict_GetItemWithError(own, keys[j]);
+        t[j] = value == nullptr ? nullptr : plain(value);
+        if (t[j] == nullptr || !t[j]->is_cuda() || t[j]->get_device() != device) {
+          PyErr_Clear();
+          Py_RETURN_NONE;
+        }
+        const bool code = narrow && (j == 1 || j == 2);
+        if (t[j]->scalar_type() != (code ? at::kFloat8_e4m3fn : at::kFloat)) Py_RETURN_NONE;
+        const bool fits = j == 0 ? t[j]->numel() == 1 : j < 3 ? same_layout(*t[j], *p) : t[j]->numel() == blocks && t[j]->is_contiguous();
+        if (!fits) Py_RETURN_NONE;
+      }
+      auto at_of = [](const at::Tensor* x) { return x == nullptr ? (uint64_t)0 : (uint64_t)x->data_ptr(); };
+      items.push_back({at_of(p), (uint64_t)g.data_ptr(), at_of(t[1]), at_of(t[2]), at_of(t[3]), at_of(t[4]), at_of(t[0]), n, (uint32_t)block0, 0u});
+    }
+    const int code = type == at::kFloat ? 0 : type == at::kBFloat16 ? 1 : type == at::kHalf ? 2 : -1;
+    if (code < 0) Py_RETURN_NONE;
+    return Py_BuildValue("(y#niiL)", reinterpret_cast<const char*>(items.data()), (Py_ssize_t)(items.size() * sizeof(AdamItem)),
+                         (Py_ssize_t)items.size(), device, code, block);
+  });
+}
+
 PyMethodDef methods[] = {
     {"addresses", addresses, METH_O, nullptr},     {"grad_addresses", grad_addresses, METH_O, nullptr}, {"usable", usable, METH_VARARGS, nullptr},
-    {"sizes", sizes, METH_O, nullptr},             {"step_fits", step_fits, METH_VARARGS, nullptr},     {nullptr, nullptr, 0, nullptr},
+    {"sizes", sizes, METH_O, nullptr},             {"step_fits", step_fits, METH_VARARGS, nullptr},
+    {"adam_items", adam_items, METH_VARARGS, nullptr}, {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_tensor_scan", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

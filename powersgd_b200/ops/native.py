@@ -12,6 +12,8 @@ import ctypes
 import os
 from typing import Optional
 
+import torch
+
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # PSGD_B200_LIB points at another build of the same library (e.g. one with development counters)
 LIB_PATH = os.environ.get("PSGD_B200_LIB") or os.path.join(os.path.dirname(_HERE), "csrc", "libpsgd_b200.so")
@@ -72,6 +74,28 @@ def check(code: int, what: str) -> None:
     if code != 0:
         msg = lib().psgd_last_error()
         raise RuntimeError(f"{what} failed (code {code}): {msg.decode() if msg else ''}")
+
+
+class on_device:
+    """`with on_device(device) as stream`: launches for tensors of `device` (an index is given), on its current stream."""
+
+    __slots__ = ("index", "back")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        now = torch._C._cuda_getDevice()
+        self.back = None
+        if now != self.index:
+            self.back = now
+            torch._C._cuda_setDevice(self.index)
+        return torch._C._cuda_getCurrentRawStream(self.index)
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            torch._C._cuda_setDevice(self.back)
+        return False
 
 
 def capture_id(stream: ctypes.c_void_p) -> int:
