@@ -9,13 +9,13 @@
 // logarithm of the sum are float32; P and dS are rounded to 16 bits as operands of the second products, as the tensor
 // core takes them, and results are rounded once.
 //
-// All three kernels work on tiles of 128 x 128 scores. Rows of Q, K, V and dO come by TMA in tiles of 128 rows, and the
-// scores never leave tensor memory and registers: a thread owns a row of a tile (a lane of tensor memory), so that a row's
-// maximum and sum need no exchange between lanes, and P and dS go back to tensor memory as the A operand of the second products.
-//   forward   a block has two tiles of queries of one head that share K and V. While the tensor core multiplies for one of
-//             them, the four warps of the other take exponentials.
-//   dQ        a block has one tile of queries and walks over keys.
-//   dK, dV    a block has one tile of keys and walks over the queries of all heads of its group, transposed: lanes are
+// Rows of Q, K, V and dO come by TMA, and the scores never leave tensor memory and registers: a thread owns a row of a tile
+// (a lane of tensor memory), so that a row's maximum and sum need no exchange between lanes, and P and dS go back to tensor
+// memory as the A operand of the second products. A step's chain (products, into registers, exponentials, back, products) is
+// much longer than the work of any one unit in it, so two chains run on every SM: two blocks, or two tiles of one.
+//   forward   tiles of 128 queries, walking over tiles of 128 keys.
+//   dQ        tiles of 128 queries, walking over tiles of 64 keys.
+//   dK, dV    tiles of 128 keys, walking over tiles of 64 queries of all heads of the group, transposed: lanes are
 //             keys, so that P^T and dS^T are A operands as they come. Nothing is added with atomics: the same inputs
 //             give the same bits. The price is that S and dP are computed twice (seven products instead of five).
 // A row of a tile that belongs to another sequence, or lies behind the last one, may hold anything: scores with it are
@@ -26,6 +26,7 @@
 //
 // Every wait is bounded: where one runs out, the block sets the status word, all its warps fall through, and the
 // kernel ends.
+#include <cooperative_groups.h>
 #include <cuda.h>
 #include <string.h>
 
@@ -33,17 +34,22 @@
 
 namespace {
 
-constexpr int AT_TILE = 128;
+namespace cg = cooperative_groups;
+
+constexpr int AT_TILE = 128;     // rows of a tile that stays
+constexpr int AT_STEP = 64;      // rows of a tile that passes, in the backward pass
 constexpr float AT_LOG2E = 1.44269504088896341f;
 
 struct AtArgs {
-  CUtensorMap q, k, v, g;        // boxes of 64 elements x 1 head x 128 rows; g: the gradient of the output
+  CUtensorMap q, k, v, g;        // boxes of 64 elements x 1 head x 64 rows; g: the gradient of the output
   const int* offsets;
   int sequences, tokens, heads, group, size;   // group: query heads per key head
   int causal;
   float scale, scale2;           // scale, scale log2(e)
+  int split;                     // dK, dV: blocks that share a tile of keys
   int blocks;                    // tiles (forward: pairs of them) that the grid has room for, per head
   const void* out;               // forward: written; backward: read. [tokens, heads, size]
+  const void* rest;              // what rounding took from the output, likewise; null where no gradient will be asked for
   const void* grad;              // the gradient of the output, as `g` addresses it
   long long grad_row, grad_head; // its strides
   float* lse;                    // [heads, tokens]: log2 of the sum of exponentials, scaled scores
@@ -58,11 +64,36 @@ __device__ __forceinline__ float at_exp2(float x) {
   return y;
 }
 
+// The largest of three; what is no number wins.
+__device__ __forceinline__ float at_max3(float x, float y, float z) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(x), "f"(y), "f"(z));
+  return r;
+}
+
+// 2^x in plain arithmetic: x = n + f with |f| <= 1/2 by rounding, a polynomial of degree 4 in f with the least maximal relative error
+// (2.8e-6; fitted with value 1 at 0), n added to the exponent. Below -127 the result is zero.
+constexpr int AT_POLY = 4;   // of 16 exponentials, those that are taken so: the special function unit has 16 results per cycle and SM
+__device__ __forceinline__ float2 at_exp2_poly(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
+  x.x = fmaxf(x.x, -127.f);
+  x.y = fmaxf(x.y, -127.f);
+  const float2 t = add2(x, magic);
+  const float2 f = fma2(add2(t, back), minus, x);
+  float2 p = make_float2(0.0095828531f, 0.0095828531f);
+  p = fma2(p, f, make_float2(0.0559064246f, 0.0559064246f));
+  p = fma2(p, f, make_float2(0.2402409861f, 0.2402409861f));
+  p = fma2(p, f, make_float2(0.6931241934f, 0.6931241934f));
+  p = fma2(p, f, make_float2(1.f, 1.f));
+  return make_float2(__uint_as_float(__float_as_uint(p.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(p.y) + (__float_as_uint(t.y) << 23)));
+}
+
 // ---- which tile --------------------------------------------------------------------------------
 // Sequences cut into pieces of `rows`; piece number `index` in the order: the pieces that have the most of their sequence before them
 // (`from_end`: behind them) first. One warp asks. Returns false where there are fewer.
 struct AtPiece {
   int start, length, piece;      // first row and rows of its sequence, its number there
+  int before, behind;            // rows that belong to no sequence: [0, before) and [behind, tokens)
 };
 __device__ __forceinline__ int at_bound(const int* offsets, int s, int tokens) { return min(max(offsets[s], 0), tokens); }
 __device__ bool at_find(const AtArgs& a, int rows, int index, bool from_end, AtPiece& out) {
@@ -73,6 +104,8 @@ __device__ bool at_find(const AtArgs& a, int rows, int index, bool from_end, AtP
     return hi > lo ? (hi - lo + rows - 1) / rows : 0;
   };
   const int mine = pieces(lane);
+  out.before = at_bound(a.offsets, 0, a.tokens);
+  out.behind = max(at_bound(a.offsets, a.sequences, a.tokens), out.before);
   // pieces at level `level` of their sequences or above
   auto above = [&](int level) {
     int n = max(mine - level, 0);
@@ -109,11 +142,10 @@ __device__ bool at_find(const AtArgs& a, int rows, int index, bool from_end, AtP
 
 // Rows of a result that belong to no sequence: zeros. Dealt out over the blocks of a head.
 template <typename T>
-__device__ void at_clear_outside(const AtArgs& a, T* out, int heads, int head, int block) {
-  const int first = at_bound(a.offsets, 0, a.tokens), last = at_bound(a.offsets, a.sequences, a.tokens);
-  const int outside = first + a.tokens - max(first, last);
+__device__ __forceinline__ void at_clear_outside(const AtArgs& a, const AtPiece& piece, T* out, int heads, int head, int block) {
+  const int outside = piece.before + a.tokens - piece.behind;
   for (int i = block; i < outside; i += a.blocks) {
-    const int row = i < first ? i : max(first, last) + i - first;
+    const int row = i < piece.before ? i : piece.behind + i - piece.before;
     T* p = out + ((long long)row * heads + head) * a.size;
     for (int e = threadIdx.x; e < a.size; e += blockDim.x) p[e] = T(0.f);
   }
@@ -125,47 +157,88 @@ struct AtWait {
   int* status;
   __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
 #pragma unroll 1
-    for (int i = 0; i < 16; ++i)   // (the clock is read only when it takes longer)
+    for (int i = 0; i < 64; ++i)   // (the clock is read only when it takes longer)
       if (psgd_mbar_try_wait(bar, parity)) return true;
     return psgd_mbar_wait(bar, parity, abort_flag, status);
   }
 };
 
-// A tile of 128 rows from `row` of one head: PANELS boxes of 64 elements.
-template <int PANELS>
-__device__ __forceinline__ void at_load_tile(uint32_t dst, const CUtensorMap* map, int head, int row, uint64_t* bar) {
-#pragma unroll
-  for (int p = 0; p < PANELS; ++p) tma_load_box3(dst + p * UMMA_PANEL, map, p * 64, head, row, bar);
+// The same for a warp that goes on as one: all of its lanes, or none.
+struct AtWaitAll {
+  AtWait one;
+  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const { return __all_sync(0xffffffffu, one(bar, parity)); }
+};
+
+// One arrival for a warp whose lanes have all done what the barrier stands for. (128 or 256 arrivals on one word of shared memory
+// took longer than the work between them.)
+__device__ __forceinline__ void at_arrive(uint64_t* bar) {
+  umma_fence_before();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) psgd_mbar_arrive(bar);
 }
 
-// Clears rows [from, 128) of a tile, by threads that have one row each.
-template <int PANELS>
-__device__ __forceinline__ void at_clear_row(uint8_t* tile, int row, int from) {
-  if (row < from) return;
+// A tile of ROWS rows from `row` of one head, in boxes of 64 rows x 64 elements.
+template <int PANELS, int ROWS>
+__device__ __forceinline__ void at_load_tile(uint32_t dst, const CUtensorMap* map, int head, int row, uint64_t* bar) {
 #pragma unroll
   for (int p = 0; p < PANELS; ++p) {
-    uint4* at = reinterpret_cast<uint4*>(tile + p * UMMA_PANEL + row * 128);
+#pragma unroll
+    for (int r = 0; r < ROWS; r += 64) tma_load_box3(dst + (p * ROWS + r) * 128, map, p * 64, head, row + r, bar);
+  }
+}
+
+// Clears a row of a tile.
+template <int PANELS, int ROWS>
+__device__ __forceinline__ void at_clear_row(uint8_t* tile, int row) {
+#pragma unroll
+  for (int p = 0; p < PANELS; ++p) {
+    uint4* at = reinterpret_cast<uint4*>(tile + (p * ROWS + row) * 128);
 #pragma unroll
     for (int i = 0; i < 8; ++i) at[i] = make_uint4(0, 0, 0, 0);
   }
 }
 
-// `columns` of an accumulator's row, times `factor`, as a row of 16-bit numbers.
+// The 32 rows of an accumulator that a warp can read, times `factor`, as rows of 16-bit numbers `pitch` elements apart, the first `rows` of them;
+// what rounding takes from them likewise to `rest`. By way of 4 KiB of shared memory of the warp's own: a lane has a row, and eight lanes
+// together write 128 bytes of one.
 template <typename T, int PANELS>
-__device__ __forceinline__ void at_write_row(uint32_t tmem, float factor, T* row, int size, bool write) {
+__device__ __forceinline__ void at_write_rows(uint32_t tmem, float factor, uint8_t* stage, T* out, T* rest, long long pitch, int rows, int size) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int c = 0; c < PANELS * 64; c += 32) {
-    if (c >= size) break;
-    float f[32];
-    tmem_load32(tmem + c, f);
+  for (int panel = 0; panel < PANELS; ++panel) {
+    if (panel * 64 >= size) break;
+    float f[64];
+    tmem_load32(tmem + panel * 64, f);
+    tmem_load32(tmem + panel * 64 + 32, f + 32);
     tmem_load_wait();
-    if (write) {
 #pragma unroll
-      for (int i = 0; i < 32; i += 8) {
-        if (c + i < size)
-          *reinterpret_cast<uint4*>(row + c + i) = make_uint4(pack2<T>(f[i] * factor, f[i + 1] * factor), pack2<T>(f[i + 2] * factor, f[i + 3] * factor),
-                                                              pack2<T>(f[i + 4] * factor, f[i + 5] * factor), pack2<T>(f[i + 6] * factor, f[i + 7] * factor));
+    for (int c = 0; c < 64; ++c) f[c] *= factor;
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+      T* to = part == 0 ? out : rest;
+      if (to == nullptr) break;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float& x = f[8 * c + 2 * e];
+          float& y = f[8 * c + 2 * e + 1];
+          w[e] = pack2<T>(x, y);
+          const float2 back = unpack2<T>(w[e]);
+          x -= back.x;
+          y -= back.y;
+        }
+        *reinterpret_cast<uint4*>(stage + lane * 128 + ((c ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
       }
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int row = i * 4 + (lane >> 3), c = lane & 7;
+        const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
+        if (row < rows && panel * 64 + c * 8 < size) *reinterpret_cast<uint4*>(to + row * pitch + panel * 64 + c * 8) = v;
+      }
+      __syncwarp();
     }
   }
 }
@@ -178,126 +251,141 @@ template <>
 struct AtType<__nv_bfloat16> { static constexpr int value = 1; };
 
 // ---- forward -----------------------------------------------------------------------------------
-constexpr int AF_THREADS = 320;   // warps 0-3 and 4-7: one tile of queries each; 8: loads; 9: products
+// TILES of queries per block: four warps each, then a warp that loads and one that issues the products.
 constexpr int AF_RING = 4;        // tiles of K and V under way
 
-template <int PANELS>
-constexpr size_t af_shared() { return 1024 + (size_t)(2 + AF_RING) * PANELS * UMMA_PANEL; }
+__host__ __device__ constexpr int af_threads(int tiles) { return 128 * tiles + 64; }
+constexpr size_t af_shared(int panels, int tiles) { return 1024 + (size_t)(tiles + AF_RING) * panels * UMMA_PANEL; }
 
-template <typename T, int PANELS>
-__global__ void __launch_bounds__(AF_THREADS, 1) psgd_attention_kernel(const __grid_constant__ AtArgs a) {
+template <typename T, int PANELS, int TILES>
+__global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_kernel(const __grid_constant__ AtArgs a) {
   constexpr int TILE_BYTES = PANELS * UMMA_PANEL;
+  constexpr int LOADER = 4 * TILES, ISSUER = LOADER + 1, COLUMNS = 256 * TILES, O = TILES * AT_TILE;   // warps; tensor memory: scores, outputs
+  // Where there is room P has columns of its own, and the next scores are multiplied as soon as these are in registers; else P takes the place
+  // of the scores, and the next ones come behind P V.
+  constexpr bool EARLY = TILES == 1 && PANELS == 1;
+  constexpr int P = EARLY ? 192 : 0;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = base;
-  uint8_t* s_ring = base + 2 * TILE_BYTES;
-  __shared__ __align__(8) uint64_t bar_q, bar_full[AF_RING], bar_empty[AF_RING], bar_s[2], bar_p[2], bar_o[2];
+  uint8_t* s_ring = base + TILES * TILE_BYTES;
+  __shared__ __align__(8) uint64_t bar_q, bar_full[AF_RING], bar_empty[AF_RING], bar_s[TILES], bar_r[TILES], bar_p[TILES][2], bar_o[TILES];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_found;
   __shared__ AtPiece s_piece;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int head = blockIdx.x % a.heads, index = blockIdx.x / a.heads;
-  at_clear_outside<T>(a, (T*)a.out, a.heads, head, index);
   if (warp == 0) {
-    AtPiece piece = {0, 0, 0};
-    const bool found = at_find(a, 2 * AT_TILE, index, false, piece);
+    AtPiece piece = {0, 0, 0, 0, 0};
+    const bool found = at_find(a, TILES * AT_TILE, index, false, piece);
     if (lane == 0) {
       s_piece = piece;
       s_found = found;
     }
   }
+  if (warp == LOADER && lane < 3) tma_prefetch_map(lane == 0 ? &a.q : lane == 1 ? &a.k : &a.v);
   if (tid == 32) {
     psgd_mbar_init(&bar_q, 1);
     for (int i = 0; i < AF_RING; ++i) {
       psgd_mbar_init(&bar_full[i], 1);
       psgd_mbar_init(&bar_empty[i], 1);
     }
-    for (int t = 0; t < 2; ++t) {
+    for (int t = 0; t < TILES; ++t) {
       psgd_mbar_init(&bar_s[t], 1);
-      psgd_mbar_init(&bar_p[t], 128);
+      psgd_mbar_init(&bar_r[t], 4);
+      psgd_mbar_init(&bar_p[t][0], 4);
+      psgd_mbar_init(&bar_p[t][1], 4);
       psgd_mbar_init(&bar_o[t], 1);
     }
     s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  __syncthreads();
-  if (!s_found) return;
-  if (warp == 9) tmem_alloc(&s_tmem, 512);
+  if (warp == ISSUER) tmem_alloc(&s_tmem, COLUMNS);
   umma_fence_before();
   __syncthreads();
   umma_fence_after();
+  at_clear_outside<T>(a, s_piece, (T*)a.out, a.heads, head, index);
+  if (!s_found) {
+    if (warp == ISSUER) tmem_free(s_tmem, COLUMNS);
+    return;
+  }
   const uint32_t tmem = s_tmem;
   const AtWait wait = {&s_abort, a.status};
-  const int start = s_piece.start, length = s_piece.length, row0 = s_piece.piece * 2 * AT_TILE;
+  const int start = s_piece.start, length = s_piece.length, row0 = s_piece.piece * TILES * AT_TILE;
   // tiles of keys that each tile of queries meets
-  int n[2];
+  int n[TILES];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int t = 0; t < TILES; ++t) {
     const int q0 = row0 + t * AT_TILE;
     n[t] = q0 >= length ? 0 : a.causal ? q0 / AT_TILE + 1 : (length + AT_TILE - 1) / AT_TILE;
   }
-  const int steps = max(n[0], n[1]);
+  const int steps = max(n[0], n[TILES - 1]);
 
-  if (warp == 8) {
+  if (warp == LOADER) {
     if (lane == 0) {
-      psgd_mbar_expect_tx(&bar_q, n[1] > 0 ? 2 * TILE_BYTES : TILE_BYTES);
-      for (int t = 0; t < 2; ++t)
-        if (n[t] > 0) at_load_tile<PANELS>(psgd_smem_u32(s_q + t * TILE_BYTES), &a.q, head, start + row0 + t * AT_TILE, &bar_q);
+      psgd_mbar_expect_tx(&bar_q, n[TILES - 1] > 0 ? TILES * TILE_BYTES : TILE_BYTES);
+      for (int t = 0; t < TILES; ++t)
+        if (n[t] > 0) at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_q + t * TILE_BYTES), &a.q, head, start + row0 + t * AT_TILE, &bar_q);
       for (int i = 0; i < 2 * steps; ++i) {   // K_0, V_0, K_1, V_1, ...
         const int slot = i % AF_RING;
         if (!wait(&bar_empty[slot], ((i / AF_RING) & 1) ^ 1)) break;
         psgd_mbar_expect_tx(&bar_full[slot], TILE_BYTES);
-        at_load_tile<PANELS>(psgd_smem_u32(s_ring + slot * TILE_BYTES), (i & 1) ? &a.v : &a.k, head / a.group, start + (i >> 1) * AT_TILE, &bar_full[slot]);
+        at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_ring + slot * TILE_BYTES), (i & 1) ? &a.v : &a.k, head / a.group, start + (i >> 1) * AT_TILE, &bar_full[slot]);
       }
     }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      const int k_steps = (a.size + 15) / 16;
-      constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_TILE);
-      const uint32_t o_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
-      const uint32_t q_at = psgd_smem_u32(s_q), ring_at = psgd_smem_u32(s_ring);
-      auto scores = [&](int t, int j) {
-        umma_rows_by_rows(tmem + t * AT_TILE, q_at + t * TILE_BYTES, ring_at + (2 * j % AF_RING) * TILE_BYTES, S_SHAPE, k_steps, false);
-        umma_arrive(&bar_s[t]);
-      };
-      bool ok = wait(&bar_q, 0) && wait(&bar_full[0], 0);
-      if (ok) {
-        umma_fence_after();
-        for (int t = 0; t < 2; ++t)
-          if (n[t] > 0) scores(t, 0);
-        umma_arrive(&bar_empty[0]);
+  } else if (warp == ISSUER) {
+    const AtWaitAll wait_all = {wait};
+    const int k_steps = (a.size + 15) / 16;
+    constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_TILE);
+    const uint32_t o_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
+    const uint32_t q_at = psgd_smem_u32(s_q), ring_at = psgd_smem_u32(s_ring);
+    bool ok = wait_all(&bar_q, 0) && wait_all(&bar_full[0], 0);
+    int have = 0;   // tiles of keys that are there
+    auto scores = [&](int t, int j) {
+      if (j > have) {
+        ok = wait_all(&bar_full[2 * j % AF_RING], (2 * j / AF_RING) & 1);
+        have = j;
       }
-      for (int j = 0; j < steps && ok; ++j) {
-        const int kv = 2 * j + 1, kn = 2 * j + 2;
-        ok = wait(&bar_full[kv % AF_RING], (kv / AF_RING) & 1);
-        bool next = false;
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (j >= n[t]) continue;
-          ok = wait(&bar_p[t], j & 1);
+      if (!ok) return;
+      umma_fence_after();
+      umma_rows_by_rows<4 * PANELS, AT_TILE>(tmem + t * AT_TILE, q_at + t * TILE_BYTES, ring_at + (2 * j % AF_RING) * TILE_BYTES, S_SHAPE, k_steps);
+      umma_arrive(&bar_s[t]);
+    };
+    for (int t = 0; t < TILES && ok; ++t)
+      if (n[t] > 0) scores(t, 0);
+    if (ok) umma_arrive(&bar_empty[0]);
+    for (int j = 0; j < steps && ok; ++j) {
+      const int kv = 2 * j + 1, kn = 2 * j + 2;
+      for (int t = 0; t < TILES && ok; ++t) {
+        if (j >= n[t]) continue;
+        if (EARLY && j + 1 < n[t]) {
+          ok = wait_all(&bar_r[t], j & 1);
+          if (ok) scores(t, j + 1);
           if (!ok) break;
-          umma_fence_after();
-          for (int s = 0; s < AT_TILE / 16; ++s)
-            umma_ts(tmem + 2 * AT_TILE + t * AT_TILE, tmem + t * AT_TILE + s * 8, umma_tile(ring_at + (kv % AF_RING) * TILE_BYTES + s * 2048), o_shape, j > 0 || s > 0);
-          umma_arrive(&bar_o[t]);
-          if (j + 1 < n[t]) {
-            if (!next) ok = wait(&bar_full[kn % AF_RING], (kn / AF_RING) & 1);
-            if (!ok) break;
-            next = true;
-            umma_fence_after();
-            scores(t, j + 1);
-          }
         }
+        if (t == 0 || n[0] <= j) ok = wait_all(&bar_full[kv % AF_RING], (kv / AF_RING) & 1);
+        const uint32_t o_at = tmem + O + t * AT_TILE, p_at = tmem + P + t * AT_TILE, v_at = ring_at + (kv % AF_RING) * TILE_BYTES;
+        ok = ok && wait_all(&bar_p[t][0], j & 1);
         if (!ok) break;
-        umma_arrive(&bar_empty[kv % AF_RING]);
-        if (j + 1 < steps) umma_arrive(&bar_empty[kn % AF_RING]);
+        umma_fence_after();
+        umma_weights_by_rows<0, 4, AT_TILE>(o_at, p_at, v_at, o_shape, j > 0);
+        ok = wait_all(&bar_p[t][1], j & 1);
+        if (!ok) break;
+        umma_fence_after();
+        umma_weights_by_rows<4, 8, AT_TILE>(o_at, p_at, v_at, o_shape, true);
+        umma_arrive(&bar_o[t]);
+        if (!EARLY && j + 1 < n[t]) scores(t, j + 1);
       }
+      if (!ok) break;
+      umma_arrive(&bar_empty[kv % AF_RING]);
+      if (j + 1 < steps) umma_arrive(&bar_empty[kn % AF_RING]);
     }
   } else {
     const int t = warp >> 2, row = tid & 127;
     const int q = row0 + t * AT_TILE + row;          // in its sequence
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_at = tmem + lanes + t * AT_TILE, o_at = tmem + lanes + 2 * AT_TILE + t * AT_TILE;
+    const uint32_t s_at = tmem + lanes + t * AT_TILE, o_at = tmem + lanes + O + t * AT_TILE, p_at = tmem + lanes + P + t * AT_TILE;
     const int limit = a.causal ? min(q, length - 1) : length - 1;   // last key that counts
     float m = -INFINITY, l = 0.f;                    // what exponents are relative to (unscaled scores), sum
     bool ok = true;
@@ -309,6 +397,7 @@ __global__ void __launch_bounds__(AF_THREADS, 1) psgd_attention_kernel(const __g
 #pragma unroll
       for (int c = 0; c < AT_TILE; c += 32) tmem_load32(s_at + c, s + c);
       tmem_load_wait();
+      if (EARLY) at_arrive(&bar_r[t]);
       if (j == n[t] - 1) {
         const int last = limit - j * AT_TILE;
 #pragma unroll
@@ -319,17 +408,27 @@ __global__ void __launch_bounds__(AF_THREADS, 1) psgd_attention_kernel(const __g
           const int kv = 2 * j + 1;
           ok = wait(&bar_full[kv % AF_RING], (kv / AF_RING) & 1);
           if (!ok) break;
-          at_clear_row<PANELS>(s_ring + (kv % AF_RING) * TILE_BYTES, row, held);
+          if (row >= held) at_clear_row<PANELS, AT_TILE>(s_ring + (kv % AF_RING) * TILE_BYTES, row);
           psgd_fence_async_shared();
         }
       }
-      float most[4] = {s[0], s[1], s[2], s[3]};
+      float most[4];
 #pragma unroll
-      for (int c = 4; c < AT_TILE; ++c) most[c & 3] = fmaxf(most[c & 3], s[c]);
-      const float largest = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-      // The sums stay relative to an older maximum while exponents stay below 2^8: accumulators are rescaled only when it moves by more.
-      const bool moves = (largest - m) * a.scale2 > 8.f || j == 0;
-      if (j > 0) {
+      for (int c = 0; c < 4; ++c) most[c] = at_max3(s[c], s[c + 4], s[c + 8]);
+#pragma unroll
+      for (int c = 12; c < AT_TILE - 4; c += 8) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most[i] = at_max3(most[i], s[c + i], s[c + i + 4]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], s[AT_TILE - 4 + i]);
+      const float largest = at_max3(at_max3(most[0], most[1], most[2]), most[3], most[3]);
+      if (j == 0) {
+        m = largest;
+      } else {
+        // The sums stay relative to an older maximum while exponents stay below 2^8: accumulators are rescaled only when it moves by
+        // more (and where it is no number).
+        const bool moves = !((largest - m) * a.scale2 <= 8.f);
         if (__any_sync(0xffffffffu, moves)) {
           ok = wait(&bar_o[t], (j - 1) & 1);
           if (!ok) break;
@@ -349,35 +448,42 @@ __global__ void __launch_bounds__(AF_THREADS, 1) psgd_attention_kernel(const __g
             tmem_store16(o_at + c + 16, reinterpret_cast<uint32_t*>(o) + 16);
           }
         }
-      } else {
-        m = largest;
       }
       const float from = m == -INFINITY ? 0.f : m * a.scale2;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const float2 factor2 = make_float2(a.scale2, a.scale2), from2 = make_float2(-from, -from);
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int c = 0; c < AT_TILE; c += 32) {
-        uint32_t p[16];
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float x = at_exp2(fmaf(s[c + i], a.scale2, -from)), y = at_exp2(fmaf(s[c + i + 1], a.scale2, -from));
-          sum[i & 3] += x;
-          sum[(i & 3) + 1] += y;
-          p[i / 2] = pack2<T>(x, y);
+        for (int c = half * 64; c < half * 64 + 64; c += 32) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const float2 x = fma2(make_float2(s[c + i], s[c + i + 1]), factor2, from2);
+            const float2 e = i % 16 < AT_POLY ? at_exp2_poly(x) : make_float2(at_exp2(x.x), at_exp2(x.y));
+            sum[(i / 2) & 1] = add2(sum[(i / 2) & 1], e);
+            p[i / 2] = pack2<T>(e.x, e.y);
+          }
+          if (EARLY && c == 0 && j > 0) {
+            ok = wait(&bar_o[t], (j - 1) & 1);   // the last P has been read
+            umma_fence_after();
+          }
+          tmem_store16(p_at + c / 2, p);
         }
-        tmem_store16(s_at + c / 2, p);
+        tmem_store_wait();
+        at_arrive(&bar_p[t][half]);
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_store_wait();
-      umma_fence_before();
-      psgd_mbar_arrive(&bar_p[t]);
+      if (!ok) break;
+      l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
     }
     if (ok && n[t] > 0) ok = wait(&bar_o[t], (n[t] - 1) & 1);
     if (ok && n[t] > 0) {
       umma_fence_after();
-      const bool held = q < length;
-      T* out = (T*)a.out + ((long long)(start + (held ? q : 0)) * a.heads + head) * a.size;
-      at_write_row<T, PANELS>(o_at, 1.f / l, out, a.size, held);
-      if (held) a.lse[(long long)head * a.tokens + start + q] = m * a.scale2 + log2f(l);
+      const int first = row0 + t * AT_TILE + (warp & 3) * 32;      // the warp's rows
+      const long long at = ((long long)(start + first) * a.heads + head) * a.size;
+      at_write_rows<T, PANELS>(o_at, 1.f / l, s_q + t * TILE_BYTES + (warp & 3) * 4096, (T*)a.out + at, a.rest == nullptr ? nullptr : (T*)a.rest + at,
+                               (long long)a.heads * a.size, length - first, a.size);
+      if (q < length) a.lse[(long long)head * a.tokens + start + q] = m * a.scale2 + log2f(l);
     }
   }
   umma_fence_before();
@@ -386,219 +492,239 @@ __global__ void __launch_bounds__(AF_THREADS, 1) psgd_attention_kernel(const __g
     psgd_let_copies_land();
     __syncthreads();
   }
-  if (warp == 9) {
+  if (warp == ISSUER) {
     __syncwarp();
-    tmem_free(tmem, 512);
+    tmem_free(tmem, COLUMNS);
   }
 }
 
 // ---- backward ----------------------------------------------------------------------------------
-constexpr int AB_THREADS = 320;   // warps 0-7: scores (0-3 columns 0-63 of a tile, 4-7 the others); 8: loads; 9: products
+constexpr int AB_MOST_SPLIT = 8;      // blocks of a cluster
+constexpr int AB_ENOUGH = 4 * 148;    // with so many blocks the heads of a group stay in one
+// CHAINS of four warps each take the steps in turn; then a warp that loads and one that issues the products. One chain where two blocks fit an SM,
+// two where one does.
+__host__ __device__ constexpr int ab_threads(int chains) { return 128 * chains + 64; }
+// Tiles that pass come in pairs (K and V, or Q and dO).
+__host__ __device__ constexpr int ab_stages(int panels, int chains) { return panels == 1 ? 3 : chains == 1 ? 1 : 4; }
+__host__ __device__ constexpr size_t ab_shared(int panels, int chains) { return 1024 + (size_t)panels * (2 * UMMA_PANEL + ab_stages(panels, chains) * UMMA_PANEL); }
 
-template <int PANELS>
-constexpr size_t ab_shared() { return 1024 + (size_t)6 * PANELS * UMMA_PANEL; }   // two tiles that stay, two stages of two that pass
-
+template <int CHAINS, int STAGES>
 struct AbBars {
-  uint64_t fixed, full[2], empty[2], s, dp, p, ds, done;
+  uint64_t fixed, full[STAGES], empty[STAGES], s[CHAINS], dp[CHAINS], p[CHAINS], ds[CHAINS], done;
+  __device__ __forceinline__ void init() {
+    psgd_mbar_init(&fixed, 1);
+    for (int i = 0; i < STAGES; ++i) {
+      psgd_mbar_init(&full[i], 1);
+      psgd_mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < CHAINS; ++i) {
+      psgd_mbar_init(&s[i], 1);
+      psgd_mbar_init(&dp[i], 1);
+      psgd_mbar_init(&p[i], 4);
+      psgd_mbar_init(&ds[i], 4);
+    }
+    psgd_mbar_init(&done, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
 };
 
-__device__ __forceinline__ void ab_init(AbBars& b) {
-  psgd_mbar_init(&b.fixed, 1);
-  for (int i = 0; i < 2; ++i) {
-    psgd_mbar_init(&b.full[i], 1);
-    psgd_mbar_init(&b.empty[i], 1);
+// 64 exponentials 2^(scale2 s - at) of a row.
+__device__ __forceinline__ void ab_exponentials(float* s, float scale2, float at) {
+  const float2 factor = make_float2(scale2, scale2), minus = make_float2(-at, -at);
+#pragma unroll
+  for (int c = 0; c < AT_STEP; c += 2) {
+    const float2 x = fma2(make_float2(s[c], s[c + 1]), factor, minus);
+    const float2 e = c % 16 < AT_POLY ? at_exp2_poly(x) : make_float2(at_exp2(x.x), at_exp2(x.y));
+    s[c] = e.x;
+    s[c + 1] = e.y;
   }
-  psgd_mbar_init(&b.s, 1);
-  psgd_mbar_init(&b.dp, 1);
-  psgd_mbar_init(&b.p, 256);
-  psgd_mbar_init(&b.ds, 256);
-  psgd_mbar_init(&b.done, 1);
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
 
-// dQ: tensor memory holds S (128 columns), dP (128; dS takes its place in halves of 32 columns at 0 and 64) and dQ.
-// S of the next tile is multiplied as soon as this one is in registers, dP of the next behind dQ of this one.
+// dQ: tensor memory holds, per chain, S and dP (64 columns each; dS takes the first half of dP's place), and dQ. S of a chain's next step is
+// multiplied as soon as this one is in registers, its dP behind dQ of this one.
 template <typename T, int PANELS>
-__global__ void __launch_bounds__(AB_THREADS, 1) psgd_attention_dq_kernel(const __grid_constant__ AtArgs a) {
-  constexpr int TILE_BYTES = PANELS * UMMA_PANEL;
+__global__ void __launch_bounds__(ab_threads(1), 2) psgd_attention_dq_kernel(const __grid_constant__ AtArgs a) {
+  constexpr int TILE_BYTES = PANELS * UMMA_PANEL, HALF = TILE_BYTES / 2, STAGES = ab_stages(PANELS, 1);
+  constexpr int DP = AT_STEP, DQ = 2 * AT_STEP, COLUMNS = 256;   // tensor memory
+  constexpr int LOADER = 4, ISSUER = 5;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = base;
   uint8_t* s_g = base + TILE_BYTES;
   uint8_t* s_ring = base + 2 * TILE_BYTES;   // stage: K, V
-  __shared__ __align__(8) AbBars bars;
-  __shared__ float s_delta[AT_TILE];
+  __shared__ __align__(8) AbBars<1, STAGES> bars;
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_found;
   __shared__ AtPiece s_piece;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int head = blockIdx.x % a.heads, index = blockIdx.x / a.heads;
-  at_clear_outside<T>(a, (T*)a.dq, a.heads, head, index);
   if (warp == 0) {
-    AtPiece piece = {0, 0, 0};
+    AtPiece piece = {0, 0, 0, 0, 0};
     const bool found = at_find(a, AT_TILE, index, false, piece);
     if (lane == 0) {
       s_piece = piece;
       s_found = found;
     }
   }
+  if (warp == LOADER && lane < 4) tma_prefetch_map(lane == 0 ? &a.q : lane == 1 ? &a.g : lane == 2 ? &a.k : &a.v);
   if (tid == 32) {
-    ab_init(bars);
+    bars.init();
     s_abort = 0;
   }
-  __syncthreads();
-  if (!s_found) return;
-  if (warp == 9) tmem_alloc(&s_tmem, 512);
+  if (warp == ISSUER) tmem_alloc(&s_tmem, COLUMNS);
   umma_fence_before();
   __syncthreads();
   umma_fence_after();
+  at_clear_outside<T>(a, s_piece, (T*)a.dq, a.heads, head, index);
+  if (!s_found) {
+    if (warp == ISSUER) tmem_free(s_tmem, COLUMNS);
+    return;
+  }
   const uint32_t tmem = s_tmem;
   const AtWait wait = {&s_abort, a.status};
   const int start = s_piece.start, length = s_piece.length, q0 = s_piece.piece * AT_TILE;
-  const int steps = a.causal ? s_piece.piece + 1 : (length + AT_TILE - 1) / AT_TILE;
-  constexpr int DP = AT_TILE, DQ = 2 * AT_TILE;   // columns
+  const int steps = (a.causal ? min(q0 + AT_TILE, length) + AT_STEP - 1 : length + AT_STEP - 1) / AT_STEP;
 
-  if (warp == 8) {
+  if (warp == LOADER) {
     if (lane == 0) {
       psgd_mbar_expect_tx(&bars.fixed, 2 * TILE_BYTES);
-      at_load_tile<PANELS>(psgd_smem_u32(s_q), &a.q, head, start + q0, &bars.fixed);
-      at_load_tile<PANELS>(psgd_smem_u32(s_g), &a.g, head, start + q0, &bars.fixed);
+      at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_q), &a.q, head, start + q0, &bars.fixed);
+      at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_g), &a.g, head, start + q0, &bars.fixed);
       for (int j = 0; j < steps; ++j) {
-        const int slot = j & 1;
-        if (!wait(&bars.empty[slot], ((j >> 1) & 1) ^ 1)) break;
-        psgd_mbar_expect_tx(&bars.full[slot], 2 * TILE_BYTES);
-        const uint32_t at = psgd_smem_u32(s_ring + slot * 2 * TILE_BYTES);
-        at_load_tile<PANELS>(at, &a.k, head / a.group, start + j * AT_TILE, &bars.full[slot]);
-        at_load_tile<PANELS>(at + TILE_BYTES, &a.v, head / a.group, start + j * AT_TILE, &bars.full[slot]);
+        const int slot = j % STAGES;
+        if (!wait(&bars.empty[slot], ((j / STAGES) & 1) ^ 1)) break;
+        psgd_mbar_expect_tx(&bars.full[slot], 2 * HALF);
+        const uint32_t at = psgd_smem_u32(s_ring + slot * TILE_BYTES);
+        at_load_tile<PANELS, AT_STEP>(at, &a.k, head / a.group, start + j * AT_STEP, &bars.full[slot]);
+        at_load_tile<PANELS, AT_STEP>(at + HALF, &a.v, head / a.group, start + j * AT_STEP, &bars.full[slot]);
       }
     }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      const int k_steps = (a.size + 15) / 16;
-      constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_TILE);
-      const uint32_t q_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
-      const uint32_t q_at = psgd_smem_u32(s_q), g_at = psgd_smem_u32(s_g), ring_at = psgd_smem_u32(s_ring);
-      auto scores = [&](int j) {
-        umma_rows_by_rows(tmem, q_at, ring_at + (j & 1) * 2 * TILE_BYTES, S_SHAPE, k_steps, false);
-        umma_arrive(&bars.s);
-      };
-      auto slopes = [&](int j) {
-        umma_rows_by_rows(tmem + DP, g_at, ring_at + (j & 1) * 2 * TILE_BYTES + TILE_BYTES, S_SHAPE, k_steps, false);
-        umma_arrive(&bars.dp);
-      };
-      bool ok = wait(&bars.fixed, 0) && wait(&bars.full[0], 0);
-      if (ok) {
-        umma_fence_after();
-        scores(0);
-        slopes(0);
-      }
-      for (int j = 0; j < steps && ok; ++j) {
-        ok = wait(&bars.p, j & 1);    // S is in registers
-        if (!ok) break;
-        umma_fence_after();
-        if (j + 1 < steps) {
-          ok = wait(&bars.full[(j + 1) & 1], ((j + 1) >> 1) & 1);
-          if (!ok) break;
-          umma_fence_after();
-          scores(j + 1);
-        }
-        ok = wait(&bars.ds, j & 1);
-        if (!ok) break;
-        umma_fence_after();
-        for (int s = 0; s < AT_TILE / 16; ++s)
-          umma_ts(tmem + DQ, tmem + DP + (s >> 2) * 64 + (s & 3) * 8, umma_tile(ring_at + (j & 1) * 2 * TILE_BYTES + s * 2048), q_shape, j > 0 || s > 0);
-        umma_arrive(&bars.empty[j & 1]);
-        if (j + 1 < steps) slopes(j + 1);
-        else umma_arrive(&bars.done);
+  } else if (warp == ISSUER) {
+    const AtWaitAll wait_all = {wait};
+    const int k_steps = (a.size + 15) / 16;
+    constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_STEP);
+    const uint32_t q_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
+    const uint32_t q_at = psgd_smem_u32(s_q), g_at = psgd_smem_u32(s_g), ring_at = psgd_smem_u32(s_ring);
+    bool ok = wait_all(&bars.fixed, 0);
+    int have = -1;
+    auto there = [&](int j) {
+      if (j > have) ok = ok && wait_all(&bars.full[j % STAGES], (j / STAGES) & 1);
+      have = j;
+      if (ok) umma_fence_after();
+      return ok;
+    };
+    auto scores = [&](int j) {
+      if (!there(j)) return;
+      umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem, q_at, ring_at + j % STAGES * TILE_BYTES, S_SHAPE, k_steps);
+      umma_arrive(&bars.s[0]);
+    };
+    auto slopes = [&](int j) {
+      if (!there(j)) return;
+      umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem + DP, g_at, ring_at + j % STAGES * TILE_BYTES + HALF, S_SHAPE, k_steps);
+      umma_arrive(&bars.dp[0]);
+    };
+    scores(0);
+    if (ok) slopes(0);
+    for (int j = 0; j < steps && ok; ++j) {
+      ok = wait_all(&bars.p[0], j & 1);    // S is in registers
+      if (!ok) break;
+      umma_fence_after();
+      // (with one stage the next keys come when dQ has been multiplied)
+      if (STAGES > 1 && j + 1 < steps) scores(j + 1);
+      ok = ok && wait_all(&bars.ds[0], j & 1);
+      if (!ok) break;
+      umma_fence_after();
+      umma_weights_by_rows<0, 4, AT_STEP>(tmem + DQ, tmem + DP, ring_at + j % STAGES * TILE_BYTES, q_shape, j > 0);
+      umma_arrive(&bars.empty[j % STAGES]);
+      if (j + 1 < steps) {
+        if (STAGES == 1) scores(j + 1);
+        if (ok) slopes(j + 1);
+      } else {
+        umma_arrive(&bars.done);
       }
     }
   } else {
-    const int half = warp >> 2, row = tid & 127, q = q0 + row;
+    const int row = tid, q = q0 + row;
     const bool held = q < length;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const long long stat = (long long)head * a.tokens + start + q;
-    // delta of the row, once for the keys' pass too
-    if (half == 0) {
-      float d = 0.f;
-      if (held) {
-        const T* o = (const T*)a.out + ((long long)(start + q) * a.heads + head) * a.size;
-        const T* g = (const T*)a.grad + (long long)(start + q) * a.grad_row + (long long)head * a.grad_head;
-        for (int c = 0; c < a.size; c += 8) {
-          const uint4 x = *reinterpret_cast<const uint4*>(o + c), y = *reinterpret_cast<const uint4*>(g + c);
-          const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    // delta of the row, for the keys' pass too. It is a small difference of large sums, and what it is off by moves a whole row of
+    // dS one way: it takes the output unrounded, in two parts. (With the rounded one dQ and dK were off by 1.7 times their own
+    // rounding, so by 1.4.)
+    float delta = 0.f, lse = 0.f;
+    if (held) {
+      const long long at = ((long long)(start + q) * a.heads + head) * a.size;
+      const T* o = (const T*)a.out + at;
+      const T* o_rest = (const T*)a.rest + at;
+      const T* g = (const T*)a.grad + (long long)(start + q) * a.grad_row + (long long)head * a.grad_head;
+      lse = a.lse[stat];
+#pragma unroll 4
+      for (int c = 0; c < a.size; c += 8) {
+        const uint4 x = *reinterpret_cast<const uint4*>(o + c), y = *reinterpret_cast<const uint4*>(g + c), z = *reinterpret_cast<const uint4*>(o_rest + c);
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 u = unpack2<T>(xs[i]), v = unpack2<T>(ys[i]);
-            d = fmaf(u.x, v.x, d);
-            d = fmaf(u.y, v.y, d);
-          }
+        for (int i = 0; i < 4; ++i) {
+          const float2 u = unpack2<T>(xs[i]), v = unpack2<T>(ys[i]), w = unpack2<T>(zs[i]);
+          delta = fmaf(u.x + w.x, v.x, delta);
+          delta = fmaf(u.y + w.y, v.y, delta);
         }
-        a.delta[stat] = d;
       }
-      s_delta[row] = d;
+      a.delta[stat] = delta;
     }
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    const float delta = s_delta[row], lse = held ? a.lse[stat] : 0.f;
-    const int limit = (a.causal ? min(q, length - 1) : length - 1) - half * 64;
+    const int limit = a.causal ? min(q, length - 1) : length - 1;    // last key that counts
     bool ok = true;
     for (int j = 0; j < steps; ++j) {
-      ok = wait(&bars.s, j & 1);
+      ok = wait(&bars.s[0], j & 1);
       if (!ok) break;
       umma_fence_after();
-      float p[64];
-      tmem_load32(tmem + lanes + half * 64, p);
-      tmem_load32(tmem + lanes + half * 64 + 32, p + 32);
+      float p[AT_STEP];
+      tmem_load32(tmem + lanes, p);
+      tmem_load32(tmem + lanes + 32, p + 32);
       tmem_load_wait();
-      umma_fence_before();
-      psgd_mbar_arrive(&bars.p);
-      const bool edge = j == steps - 1;
-      const int last = limit - j * AT_TILE;
-#pragma unroll
-      for (int c = 0; c < 64; ++c) p[c] = at_exp2(fmaf(p[c], a.scale2, -lse));
+      at_arrive(&bars.p[0]);
+      ab_exponentials(p, a.scale2, lse);
+      const int last = limit - j * AT_STEP;
+      const bool edge = (j + 1) * AT_STEP > (a.causal ? min(q0 + 1, length) : length);     // some key of this step does not count for some row
       if (edge) {
-#pragma unroll
-        for (int c = 0; c < 64; ++c)
-          if (c > last) p[c] = 0.f;
-        const int keys = length - j * AT_TILE;
-        if (keys < AT_TILE) {
-          ok = wait(&bars.full[j & 1], (j >> 1) & 1);
+        const int keys = length - j * AT_STEP;
+        if (keys < AT_STEP) {
+          ok = wait(&bars.full[j % STAGES], (j / STAGES) & 1);
           if (!ok) break;
-          if (half == 0) at_clear_row<PANELS>(s_ring + (j & 1) * 2 * TILE_BYTES, row, keys);
+          if (row >= keys && row < AT_STEP) at_clear_row<PANELS, AT_STEP>(s_ring + j % STAGES * TILE_BYTES, row);
           psgd_fence_async_shared();
         }
       }
-      ok = wait(&bars.dp, j & 1);
+      ok = wait(&bars.dp[0], j & 1);
       if (!ok) break;
       umma_fence_after();
+      const float2 minus = make_float2(-delta, -delta);
 #pragma unroll
-      for (int c = 0; c < 64; c += 32) {
+      for (int c = 0; c < AT_STEP; c += 32) {
         float d[32];
-        tmem_load32(tmem + lanes + DP + half * 64 + c, d);
+        tmem_load32(tmem + lanes + DP + c, d);
         tmem_load_wait();
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float x = p[c + i] * (d[i] - delta), y = p[c + i + 1] * (d[i + 1] - delta);
-          if (edge) {   // (a masked key may hold anything)
-            if (c + i > last) x = 0.f;
-            if (c + i + 1 > last) y = 0.f;
+          float2 x = mul2(make_float2(p[c + i], p[c + i + 1]), add2(make_float2(d[i], d[i + 1]), minus));
+          if (edge) {   // (a key that does not count may hold anything)
+            if (c + i > last) x.x = 0.f;
+            if (c + i + 1 > last) x.y = 0.f;
           }
-          w[i / 2] = pack2<T>(x, y);
+          w[i / 2] = pack2<T>(x.x, x.y);
         }
-        tmem_store16(tmem + lanes + DP + half * 64 + c / 2, w);
+        tmem_store16(tmem + lanes + DP + c / 2, w);
       }
       tmem_store_wait();
-      umma_fence_before();
-      psgd_mbar_arrive(&bars.ds);
+      at_arrive(&bars.ds[0]);
     }
     if (ok) ok = wait(&bars.done, 0);
     if (ok) {
       umma_fence_after();
-      if (half == 0) {
-        T* out = (T*)a.dq + ((long long)(start + (held ? q : 0)) * a.heads + head) * a.size;
-        at_write_row<T, PANELS>(tmem + lanes + DQ, a.scale, out, a.size, held);
-      }
+      const int first = q0 + warp * 32;
+      at_write_rows<T, PANELS>(tmem + lanes + DQ, a.scale, s_q + warp * 4096, (T*)a.dq + ((long long)(start + first) * a.heads + head) * a.size, (T*)nullptr,
+                               (long long)a.heads * a.size, length - first, a.size);
     }
   }
   umma_fence_before();
@@ -607,211 +733,246 @@ __global__ void __launch_bounds__(AB_THREADS, 1) psgd_attention_dq_kernel(const 
     psgd_let_copies_land();
     __syncthreads();
   }
-  if (warp == 9) {
+  if (warp == ISSUER) {
     __syncwarp();
-    tmem_free(tmem, 512);
+    tmem_free(tmem, COLUMNS);
   }
 }
 
-// dK, dV: tensor memory holds S^T (P^T takes its place), dP^T (dS^T likewise), dV and dK: 4 x 128 columns. dV of a tile and S^T of the
-// next are multiplied while dS^T is formed, dK and dP^T of the next while the next exponentials are taken.
+// dK, dV: tensor memory holds, per chain, S^T (P^T takes the first half of its place) and dP^T (dS^T likewise), 64 columns each, and dV and dK. dV
+// of a step and S^T of the chain's next are multiplied while dS^T is formed, dK and the next dP^T while the next exponentials are
+// taken. Where few tiles of keys share many query heads, the heads are dealt out over a cluster of blocks (`split`), whose sums are
+// added in shared memory, in the order of their rank.
 template <typename T, int PANELS>
-__global__ void __launch_bounds__(AB_THREADS, 1) psgd_attention_dkv_kernel(const __grid_constant__ AtArgs a) {
-  constexpr int TILE_BYTES = PANELS * UMMA_PANEL;
+__global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention_dkv_kernel(const __grid_constant__ AtArgs a) {
+  constexpr int CHAINS = PANELS;
+  constexpr int TILE_BYTES = PANELS * UMMA_PANEL, HALF = TILE_BYTES / 2, STAGES = ab_stages(PANELS, CHAINS);
+  constexpr int DV = 2 * AT_STEP * CHAINS, DK = DV + 64 * PANELS, COLUMNS = 256 * CHAINS;   // tensor memory; chain c has its scores at 128 c, slopes behind
+  constexpr int LOADER = 4 * CHAINS, ISSUER = LOADER + 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_k = base;
   uint8_t* s_v = base + TILE_BYTES;
   uint8_t* s_ring = base + 2 * TILE_BYTES;   // stage: Q, dO
-  __shared__ __align__(8) AbBars bars;
-  __shared__ __align__(16) float s_lse[3][AT_TILE], s_delta[3][AT_TILE];   // of tile i in place i % 3, see below
+  __shared__ __align__(8) AbBars<CHAINS, STAGES> bars;
+  __shared__ __align__(16) float s_stats[CHAINS][3][2 * AT_STEP];   // of a chain's i-th step in place i % 3 (see below): logarithms, then deltas
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_found;
   __shared__ AtPiece s_piece;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int kv_heads = a.heads / a.group, head = blockIdx.x % kv_heads, index = blockIdx.x / kv_heads;
-  at_clear_outside<T>(a, (T*)a.dk, kv_heads, head, index);
-  at_clear_outside<T>(a, (T*)a.dv, kv_heads, head, index);
+  const int kv_heads = a.heads / a.group, rank = blockIdx.x % a.split, block = blockIdx.x / a.split;
+  const int head = block % kv_heads, index = block / kv_heads;
   if (warp == 0) {
-    AtPiece piece = {0, 0, 0};
+    AtPiece piece = {0, 0, 0, 0, 0};
     const bool found = at_find(a, AT_TILE, index, true, piece);
     if (lane == 0) {
       s_piece = piece;
       s_found = found;
     }
   }
+  if (warp == LOADER && lane < 4) tma_prefetch_map(lane == 0 ? &a.q : lane == 1 ? &a.g : lane == 2 ? &a.k : &a.v);
   if (tid == 32) {
-    ab_init(bars);
+    bars.init();
     s_abort = 0;
   }
-  __syncthreads();
-  if (!s_found) return;
-  if (warp == 9) tmem_alloc(&s_tmem, 512);
+  if (warp == ISSUER) tmem_alloc(&s_tmem, COLUMNS);
   umma_fence_before();
   __syncthreads();
   umma_fence_after();
+  if (rank == 0) {
+    at_clear_outside<T>(a, s_piece, (T*)a.dk, kv_heads, head, index);
+    at_clear_outside<T>(a, s_piece, (T*)a.dv, kv_heads, head, index);
+  }
+  if (!s_found) {   // (so for all blocks of the cluster)
+    if (warp == ISSUER) tmem_free(s_tmem, COLUMNS);
+    return;
+  }
   const uint32_t tmem = s_tmem;
   const AtWait wait = {&s_abort, a.status};
   const int start = s_piece.start, length = s_piece.length, k0 = s_piece.piece * AT_TILE;
-  const int first = a.causal ? s_piece.piece : 0;                     // first tile of queries
-  const int per_head = (length + AT_TILE - 1) / AT_TILE - first, steps = per_head * a.group;
-  constexpr int DP = AT_TILE, DV = 2 * AT_TILE, DK = 3 * AT_TILE;     // columns
-  auto q_head = [&](int i) { return head * a.group + i / per_head; };
-  auto q_row = [&](int i) { return (first + i % per_head) * AT_TILE; };
+  const int first = a.causal ? k0 / AT_STEP : 0;                      // first step of queries
+  const int per_head = (length + AT_STEP - 1) / AT_STEP - first, heads = a.group / a.split, steps = per_head * heads;
+  const int head0 = head * a.group + rank * heads;
+  auto q_head = [&](int i) { return head0 + i / per_head; };
+  auto q_row = [&](int i) { return (first + i % per_head) * AT_STEP; };
 
-  if (warp == 8) {
+  if (warp == LOADER) {
     if (lane == 0) {
       psgd_mbar_expect_tx(&bars.fixed, 2 * TILE_BYTES);
-      at_load_tile<PANELS>(psgd_smem_u32(s_k), &a.k, head, start + k0, &bars.fixed);
-      at_load_tile<PANELS>(psgd_smem_u32(s_v), &a.v, head, start + k0, &bars.fixed);
+      at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_k), &a.k, head, start + k0, &bars.fixed);
+      at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_v), &a.v, head, start + k0, &bars.fixed);
       for (int i = 0; i < steps; ++i) {
-        const int slot = i & 1;
-        if (!wait(&bars.empty[slot], ((i >> 1) & 1) ^ 1)) break;
-        psgd_mbar_expect_tx(&bars.full[slot], 2 * TILE_BYTES);
-        const uint32_t at = psgd_smem_u32(s_ring + slot * 2 * TILE_BYTES);
-        at_load_tile<PANELS>(at, &a.q, q_head(i), start + q_row(i), &bars.full[slot]);
-        at_load_tile<PANELS>(at + TILE_BYTES, &a.g, q_head(i), start + q_row(i), &bars.full[slot]);
+        const int slot = i % STAGES;
+        if (!wait(&bars.empty[slot], ((i / STAGES) & 1) ^ 1)) break;
+        psgd_mbar_expect_tx(&bars.full[slot], 2 * HALF);
+        const uint32_t at = psgd_smem_u32(s_ring + slot * TILE_BYTES);
+        at_load_tile<PANELS, AT_STEP>(at, &a.q, q_head(i), start + q_row(i), &bars.full[slot]);
+        at_load_tile<PANELS, AT_STEP>(at + HALF, &a.g, q_head(i), start + q_row(i), &bars.full[slot]);
       }
     }
-  } else if (warp == 9) {
-    if (lane == 0) {
-      const int k_steps = (a.size + 15) / 16;
-      constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_TILE);
-      const uint32_t o_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
-      const uint32_t k_at = psgd_smem_u32(s_k), v_at = psgd_smem_u32(s_v), ring_at = psgd_smem_u32(s_ring);
-      auto scores = [&](int i) {
-        umma_rows_by_rows(tmem, k_at, ring_at + (i & 1) * 2 * TILE_BYTES, S_SHAPE, k_steps, false);
-        umma_arrive(&bars.s);
-      };
-      auto slopes = [&](int i) {
-        umma_rows_by_rows(tmem + DP, v_at, ring_at + (i & 1) * 2 * TILE_BYTES + TILE_BYTES, S_SHAPE, k_steps, false);
-        umma_arrive(&bars.dp);
-      };
-      // the halves of P^T and dS^T lie 64 columns apart
-      auto second = [&](uint32_t d, uint32_t p, uint32_t tile, bool more) {
-        for (int s = 0; s < AT_TILE / 16; ++s) umma_ts(tmem + d, tmem + p + (s >> 2) * 64 + (s & 3) * 8, umma_tile(tile + s * 2048), o_shape, more || s > 0);
-      };
-      bool ok = wait(&bars.fixed, 0) && wait(&bars.full[0], 0);
-      if (ok) {
-        umma_fence_after();
-        scores(0);
-        slopes(0);
-      }
-      for (int i = 0; i < steps && ok; ++i) {
-        const uint32_t stage = ring_at + (i & 1) * 2 * TILE_BYTES;
-        ok = wait(&bars.p, i & 1);
-        if (!ok) break;
-        umma_fence_after();
-        second(DV, 0, stage + TILE_BYTES, i > 0);
-        if (i + 1 < steps) {
-          ok = wait(&bars.full[(i + 1) & 1], ((i + 1) >> 1) & 1);
-          if (!ok) break;
-          umma_fence_after();
-          scores(i + 1);
-        }
-        ok = wait(&bars.ds, i & 1);
-        if (!ok) break;
-        umma_fence_after();
-        second(DK, DP, stage, i > 0);
-        umma_arrive(&bars.empty[i & 1]);
-        if (i + 1 < steps) slopes(i + 1);
-        else umma_arrive(&bars.done);
-      }
-    }
-  } else {
-    const int half = warp >> 2, row = tid & 127, key = k0 + row;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-    auto statistic = [&](int i) {   // of query `row` of tile i: log of the sum, or delta
-      const int q = q_row(i) + row;
-      if (q >= length) return 0.f;
-      return (half == 0 ? a.lse : a.delta)[(long long)q_head(i) * a.tokens + start + q];
+  } else if (warp == ISSUER) {
+    const AtWaitAll wait_all = {wait};
+    const int k_steps = (a.size + 15) / 16;
+    constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_STEP);
+    const uint32_t o_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
+    const uint32_t k_at = psgd_smem_u32(s_k), v_at = psgd_smem_u32(s_v), ring_at = psgd_smem_u32(s_ring);
+    bool ok = wait_all(&bars.fixed, 0);
+    int have = -1;
+    auto there = [&](int i) {
+      if (i > have) ok = ok && wait_all(&bars.full[i % STAGES], (i / STAGES) & 1);
+      have = max(have, i);
+      if (ok) umma_fence_after();
+      return ok;
     };
-    float (*mine)[AT_TILE] = half == 0 ? s_lse : s_delta;
-    mine[0][row] = statistic(0);
-    asm volatile("bar.sync 1, 256;" ::: "memory");
-    bool ok = true;
-    for (int i = 0; i < steps; ++i) {
-      const float ahead = i + 1 < steps ? statistic(i + 1) : 0.f;
-      const int q0 = q_row(i) + half * 64, queries = length - q_row(i);
-      // queries [from, to) of this thread's columns meet its key
-      const int from = a.causal ? key - q0 : 0, to = length - q0;
-      const bool edge = (a.causal && i % per_head == 0) || queries < AT_TILE;
-      // The statistics of tile i were written before the arrivals for tile i - 1. A warp may be behind by the second half of a tile, no
-      // more: two places would not do, three do.
-      ok = (i == 0 || wait(&bars.p, (i - 1) & 1)) && wait(&bars.s, i & 1);
+    auto scores = [&](int i) {
+      if (!there(i)) return;
+      umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem + i % CHAINS * 128, k_at, ring_at + i % STAGES * TILE_BYTES, S_SHAPE, k_steps);
+      umma_arrive(&bars.s[i % CHAINS]);
+    };
+    auto slopes = [&](int i) {
+      if (!there(i)) return;
+      umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem + i % CHAINS * 128 + AT_STEP, v_at, ring_at + i % STAGES * TILE_BYTES + HALF, S_SHAPE, k_steps);
+      umma_arrive(&bars.dp[i % CHAINS]);
+    };
+    for (int i = 0; i < CHAINS && i < steps && ok; ++i) {
+      scores(i);
+      if (ok) slopes(i);
+    }
+    for (int i = 0; i < steps && ok; ++i) {
+      const int chain = i % CHAINS;
+      const uint32_t parity = (i / CHAINS) & 1, stage = ring_at + i % STAGES * TILE_BYTES;
+      ok = wait_all(&bars.p[chain], parity);
       if (!ok) break;
       umma_fence_after();
-      float p[64];
-      tmem_load32(tmem + lanes + half * 64, p);
-      tmem_load32(tmem + lanes + half * 64 + 32, p + 32);
+      umma_weights_by_rows<0, 4, AT_STEP>(tmem + DV, tmem + chain * 128, stage + HALF, o_shape, i > 0);
+      if (i + CHAINS < steps) scores(i + CHAINS);
+      ok = ok && wait_all(&bars.ds[chain], parity);
+      if (!ok) break;
+      umma_fence_after();
+      umma_weights_by_rows<0, 4, AT_STEP>(tmem + DK, tmem + chain * 128 + AT_STEP, stage, o_shape, i > 0);
+      umma_arrive(&bars.empty[i % STAGES]);
+      if (i + CHAINS < steps) slopes(i + CHAINS);
+      if (i == steps - 1) umma_arrive(&bars.done);
+    }
+  } else {
+    const int chain = warp >> 2, row = tid & 127, key = k0 + row;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + chain * 128, dp_at = s_at + AT_STEP;
+    auto statistic = [&](int i) {   // of query row % 64 of step i: logarithm of the sum, or delta
+      const int q = q_row(i) + row % AT_STEP;
+      if (q >= length) return 0.f;
+      return (row < AT_STEP ? a.lse : a.delta)[(long long)q_head(i) * a.tokens + start + q];
+    };
+    float (*stats)[2 * AT_STEP] = s_stats[chain];
+    if (chain < steps) stats[0][row] = statistic(chain);
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + chain) : "memory");
+    bool ok = true;
+    int mine = 0;                   // steps of this chain so far
+    for (int i = chain; i < steps; i += CHAINS, ++mine) {
+      const float ahead = i + CHAINS < steps ? statistic(i + CHAINS) : 0.f;
+      const int q0 = q_row(i), queries = length - q0;
+      // queries [from, to) of the step meet this thread's key
+      const int from = a.causal ? key - q0 : 0, to = queries;
+      const bool edge = (a.causal && q0 < k0 + AT_TILE) || queries < AT_STEP;
+      const float* now = stats[mine % 3];
+      // The statistics of a step were written before the arrivals for the one before. A warp may be behind by the second half of a step, no
+      // more: two places would not do, three do.
+      ok = (mine == 0 || wait(&bars.p[chain], (mine - 1) & 1)) && wait(&bars.s[chain], mine & 1);
+      if (!ok) break;
+      umma_fence_after();
+      float p[AT_STEP];
+      tmem_load32(s_at, p);
+      tmem_load32(s_at + 32, p + 32);
       tmem_load_wait();
-      const float4* lse = reinterpret_cast<const float4*>(&s_lse[i % 3][half * 64]);
+      const float2 factor = make_float2(a.scale2, a.scale2);
 #pragma unroll
-      for (int c = 0; c < 64; c += 4) {
-        const float4 x = lse[c / 4];
-        p[c] = at_exp2(fmaf(p[c], a.scale2, -x.x));
-        p[c + 1] = at_exp2(fmaf(p[c + 1], a.scale2, -x.y));
-        p[c + 2] = at_exp2(fmaf(p[c + 2], a.scale2, -x.z));
-        p[c + 3] = at_exp2(fmaf(p[c + 3], a.scale2, -x.w));
+      for (int c = 0; c < AT_STEP; c += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(now + c);
+#pragma unroll
+        for (int h = 0; h < 4; h += 2) {
+          const float2 y = fma2(make_float2(p[c + h], p[c + h + 1]), factor, h ? make_float2(-x.z, -x.w) : make_float2(-x.x, -x.y));
+          const float2 e = (c + h) % 16 < AT_POLY ? at_exp2_poly(y) : make_float2(at_exp2(y.x), at_exp2(y.y));
+          p[c + h] = e.x;
+          p[c + h + 1] = e.y;
+        }
       }
       if (edge) {
 #pragma unroll
-        for (int c = 0; c < 64; ++c)
+        for (int c = 0; c < AT_STEP; ++c)
           if (c < from || c >= to) p[c] = 0.f;
-        if (queries < AT_TILE) {
-          ok = wait(&bars.full[i & 1], (i >> 1) & 1);
+        if (queries < AT_STEP) {
+          ok = wait(&bars.full[i % STAGES], (i / STAGES) & 1);
           if (!ok) break;
-          at_clear_row<PANELS>(s_ring + (i & 1) * 2 * TILE_BYTES + half * TILE_BYTES, row, queries);
+          const int r = row % AT_STEP;
+          if (r >= queries) at_clear_row<PANELS, AT_STEP>(s_ring + i % STAGES * TILE_BYTES + (row < AT_STEP ? 0 : HALF), r);
           psgd_fence_async_shared();
         }
       }
-      // S^T is 128 columns wide and P^T takes 32 of each half: a half is written by the warps that read it
 #pragma unroll
-      for (int c = 0; c < 64; c += 32) {
+      for (int c = 0; c < AT_STEP; c += 32) {
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) w[e / 2] = pack2<T>(p[c + e], p[c + e + 1]);
-        tmem_store16(tmem + lanes + half * 64 + c / 2, w);
+        tmem_store16(s_at + c / 2, w);
       }
-      mine[(i + 1) % 3][row] = ahead;
+      stats[(mine + 1) % 3][row] = ahead;
       tmem_store_wait();
-      umma_fence_before();
-      psgd_mbar_arrive(&bars.p);
-      ok = wait(&bars.dp, i & 1);
+      at_arrive(&bars.p[chain]);
+      ok = wait(&bars.dp[chain], mine & 1);
       if (!ok) break;
       umma_fence_after();
-      const float4* delta = reinterpret_cast<const float4*>(&s_delta[i % 3][half * 64]);
 #pragma unroll
-      for (int c = 0; c < 64; c += 32) {
+      for (int c = 0; c < AT_STEP; c += 32) {
         float d[32];
-        tmem_load32(tmem + lanes + DP + half * 64 + c, d);
+        tmem_load32(dp_at + c, d);
         tmem_load_wait();
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
-          const float4 x = delta[(c + e) / 4];
-          float f[4] = {p[c + e] * (d[e] - x.x), p[c + e + 1] * (d[e + 1] - x.y), p[c + e + 2] * (d[e + 2] - x.z), p[c + e + 3] * (d[e + 3] - x.w)};
-          if (edge) {
+          const float4 x = *reinterpret_cast<const float4*>(now + AT_STEP + c + e);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              if (c + e + u < from || c + e + u >= to) f[u] = 0.f;
+          for (int h = 0; h < 4; h += 2) {
+            const int at = c + e + h;
+            float2 f = mul2(make_float2(p[at], p[at + 1]), add2(make_float2(d[e + h], d[e + h + 1]), h ? make_float2(-x.z, -x.w) : make_float2(-x.x, -x.y)));
+            if (edge) {
+              if (at < from || at >= to) f.x = 0.f;
+              if (at + 1 < from || at + 1 >= to) f.y = 0.f;
+            }
+            w[(e + h) / 2] = pack2<T>(f.x, f.y);
           }
-          w[e / 2] = pack2<T>(f[0], f[1]);
-          w[e / 2 + 1] = pack2<T>(f[2], f[3]);
         }
-        tmem_store16(tmem + lanes + DP + half * 64 + c / 2, w);
+        tmem_store16(dp_at + c / 2, w);
       }
       tmem_store_wait();
-      umma_fence_before();
-      psgd_mbar_arrive(&bars.ds);
+      at_arrive(&bars.ds[chain]);
     }
     if (ok) ok = wait(&bars.done, 0);
     if (ok) {
       umma_fence_after();
-      const bool held = key < length;
-      T* out = (T*)(half == 0 ? a.dv : a.dk) + ((long long)(start + (held ? key : 0)) * kv_heads + head) * a.size;
-      at_write_row<T, PANELS>(tmem + lanes + (half == 0 ? DV : DK), half == 0 ? 1.f : a.scale, out, a.size, held);
+      // dV by the first chain, dK by the last
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        if (CHAINS == 2 && which != chain) continue;
+        const uint32_t at = tmem + lanes + (which == 0 ? DV : DK);
+        if (a.split == 1) {
+          const int first_row = k0 + (warp & 3) * 32;
+          at_write_rows<T, PANELS>(at, which == 0 ? 1.f : a.scale, (which == 0 ? s_v : s_k) + (warp & 3) * 4096,
+                                   (T*)(which == 0 ? a.dv : a.dk) + ((long long)(start + first_row) * kv_heads + head) * a.size, (T*)nullptr,
+                                   (long long)kv_heads * a.size, length - first_row, a.size);
+        } else {
+          // this block's share: [dV, dK][128 rows][64 PANELS] float32, groups of four elements where no two lanes meet in a bank
+          float* share = reinterpret_cast<float*>(base) + (which * AT_TILE + row) * 64 * PANELS;
+#pragma unroll
+          for (int c = 0; c < PANELS * 64; c += 32) {
+            float f[32];
+            tmem_load32(at + c, f);
+            tmem_load_wait();
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(share + ((c + e) ^ ((row & 7) << 2))) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+          }
+        }
+      }
     }
   }
   umma_fence_before();
@@ -820,9 +981,33 @@ __global__ void __launch_bounds__(AB_THREADS, 1) psgd_attention_dkv_kernel(const
     psgd_let_copies_land();
     __syncthreads();
   }
-  if (warp == 9) {
+  if (warp == ISSUER) {
     __syncwarp();
-    tmem_free(tmem, 512);
+    tmem_free(tmem, COLUMNS);
+  }
+  if (a.split > 1) {
+    // Rows rank, rank + split, ... of both, by this block. (Where a wait has run out somewhere the sums are not valid, and the
+    // status word says so.)
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    constexpr int FOURS = 16 * PANELS;
+    for (int e = tid; e < 2 * AT_TILE * FOURS; e += ab_threads(CHAINS)) {
+      const int which = e / (AT_TILE * FOURS), r = e / FOURS % AT_TILE, c = e % FOURS * 4;
+      if (r % a.split != rank || k0 + r >= length || c >= a.size) continue;
+      float* at = reinterpret_cast<float*>(base) + (which * AT_TILE + r) * 64 * PANELS + (c ^ ((r & 7) << 2));
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int b = 0; b < a.split; ++b) {
+        const float4 x = *reinterpret_cast<const float4*>(cluster.map_shared_rank(at, b));
+        sum.x += x.x;
+        sum.y += x.y;
+        sum.z += x.z;
+        sum.w += x.w;
+      }
+      const float f = which == 0 ? 1.f : a.scale;
+      T* out = (T*)(which == 0 ? a.dv : a.dk) + ((long long)(start + k0 + r) * kv_heads + head) * a.size + c;
+      *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(sum.x * f, sum.y * f), pack2<T>(sum.z * f, sum.w * f));
+    }
+    cluster.sync();   // nobody leaves while its share is read
   }
 }
 
@@ -830,7 +1015,10 @@ __global__ void __launch_bounds__(AB_THREADS, 1) psgd_attention_dkv_kernel(const
 typedef CUresult (*AtEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// [tokens, heads, size] with `row` and `head` elements between rows and heads: boxes of 64 elements of one head in 128 rows, zeros outside.
+// Tiles of queries per block of the forward pass.
+constexpr int at_tiles(int size) { return size <= 64 ? 1 : 2; }
+
+// [tokens, heads, size] with `row` and `head` elements between rows and heads: boxes of 64 elements of one head in 64 rows, zeros outside.
 int at_encode(CUtensorMap* map, const void* at, int type, int tokens, int heads, int size, long long row, long long head) {
   static AtEncodeFn fn = nullptr;
   if (fn == nullptr) {
@@ -844,7 +1032,7 @@ int at_encode(CUtensorMap* map, const void* at, int type, int tokens, int heads,
   }
   const cuuint64_t dims[3] = {(cuuint64_t)size, (cuuint64_t)heads, (cuuint64_t)tokens};
   const cuuint64_t strides[2] = {(cuuint64_t)head * 2, (cuuint64_t)row * 2};
-  const cuuint32_t box[3] = {64, 1, AT_TILE}, elem[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, 1, 64}, elem[3] = {1, 1, 1};
   const CUresult rc = fn(map, type == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, (void*)at, dims, strides, box, elem,
                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (rc != CUDA_SUCCESS) {
@@ -890,29 +1078,37 @@ int at_fill(AtArgs& a, const void* q, const void* k, const void* v, const long l
 
 template <typename T, int PANELS>
 int at_forward(const AtArgs& a, cudaStream_t stream) {
+  constexpr int TILES = at_tiles(PANELS * 64);
   static unsigned long long devices = 0;
-  if (const int code = psgd_allow_shared((const void*)psgd_attention_kernel<T, PANELS>, af_shared<PANELS>(), devices)) return code;
-  return psgd_launch(psgd_attention_kernel<T, PANELS>, a.blocks * a.heads, AF_THREADS, af_shared<PANELS>(), stream, 0, a);
+  if (const int code = psgd_allow_shared((const void*)psgd_attention_kernel<T, PANELS, TILES>, af_shared(PANELS, TILES), devices)) return code;
+  return psgd_launch(psgd_attention_kernel<T, PANELS, TILES>, a.blocks * a.heads, af_threads(TILES), af_shared(PANELS, TILES), stream, 0, a);
 }
 template <typename T, int PANELS>
-int at_backward(const AtArgs& a, cudaStream_t stream) {
+int at_backward(AtArgs a, cudaStream_t stream) {
   static unsigned long long q_devices = 0, kv_devices = 0;
-  if (const int code = psgd_allow_shared((const void*)psgd_attention_dq_kernel<T, PANELS>, ab_shared<PANELS>(), q_devices)) return code;
-  if (const int code = psgd_allow_shared((const void*)psgd_attention_dkv_kernel<T, PANELS>, ab_shared<PANELS>(), kv_devices)) return code;
+  if (const int code = psgd_allow_shared((const void*)psgd_attention_dq_kernel<T, PANELS>, ab_shared(PANELS, 1), q_devices)) return code;
+  if (const int code = psgd_allow_shared((const void*)psgd_attention_dkv_kernel<T, PANELS>, ab_shared(PANELS, PANELS), kv_devices)) return code;
   // (delta comes from the first)
-  if (const int code = psgd_launch(psgd_attention_dq_kernel<T, PANELS>, a.blocks * a.heads, AB_THREADS, ab_shared<PANELS>(), stream, 0, a)) return code;
-  return psgd_launch(psgd_attention_dkv_kernel<T, PANELS>, a.blocks * (a.heads / a.group), AB_THREADS, ab_shared<PANELS>(), stream, 0, a);
+  if (const int code = psgd_launch(psgd_attention_dq_kernel<T, PANELS>, a.blocks * a.heads, ab_threads(1), ab_shared(PANELS, 1), stream, 0, a)) return code;
+  const int kv_heads = a.heads / a.group;
+  a.split = 1;
+  for (int split = 2; split <= AB_MOST_SPLIT && split <= a.group && (long long)a.blocks * kv_heads * a.split < AB_ENOUGH; ++split)
+    if (a.group % split == 0) a.split = split;
+  if ((long long)a.blocks * kv_heads * a.split > 0x7fffffffll) a.split = 1;
+  return psgd_launch_clusters(psgd_attention_dkv_kernel<T, PANELS>, a.blocks * kv_heads * a.split, ab_threads(PANELS), ab_shared(PANELS, PANELS), stream, 0,
+                              a.split, a);
 }
 
 }  // namespace
 
 // dtype: 1 bfloat16, 2 float16. strides: rows and heads of q, k and v, in elements, multiples of 8; addresses on 16-byte boundaries. `out` is
-// [tokens, heads, size], contiguous, lse [heads, tokens]. Rows of `out` outside the sequences become zeros.
+// [tokens, heads, size], contiguous, `rest` (what rounding takes from it: the backward pass wants it) likewise or null, lse [heads, tokens]. Rows of `out` outside the sequences become zeros.
 PSGD_API int psgd_attention(const void* q, const void* k, const void* v, const long long* strides, const int* offsets, int sequences, int tokens, int heads,
-                            int kv_heads, int size, int dtype, int causal, float scale, void* out, float* lse, int* status, cudaStream_t stream) {
+                            int kv_heads, int size, int dtype, int causal, float scale, void* out, void* rest, float* lse, int* status, cudaStream_t stream) {
   AtArgs a;
-  if (at_fill(a, q, k, v, strides, offsets, sequences, tokens, heads, kv_heads, size, dtype, causal, scale, 2 * AT_TILE, heads, status)) return -1;
+  if (at_fill(a, q, k, v, strides, offsets, sequences, tokens, heads, kv_heads, size, dtype, causal, scale, at_tiles(size) * AT_TILE, heads, status)) return -1;
   a.out = out;
+  a.rest = rest;
   a.lse = lse;
   if (dtype == 1) return size <= 64 ? at_forward<__nv_bfloat16, 1>(a, stream) : at_forward<__nv_bfloat16, 2>(a, stream);
   return size <= 64 ? at_forward<__half, 1>(a, stream) : at_forward<__half, 2>(a, stream);
@@ -920,12 +1116,13 @@ PSGD_API int psgd_attention(const void* q, const void* k, const void* v, const l
 
 // strides: those of q, k, v and of the output's gradient. delta: scratch, [heads, tokens]. dq, dk, dv are contiguous.
 PSGD_API int psgd_attention_backward(const void* q, const void* k, const void* v, const void* grad, const long long* strides, const int* offsets, int sequences,
-                                     int tokens, int heads, int kv_heads, int size, int dtype, int causal, float scale, const void* out, const float* lse,
+                                     int tokens, int heads, int kv_heads, int size, int dtype, int causal, float scale, const void* out, const void* rest, const float* lse,
                                      float* delta, void* dq, void* dk, void* dv, int* status, cudaStream_t stream) {
   AtArgs a;
   if (at_fill(a, q, k, v, strides, offsets, sequences, tokens, heads, kv_heads, size, dtype, causal, scale, AT_TILE, heads, status)) return -1;
   if (at_encode(&a.g, grad, dtype, tokens, heads, size, strides[6], strides[7])) return -1;
   a.out = out;
+  a.rest = rest;
   a.grad = grad;
   a.grad_row = strides[6];
   a.grad_head = strides[7];

@@ -7,16 +7,16 @@
 
 #include "psgd_async.cuh"
 
-// A tile of 128 rows x 64 elements of 16 bits is 128 rows of 128 bytes, 16 KiB, as a TMA load with the 128-byte swizzle leaves it (eight rows, 1 KiB,
-// are one swizzle atom). Wider tiles are several of them, one behind another.
+// A panel is 64 or 128 rows of 64 elements of 16 bits, 128 bytes per row, as a TMA load with the 128-byte swizzle leaves it (eight rows, 1 KiB,
+// are one swizzle atom). Wider tiles are several panels, one behind another.
 constexpr int UMMA_ROWS = 128;
-constexpr int UMMA_PANEL = UMMA_ROWS * 128;
+constexpr int UMMA_PANEL = UMMA_ROWS * 128;   // bytes
 
 // Shared-memory descriptor of such a tile, 128-byte swizzle. Read along its rows (K-major): atoms follow each other along M or N
 // every 1024 bytes; a step of 16 along K is 32 bytes further. Read across (MN-major: the rows are K): atoms follow each other along K every
-// 1024 bytes, panels of 64 along N every UMMA_PANEL; a step of 16 along K is 2048 bytes further.
-__device__ __forceinline__ uint64_t umma_tile(uint32_t saddr) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(UMMA_PANEL >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// 1024 bytes, along N every `panel` bytes; a step of 16 along K is 2048 bytes further.
+__device__ __forceinline__ uint64_t umma_tile(uint32_t saddr, uint32_t panel) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(panel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
 }
 
 // Instruction descriptor: D float32, A and B of one type (0 float16, 1 bfloat16), M = 128.
@@ -24,31 +24,46 @@ __host__ __device__ constexpr uint32_t umma_shape(int type, bool b_across, int n
   return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((b_across ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(UMMA_ROWS >> 4) << 24);
 }
 
+// The products are issued by a whole warp in step, one elected lane of it doing so: descriptors stay in uniform registers, where the
+// instruction wants them. (Issued from a branch that one lane takes, a product took 80 cycles to issue and 32 to execute.)
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(shape), "r"((uint32_t)accumulate)
       : "memory");
 }
 __device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool accumulate) {   // A in tensor memory, K-major
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"((uint32_t)accumulate)
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(shape), "r"((uint32_t)accumulate)
       : "memory");
 }
-// Arrives on `bar` when the products issued by this thread so far are complete.
+// Arrives on `bar` when the products issued by this warp so far are complete.
 __device__ __forceinline__ void umma_arrive(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(psgd_smem_u32(bar)) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(psgd_smem_u32(bar))
+      : "memory");
 }
 __device__ __forceinline__ void umma_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void umma_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// D[128 x n] (+)= A B^T over k elements: tiles of rows along K, both in shared memory.
-__device__ __forceinline__ void umma_rows_by_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, int steps, bool accumulate) {
-  for (int s = 0; s < steps; ++s) {
-    const uint32_t off = (uint32_t)(s >> 2) * UMMA_PANEL + (uint32_t)(s & 3) * 32;
-    umma_ss(d, umma_tile(a + off), umma_tile(b + off), shape, accumulate || s > 0);
+// D[128 x n] = A B^T over 16 `steps` elements: 128 rows of A, n of B (a panel of B has B_ROWS), both in shared memory.
+template <int MOST_STEPS, int B_ROWS>
+__device__ __forceinline__ void umma_rows_by_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, int steps) {
+  const uint64_t ta = umma_tile(a, UMMA_PANEL), tb = umma_tile(b, B_ROWS * 128);
+#pragma unroll
+  for (int s = 0; s < MOST_STEPS; ++s) {
+    if (s >= steps) break;   // (addresses are below 256 KiB: nothing is carried out of their field)
+    umma_ss(d, ta + (((s >> 2) * UMMA_PANEL + (s & 3) * 32) >> 4), tb + (((s >> 2) * B_ROWS * 128 + (s & 3) * 32) >> 4), shape, s > 0);
   }
+}
+// D[128 x n] (+)= A B over rows [16 FROM, 16 TO) of B: A in tensor memory, eight columns for every 16 of K; B_ROWS rows of B are K.
+template <int FROM, int TO, int B_ROWS>
+__device__ __forceinline__ void umma_weights_by_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, bool accumulate) {
+  const uint64_t tb = umma_tile(b, B_ROWS * 128);
+#pragma unroll
+  for (int s = FROM; s < TO; ++s) umma_ts(d, a + s * 8, tb + (s * 2048 >> 4), shape, accumulate || s > 0);
 }
 
 // 32 columns of the 32 lanes of this warp. A wait must follow before the registers are used.
@@ -77,6 +92,7 @@ __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t columns) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(columns) : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 // Loads one box of a three-dimensional tensor.
 __device__ __forceinline__ void tma_load_box3(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst), "l"(map),
@@ -106,4 +122,24 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Two float32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+      : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }

@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import Optional, Tuple
+from typing import Optional
 
 import torch
 
@@ -38,7 +38,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _PackedAttention.apply(q, k, v, offsets, bool(causal), scale)
-    return _forward(q, k, v, offsets, bool(causal), scale)[0]
+    return _forward(q, k, v, offsets, bool(causal), scale, False)[0]
 
 
 def check(q, k, v, offsets, scale) -> None:
@@ -100,26 +100,28 @@ def _strides(*tensors) -> ctypes.Array:
     return (ctypes.c_longlong * len(out))(*out)
 
 
-def _forward(q, k, v, offsets, causal, scale) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+def _forward(q, k, v, offsets, causal, scale, gradient: bool):
+    """The output, and for a backward pass the logarithms of the sums and what rounding took from the output."""
     if not _native(q):
         return _forward_torch(q, k, v, offsets, causal, scale)
     tokens, heads, size = q.shape
     sequences = offsets.shape[0] - 1
     out = torch.empty((tokens, heads, size), dtype=q.dtype, device=q.device)
     if tokens == 0 or sequences == 0:
-        return out.zero_(), None
+        return out.zero_(), None, None
     lse = torch.empty((heads, tokens), dtype=torch.float32, device=q.device)
+    rest = torch.empty_like(out) if gradient else None
     q, k, v, offsets = _usable(q), _usable(k), _usable(v), offsets.contiguous()
     with native.on_device(q.device) as stream:
         code = native.lib().psgd_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), offsets.data_ptr(), sequences, tokens, heads, k.shape[1], size, DTYPES[q.dtype],
-            causal, scale, out.data_ptr(), lse.data_ptr(), _status(q.device), stream,
+            causal, scale, out.data_ptr(), rest.data_ptr() if gradient else None, lse.data_ptr(), _status(q.device), stream,
         )
     native.check(code, "psgd_attention")
-    return out, lse
+    return out, lse, rest
 
 
-def _backward(q, k, v, offsets, out, lse, grad, causal, scale):
+def _backward(q, k, v, offsets, out, lse, rest, grad, causal, scale):
     if not _native(q):
         return _backward_torch(q, k, v, offsets, out, grad, causal, scale)
     tokens, heads, size = q.shape
@@ -134,7 +136,7 @@ def _backward(q, k, v, offsets, out, lse, grad, causal, scale):
     with native.on_device(q.device) as stream:
         code = native.lib().psgd_attention_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), grad.data_ptr(), _strides(q, k, v, grad), offsets.data_ptr(), sequences, tokens, heads, groups, size,
-            DTYPES[q.dtype], causal, scale, out.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+            DTYPES[q.dtype], causal, scale, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
             _status(q.device), stream,
         )
     native.check(code, "psgd_attention_backward")
@@ -144,16 +146,16 @@ def _backward(q, k, v, offsets, out, lse, grad, causal, scale):
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, causal, scale):
-        out, lse = _forward(q, k, v, offsets, causal, scale)
-        ctx.save_for_backward(q, k, v, offsets, out, lse)
+        out, lse, rest = _forward(q, k, v, offsets, causal, scale, True)
+        ctx.save_for_backward(q, k, v, offsets, out, lse, rest)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        q, k, v, offsets, out, lse = ctx.saved_tensors
-        return (*_backward(q, k, v, offsets, out, lse, grad, ctx.causal, ctx.scale), None, None, None)
+        q, k, v, offsets, out, lse, rest = ctx.saved_tensors
+        return (*_backward(q, k, v, offsets, out, lse, rest, grad, ctx.causal, ctx.scale), None, None, None)
 
 
 # ---- the same in torch operations --------------------------------------------------------------
@@ -183,7 +185,7 @@ def _forward_torch(q, k, v, offsets, causal, scale):
     for lo, hi in _sequences(offsets, q.shape[0]):
         p = _weights(_wide(q[lo:hi]), _wide(k[lo:hi], group), causal, scale)
         out[lo:hi] = (p @ _wide(v[lo:hi], group)).transpose(0, 1).to(q.dtype)
-    return out, None
+    return out, None, None
 
 
 def _backward_torch(q, k, v, offsets, out, grad, causal, scale):
