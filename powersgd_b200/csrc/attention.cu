@@ -73,7 +73,7 @@ __device__ __forceinline__ float at_max3(float x, float y, float z) {
 
 // 2^x in plain arithmetic: x = n + f with |f| <= 1/2 by rounding, a polynomial of degree 4 in f with the least maximal relative error
 // (2.8e-6; fitted with value 1 at 0), n added to the exponent. Below -127 the result is zero.
-constexpr int AT_POLY = 4;   // of 16 exponentials, those that are taken so: the special function unit has 16 results per cycle and SM
+constexpr int AT_POLY = 2;   // of 16 exponentials, those that are taken so: the special function unit has 16 results per cycle and SM
 __device__ __forceinline__ float2 at_exp2_poly(float2 x) {
   const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
   x.x = fmaxf(x.x, -127.f);
@@ -98,22 +98,25 @@ struct AtPiece {
 __device__ __forceinline__ int at_bound(const int* offsets, int s, int tokens) { return min(max(offsets[s], 0), tokens); }
 __device__ bool at_find(const AtArgs& a, int rows, int index, bool from_end, AtPiece& out) {
   const int lane = threadIdx.x & 31;
-  auto pieces = [&](int s) {
+  auto pieces = [&](int s, int& begin, int& length) {
+    begin = length = 0;
     if (s >= a.sequences) return 0;
-    const int lo = at_bound(a.offsets, s, a.tokens), hi = at_bound(a.offsets, s + 1, a.tokens);
-    return hi > lo ? (hi - lo + rows - 1) / rows : 0;
+    begin = at_bound(a.offsets, s, a.tokens);
+    length = max(at_bound(a.offsets, s + 1, a.tokens) - begin, 0);
+    return (length + rows - 1) / rows;
   };
-  const int mine = pieces(lane);
+  int begin, length, b, l;       // of the sequence that this lane has (of the first 32)
+  const int mine = pieces(lane, begin, length);
   out.before = at_bound(a.offsets, 0, a.tokens);
   out.behind = max(at_bound(a.offsets, a.sequences, a.tokens), out.before);
   // pieces at level `level` of their sequences or above
   auto above = [&](int level) {
     int n = max(mine - level, 0);
-    for (int s = lane + 32; s < a.sequences; s += 32) n += max(pieces(s) - level, 0);
+    for (int s = lane + 32; s < a.sequences; s += 32) n += max(pieces(s, b, l) - level, 0);
     return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
   };
   int most = mine;
-  for (int s = lane + 32; s < a.sequences; s += 32) most = max(most, pieces(s));
+  for (int s = lane + 32; s < a.sequences; s += 32) most = max(most, pieces(s, b, l));
   most = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
   if (index >= above(0)) return false;
   int lo = 0, hi = most;         // above(lo) > index >= above(hi)
@@ -124,17 +127,18 @@ __device__ bool at_find(const AtArgs& a, int rows, int index, bool from_end, AtP
   }
   int left = index - above(lo + 1);   // the left-th sequence with more than `lo` pieces
   for (int s0 = 0; s0 < a.sequences; s0 += 32) {
-    const bool has = (s0 ? pieces(s0 + lane) : mine) > lo;
+    const int count = s0 ? pieces(s0 + lane, begin, length) : mine;
+    const bool has = count > lo;
     const unsigned votes = __ballot_sync(0xffffffffu, has);
     const int n = __popc(votes);
     if (left >= n) {
       left -= n;
       continue;
     }
-    const int s = s0 + __fns(votes, 0, left + 1);
-    out.start = at_bound(a.offsets, s, a.tokens);
-    out.length = at_bound(a.offsets, s + 1, a.tokens) - out.start;
-    out.piece = from_end ? (out.length + rows - 1) / rows - 1 - lo : lo;
+    const int from = __fns(votes, 0, left + 1);
+    out.start = __shfl_sync(0xffffffffu, begin, from);
+    out.length = __shfl_sync(0xffffffffu, length, from);
+    out.piece = from_end ? __shfl_sync(0xffffffffu, count, from) - 1 - lo : lo;
     return true;
   }
   return false;
@@ -210,7 +214,7 @@ __device__ __forceinline__ void at_write_rows(uint32_t tmem, float factor, uint8
     float f[64];
     tmem_load32(tmem + panel * 64, f);
     tmem_load32(tmem + panel * 64 + 32, f + 32);
-    tmem_load_wait();
+    tmem_load_wait<64>(f);
 #pragma unroll
     for (int c = 0; c < 64; ++c) f[c] *= factor;
 #pragma unroll 1
@@ -274,7 +278,7 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
   __shared__ int s_abort, s_found;
   __shared__ AtPiece s_piece;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int head = blockIdx.x % a.heads, index = blockIdx.x / a.heads;
   if (warp == 0) {
     AtPiece piece = {0, 0, 0, 0, 0};
@@ -310,9 +314,9 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
     if (warp == ISSUER) tmem_free(s_tmem, COLUMNS);
     return;
   }
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = warp_uniform(s_tmem);
   const AtWait wait = {&s_abort, a.status};
-  const int start = s_piece.start, length = s_piece.length, row0 = s_piece.piece * TILES * AT_TILE;
+  const int start = s_piece.start, length = warp_uniform(s_piece.length), row0 = warp_uniform(s_piece.piece) * TILES * AT_TILE;
   // tiles of keys that each tile of queries meets
   int n[TILES];
 #pragma unroll
@@ -339,7 +343,7 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
     const int k_steps = (a.size + 15) / 16;
     constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_TILE);
     const uint32_t o_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
-    const uint32_t q_at = psgd_smem_u32(s_q), ring_at = psgd_smem_u32(s_ring);
+    const uint32_t q_at = warp_uniform(psgd_smem_u32(s_q)), ring_at = q_at + TILES * TILE_BYTES;
     bool ok = wait_all(&bar_q, 0) && wait_all(&bar_full[0], 0);
     int have = 0;   // tiles of keys that are there
     auto scores = [&](int t, int j) {
@@ -396,7 +400,7 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
       float s[AT_TILE];
 #pragma unroll
       for (int c = 0; c < AT_TILE; c += 32) tmem_load32(s_at + c, s + c);
-      tmem_load_wait();
+      tmem_load_wait<AT_TILE>(s);
       if (EARLY) at_arrive(&bar_r[t]);
       if (j == n[t] - 1) {
         const int last = limit - j * AT_TILE;
@@ -441,7 +445,7 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
             if (c >= a.size) break;
             float o[32];
             tmem_load32(o_at + c, o);
-            tmem_load_wait();
+            tmem_load_wait<32>(o);
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] *= f;
             tmem_store16(o_at + c, reinterpret_cast<uint32_t*>(o));
@@ -505,8 +509,8 @@ constexpr int AB_ENOUGH = 4 * 148;    // with so many blocks the heads of a grou
 // two where one does.
 __host__ __device__ constexpr int ab_threads(int chains) { return 128 * chains + 64; }
 // Tiles that pass come in pairs (K and V, or Q and dO).
-__host__ __device__ constexpr int ab_stages(int panels, int chains) { return panels == 1 ? 3 : chains == 1 ? 1 : 4; }
-__host__ __device__ constexpr size_t ab_shared(int panels, int chains) { return 1024 + (size_t)panels * (2 * UMMA_PANEL + ab_stages(panels, chains) * UMMA_PANEL); }
+__host__ __device__ constexpr int ab_stages(int panels) { return panels == 1 ? 3 : 4; }
+__host__ __device__ constexpr size_t ab_shared(int panels) { return 1024 + (size_t)panels * (2 + ab_stages(panels)) * UMMA_PANEL; }
 
 template <int CHAINS, int STAGES>
 struct AbBars {
@@ -534,30 +538,30 @@ __device__ __forceinline__ void ab_exponentials(float* s, float scale2, float at
 #pragma unroll
   for (int c = 0; c < AT_STEP; c += 2) {
     const float2 x = fma2(make_float2(s[c], s[c + 1]), factor, minus);
-    const float2 e = c % 16 < AT_POLY ? at_exp2_poly(x) : make_float2(at_exp2(x.x), at_exp2(x.y));
-    s[c] = e.x;
-    s[c + 1] = e.y;
+    s[c] = at_exp2(x.x);
+    s[c + 1] = at_exp2(x.y);
   }
 }
 
 // dQ: tensor memory holds, per chain, S and dP (64 columns each; dS takes the first half of dP's place), and dQ. S of a chain's next step is
 // multiplied as soon as this one is in registers, its dP behind dQ of this one.
 template <typename T, int PANELS>
-__global__ void __launch_bounds__(ab_threads(1), 2) psgd_attention_dq_kernel(const __grid_constant__ AtArgs a) {
-  constexpr int TILE_BYTES = PANELS * UMMA_PANEL, HALF = TILE_BYTES / 2, STAGES = ab_stages(PANELS, 1);
-  constexpr int DP = AT_STEP, DQ = 2 * AT_STEP, COLUMNS = 256;   // tensor memory
-  constexpr int LOADER = 4, ISSUER = 5;
+__global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention_dq_kernel(const __grid_constant__ AtArgs a) {
+  constexpr int TILE_BYTES = PANELS * UMMA_PANEL, HALF = TILE_BYTES / 2, CHAINS = PANELS, STAGES = ab_stages(PANELS);
+  constexpr int DQ = 2 * AT_STEP * CHAINS, COLUMNS = 256 * CHAINS;   // tensor memory; chain c has its scores at 128 c, slopes behind
+  constexpr int LOADER = 4 * CHAINS, ISSUER = LOADER + 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = base;
   uint8_t* s_g = base + TILE_BYTES;
   uint8_t* s_ring = base + 2 * TILE_BYTES;   // stage: K, V
-  __shared__ __align__(8) AbBars<1, STAGES> bars;
+  __shared__ __align__(8) AbBars<CHAINS, STAGES> bars;
+  __shared__ float s_delta[AT_TILE];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_found;
   __shared__ AtPiece s_piece;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int head = blockIdx.x % a.heads, index = blockIdx.x / a.heads;
   if (warp == 0) {
     AtPiece piece = {0, 0, 0, 0, 0};
@@ -581,9 +585,9 @@ __global__ void __launch_bounds__(ab_threads(1), 2) psgd_attention_dq_kernel(con
     if (warp == ISSUER) tmem_free(s_tmem, COLUMNS);
     return;
   }
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = warp_uniform(s_tmem);
   const AtWait wait = {&s_abort, a.status};
-  const int start = s_piece.start, length = s_piece.length, q0 = s_piece.piece * AT_TILE;
+  const int start = s_piece.start, length = warp_uniform(s_piece.length), q0 = warp_uniform(s_piece.piece) * AT_TILE;
   const int steps = (a.causal ? min(q0 + AT_TILE, length) + AT_STEP - 1 : length + AT_STEP - 1) / AT_STEP;
 
   if (warp == LOADER) {
@@ -605,60 +609,59 @@ __global__ void __launch_bounds__(ab_threads(1), 2) psgd_attention_dq_kernel(con
     const int k_steps = (a.size + 15) / 16;
     constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_STEP);
     const uint32_t q_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
-    const uint32_t q_at = psgd_smem_u32(s_q), g_at = psgd_smem_u32(s_g), ring_at = psgd_smem_u32(s_ring);
+    const uint32_t q_at = warp_uniform(psgd_smem_u32(s_q)), g_at = q_at + TILE_BYTES, ring_at = q_at + 2 * TILE_BYTES;
     bool ok = wait_all(&bars.fixed, 0);
     int have = -1;
     auto there = [&](int j) {
       if (j > have) ok = ok && wait_all(&bars.full[j % STAGES], (j / STAGES) & 1);
-      have = j;
+      have = max(have, j);
       if (ok) umma_fence_after();
       return ok;
     };
     auto scores = [&](int j) {
       if (!there(j)) return;
-      umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem, q_at, ring_at + j % STAGES * TILE_BYTES, S_SHAPE, k_steps);
-      umma_arrive(&bars.s[0]);
+      umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem + j % CHAINS * 128, q_at, ring_at + j % STAGES * TILE_BYTES, S_SHAPE, k_steps);
+      umma_arrive(&bars.s[j % CHAINS]);
     };
     auto slopes = [&](int j) {
       if (!there(j)) return;
-      umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem + DP, g_at, ring_at + j % STAGES * TILE_BYTES + HALF, S_SHAPE, k_steps);
-      umma_arrive(&bars.dp[0]);
+      umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem + j % CHAINS * 128 + AT_STEP, g_at, ring_at + j % STAGES * TILE_BYTES + HALF, S_SHAPE, k_steps);
+      umma_arrive(&bars.dp[j % CHAINS]);
     };
-    scores(0);
-    if (ok) slopes(0);
+    for (int j = 0; j < CHAINS && j < steps && ok; ++j) {
+      scores(j);
+      if (ok) slopes(j);
+    }
     for (int j = 0; j < steps && ok; ++j) {
-      ok = wait_all(&bars.p[0], j & 1);    // S is in registers
+      const int chain = j % CHAINS;
+      const uint32_t parity = (j / CHAINS) & 1;
+      ok = wait_all(&bars.p[chain], parity);    // S is in registers
       if (!ok) break;
       umma_fence_after();
-      // (with one stage the next keys come when dQ has been multiplied)
-      if (STAGES > 1 && j + 1 < steps) scores(j + 1);
-      ok = ok && wait_all(&bars.ds[0], j & 1);
+      if (j + CHAINS < steps) scores(j + CHAINS);
+      ok = ok && wait_all(&bars.ds[chain], parity);
       if (!ok) break;
       umma_fence_after();
-      umma_weights_by_rows<0, 4, AT_STEP>(tmem + DQ, tmem + DP, ring_at + j % STAGES * TILE_BYTES, q_shape, j > 0);
+      umma_weights_by_rows<0, 4, AT_STEP>(tmem + DQ, tmem + chain * 128 + AT_STEP, ring_at + j % STAGES * TILE_BYTES, q_shape, j > 0);
       umma_arrive(&bars.empty[j % STAGES]);
-      if (j + 1 < steps) {
-        if (STAGES == 1) scores(j + 1);
-        if (ok) slopes(j + 1);
-      } else {
-        umma_arrive(&bars.done);
-      }
+      if (j + CHAINS < steps) slopes(j + CHAINS);
+      if (j == steps - 1) umma_arrive(&bars.done);
     }
   } else {
-    const int row = tid, q = q0 + row;
+    const int chain = warp >> 2, row = tid & 127, q = q0 + row;
     const bool held = q < length;
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + chain * 128, dp_at = s_at + AT_STEP;
     const long long stat = (long long)head * a.tokens + start + q;
     // delta of the row, for the keys' pass too. It is a small difference of large sums, and what it is off by moves a whole row of
     // dS one way: it takes the output unrounded, in two parts. (With the rounded one dQ and dK were off by 1.7 times their own
     // rounding, so by 1.4.)
-    float delta = 0.f, lse = 0.f;
-    if (held) {
+    float delta = 0.f;
+    const float lse = held ? a.lse[stat] : 0.f;
+    if (held && chain == 0) {
       const long long at = ((long long)(start + q) * a.heads + head) * a.size;
       const T* o = (const T*)a.out + at;
       const T* o_rest = (const T*)a.rest + at;
       const T* g = (const T*)a.grad + (long long)(start + q) * a.grad_row + (long long)head * a.grad_head;
-      lse = a.lse[stat];
 #pragma unroll 4
       for (int c = 0; c < a.size; c += 8) {
         const uint4 x = *reinterpret_cast<const uint4*>(o + c), y = *reinterpret_cast<const uint4*>(g + c), z = *reinterpret_cast<const uint4*>(o_rest + c);
@@ -672,22 +675,31 @@ __global__ void __launch_bounds__(ab_threads(1), 2) psgd_attention_dq_kernel(con
       }
       a.delta[stat] = delta;
     }
+    if (CHAINS == 2) {
+      if (chain == 0) s_delta[row] = delta;
+      asm volatile("bar.sync 1, 256;" ::: "memory");
+      delta = s_delta[row];
+    }
     const int limit = a.causal ? min(q, length - 1) : length - 1;    // last key that counts
     bool ok = true;
-    for (int j = 0; j < steps; ++j) {
-      ok = wait(&bars.s[0], j & 1);
+    for (int j = chain; j < steps; j += CHAINS) {
+      const uint32_t parity = (j / CHAINS) & 1;
+      ok = wait(&bars.s[chain], parity);
       if (!ok) break;
       umma_fence_after();
       float p[AT_STEP];
-      tmem_load32(tmem + lanes, p);
-      tmem_load32(tmem + lanes + 32, p + 32);
-      tmem_load_wait();
-      at_arrive(&bars.p[0]);
+      tmem_load32(s_at, p);
+      tmem_load32(s_at + 32, p + 32);
+      tmem_load_wait<AT_STEP>(p);
+      at_arrive(&bars.p[chain]);
       ab_exponentials(p, a.scale2, lse);
       const int last = limit - j * AT_STEP;
       const bool edge = (j + 1) * AT_STEP > (a.causal ? min(q0 + 1, length) : length);     // some key of this step does not count for some row
+      const int keys = length - j * AT_STEP;
       if (edge) {
-        const int keys = length - j * AT_STEP;
+#pragma unroll
+        for (int c = 0; c < AT_STEP; ++c)
+          if (c > last) p[c] = 0.f;
         if (keys < AT_STEP) {
           ok = wait(&bars.full[j % STAGES], (j / STAGES) & 1);
           if (!ok) break;
@@ -695,35 +707,36 @@ __global__ void __launch_bounds__(ab_threads(1), 2) psgd_attention_dq_kernel(con
           psgd_fence_async_shared();
         }
       }
-      ok = wait(&bars.dp[0], j & 1);
+      ok = wait(&bars.dp[chain], parity);
       if (!ok) break;
       umma_fence_after();
       const float2 minus = make_float2(-delta, -delta);
+      float d[AT_STEP];
+      tmem_load32(dp_at, d);
+      tmem_load32(dp_at + 32, d + 32);
+      tmem_load_wait<AT_STEP>(d);
 #pragma unroll
       for (int c = 0; c < AT_STEP; c += 32) {
-        float d[32];
-        tmem_load32(tmem + lanes + DP + c, d);
-        tmem_load_wait();
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float2 x = mul2(make_float2(p[c + i], p[c + i + 1]), add2(make_float2(d[i], d[i + 1]), minus));
-          if (edge) {   // (a key that does not count may hold anything)
+          float2 x = mul2(make_float2(p[c + i], p[c + i + 1]), add2(make_float2(d[c + i], d[c + i + 1]), minus));
+          if (keys < AT_STEP) {   // (behind the sequence dP may be anything: no factor of zero does)
             if (c + i > last) x.x = 0.f;
             if (c + i + 1 > last) x.y = 0.f;
           }
           w[i / 2] = pack2<T>(x.x, x.y);
         }
-        tmem_store16(tmem + lanes + DP + c / 2, w);
+        tmem_store16(dp_at + c / 2, w);
       }
       tmem_store_wait();
-      at_arrive(&bars.ds[0]);
+      at_arrive(&bars.ds[chain]);
     }
     if (ok) ok = wait(&bars.done, 0);
     if (ok) {
       umma_fence_after();
       const int first = q0 + warp * 32;
-      at_write_rows<T, PANELS>(tmem + lanes + DQ, a.scale, s_q + warp * 4096, (T*)a.dq + ((long long)(start + first) * a.heads + head) * a.size, (T*)nullptr,
+      if (chain == 0) at_write_rows<T, PANELS>(tmem + lanes + DQ, a.scale, s_q + warp * 4096, (T*)a.dq + ((long long)(start + first) * a.heads + head) * a.size, (T*)nullptr,
                                (long long)a.heads * a.size, length - first, a.size);
     }
   }
@@ -746,7 +759,7 @@ __global__ void __launch_bounds__(ab_threads(1), 2) psgd_attention_dq_kernel(con
 template <typename T, int PANELS>
 __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention_dkv_kernel(const __grid_constant__ AtArgs a) {
   constexpr int CHAINS = PANELS;
-  constexpr int TILE_BYTES = PANELS * UMMA_PANEL, HALF = TILE_BYTES / 2, STAGES = ab_stages(PANELS, CHAINS);
+  constexpr int TILE_BYTES = PANELS * UMMA_PANEL, HALF = TILE_BYTES / 2, STAGES = ab_stages(PANELS);
   constexpr int DV = 2 * AT_STEP * CHAINS, DK = DV + 64 * PANELS, COLUMNS = 256 * CHAINS;   // tensor memory; chain c has its scores at 128 c, slopes behind
   constexpr int LOADER = 4 * CHAINS, ISSUER = LOADER + 1;
   extern __shared__ uint8_t smem_raw[];
@@ -760,7 +773,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
   __shared__ int s_abort, s_found;
   __shared__ AtPiece s_piece;
 
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int kv_heads = a.heads / a.group, rank = blockIdx.x % a.split, block = blockIdx.x / a.split;
   const int head = block % kv_heads, index = block / kv_heads;
   if (warp == 0) {
@@ -788,27 +801,37 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
     if (warp == ISSUER) tmem_free(s_tmem, COLUMNS);
     return;
   }
-  const uint32_t tmem = s_tmem;
+  const uint32_t tmem = warp_uniform(s_tmem);
   const AtWait wait = {&s_abort, a.status};
-  const int start = s_piece.start, length = s_piece.length, k0 = s_piece.piece * AT_TILE;
+  const int start = s_piece.start, length = warp_uniform(s_piece.length), k0 = warp_uniform(s_piece.piece) * AT_TILE;
   const int first = a.causal ? k0 / AT_STEP : 0;                      // first step of queries
   const int per_head = (length + AT_STEP - 1) / AT_STEP - first, heads = a.group / a.split, steps = per_head * heads;
   const int head0 = head * a.group + rank * heads;
-  auto q_head = [&](int i) { return head0 + i / per_head; };
-  auto q_row = [&](int i) { return (first + i % per_head) * AT_STEP; };
+  // Head and first query of a step, counted on without a division.
+  struct Step {
+    int head, row;
+  };
+  auto next = [&](Step& at, int by) {
+    at.row += by * AT_STEP;
+    while (at.row >= (first + per_head) * AT_STEP) {
+      at.row -= per_head * AT_STEP;
+      ++at.head;
+    }
+  };
 
   if (warp == LOADER) {
     if (lane == 0) {
       psgd_mbar_expect_tx(&bars.fixed, 2 * TILE_BYTES);
       at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_k), &a.k, head, start + k0, &bars.fixed);
       at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_v), &a.v, head, start + k0, &bars.fixed);
-      for (int i = 0; i < steps; ++i) {
+      Step step = {head0, first * AT_STEP};
+      for (int i = 0; i < steps; ++i, next(step, 1)) {
         const int slot = i % STAGES;
         if (!wait(&bars.empty[slot], ((i / STAGES) & 1) ^ 1)) break;
         psgd_mbar_expect_tx(&bars.full[slot], 2 * HALF);
         const uint32_t at = psgd_smem_u32(s_ring + slot * TILE_BYTES);
-        at_load_tile<PANELS, AT_STEP>(at, &a.q, q_head(i), start + q_row(i), &bars.full[slot]);
-        at_load_tile<PANELS, AT_STEP>(at + HALF, &a.g, q_head(i), start + q_row(i), &bars.full[slot]);
+        at_load_tile<PANELS, AT_STEP>(at, &a.q, step.head, start + step.row, &bars.full[slot]);
+        at_load_tile<PANELS, AT_STEP>(at + HALF, &a.g, step.head, start + step.row, &bars.full[slot]);
       }
     }
   } else if (warp == ISSUER) {
@@ -816,7 +839,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
     const int k_steps = (a.size + 15) / 16;
     constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_STEP);
     const uint32_t o_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
-    const uint32_t k_at = psgd_smem_u32(s_k), v_at = psgd_smem_u32(s_v), ring_at = psgd_smem_u32(s_ring);
+    const uint32_t k_at = warp_uniform(psgd_smem_u32(s_k)), v_at = k_at + TILE_BYTES, ring_at = k_at + 2 * TILE_BYTES;
     bool ok = wait_all(&bars.fixed, 0);
     int have = -1;
     auto there = [&](int i) {
@@ -858,19 +881,23 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
   } else {
     const int chain = warp >> 2, row = tid & 127, key = k0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + chain * 128, dp_at = s_at + AT_STEP;
-    auto statistic = [&](int i) {   // of query row % 64 of step i: logarithm of the sum, or delta
-      const int q = q_row(i) + row % AT_STEP;
-      if (q >= length) return 0.f;
-      return (row < AT_STEP ? a.lse : a.delta)[(long long)q_head(i) * a.tokens + start + q];
+    const float* statistics = (row < AT_STEP ? a.lse : a.delta) + start + row % AT_STEP;
+    auto statistic = [&](const Step& at) {   // of query row % 64 of a step, negative: logarithm of the sum, or delta
+      return at.row + row % AT_STEP < length ? -statistics[(long long)at.head * a.tokens + at.row] : 0.f;
     };
     float (*stats)[2 * AT_STEP] = s_stats[chain];
-    if (chain < steps) stats[0][row] = statistic(chain);
+    Step step = {head0, first * AT_STEP}, later;
+    next(step, chain);
+    if (chain < steps) stats[0][row] = statistic(step);
+    later = step;
     asm volatile("bar.sync %0, 128;" ::"r"(1 + chain) : "memory");
     bool ok = true;
     int mine = 0;                   // steps of this chain so far
     for (int i = chain; i < steps; i += CHAINS, ++mine) {
-      const float ahead = i + CHAINS < steps ? statistic(i + CHAINS) : 0.f;
-      const int q0 = q_row(i), queries = length - q0;
+      const int q0 = step.row, queries = length - q0;
+      next(later, CHAINS);
+      const float ahead = i + CHAINS < steps ? statistic(later) : 0.f;
+      step = later;
       // queries [from, to) of the step meet this thread's key
       const int from = a.causal ? key - q0 : 0, to = queries;
       const bool edge = (a.causal && q0 < k0 + AT_TILE) || queries < AT_STEP;
@@ -883,24 +910,26 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       float p[AT_STEP];
       tmem_load32(s_at, p);
       tmem_load32(s_at + 32, p + 32);
-      tmem_load_wait();
+      tmem_load_wait<AT_STEP>(p);
       const float2 factor = make_float2(a.scale2, a.scale2);
 #pragma unroll
       for (int c = 0; c < AT_STEP; c += 4) {
         const float4 x = *reinterpret_cast<const float4*>(now + c);
 #pragma unroll
         for (int h = 0; h < 4; h += 2) {
-          const float2 y = fma2(make_float2(p[c + h], p[c + h + 1]), factor, h ? make_float2(-x.z, -x.w) : make_float2(-x.x, -x.y));
-          const float2 e = (c + h) % 16 < AT_POLY ? at_exp2_poly(y) : make_float2(at_exp2(y.x), at_exp2(y.y));
-          p[c + h] = e.x;
-          p[c + h + 1] = e.y;
+          const float2 y = fma2(make_float2(p[c + h], p[c + h + 1]), factor, h ? make_float2(x.z, x.w) : make_float2(x.x, x.y));
+          p[c + h] = at_exp2(y.x);
+          p[c + h + 1] = at_exp2(y.y);
         }
       }
       if (edge) {
 #pragma unroll
         for (int c = 0; c < AT_STEP; ++c)
-          if (c < from || c >= to) p[c] = 0.f;
+          if (c < from) p[c] = 0.f;
         if (queries < AT_STEP) {
+#pragma unroll
+          for (int c = 0; c < AT_STEP; ++c)
+            if (c >= to) p[c] = 0.f;
           ok = wait(&bars.full[i % STAGES], (i / STAGES) & 1);
           if (!ok) break;
           const int r = row % AT_STEP;
@@ -921,11 +950,12 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       ok = wait(&bars.dp[chain], mine & 1);
       if (!ok) break;
       umma_fence_after();
+      float d[AT_STEP];
+      tmem_load32(dp_at, d);
+      tmem_load32(dp_at + 32, d + 32);
+      tmem_load_wait<AT_STEP>(d);
 #pragma unroll
       for (int c = 0; c < AT_STEP; c += 32) {
-        float d[32];
-        tmem_load32(dp_at + c, d);
-        tmem_load_wait();
         uint32_t w[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 4) {
@@ -933,8 +963,8 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
 #pragma unroll
           for (int h = 0; h < 4; h += 2) {
             const int at = c + e + h;
-            float2 f = mul2(make_float2(p[at], p[at + 1]), add2(make_float2(d[e + h], d[e + h + 1]), h ? make_float2(-x.z, -x.w) : make_float2(-x.x, -x.y)));
-            if (edge) {
+            float2 f = mul2(make_float2(p[at], p[at + 1]), add2(make_float2(d[at], d[at + 1]), h ? make_float2(x.z, x.w) : make_float2(x.x, x.y)));
+            if (queries < AT_STEP) {   // (behind the sequence dP may be anything: no factor of zero does)
               if (at < from || at >= to) f.x = 0.f;
               if (at + 1 < from || at + 1 >= to) f.y = 0.f;
             }
@@ -966,7 +996,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
           for (int c = 0; c < PANELS * 64; c += 32) {
             float f[32];
             tmem_load32(at + c, f);
-            tmem_load_wait();
+            tmem_load_wait<32>(f);
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
               *reinterpret_cast<float4*>(share + ((c + e) ^ ((row & 7) << 2))) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
@@ -1086,16 +1116,16 @@ int at_forward(const AtArgs& a, cudaStream_t stream) {
 template <typename T, int PANELS>
 int at_backward(AtArgs a, cudaStream_t stream) {
   static unsigned long long q_devices = 0, kv_devices = 0;
-  if (const int code = psgd_allow_shared((const void*)psgd_attention_dq_kernel<T, PANELS>, ab_shared(PANELS, 1), q_devices)) return code;
-  if (const int code = psgd_allow_shared((const void*)psgd_attention_dkv_kernel<T, PANELS>, ab_shared(PANELS, PANELS), kv_devices)) return code;
+  if (const int code = psgd_allow_shared((const void*)psgd_attention_dq_kernel<T, PANELS>, ab_shared(PANELS), q_devices)) return code;
+  if (const int code = psgd_allow_shared((const void*)psgd_attention_dkv_kernel<T, PANELS>, ab_shared(PANELS), kv_devices)) return code;
   // (delta comes from the first)
-  if (const int code = psgd_launch(psgd_attention_dq_kernel<T, PANELS>, a.blocks * a.heads, ab_threads(1), ab_shared(PANELS, 1), stream, 0, a)) return code;
+  if (const int code = psgd_launch(psgd_attention_dq_kernel<T, PANELS>, a.blocks * a.heads, ab_threads(PANELS), ab_shared(PANELS), stream, 0, a)) return code;
   const int kv_heads = a.heads / a.group;
   a.split = 1;
   for (int split = 2; split <= AB_MOST_SPLIT && split <= a.group && (long long)a.blocks * kv_heads * a.split < AB_ENOUGH; ++split)
     if (a.group % split == 0) a.split = split;
   if ((long long)a.blocks * kv_heads * a.split > 0x7fffffffll) a.split = 1;
-  return psgd_launch_clusters(psgd_attention_dkv_kernel<T, PANELS>, a.blocks * kv_heads * a.split, ab_threads(PANELS), ab_shared(PANELS, PANELS), stream, 0,
+  return psgd_launch_clusters(psgd_attention_dkv_kernel<T, PANELS>, a.blocks * kv_heads * a.split, ab_threads(PANELS), ab_shared(PANELS), stream, 0,
                               a.split, a);
 }
 

@@ -75,25 +75,29 @@ def scan_target() -> str:
     return f"torch {torch.__version__} {torch.version.git_version}, python {platform.python_version()}"
 
 
-def _build_scan() -> None:
-    """The list checks (host/tensor_scan.cpp), a CPython extension for the PyTorch of this interpreter."""
-    src = os.path.join(HERE, "host", "tensor_scan.cpp")
+def _build_host(name: str, lib: str, cuda: bool = False) -> None:
+    """host/<name>.cpp, a CPython extension for the PyTorch of this interpreter."""
+    src = os.path.join(HERE, "host", name + ".cpp")
     import sysconfig
 
     import torch
 
-    stamp_path = os.path.join(OBJ_DIR, "scan_stamp.txt")
+    stamp_path = os.path.join(OBJ_DIR, name + "_stamp.txt")
     stamp = f"{_digest([src])} {scan_target()}"
-    if os.path.exists(SCAN_LIB) and os.path.exists(stamp_path):
+    if os.path.exists(lib) and os.path.exists(stamp_path):
         with open(stamp_path) as fp:
             if fp.read() == stamp:
                 return
     base = os.path.dirname(os.path.abspath(torch.__file__))
     includes = [os.path.join(base, "include"), os.path.join(base, "include", "torch", "csrc", "api", "include"), sysconfig.get_paths()["include"]]
+    links = ["-lc10", "-ltorch_cpu", "-ltorch_python"]
+    if cuda:
+        includes.append(os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_nvcc()))), "include"))
+        links.append("-lc10_cuda")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DPSGD_SCAN_TARGET="{scan_target()}"',
-           *[f"-isystem{i}" for i in includes], src, "-o", SCAN_LIB,
-           f"-L{os.path.join(base, 'lib')}", "-lc10", "-ltorch_cpu", "-ltorch_python"]
+           *[f"-isystem{i}" for i in includes], src, "-o", lib,
+           f"-L{os.path.join(base, 'lib')}", *links]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"{cmd[0]} failed on {src}:\n{res.stdout}\n{res.stderr}")
@@ -101,15 +105,22 @@ def _build_scan() -> None:
         fp.write(stamp)
 
 
+def operators_lib() -> str:
+    """Where the calls of the language-model operators are built to (host/operators.cpp), beside the list checks."""
+    return os.path.join(os.path.dirname(SCAN_LIB), "_operators.so")
+
+
 def build(force: bool = False, verbose: bool = False, debug: bool = False) -> str:
     """`debug=True` builds the bounds-checked variant (libpsgd_b200_debug.so) instead."""
     os.makedirs(OBJ_DIR, exist_ok=True)
-    try:
-        _build_scan()
-    except Exception as exc:   # no PyTorch, headers of Python or host compiler: the package asks in Python instead, more slowly
-        if os.path.exists(SCAN_LIB):
-            os.remove(SCAN_LIB)
-        warnings.warn(f"list checks not built ({exc})", stacklevel=2)
+    # no PyTorch, headers of Python or host compiler: the package asks in Python instead, more slowly
+    for what, name, path, cuda in (("list checks", "tensor_scan", SCAN_LIB, False), ("operator calls", "operators", operators_lib(), True)):
+        try:
+            _build_host(name, path, cuda)
+        except Exception as exc:
+            if os.path.exists(path):
+                os.remove(path)
+            warnings.warn(f"{what} not built ({exc})", stacklevel=2)
     srcs = sources()
     headers = [os.path.join(HERE, f) for f in os.listdir(HERE) if f.endswith((".h", ".cuh"))]
     obj_dir, lib = (DEBUG_OBJ_DIR, DEBUG_LIB) if debug else (OBJ_DIR, LIB)

@@ -24,6 +24,11 @@ __host__ __device__ constexpr uint32_t umma_shape(int type, bool b_across, int n
   return (1u << 4) | ((uint32_t)type << 7) | ((uint32_t)type << 10) | ((b_across ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(UMMA_ROWS >> 4) << 24);
 }
 
+// A value that all lanes of the warp have, said so that the compiler knows: what follows from it lives in uniform registers, and a branch on it
+// does not part the warp.
+template <typename T>
+__device__ __forceinline__ T warp_uniform(T x) { return __shfl_sync(0xffffffffu, x, 0); }
+
 // The products are issued by a whole warp in step, one elected lane of it doing so: descriptors stay in uniform registers, where the
 // instruction wants them. (Issued from a branch that one lane takes, a product took 80 cycles to issue and 32 to execute.)
 __device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool accumulate) {
@@ -76,7 +81,13 @@ __device__ __forceinline__ void tmem_load32(uint32_t addr, float* f) {
         "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(addr));
 }
-__device__ __forceinline__ void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// Waits for the loads of this thread; `f` is what they fill (said to the compiler, which must not use it earlier).
+template <int N>
+__device__ __forceinline__ void tmem_load_wait(float* f) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+f"(f[i])::"memory");
+}
 __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
                "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),

@@ -13,6 +13,7 @@ from typing import Optional
 import torch
 
 from . import native
+from .host import operators
 
 DTYPES = {torch.bfloat16: 1, torch.float16: 2}
 MOST_SIZE = 128
@@ -34,6 +35,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     Differentiable (once) in q, k and v, whose gradients have the shapes of these; the result and the gradients are the same
     in every run. Tensors may be views, as parts of one projection are: rows and heads that do not begin on 16-byte boundaries, or
     elements that do not lie side by side, are copied first. Under float16 a gradient beyond its range becomes infinite."""
+    if operators is not None and (scale is None or scale > 0):
+        out = operators.packed_attention(q, k, v, offsets, causal, 0.0 if scale is None else scale)
+        if out is not None:
+            return out
     check(q, k, v, offsets, scale)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -75,6 +80,8 @@ def _status(device: torch.device):
         with native.relaxed_capture():
             native.check(native.lib().psgd_status_alloc(ctypes.byref(host), ctypes.byref(dev)), "psgd_status_alloc")
         word = _statuses[device] = (host, ctypes.cast(dev, ctypes.c_void_p).value)
+        if operators is not None:
+            operators.status(device.index, ctypes.cast(host, ctypes.c_void_p).value, word[1])
     code = word[0][0]
     if code:
         word[0][0] = 0

@@ -13,6 +13,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import native
+from .host import operators
 
 MOST_TOP = 32
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -35,6 +36,9 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0
     the same. A target outside the vocabulary has log probability NaN: nothing is read for it. Masked tokens have logits of
     -inf; a row that has only those is no distribution: log probability -inf, entropy zero, no gradient. A row that
     holds +inf or NaN gives NaN, and any tokens. Returned statistics are float32."""
+    out = operators.token_log_probs(logits, targets, top, entropy, ignore_index, temperature) if operators is not None else None
+    if out is not None:
+        return TokenLogProbs(*out)
     check(logits, targets, top, ignore_index, temperature)
     if torch.is_grad_enabled() and logits.requires_grad:
         out = _TokenLogProbs.apply(logits, targets, int(top), bool(entropy), int(ignore_index), float(temperature))
