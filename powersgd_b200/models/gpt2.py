@@ -4,15 +4,23 @@ Not part of the reference repository; it is the fifth benchmark configuration (G
 24 layers, d = 1024, 16 heads, vocabulary 50 257, sequence 1024, bf16 autocast with float32
 gradients). Attention uses PyTorch's scaled-dot-product kernel; gradient compression is
 independent of the sequence length, so no sequence parallelism is involved.
+
+Documents of different lengths are trained on without padding, packed one behind another: `model.loss(tokens, targets,
+offsets)` with the rows of document i from offsets[i] to offsets[i + 1]. Attention then is `packed_attention` and the
+loss `token_log_probs`; both keep off the host, so that the lengths may change from step to step of a recorded graph.
 """
 from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from typing import Optional
 
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from ..ops.attention import packed_attention
+from ..ops.tokens import TokenLogProbs, token_log_probs
 
 
 @dataclass
@@ -48,7 +56,12 @@ class Block(nn.Module):
         self.mlp_proj = nn.Linear(4 * cfg.n_embd, cfg.n_embd)
         self.n_head, self.dropout = cfg.n_head, cfg.dropout
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        if offsets is not None:
+            t, c = x.shape
+            q, k, v = self.attn_qkv(self.ln_1(x)).view(t, 3, self.n_head, c // self.n_head).unbind(1)
+            x = x + self.attn_proj(packed_attention(q, k, v, offsets).reshape(t, c))
+            return x + self.mlp_proj(F.gelu(self.mlp_fc(self.ln_2(x)), approximate="tanh"))
         b, t, c = x.shape
         q, k, v = self.attn_qkv(self.ln_1(x)).split(c, dim=2)
         shape = (b, t, self.n_head, c // self.n_head)
@@ -78,14 +91,32 @@ class GPT2(nn.Module):
         if isinstance(module, nn.Linear) and module.bias is not None:
             nn.init.zeros_(module.bias)
 
-    def forward(self, tokens: torch.Tensor) -> torch.Tensor:
-        _, t = tokens.shape
-        pos = torch.arange(t, device=tokens.device)
+    def forward(self, tokens: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Logits of [batch, time] tokens, or of [rows] tokens of packed documents (`offsets`: int32, see `packed_attention`; on the GPU
+        under bf16 or fp16 autocast). A document's positions begin at zero; rows that belong to no document give logits of no meaning."""
+        if offsets is not None and self.cfg.dropout and self.training:
+            raise ValueError("GPT2: packed documents are trained on without dropout")
+        if tokens.dim() != (2 if offsets is None else 1):
+            raise ValueError(f"GPT2: tokens {tuple(tokens.shape)}; [batch, time] is expected, or [rows] with offsets")
+        t = tokens.shape[-1]
+        pos = torch.arange(t, device=tokens.device, dtype=torch.int64 if offsets is None else torch.int32)
+        if offsets is not None:
+            document = torch.searchsorted(offsets[1:].contiguous(), pos, right=True, out_int32=True)
+            pos = (pos - offsets[document]).clamp(0, self.cfg.n_positions - 1)
         x = self.wte(tokens) + self.wpe(pos)
         for block in self.h:
-            x = block(x)
+            x = block(x) if offsets is None else block(x, offsets)
         return F.linear(self.ln_f(x), self.wte.weight)  # tied output embedding
 
-    def loss(self, tokens: torch.Tensor, targets: torch.Tensor) -> torch.Tensor:
+    def loss(self, tokens: torch.Tensor, targets: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Mean negative log probability of the targets; with `offsets`, of those that are not -100 (the end of a document, rows that belong to
+        none)."""
+        if offsets is not None:
+            log_probs = self.score(tokens, targets, offsets).log_probs
+            return -log_probs.sum() / (targets != -100).sum().clamp(min=1)
         logits = self(tokens)
         return F.cross_entropy(logits.view(-1, logits.size(-1)).float(), targets.reshape(-1))
+
+    def score(self, tokens: torch.Tensor, targets: torch.Tensor, offsets: Optional[torch.Tensor] = None, **options) -> TokenLogProbs:
+        """Log probabilities of the targets; `top`, `entropy` and `temperature` as in `token_log_probs`."""
+        return token_log_probs(self(tokens, offsets), targets, **options)
