@@ -194,15 +194,126 @@ struct LpList {
   }
 };
 
+// The `top` largest of a part of a row, in descending order to s_best (zeros behind them), once the part has been read. Every thread brings the
+// largest value it has seen; of these, or of groups of them, 32 or 64 values are made. The top-th largest of those is a bound that
+// at least `top` elements reach, and few others. The elements of the threads that reach it, a few per cent of the row, are looked through again,
+// those of one thread by a whole warp, and what reaches the bound is collected. Where more does than there is room for (equal logits,
+// a row that is masked but for a few) every warp keeps a list of all it sees instead: with that alone a batch of 1023 x 33281 float16
+// logits took 84 us, without alternatives it takes 14.
+constexpr int LP_CANDIDATES = 512;
+template <typename T, int THREADS>
+__device__ __forceinline__ void lp_select(const T* z, int lead, int v0, int v1, int extra, float most, int top, unsigned long long* s_keys,
+                                          unsigned long long* s_best) {
+  using V = LpVec<T>;
+  constexpr int WARPS = THREADS / 32, KEYS = THREADS < 64 ? 32 : 64, GROUP = THREADS / KEYS, AHEAD = 4;
+  __shared__ __align__(16) uint32_t s_most[KEYS];
+  __shared__ uint32_t s_bound;
+  __shared__ int s_count, s_flagged;
+  __shared__ short s_threads[THREADS];
+  __shared__ unsigned long long s_least;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t mine = lp_order(most);
+  uint32_t group = mine;
+#pragma unroll
+  for (int o = 1; o < GROUP; o *= 2) group = max(group, __shfl_xor_sync(0xffffffffu, group, o));
+  if (tid % GROUP == 0) s_most[tid / GROUP] = group;
+  if (tid == 0) {
+    s_count = s_flagged = 0;
+    s_least = 0;
+  }
+  if (tid < LP_MAX_TOP) s_best[tid] = 0;
+  __syncthreads();
+  {   // the place of a group among the groups: its threads compare it with a share each
+    constexpr int SHARE = KEYS / GROUP < 4 ? 4 : KEYS / GROUP;
+    int above = 0, reach = 0;
+#pragma unroll
+    for (int i = 0; i < SHARE; i += 4) {
+      const uint4 x = *reinterpret_cast<const uint4*>(s_most + tid % GROUP * SHARE + i);
+      above += (x.x > group) + (x.y > group) + (x.z > group) + (x.w > group);
+      reach += (x.x >= group) + (x.y >= group) + (x.z >= group) + (x.w >= group);
+    }
+#pragma unroll
+    for (int o = 1; o < GROUP; o *= 2) {
+      above += __shfl_xor_sync(0xffffffffu, above, o);
+      reach += __shfl_xor_sync(0xffffffffu, reach, o);
+    }
+    if (above < top && reach >= top) s_bound = group;   // (equal ones write the same)
+  }
+  __syncthreads();
+  const uint32_t bound = s_bound;
+  const uint4* zv = reinterpret_cast<const uint4*>(z + lead);
+  auto take = [&](float v, int index) {
+    if (lp_order(v) < bound) return;
+    const int at = atomicAdd(&s_count, 1);
+    if (at < LP_CANDIDATES) s_keys[at] = lp_key(v, index);
+  };
+  if (mine >= bound) {
+    s_threads[atomicAdd(&s_flagged, 1)] = (short)tid;
+    if (extra >= 0) take(V::one(z + extra), extra);
+  }
+  __syncthreads();
+  const int flagged = s_flagged;
+  const int per_thread = (v1 - v0 + THREADS - 1) / THREADS;      // vectors, at most
+  for (int f = warp * AHEAD; f < flagged; f += WARPS * AHEAD) {
+    for (int i = lane; i - lane < per_thread; i += 32) {
+      uint4 r[AHEAD];
+      int at[AHEAD];
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        at[u] = f + u < flagged ? v0 + s_threads[f + u] + i * THREADS : v1;
+        if (at[u] < v1) r[u] = zv[at[u]];
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (at[u] >= v1 || lp_order(V::largest(r[u])) < bound) continue;
+        float x[V::N];
+        V::unpack(r[u], x);
+#pragma unroll
+        for (int e = 0; e < V::N; ++e) take(x[e], lead + at[u] * V::N + e);
+      }
+    }
+  }
+  __syncthreads();
+  int count = s_count;
+  if (count > LP_CANDIDATES) {
+    __syncthreads();
+    LpList list;
+    list.init();
+    for (int v = v0 + tid; v - tid < v1; v += THREADS) {
+      const bool valid = v < v1;
+      uint4 r = make_uint4(0, 0, 0, 0);
+      if (valid) r = zv[v];
+      const unsigned long long seen = *(volatile unsigned long long*)&s_least;
+      if (seen > list.least) list.least = seen;
+      if (!__any_sync(0xffffffffu, valid && lp_order(V::largest(r)) >= (uint32_t)(list.least >> 32))) continue;
+      float f[V::N];
+      V::unpack(r, f);
+#pragma unroll
+      for (int i = 0; i < V::N; ++i) list.offer(lp_key(f[i], lead + v * V::N + i), valid, top, &s_least);
+    }
+    list.offer(extra >= 0 ? lp_key(V::one(z + extra), extra) : 0, extra >= 0, top, &s_least);
+    s_keys[tid] = lane < top ? list.mine : 0;
+    count = THREADS;
+    __syncthreads();
+  }
+  for (int c = tid; c < count; c += THREADS) {   // a key's place is the number of larger ones
+    const unsigned long long key = s_keys[c];
+    int place = 0;
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) place += s_keys[i] > key;
+    if (key != 0 && place < top) s_best[place] = key;
+  }
+  __syncthreads();
+}
+
 template <typename T, int THREADS, bool TOP, bool ENT>
 __global__ void __launch_bounds__(THREADS) psgd_token_logprob_kernel(const __grid_constant__ LpArgs a) {
   using V = LpVec<T>;
-  constexpr int U = 4, WARPS = THREADS / 32;
+  constexpr int U = sizeof(T) == 4 ? 8 : 4, WARPS = THREADS / 32;
   __shared__ LpSum s_sum[WARPS];
   __shared__ LpSum s_parts[LP_MAX_CLUSTER];
-  __shared__ unsigned long long s_keys[TOP ? WARPS * LP_MAX_TOP : 1], s_best[TOP ? LP_MAX_TOP : 1];
+  __shared__ unsigned long long s_keys[TOP ? LP_CANDIDATES : 1], s_best[TOP ? LP_MAX_TOP : 1];
   __shared__ unsigned long long s_cluster_keys[TOP ? LP_MAX_CLUSTER * LP_MAX_TOP : 1];
-  __shared__ unsigned long long s_least;
 
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
@@ -221,12 +332,6 @@ __global__ void __launch_bounds__(THREADS) psgd_token_logprob_kernel(const __gri
   const bool known = target >= 0 && target < a.vocab;
   float z_target = 0.f;
   if (part == 0 && tid == 0 && known) z_target = V::one(z + target);   // on its way while the row is read
-  if (TOP) {
-    if (tid == 0) s_least = 0;
-    if (tid < LP_MAX_TOP) s_best[tid] = 0;
-    __syncthreads();
-  }
-
   const int lead = lp_lead(z, a.vocab);
   const int nvec = (a.vocab - lead) / V::N;
   const int share = (nvec + parts - 1) / parts;
@@ -234,8 +339,6 @@ __global__ void __launch_bounds__(THREADS) psgd_token_logprob_kernel(const __gri
   const uint4* zv = reinterpret_cast<const uint4*>(z + lead);
 
   LpSum t = {-INFINITY, 0.f, 0.f};
-  LpList list;
-  if (TOP) list.init();
   auto move_to = [&](float m) {   // the maximum moves to m
     if (m > t.m) {
       const float d = (t.m - m) * a.k, f = lp_exp2(d);
@@ -249,17 +352,6 @@ __global__ void __launch_bounds__(THREADS) psgd_token_logprob_kernel(const __gri
     t.s += e;
     if (ENT) t.a = fmaf(e, fmaxf(d, LP_FLOOR), t.a);
   };
-  auto offer = [&](const uint4& r, int index, bool valid) {
-    float f[V::N];
-    V::unpack(r, f);
-#pragma unroll
-    for (int i = 0; i < V::N; ++i) list.offer(lp_key(f[i], index + i), valid, a.top, &s_least);
-  };
-  auto refresh = [&]() {
-    const unsigned long long seen = *(volatile unsigned long long*)&s_least;
-    if (seen > list.least) list.least = seen;
-  };
-
   int v = v0 + tid;
   for (; v - tid + U * THREADS <= v1; v += U * THREADS) {
     uint4 r[U];
@@ -268,7 +360,10 @@ __global__ void __launch_bounds__(THREADS) psgd_token_logprob_kernel(const __gri
     float most[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) most[u] = V::largest(r[u]);
-    move_to(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
+    float largest = most[0];
+#pragma unroll
+    for (int u = 1; u < U; ++u) largest = fmaxf(largest, most[u]);
+    move_to(largest);
     const float b = lp_base(t.m);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -277,44 +372,29 @@ __global__ void __launch_bounds__(THREADS) psgd_token_logprob_kernel(const __gri
 #pragma unroll
       for (int i = 0; i < V::N; ++i) add(f[i], b);
     }
-    if (TOP) {
-      refresh();
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (__any_sync(0xffffffffu, lp_order(most[u]) >= (uint32_t)(list.least >> 32))) offer(r[u], lead + (v + u * THREADS) * V::N, true);
-    }
   }
-  for (; v - tid < v1; v += THREADS) {   // the last vectors: the warps take part whole
-    const bool valid = v < v1;
-    uint4 r = make_uint4(0, 0, 0, 0);
-    if (valid) {
-      r = lp_load(zv + v);
-      move_to(V::largest(r));
-      const float b = lp_base(t.m);
-      float f[V::N];
-      V::unpack(r, f);
+  for (; v < v1; v += THREADS) {
+    const uint4 r = lp_load(zv + v);
+    move_to(V::largest(r));
+    const float b = lp_base(t.m);
+    float f[V::N];
+    V::unpack(r, f);
 #pragma unroll
-      for (int i = 0; i < V::N; ++i) add(f[i], b);
-    }
-    if (TOP) {
-      refresh();
-      offer(r, lead + v * V::N, valid);
-    }
+    for (int i = 0; i < V::N; ++i) add(f[i], b);
   }
   // what lies before the first and behind the last whole vector: at most 14 elements, in warp 0
+  int extra = -1;
   if (warp == 0) {
     const int tail0 = lead + nvec * V::N, tail = a.vocab - tail0;
-    int index = -1;
-    if (part == 0 && lane < lead) index = lane;
-    if (part == parts - 1 && lane >= 16 && lane - 16 < tail) index = tail0 + lane - 16;
-    float f = 0.f;
-    if (index >= 0) {
-      f = V::one(z + index);
+    if (part == 0 && lane < lead) extra = lane;
+    if (part == parts - 1 && lane >= 16 && lane - 16 < tail) extra = tail0 + lane - 16;
+    if (extra >= 0) {
+      const float f = V::one(z + extra);
       move_to(f);
       add(f, lp_base(t.m));
     }
-    if (TOP) list.offer(lp_key(f, index), index >= 0, a.top, &s_least);
   }
+  if (TOP) lp_select<T, THREADS>(z, lead, v0, v1, extra, t.m, a.top, s_keys, s_best);
 
   // over the warp, the block, the cluster
 #pragma unroll
@@ -326,20 +406,7 @@ __global__ void __launch_bounds__(THREADS) psgd_token_logprob_kernel(const __gri
     t = lp_join<ENT>(t, y, a.k);
   }
   if (lane == 0) s_sum[warp] = t;
-  if (TOP) s_keys[warp * LP_MAX_TOP + lane] = lane < a.top ? list.mine : 0;
   __syncthreads();
-  if (TOP) {   // a key's place is the number of larger ones
-    unsigned long long key = 0;
-    int place = LP_MAX_TOP;
-    if (tid < WARPS * LP_MAX_TOP && (tid & 31) < a.top) {
-      key = s_keys[tid];
-      place = 0;
-      for (int w = 0; w < WARPS; ++w)
-        for (int j = 0; j < a.top; ++j) place += s_keys[w * LP_MAX_TOP + j] > key;
-    }
-    if (key != 0 && place < a.top) s_best[place] = key;
-    __syncthreads();
-  }
   if (tid == 0) {
     for (int w = 1; w < WARPS; ++w) t = lp_join<ENT>(t, s_sum[w], a.k);
     if (parts > 1) *cluster.map_shared_rank(&s_parts[part], 0) = t;
@@ -406,7 +473,7 @@ struct LpGradArgs {
   const float* g_top;
 };
 
-constexpr int LG_THREADS = 256, LG_U = 2;
+constexpr int LG_THREADS = 256, LG_U = 4;
 
 // One chunk of a row per block: elementwise, so nothing waits for anything.
 template <typename T, bool ENT, bool TOP>
@@ -503,7 +570,10 @@ int lp_forward(const LpArgs& a, long long rows, int cluster, cudaStream_t stream
 
 template <typename T>
 int lp_dispatch(const LpArgs& a, long long rows, cudaStream_t stream) {
-  if (a.vocab * (int)sizeof(T) <= 8192) return lp_forward<T, 64>(a, rows, 1, stream);
+  // Short rows: a warp each, without barriers; with many alternatives two, since the bound of 32 values is a low one where most of them are
+  // asked for (16384 x 1000 float16: 15 us by one warp, 17 by two; with 8 alternatives 45 and 45, with 20 86 and 52).
+  if (a.vocab * (long long)sizeof(T) <= 4096 && a.top <= 8) return lp_forward<T, 32>(a, rows, 1, stream);
+  if (a.vocab * (long long)sizeof(T) <= 8192) return lp_forward<T, 64>(a, rows, 1, stream);
   // Few rows: a cluster shares one, so that the row is read by several SMs at a time.
   int cluster = 1;
   while (cluster < LP_MAX_CLUSTER && rows * cluster < 296 && a.vocab / (2 * cluster) >= 2048) cluster *= 2;
