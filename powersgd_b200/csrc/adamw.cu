@@ -119,8 +119,10 @@ __device__ __forceinline__ AwFactors aw_factors(const AwHyper& h, float t) {
 // Products and sums are rounded one by one, without fused multiply-adds: moments are the same bits that elementwise operations give, and
 // 8-bit codes that follow from them are too, in this step and in all later ones.
 __device__ __forceinline__ void aw_moments(const AwHyper& h, float2 g, float2& m, float2& v) {
-  m = add2(mul2(m, make_float2(h.beta1, h.beta1)), mul2(g, make_float2(h.rest1, h.rest1)));
-  v = add2(mul2(v, make_float2(h.beta2, h.beta2)), mul2(mul2(g, g), make_float2(h.rest2, h.rest2)));
+  const float2 m0 = mul2(m, make_float2(h.beta1, h.beta1)), m1 = mul2(g, make_float2(h.rest1, h.rest1));
+  const float2 v0 = mul2(v, make_float2(h.beta2, h.beta2)), v1 = mul2(mul2(g, g), make_float2(h.rest2, h.rest2));
+  m = make_float2(__fadd_rn(m0.x, m1.x), __fadd_rn(m0.y, m1.y));   // (sums of pairs would be fused with the products)
+  v = make_float2(__fadd_rn(v0.x, v1.x), __fadd_rn(v0.y, v1.y));
 }
 __device__ __forceinline__ float aw_reciprocal(float x) {   // (1 ulp; the update is small beside p)
   float y;

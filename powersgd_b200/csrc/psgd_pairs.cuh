@@ -1,4 +1,5 @@
-// Two float32 operations in one instruction, each rounded as one by itself.
+// Two float32 operations in one instruction. The compiler fuses a product of pairs with a sum of pairs that takes it, although both say how
+// they are rounded: where each has to be rounded by itself, the sum is made of scalars (__fadd_rn).
 #pragma once
 #include <cuda_runtime.h>
 

@@ -196,6 +196,23 @@ def test_same_as_the_cpu_and_repeatable():
         assert ((a - b).abs() > 1e-5).float().mean() < 0.01      # a code that goes the other way moves its element
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_moments_are_those_of_torch_operations_bit_for_bit(dtype, bits):
+    """Products and sums rounded one by one: otherwise a code now and then goes the other way, and takes its element with it."""
+    p, opt = _make([(300, 1000)], dtype, bits)
+    p = p[0]
+    q, state = p.detach().clone(), adamw.new_state(p, bits)
+    names = adamw.state_names(bits)
+    for step in range(3):
+        _grads([p], step)
+        adamw._step_torch(q, p.grad, [state[n] for n in names], state["step"], bits, LR, B1, B2, EPS, WD, 77, 0)
+        opt.step()
+        for name in names:
+            assert torch.equal(state[name].view(torch.uint8), opt.state[p][name].view(torch.uint8)), name
+        assert (p.double() - q.double()).norm() <= 2.0**-20 * q.double().norm() if dtype == torch.float32 else (p != q).float().mean() < 1e-3
+
+
 def test_infinite_gradients_stay_in_their_block():
     p = torch.nn.Parameter(torch.ones(1024, device="cuda"))
     p.grad = torch.ones(1024, device="cuda")
