@@ -1,4 +1,4 @@
-// Calls of token_log_probs and packed_attention from Python, as a CPython extension against PyTorch's C++ interface.
+// Calls of token_log_probs, packed_attention and AdamW from Python, as a CPython extension against PyTorch's C++ interface.
 //
 // Through Python and a foreign function call a forward pass took 25 us of the host, and a backward pass, whose node the autograd
 // engine runs on a thread of its own that must first get the interpreter lock, 80 us besides the engine's own 45: more than the kernels
@@ -38,6 +38,7 @@ struct Entry {
                    void*) = nullptr;
   int (*attention_backward)(const void*, const void*, const void*, const void*, const long long*, const int*, int, int, int, int, int, int, int, float,
                             const void*, const void*, const float*, float*, void*, void*, void*, int*, void*) = nullptr;
+  int (*adamw)(const void*, int, int, int, double, const float*, double, double, double, double, double, double, unsigned, int*, void*) = nullptr;
 } entry;
 
 constexpr int MOST_DEVICES = 64;
@@ -354,16 +355,36 @@ PyObject* packed_attention(PyObject*, PyObject* args) {
   });
 }
 
+// ---- AdamW --------------------------------------------------------------------------------------
+// adamw_step(items, count, device, type, bits, lr, address of lr, betas and their logarithms, eps, decay, seed, ticket): the native step on the
+// device's current stream. Returns its code.
+PyObject* adamw_step(PyObject*, PyObject* args) {
+  return guarded([&]() -> PyObject* {
+    const char* items;
+    Py_ssize_t bytes;
+    int count, device, type, bits;
+    double lr, beta1, beta2, log1, log2, eps, decay;
+    unsigned long long lr_at, ticket;
+    unsigned int seed;
+    if (!PyArg_ParseTuple(args, "y#iiiidKddddddIK", &items, &bytes, &count, &device, &type, &bits, &lr, &lr_at, &beta1, &beta2, &log1, &log2, &eps, &decay, &seed, &ticket))
+      return nullptr;
+    const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+    void* stream = (void*)c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)device).stream();
+    return PyLong_FromLong(entry.adamw(items, count, type, bits, lr, (const float*)lr_at, beta1, beta2, log1, log2, eps, decay, seed, (int*)ticket, stream));
+  });
+}
+
 // ---- what Python hands over ---------------------------------------------------------------------
-// bind(error, token, token_grad, attention, attention_backward): addresses of the native library's entry points.
+// bind(error, token, token_grad, attention, attention_backward, adamw): addresses of the native library's entry points.
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[5];
-  if (!PyArg_ParseTuple(args, "KKKKK", a, a + 1, a + 2, a + 3, a + 4)) return nullptr;
+  unsigned long long a[6];
+  if (!PyArg_ParseTuple(args, "KKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5)) return nullptr;
   entry.error = (decltype(entry.error))a[0];
   entry.token = (decltype(entry.token))a[1];
   entry.token_grad = (decltype(entry.token_grad))a[2];
   entry.attention = (decltype(entry.attention))a[3];
   entry.attention_backward = (decltype(entry.attention_backward))a[4];
+  entry.adamw = (decltype(entry.adamw))a[5];
   Py_RETURN_NONE;
 }
 // status(device, host address, device address): the status word of a device.
@@ -383,6 +404,7 @@ PyMethodDef methods[] = {
     {"status", status, METH_VARARGS, nullptr},
     {"token_log_probs", token_log_probs, METH_VARARGS, nullptr},
     {"packed_attention", packed_attention, METH_VARARGS, nullptr},
+    {"adamw_step", adamw_step, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -392,7 +414,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods,
 PyMODINIT_FUNC PyInit__operators() {
   PyObject* m = PyModule_Create(&module);
   // what this was compiled for, which the loader compares (csrc/build.py, scan_target)
-  if (m != nullptr && PyModule_AddStringConstant(m, "target", PSGD_SCAN_TARGET) != 0) {
+  if (m != nullptr && (PyModule_AddStringConstant(m, "target", PSGD_SCAN_TARGET) != 0 || PyModule_AddIntConstant(m, "entry_points", 6) != 0)) {
     Py_DECREF(m);
     return nullptr;
   }

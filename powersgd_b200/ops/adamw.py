@@ -10,7 +10,6 @@ random bits that are a hash of `seed`, the number of steps and the element's pla
 """
 from __future__ import annotations
 
-import ctypes
 import math
 from typing import List, Optional, Sequence
 
@@ -18,7 +17,7 @@ import numpy as np
 import torch
 
 from . import native, scan
-from .recording import is_recorded, keep_with_graph
+from .host import operators
 
 BLOCK = 256             # elements that share a scale
 E4M3_MAX = 448.0
@@ -131,14 +130,15 @@ def launch(items: bytes, count: int, device: torch.device, dtype: int, *, bits, 
             lr_at, lr = lr, 0.0
         else:
             lr = float(lr)
-    with native.on_device(device) as stream:
-        native.check(
-            native.lib().psgd_adamw_step(
-                items, count, dtype, bits, lr, None if lr_at is None else lr_at.data_ptr(), beta1, beta2, math.log(beta1) if beta1 > 0 else -math.inf,
-                math.log(beta2) if beta2 > 0 else -math.inf, eps, weight_decay, seed, ticket.data_ptr(), stream,
-            ),
-            "psgd_adamw_step",
-        )
+    call = (items, count, dtype, bits, lr, 0 if lr_at is None else lr_at.data_ptr(), beta1, beta2, math.log(beta1) if beta1 > 0 else -math.inf,
+            math.log(beta2) if beta2 > 0 else -math.inf, eps, weight_decay, seed, ticket.data_ptr())
+    if operators is not None:
+        code = operators.adamw_step(*call[:2], device.index, *call[2:])
+    else:
+        with native.on_device(device) as stream:
+            code = native.lib().psgd_adamw_step(*call, stream)
+    if code:
+        native.check(code, "psgd_adamw_step")
 
 
 # ---- the step in torch operations --------------------------------------------------------------

@@ -8,7 +8,7 @@ import os
 from ..csrc.build import operators_lib, scan_target
 from . import native
 
-ENTRY_POINTS = ("psgd_last_error", "psgd_token_logprob", "psgd_token_logprob_grad", "psgd_attention", "psgd_attention_backward")
+ENTRY_POINTS = ("psgd_last_error", "psgd_token_logprob", "psgd_token_logprob_grad", "psgd_attention", "psgd_attention_backward", "psgd_adamw_step")
 
 
 def _load():
@@ -22,8 +22,8 @@ def _load():
         spec.loader.exec_module(module)
     except ImportError:   # symbols or libraries that are not there
         return None
-    if getattr(module, "target", None) != scan_target():
-        return None
+    if getattr(module, "target", None) != scan_target() or getattr(module, "entry_points", 0) != len(ENTRY_POINTS):
+        return None   # of another PyTorch, or of an earlier state of the sources
     module.bind(*[ctypes.cast(getattr(native.lib(), name), ctypes.c_void_p).value for name in ENTRY_POINTS])
     return module
 

@@ -9,7 +9,7 @@ import torch
 from .aggregators import Aggregator
 from .ops import adamw as _adamw
 from .ops import native, scan
-from .ops.recording import is_recorded, keep_with_graph, outside_capture
+from .ops.recording import keep_with_graph, outside_capture
 from .utils import params_in_optimizer
 
 
@@ -99,13 +99,12 @@ class AdamW(torch.optim.Optimizer):
             if p.dtype not in _adamw.DTYPES:
                 raise TypeError(f"AdamW: parameter {i} is {p.dtype}; float32, bfloat16 and float16 are supported")
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        first_block = 0
+        first_block = 0    # of each parameter in the stream of random numbers
         for group in self.param_groups:
             first_block = self._step_group(group, first_block)
         return loss
@@ -118,7 +117,12 @@ class AdamW(torch.optim.Optimizer):
             items, count, device, dtype, end = known
             if count and native.use_for_cuda():
                 device = torch.device("cuda", device)
-                self._launch_items(group, items, count, device, dtype)
+                ticket = self._ticket(device)
+                if torch.cuda.is_current_stream_capturing():
+                    self._keep(group["params"], [self.state[p] for p in group["params"] if p.grad is not None], ticket)
+                beta1, beta2 = group["betas"]
+                _adamw.launch(items, count, device, dtype, bits=bits, lr=group["lr"], beta1=beta1, beta2=beta2, eps=group["eps"],
+                              weight_decay=group["weight_decay"], seed=group["seed"], ticket=ticket)
                 return end
         lists, at = {}, first_block
         for p in group["params"]:
@@ -137,7 +141,8 @@ class AdamW(torch.optim.Optimizer):
             ticket = None
             if device.type == "cuda" and native.use_for_cuda():
                 ticket = self._ticket(device)
-                self._keep(device, params, states)
+                if torch.cuda.is_current_stream_capturing():
+                    self._keep(params, states, ticket)
             missing = [name for name in ("step", *names) if any(name not in s for s in states)]
             if missing:
                 raise ValueError(f"AdamW: the state has no {missing[0]}; it belongs to moments of another number of bits than {bits}")
@@ -146,12 +151,6 @@ class AdamW(torch.optim.Optimizer):
                               seed=group["seed"], first_blocks=blocks, ticket=ticket)
         return at
 
-    def _launch_items(self, group: dict, items: bytes, count: int, device: torch.device, dtype: int) -> None:
-        ticket = self._ticket(device)
-        self._keep(device, group["params"], [self.state[p] for p in group["params"] if p.grad is not None] if self._recorded(device) else ())
-        _adamw.launch(items, count, device, dtype, bits=group["state_bits"], lr=group["lr"], beta1=group["betas"][0], beta2=group["betas"][1],
-                      eps=group["eps"], weight_decay=group["weight_decay"], seed=group["seed"], ticket=ticket)
-
     def _ticket(self, device: torch.device) -> torch.Tensor:
         ticket = self._tickets.get(device)
         if ticket is None:
@@ -159,14 +158,9 @@ class AdamW(torch.optim.Optimizer):
                 ticket = self._tickets[device] = torch.zeros(1, dtype=torch.int32, device=device)
         return ticket
 
-    @staticmethod
-    def _recorded(device: torch.device) -> bool:
-        return is_recorded(torch._C._cuda_getCurrentRawStream(device.index))
-
-    def _keep(self, device: torch.device, params, states) -> None:
-        """What a graph that is being recorded refers to stays, whatever is loaded later."""
-        if self._recorded(device):
-            keep_with_graph(self._held, *params, *[t for s in states for t in s.values()], self._tickets[device])
+    def _keep(self, params, states, ticket: torch.Tensor) -> None:
+        """What the graph that is being recorded refers to stays, whatever is loaded later."""
+        keep_with_graph(self._held, *params, *[t for s in states for t in s.values()], ticket)
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As in `torch.optim`, except that moments and numbers of steps keep their own types."""
