@@ -18,8 +18,8 @@
 //   dK, dV    tiles of 128 keys, walking over tiles of 64 queries of all heads of the group, transposed: lanes are
 //             keys, so that P^T and dS^T are A operands as they come. Nothing is added with atomics: the same inputs
 //             give the same bits. The price is that S and dP are computed twice (seven products instead of five).
-// A row of a tile that belongs to another sequence, or lies behind the last one, may hold anything: scores with it are
-// replaced, and where it would be multiplied by their zeros its row in shared memory is cleared.
+// A row of a tile that belongs to another sequence, or lies behind the last one, may hold anything: before it is multiplied with anything
+// but scores that are replaced, its row in shared memory is cleared.
 //
 // Blocks are dealt out with the longest first: the device finds the n-th tile in the order of its distance from the
 // sequence's beginning (causal: of its work), from the offsets alone.
@@ -156,25 +156,21 @@ __device__ __forceinline__ void at_clear_outside(const AtArgs& a, const AtPiece&
 }
 
 // ---- pieces of the pipelines -------------------------------------------------------------------
+// Waits for a whole warp, which goes on as one: all of its lanes, or none. (A lane that gave up alone would leave the others waiting for it at their next
+// common instruction.)
 struct AtWait {
   volatile int* abort_flag;
   int* status;
-  __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const {
+  __device__ __forceinline__ bool one(uint64_t* bar, uint32_t parity) const {
 #pragma unroll 1
     for (int i = 0; i < 64; ++i)   // (the clock is read only when it takes longer)
       if (psgd_mbar_try_wait(bar, parity)) return true;
     return psgd_mbar_wait(bar, parity, abort_flag, status);
   }
-};
-
-// The same for a warp that goes on as one: all of its lanes, or none.
-struct AtWaitAll {
-  AtWait one;
   __device__ __forceinline__ bool operator()(uint64_t* bar, uint32_t parity) const { return __all_sync(0xffffffffu, one(bar, parity)); }
 };
 
-// One arrival for a warp whose lanes have all done what the barrier stands for. (128 or 256 arrivals on one word of shared memory
-// took longer than the work between them.)
+// One arrival for a warp whose lanes have all done what the barrier stands for.
 __device__ __forceinline__ void at_arrive(uint64_t* bar) {
   umma_fence_before();
   __syncwarp();
@@ -191,15 +187,17 @@ __device__ __forceinline__ void at_load_tile(uint32_t dst, const CUtensorMap* ma
   }
 }
 
-// Clears a row of a tile.
+// Clears the rows of a tile from `from` on, which do not belong to the sequence and may hold anything: by the warp that issues the products, before
+// it does so.
 template <int PANELS, int ROWS>
-__device__ __forceinline__ void at_clear_row(uint8_t* tile, int row) {
-#pragma unroll
+__device__ __forceinline__ void at_clear_rows(uint8_t* tile, int from) {
+#pragma unroll 1
   for (int p = 0; p < PANELS; ++p) {
-    uint4* at = reinterpret_cast<uint4*>(tile + (p * ROWS + row) * 128);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) at[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int i = from * 8 + (int)(threadIdx.x & 31); i < ROWS * 8; i += 32) reinterpret_cast<uint4*>(tile + p * ROWS * 128)[i] = make_uint4(0, 0, 0, 0);
   }
+  psgd_fence_async_shared();
+  __syncwarp();
 }
 
 // The 32 rows of an accumulator that a warp can read, times `factor`, as rows of 16-bit numbers `pitch` elements apart, the first `rows` of them;
@@ -327,28 +325,28 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
   const int steps = max(n[0], n[TILES - 1]);
 
   if (warp == LOADER) {
-    if (lane == 0) {
-      psgd_mbar_expect_tx(&bar_q, n[TILES - 1] > 0 ? TILES * TILE_BYTES : TILE_BYTES);
+    {
+      if (lane == 0) psgd_mbar_expect_tx(&bar_q, n[TILES - 1] > 0 ? TILES * TILE_BYTES : TILE_BYTES);
       for (int t = 0; t < TILES; ++t)
-        if (n[t] > 0) at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_q + t * TILE_BYTES), &a.q, head, start + row0 + t * AT_TILE, &bar_q);
+        if (n[t] > 0 && lane == 0) at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_q + t * TILE_BYTES), &a.q, head, start + row0 + t * AT_TILE, &bar_q);
       for (int i = 0; i < 2 * steps; ++i) {   // K_0, V_0, K_1, V_1, ...
         const int slot = i % AF_RING;
         if (!wait(&bar_empty[slot], ((i / AF_RING) & 1) ^ 1)) break;
+        if (lane != 0) continue;
         psgd_mbar_expect_tx(&bar_full[slot], TILE_BYTES);
         at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_ring + slot * TILE_BYTES), (i & 1) ? &a.v : &a.k, head / a.group, start + (i >> 1) * AT_TILE, &bar_full[slot]);
       }
     }
   } else if (warp == ISSUER) {
-    const AtWaitAll wait_all = {wait};
     const int k_steps = (a.size + 15) / 16;
     constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_TILE);
     const uint32_t o_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
     const uint32_t q_at = warp_uniform(psgd_smem_u32(s_q)), ring_at = q_at + TILES * TILE_BYTES;
-    bool ok = wait_all(&bar_q, 0) && wait_all(&bar_full[0], 0);
+    bool ok = wait(&bar_q, 0) && wait(&bar_full[0], 0);
     int have = 0;   // tiles of keys that are there
     auto scores = [&](int t, int j) {
       if (j > have) {
-        ok = wait_all(&bar_full[2 * j % AF_RING], (2 * j / AF_RING) & 1);
+        ok = wait(&bar_full[2 * j % AF_RING], (2 * j / AF_RING) & 1);
         have = j;
       }
       if (!ok) return;
@@ -364,17 +362,20 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
       for (int t = 0; t < TILES && ok; ++t) {
         if (j >= n[t]) continue;
         if (EARLY && j + 1 < n[t]) {
-          ok = wait_all(&bar_r[t], j & 1);
+          ok = wait(&bar_r[t], j & 1);
           if (ok) scores(t, j + 1);
           if (!ok) break;
         }
-        if (t == 0 || n[0] <= j) ok = wait_all(&bar_full[kv % AF_RING], (kv / AF_RING) & 1);
+        if (t == 0 || n[0] <= j) {
+          ok = wait(&bar_full[kv % AF_RING], (kv / AF_RING) & 1);
+          if (ok && length - j * AT_TILE < AT_TILE) at_clear_rows<PANELS, AT_TILE>(s_ring + (kv % AF_RING) * TILE_BYTES, length - j * AT_TILE);
+        }
         const uint32_t o_at = tmem + O + t * AT_TILE, p_at = tmem + P + t * AT_TILE, v_at = ring_at + (kv % AF_RING) * TILE_BYTES;
-        ok = ok && wait_all(&bar_p[t][0], j & 1);
+        ok = ok && wait(&bar_p[t][0], j & 1);
         if (!ok) break;
         umma_fence_after();
         umma_weights_by_rows<0, 4, AT_TILE>(o_at, p_at, v_at, o_shape, j > 0);
-        ok = wait_all(&bar_p[t][1], j & 1);
+        ok = wait(&bar_p[t][1], j & 1);
         if (!ok) break;
         umma_fence_after();
         umma_weights_by_rows<4, 8, AT_TILE>(o_at, p_at, v_at, o_shape, true);
@@ -407,14 +408,6 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
 #pragma unroll
         for (int c = 0; c < AT_TILE; ++c)
           if (c > last) s[c] = -INFINITY;
-        const int held = length - j * AT_TILE;       // keys of this tile that belong to the sequence
-        if (held < AT_TILE) {
-          const int kv = 2 * j + 1;
-          ok = wait(&bar_full[kv % AF_RING], (kv / AF_RING) & 1);
-          if (!ok) break;
-          if (row >= held) at_clear_row<PANELS, AT_TILE>(s_ring + (kv % AF_RING) * TILE_BYTES, row);
-          psgd_fence_async_shared();
-        }
       }
       float most[4];
 #pragma unroll
@@ -591,13 +584,16 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
   const int steps = (a.causal ? min(q0 + AT_TILE, length) + AT_STEP - 1 : length + AT_STEP - 1) / AT_STEP;
 
   if (warp == LOADER) {
-    if (lane == 0) {
-      psgd_mbar_expect_tx(&bars.fixed, 2 * TILE_BYTES);
-      at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_q), &a.q, head, start + q0, &bars.fixed);
-      at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_g), &a.g, head, start + q0, &bars.fixed);
+    {
+      if (lane == 0) psgd_mbar_expect_tx(&bars.fixed, 2 * TILE_BYTES);
+      if (lane == 0) {
+        at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_q), &a.q, head, start + q0, &bars.fixed);
+        at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_g), &a.g, head, start + q0, &bars.fixed);
+      }
       for (int j = 0; j < steps; ++j) {
         const int slot = j % STAGES;
         if (!wait(&bars.empty[slot], ((j / STAGES) & 1) ^ 1)) break;
+        if (lane != 0) continue;
         psgd_mbar_expect_tx(&bars.full[slot], 2 * HALF);
         const uint32_t at = psgd_smem_u32(s_ring + slot * TILE_BYTES);
         at_load_tile<PANELS, AT_STEP>(at, &a.k, head / a.group, start + j * AT_STEP, &bars.full[slot]);
@@ -605,16 +601,21 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       }
     }
   } else if (warp == ISSUER) {
-    const AtWaitAll wait_all = {wait};
     const int k_steps = (a.size + 15) / 16;
     constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_STEP);
     const uint32_t q_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
     const uint32_t q_at = warp_uniform(psgd_smem_u32(s_q)), g_at = q_at + TILE_BYTES, ring_at = q_at + 2 * TILE_BYTES;
-    bool ok = wait_all(&bars.fixed, 0);
+    bool ok = wait(&bars.fixed, 0);
     int have = -1;
     auto there = [&](int j) {
-      if (j > have) ok = ok && wait_all(&bars.full[j % STAGES], (j / STAGES) & 1);
-      have = max(have, j);
+      if (j > have) {
+        ok = ok && wait(&bars.full[j % STAGES], (j / STAGES) & 1);
+        have = j;
+        if (ok && length - j * AT_STEP < AT_STEP) {
+          at_clear_rows<PANELS, AT_STEP>(s_ring + j % STAGES * TILE_BYTES, length - j * AT_STEP);
+          at_clear_rows<PANELS, AT_STEP>(s_ring + j % STAGES * TILE_BYTES + HALF, length - j * AT_STEP);
+        }
+      }
       if (ok) umma_fence_after();
       return ok;
     };
@@ -635,11 +636,11 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
     for (int j = 0; j < steps && ok; ++j) {
       const int chain = j % CHAINS;
       const uint32_t parity = (j / CHAINS) & 1;
-      ok = wait_all(&bars.p[chain], parity);    // S is in registers
+      ok = wait(&bars.p[chain], parity);    // S is in registers
       if (!ok) break;
       umma_fence_after();
       if (j + CHAINS < steps) scores(j + CHAINS);
-      ok = ok && wait_all(&bars.ds[chain], parity);
+      ok = ok && wait(&bars.ds[chain], parity);
       if (!ok) break;
       umma_fence_after();
       umma_weights_by_rows<0, 4, AT_STEP>(tmem + DQ, tmem + chain * 128 + AT_STEP, ring_at + j % STAGES * TILE_BYTES, q_shape, j > 0);
@@ -680,7 +681,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       asm volatile("bar.sync 1, 256;" ::: "memory");
       delta = s_delta[row];
     }
-    const int limit = a.causal ? min(q, length - 1) : length - 1;    // last key that counts
+    const int limit = a.causal ? q : length - 1;    // last key that counts
     bool ok = true;
     for (int j = chain; j < steps; j += CHAINS) {
       const uint32_t parity = (j / CHAINS) & 1;
@@ -693,19 +694,11 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       tmem_load_wait<AT_STEP>(p);
       at_arrive(&bars.p[chain]);
       ab_exponentials(p, a.scale2, lse);
-      const int last = limit - j * AT_STEP;
-      const bool edge = (j + 1) * AT_STEP > (a.causal ? min(q0 + 1, length) : length);     // some key of this step does not count for some row
-      const int keys = length - j * AT_STEP;
-      if (edge) {
+      if ((j + 1) * AT_STEP > (a.causal ? q0 + 1 : length)) {     // some keys do not count for some rows
+        const int last = limit - j * AT_STEP;
 #pragma unroll
         for (int c = 0; c < AT_STEP; ++c)
           if (c > last) p[c] = 0.f;
-        if (keys < AT_STEP) {
-          ok = wait(&bars.full[j % STAGES], (j / STAGES) & 1);
-          if (!ok) break;
-          if (row >= keys && row < AT_STEP) at_clear_row<PANELS, AT_STEP>(s_ring + j % STAGES * TILE_BYTES, row);
-          psgd_fence_async_shared();
-        }
       }
       ok = wait(&bars.dp[chain], parity);
       if (!ok) break;
@@ -720,11 +713,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
-          float2 x = mul2(make_float2(p[c + i], p[c + i + 1]), add2(make_float2(d[c + i], d[c + i + 1]), minus));
-          if (keys < AT_STEP) {   // (behind the sequence dP may be anything: no factor of zero does)
-            if (c + i > last) x.x = 0.f;
-            if (c + i + 1 > last) x.y = 0.f;
-          }
+          const float2 x = mul2(make_float2(p[c + i], p[c + i + 1]), add2(make_float2(d[c + i], d[c + i + 1]), minus));
           w[i / 2] = pack2<T>(x.x, x.y);
         }
         tmem_store16(dp_at + c / 2, w);
@@ -820,14 +809,17 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
   };
 
   if (warp == LOADER) {
-    if (lane == 0) {
-      psgd_mbar_expect_tx(&bars.fixed, 2 * TILE_BYTES);
-      at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_k), &a.k, head, start + k0, &bars.fixed);
-      at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_v), &a.v, head, start + k0, &bars.fixed);
+    {
+      if (lane == 0) psgd_mbar_expect_tx(&bars.fixed, 2 * TILE_BYTES);
+      if (lane == 0) {
+        at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_k), &a.k, head, start + k0, &bars.fixed);
+        at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_v), &a.v, head, start + k0, &bars.fixed);
+      }
       Step step = {head0, first * AT_STEP};
       for (int i = 0; i < steps; ++i, next(step, 1)) {
         const int slot = i % STAGES;
         if (!wait(&bars.empty[slot], ((i / STAGES) & 1) ^ 1)) break;
+        if (lane != 0) continue;
         psgd_mbar_expect_tx(&bars.full[slot], 2 * HALF);
         const uint32_t at = psgd_smem_u32(s_ring + slot * TILE_BYTES);
         at_load_tile<PANELS, AT_STEP>(at, &a.q, step.head, start + step.row, &bars.full[slot]);
@@ -835,16 +827,24 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       }
     }
   } else if (warp == ISSUER) {
-    const AtWaitAll wait_all = {wait};
     const int k_steps = (a.size + 15) / 16;
     constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_STEP);
     const uint32_t o_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
     const uint32_t k_at = warp_uniform(psgd_smem_u32(s_k)), v_at = k_at + TILE_BYTES, ring_at = k_at + 2 * TILE_BYTES;
-    bool ok = wait_all(&bars.fixed, 0);
+    bool ok = wait(&bars.fixed, 0);
     int have = -1;
+    Step step = {head0, first * AT_STEP};     // the one behind `have`
     auto there = [&](int i) {
-      if (i > have) ok = ok && wait_all(&bars.full[i % STAGES], (i / STAGES) & 1);
-      have = max(have, i);
+      if (i > have) {
+        ok = ok && wait(&bars.full[i % STAGES], (i / STAGES) & 1);
+        have = i;
+        const int queries = length - step.row;
+        next(step, 1);
+        if (ok && queries < AT_STEP) {
+          at_clear_rows<PANELS, AT_STEP>(s_ring + i % STAGES * TILE_BYTES, queries);
+          at_clear_rows<PANELS, AT_STEP>(s_ring + i % STAGES * TILE_BYTES + HALF, queries);
+        }
+      }
       if (ok) umma_fence_after();
       return ok;
     };
@@ -865,12 +865,12 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
     for (int i = 0; i < steps && ok; ++i) {
       const int chain = i % CHAINS;
       const uint32_t parity = (i / CHAINS) & 1, stage = ring_at + i % STAGES * TILE_BYTES;
-      ok = wait_all(&bars.p[chain], parity);
+      ok = wait(&bars.p[chain], parity);
       if (!ok) break;
       umma_fence_after();
       umma_weights_by_rows<0, 4, AT_STEP>(tmem + DV, tmem + chain * 128, stage + HALF, o_shape, i > 0);
       if (i + CHAINS < steps) scores(i + CHAINS);
-      ok = ok && wait_all(&bars.ds[chain], parity);
+      ok = ok && wait(&bars.ds[chain], parity);
       if (!ok) break;
       umma_fence_after();
       umma_weights_by_rows<0, 4, AT_STEP>(tmem + DK, tmem + chain * 128 + AT_STEP, stage, o_shape, i > 0);
@@ -894,13 +894,10 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
     bool ok = true;
     int mine = 0;                   // steps of this chain so far
     for (int i = chain; i < steps; i += CHAINS, ++mine) {
-      const int q0 = step.row, queries = length - q0;
+      const int q0 = step.row;
       next(later, CHAINS);
       const float ahead = i + CHAINS < steps ? statistic(later) : 0.f;
       step = later;
-      // queries [from, to) of the step meet this thread's key
-      const int from = a.causal ? key - q0 : 0, to = queries;
-      const bool edge = (a.causal && q0 < k0 + AT_TILE) || queries < AT_STEP;
       const float* now = stats[mine % 3];
       // The statistics of a step were written before the arrivals for the one before. A warp may be behind by the second half of a step, no
       // more: two places would not do, three do.
@@ -922,21 +919,13 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
           p[c + h + 1] = at_exp2(y.y);
         }
       }
-      if (edge) {
+      if (a.causal && q0 < k0 + AT_TILE) {     // some queries come before some keys
+        const int from = key - q0;
 #pragma unroll
         for (int c = 0; c < AT_STEP; ++c)
           if (c < from) p[c] = 0.f;
-        if (queries < AT_STEP) {
-#pragma unroll
-          for (int c = 0; c < AT_STEP; ++c)
-            if (c >= to) p[c] = 0.f;
-          ok = wait(&bars.full[i % STAGES], (i / STAGES) & 1);
-          if (!ok) break;
-          const int r = row % AT_STEP;
-          if (r >= queries) at_clear_row<PANELS, AT_STEP>(s_ring + i % STAGES * TILE_BYTES + (row < AT_STEP ? 0 : HALF), r);
-          psgd_fence_async_shared();
-        }
       }
+      // (Queries behind the sequence have rows of zeros and deltas of zero: their weights are multiplied by zeros, their slopes are zeros.)
 #pragma unroll
       for (int c = 0; c < AT_STEP; c += 32) {
         uint32_t w[16];
@@ -963,11 +952,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
 #pragma unroll
           for (int h = 0; h < 4; h += 2) {
             const int at = c + e + h;
-            float2 f = mul2(make_float2(p[at], p[at + 1]), add2(make_float2(d[at], d[at + 1]), h ? make_float2(x.z, x.w) : make_float2(x.x, x.y)));
-            if (queries < AT_STEP) {   // (behind the sequence dP may be anything: no factor of zero does)
-              if (at < from || at >= to) f.x = 0.f;
-              if (at + 1 < from || at + 1 >= to) f.y = 0.f;
-            }
+            const float2 f = mul2(make_float2(p[at], p[at + 1]), add2(make_float2(d[at], d[at + 1]), h ? make_float2(x.z, x.w) : make_float2(x.x, x.y)));
             w[(e + h) / 2] = pack2<T>(f.x, f.y);
           }
         }

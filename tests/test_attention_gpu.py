@@ -108,6 +108,17 @@ def test_large_scores(dtype):
     _check((q + ramp.flip(0)).to(dtype), k, v, g, _offsets([700]))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("size", [64, 128])
+def test_scores_far_below_zero(size, causal):
+    """Weights relative to a row's own sum would be infinite for a score of zero, which a key that does not exist has."""
+    for lengths in ([70, 200], [129, 1, 300]):
+        q, k, v, g = _inputs(sum(lengths), 2, 1, size, torch.bfloat16, scale=0.25)
+        q[..., 0] = 32.0
+        k[..., 0] = -32.0
+        _check(q, k, v, g, _offsets(lengths), causal=causal, scale=0.5)
+
+
 def test_views_of_one_projection():
     lengths = [200, 31, 150]
     qkv = torch.randn(sum(lengths), 3, 4, 64, device="cuda").bfloat16()
