@@ -556,6 +556,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
 
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
   const int head = blockIdx.x % a.heads, index = blockIdx.x / a.heads;
+  psgd_launch_dependents();      // (the pass over the keys begins beside the end of this one)
   if (warp == 0) {
     AtPiece piece = {0, 0, 0, 0, 0};
     const bool found = at_find(a, AT_TILE, index, false, piece);
@@ -787,6 +788,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
     at_clear_outside<T>(a, s_piece, (T*)a.dv, kv_heads, head, index);
   }
   if (!s_found) {   // (so for all blocks of the cluster)
+    psgd_wait_for_predecessor();
     if (warp == ISSUER) tmem_free(s_tmem, COLUMNS);
     return;
   }
@@ -825,6 +827,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
         at_load_tile<PANELS, AT_STEP>(at, &a.q, step.head, start + step.row, &bars.full[slot]);
         at_load_tile<PANELS, AT_STEP>(at + HALF, &a.g, step.head, start + step.row, &bars.full[slot]);
       }
+      psgd_wait_for_predecessor();
     }
   } else if (warp == ISSUER) {
     const int k_steps = (a.size + 15) / 16;
@@ -878,9 +881,11 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       if (i + CHAINS < steps) slopes(i + CHAINS);
       if (i == steps - 1) umma_arrive(&bars.done);
     }
+    psgd_wait_for_predecessor();
   } else {
     const int chain = warp >> 2, row = tid & 127, key = k0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + chain * 128, dp_at = s_at + AT_STEP;
+    psgd_wait_for_predecessor();   // delta is complete
     const float* statistics = (row < AT_STEP ? a.lse : a.delta) + start + row % AT_STEP;
     auto statistic = [&](const Step& at) {   // of query row % 64 of a step, negative: logarithm of the sum, or delta
       return at.row + row % AT_STEP < length ? -statistics[(long long)at.head * a.tokens + at.row] : 0.f;
@@ -1110,7 +1115,7 @@ int at_backward(AtArgs a, cudaStream_t stream) {
   for (int split = 2; split <= AB_MOST_SPLIT && split <= a.group && (long long)a.blocks * kv_heads * a.split < AB_ENOUGH; ++split)
     if (a.group % split == 0) a.split = split;
   if ((long long)a.blocks * kv_heads * a.split > 0x7fffffffll) a.split = 1;
-  return psgd_launch_clusters(psgd_attention_dkv_kernel<T, PANELS>, a.blocks * kv_heads * a.split, ab_threads(PANELS), ab_shared(PANELS), stream, 0,
+  return psgd_launch_clusters(psgd_attention_dkv_kernel<T, PANELS>, a.blocks * kv_heads * a.split, ab_threads(PANELS), ab_shared(PANELS), stream, 1,
                               a.split, a);
 }
 
