@@ -43,6 +43,7 @@ constexpr float AT_LOG2E = 1.44269504088896341f;
 struct AtArgs {
   CUtensorMap q, k, v, g;        // boxes of 64 elements x 1 head x 64 rows; g: the gradient of the output
   const int* offsets;
+  const int* plan;               // where there are more sequences than a warp has lanes: see below; else null
   int sequences, tokens, heads, group, size;   // group: query heads per key head
   int causal;
   float scale, scale2;           // scale, scale log2(e)
@@ -98,50 +99,98 @@ struct AtPiece {
 __device__ __forceinline__ int at_bound(const int* offsets, int s, int tokens) { return min(max(offsets[s], 0), tokens); }
 __device__ bool at_find(const AtArgs& a, int rows, int index, bool from_end, AtPiece& out) {
   const int lane = threadIdx.x & 31;
-  auto pieces = [&](int s, int& begin, int& length) {
-    begin = length = 0;
-    if (s >= a.sequences) return 0;
-    begin = at_bound(a.offsets, s, a.tokens);
-    length = max(at_bound(a.offsets, s + 1, a.tokens) - begin, 0);
-    return (length + rows - 1) / rows;
-  };
-  int begin, length, b, l;       // of the sequence that this lane has (of the first 32)
-  const int mine = pieces(lane, begin, length);
+  if (a.plan != nullptr) {       // the order has been written down: how many there are, then start, length and level of each
+    out.before = at_bound(a.offsets, 0, a.tokens);
+    out.behind = max(at_bound(a.offsets, a.sequences, a.tokens), out.before);
+    if (index >= a.plan[0]) return false;
+    const int* x = a.plan + 1 + 3 * index;
+    out.start = x[0];
+    out.length = x[1];
+    out.piece = from_end ? (out.length + rows - 1) / rows - 1 - x[2] : x[2];
+    return true;
+  }
+  int begin = 0, length = 0;     // of the sequence that this lane has
+  if (lane < a.sequences) {
+    begin = at_bound(a.offsets, lane, a.tokens);
+    length = max(at_bound(a.offsets, lane + 1, a.tokens) - begin, 0);
+  }
+  const int mine = (length + rows - 1) / rows;
   out.before = at_bound(a.offsets, 0, a.tokens);
   out.behind = max(at_bound(a.offsets, a.sequences, a.tokens), out.before);
   // pieces at level `level` of their sequences or above
-  auto above = [&](int level) {
-    int n = max(mine - level, 0);
-    for (int s = lane + 32; s < a.sequences; s += 32) n += max(pieces(s, b, l) - level, 0);
-    return (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
-  };
-  int most = mine;
-  for (int s = lane + 32; s < a.sequences; s += 32) most = max(most, pieces(s, b, l));
-  most = (int)__reduce_max_sync(0xffffffffu, (unsigned)most);
+  auto above = [&](int level) { return (int)__reduce_add_sync(0xffffffffu, (unsigned)max(mine - level, 0)); };
   if (index >= above(0)) return false;
-  int lo = 0, hi = most;         // above(lo) > index >= above(hi)
+  int lo = 0, hi = (int)__reduce_max_sync(0xffffffffu, (unsigned)mine);         // above(lo) > index >= above(hi)
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (above(mid) > index) lo = mid;
     else hi = mid;
   }
-  int left = index - above(lo + 1);   // the left-th sequence with more than `lo` pieces
-  for (int s0 = 0; s0 < a.sequences; s0 += 32) {
-    const int count = s0 ? pieces(s0 + lane, begin, length) : mine;
-    const bool has = count > lo;
-    const unsigned votes = __ballot_sync(0xffffffffu, has);
-    const int n = __popc(votes);
-    if (left >= n) {
-      left -= n;
-      continue;
-    }
-    const int from = __fns(votes, 0, left + 1);
-    out.start = __shfl_sync(0xffffffffu, begin, from);
-    out.length = __shfl_sync(0xffffffffu, length, from);
-    out.piece = from_end ? __shfl_sync(0xffffffffu, count, from) - 1 - lo : lo;
-    return true;
+  // the sequence that has more than `lo` pieces as the index says
+  const int from = __fns(__ballot_sync(0xffffffffu, mine > lo), 0, index - above(lo + 1) + 1);
+  out.start = __shfl_sync(0xffffffffu, begin, from);
+  out.length = __shfl_sync(0xffffffffu, length, from);
+  out.piece = from_end ? __shfl_sync(0xffffffffu, mine, from) - 1 - lo : lo;
+  return true;
+}
+
+// The same order written down, for more sequences than 32: block `level` has the pieces of that level. Their places follow those of all higher levels,
+// in the order of their sequences. (A block that asked for itself as above, in turns of 32 sequences, would read all offsets again for every
+// question: with thousands of sequences that is more than its work.)
+constexpr int AT_PLAN_THREADS = 256;
+__global__ void __launch_bounds__(AT_PLAN_THREADS) psgd_attention_plan_kernel(const int* offsets, int sequences, int tokens, int rows, int capacity, int* plan) {
+  __shared__ int s_sum[AT_PLAN_THREADS / 32];
+  const int level = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  auto sum = [&](int x) {        // over the block
+    x = (int)__reduce_add_sync(0xffffffffu, (unsigned)x);
+    __syncthreads();
+    if (lane == 0) s_sum[warp] = x;
+    __syncthreads();
+    int all = 0;
+    for (int w = 0; w < AT_PLAN_THREADS / 32; ++w) all += s_sum[w];
+    return all;
+  };
+  int higher = 0, here = 0, total = 0;
+  for (int s = threadIdx.x; s < sequences; s += AT_PLAN_THREADS) {
+    const int n = (max(at_bound(offsets, s + 1, tokens) - at_bound(offsets, s, tokens), 0) + rows - 1) / rows;
+    higher += max(n - level - 1, 0);
+    here += n > level;
+    total += n;
   }
-  return false;
+  higher = sum(higher);
+  here = sum(here);
+  if (level == 0) {
+    total = sum(total);
+    if (threadIdx.x == 0) plan[0] = min(total, capacity);
+  }
+  if (here == 0) return;
+  int at = higher;
+  for (int s0 = 0; s0 < sequences; s0 += AT_PLAN_THREADS) {
+    const int s = s0 + threadIdx.x;
+    int begin = 0, length = 0;
+    if (s < sequences) {
+      begin = at_bound(offsets, s, tokens);
+      length = max(at_bound(offsets, s + 1, tokens) - begin, 0);
+    }
+    const bool has = (length + rows - 1) / rows > level;
+    const unsigned votes = __ballot_sync(0xffffffffu, has);
+    __syncthreads();
+    if (lane == 0) s_sum[warp] = __popc(votes);
+    __syncthreads();
+    int before = __popc(votes & ((1u << lane) - 1)), all = 0;
+    for (int w = 0; w < AT_PLAN_THREADS / 32; ++w) {
+      before += w < warp ? s_sum[w] : 0;
+      all += s_sum[w];
+    }
+    const int place = at + before;
+    if (has && place < capacity) {
+      int* x = plan + 1 + 3 * place;
+      x[0] = begin;
+      x[1] = length;
+      x[2] = level;
+    }
+    at += all;
+  }
 }
 
 // Rows of a result that belong to no sequence: zeros. Dealt out over the blocks of a head.
@@ -1062,6 +1111,9 @@ int at_encode(CUtensorMap* map, const void* at, int type, int tokens, int heads,
   return 0;
 }
 
+// Pieces of `rows` that the tokens of one head can make: each sequence may leave one unfilled.
+long long at_most_pieces(int sequences, int tokens, int rows) { return (long long)tokens / rows + (sequences < tokens ? sequences : tokens); }
+
 int at_fill(AtArgs& a, const void* q, const void* k, const void* v, const long long* strides, const int* offsets, int sequences, int tokens, int heads,
             int kv_heads, int size, int type, int causal, float scale, int rows, int grid_heads, int* status) {
   if (sequences < 1 || tokens < 1 || kv_heads < 1 || heads % kv_heads != 0 || size < 8 || size > 128 || size % 8 != 0) {
@@ -1086,7 +1138,7 @@ int at_fill(AtArgs& a, const void* q, const void* k, const void* v, const long l
   a.causal = causal;
   a.scale = scale;
   a.scale2 = scale * AT_LOG2E;
-  const long long blocks = (long long)tokens / rows + (sequences < tokens ? sequences : tokens);   // each sequence may leave one piece unfilled
+  const long long blocks = at_most_pieces(sequences, tokens, rows);
   if (blocks * grid_heads > 0x7fffffffll) {
     psgd_set_error("packed attention: %lld tiles of %d heads are more than a grid holds", blocks, grid_heads);
     return -1;
@@ -1094,6 +1146,17 @@ int at_fill(AtArgs& a, const void* q, const void* k, const void* v, const long l
   a.blocks = (int)blocks;
   a.status = status;
   return 0;
+}
+
+// Writes the order down where a warp cannot find it by itself. `plan`: psgd_attention_plan_ints of memory.
+int at_plan(AtArgs& a, int rows, int* plan, cudaStream_t stream) {
+  if (a.sequences <= 32) return 0;
+  if (plan == nullptr) {
+    psgd_set_error("packed attention: %d sequences need a plan", a.sequences);
+    return -1;
+  }
+  a.plan = plan;
+  return psgd_launch(psgd_attention_plan_kernel, a.tokens / rows + 1, AT_PLAN_THREADS, 0, stream, 0, a.offsets, a.sequences, a.tokens, rows, a.blocks, plan);
 }
 
 template <typename T, int PANELS>
@@ -1121,15 +1184,20 @@ int at_backward(AtArgs a, cudaStream_t stream) {
 
 }  // namespace
 
+// Ints of scratch that a call needs as `plan`; with 0 it may be null.
+PSGD_API long long psgd_attention_plan_ints(int sequences, int tokens) { return sequences <= 32 ? 0 : 1 + 3 * at_most_pieces(sequences, tokens, AT_TILE); }
+
 // dtype: 1 bfloat16, 2 float16. strides: rows and heads of q, k and v, in elements, multiples of 8; addresses on 16-byte boundaries. `out` is
 // [tokens, heads, size], contiguous, `rest` (what rounding takes from it: the backward pass wants it) likewise or null, lse [heads, tokens]. Rows of `out` outside the sequences become zeros.
 PSGD_API int psgd_attention(const void* q, const void* k, const void* v, const long long* strides, const int* offsets, int sequences, int tokens, int heads,
-                            int kv_heads, int size, int dtype, int causal, float scale, void* out, void* rest, float* lse, int* status, cudaStream_t stream) {
+                            int kv_heads, int size, int dtype, int causal, float scale, void* out, void* rest, float* lse, int* plan, int* status,
+                            cudaStream_t stream) {
   AtArgs a;
   if (at_fill(a, q, k, v, strides, offsets, sequences, tokens, heads, kv_heads, size, dtype, causal, scale, at_tiles(size) * AT_TILE, heads, status)) return -1;
   a.out = out;
   a.rest = rest;
   a.lse = lse;
+  if (const int code = at_plan(a, at_tiles(size) * AT_TILE, plan, stream)) return code;
   if (dtype == 1) return size <= 64 ? at_forward<__nv_bfloat16, 1>(a, stream) : at_forward<__nv_bfloat16, 2>(a, stream);
   return size <= 64 ? at_forward<__half, 1>(a, stream) : at_forward<__half, 2>(a, stream);
 }
@@ -1137,7 +1205,7 @@ PSGD_API int psgd_attention(const void* q, const void* k, const void* v, const l
 // strides: those of q, k, v and of the output's gradient. delta: scratch, [heads, tokens]. dq, dk, dv are contiguous.
 PSGD_API int psgd_attention_backward(const void* q, const void* k, const void* v, const void* grad, const long long* strides, const int* offsets, int sequences,
                                      int tokens, int heads, int kv_heads, int size, int dtype, int causal, float scale, const void* out, const void* rest, const float* lse,
-                                     float* delta, void* dq, void* dk, void* dv, int* status, cudaStream_t stream) {
+                                     float* delta, void* dq, void* dk, void* dv, int* plan, int* status, cudaStream_t stream) {
   AtArgs a;
   if (at_fill(a, q, k, v, strides, offsets, sequences, tokens, heads, kv_heads, size, dtype, causal, scale, AT_TILE, heads, status)) return -1;
   if (at_encode(&a.g, grad, dtype, tokens, heads, size, strides[6], strides[7])) return -1;
@@ -1151,6 +1219,7 @@ PSGD_API int psgd_attention_backward(const void* q, const void* k, const void* v
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;
+  if (const int code = at_plan(a, AT_TILE, plan, stream)) return code;
   if (dtype == 1) return size <= 64 ? at_backward<__nv_bfloat16, 1>(a, stream) : at_backward<__nv_bfloat16, 2>(a, stream);
   return size <= 64 ? at_backward<__half, 1>(a, stream) : at_backward<__half, 2>(a, stream);
 }

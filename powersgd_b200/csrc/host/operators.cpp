@@ -34,10 +34,11 @@ struct Entry {
   int (*token)(const void*, int, long long, int, long long, const void*, int, long long, float, int, float*, float*, float*, float*, long long*, void*) = nullptr;
   int (*token_grad)(const void*, int, long long, int, long long, void*, long long, const void*, int, long long, float, int, const float*, const float*,
                     const long long*, const float*, const float*, const float*, void*) = nullptr;
-  int (*attention)(const void*, const void*, const void*, const long long*, const int*, int, int, int, int, int, int, int, float, void*, void*, float*, int*,
+  int (*attention)(const void*, const void*, const void*, const long long*, const int*, int, int, int, int, int, int, int, float, void*, void*, float*, int*, int*,
                    void*) = nullptr;
+  long long (*attention_plan_ints)(int, int) = nullptr;
   int (*attention_backward)(const void*, const void*, const void*, const void*, const long long*, const int*, int, int, int, int, int, int, int, float,
-                            const void*, const void*, const float*, float*, void*, void*, void*, int*, void*) = nullptr;
+                            const void*, const void*, const float*, float*, void*, void*, void*, int*, int*, void*) = nullptr;
   int (*adamw)(const void*, int, int, int, double, const float*, double, double, double, double, double, double, unsigned, int*, void*) = nullptr;
 } entry;
 
@@ -217,7 +218,7 @@ PyObject* token_log_probs(PyObject*, PyObject* args) {
     const auto index = targets->scalar_type();
     if (!logits->is_cuda() || logits->device() != targets->device() || type_code(logits->scalar_type()) < 0 || (index != at::kLong && index != at::kInt) || vocab < 1 ||
         vocab >= (1ll << 31) - (1 << 16) || logits->sizes().slice(0, logits->dim() - 1) != targets->sizes() || top < 0 || top > 32 || top > vocab ||
-        !(std::isfinite(temperature) && temperature > 0))
+        !(temperature >= 0x1p-100 && temperature <= 0x1p100))
       Py_RETURN_NONE;
     Tensor out[4];
     if (at::GradMode::is_enabled() && logits->requires_grad()) {
@@ -257,6 +258,12 @@ int* status_of(const Tensor& t) {
   return s.device;
 }
 
+// Scratch for the order of the tiles, where there are many sequences.
+Tensor plan_of(int64_t sequences, int64_t tokens, const Tensor& like) {
+  const long long ints = entry.attention_plan_ints((int)sequences, (int)tokens);
+  return ints ? at::empty({ints}, like.options().dtype(at::kInt)) : Tensor();
+}
+
 struct Attended {
   Tensor out, lse, rest;
 };
@@ -271,14 +278,14 @@ Attended attention_forward(const Tensor& q0, const Tensor& k0, const Tensor& v0,
   }
   o.lse = at::empty({heads, tokens}, q0.options().dtype(at::kFloat));
   if (gradient) o.rest = at::empty({tokens, heads, size}, q0.options());
-  const Tensor q = usable(q0.detach()), k = usable(k0.detach()), v = usable(v0.detach()), offsets = offsets0.contiguous();
+  const Tensor q = usable(q0.detach()), k = usable(k0.detach()), v = usable(v0.detach()), offsets = offsets0.contiguous(), plan = plan_of(sequences, tokens, q);
   long long strides[6];
   strides_of(q, strides);
   strides_of(k, strides + 2);
   strides_of(v, strides + 4);
   check(entry.attention(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), strides, (const int*)offsets.const_data_ptr(), (int)sequences, (int)tokens, (int)heads,
                         (int)k.size(1), (int)size, type_code(q.scalar_type()), causal, (float)scale, o.out.data_ptr(), gradient ? o.rest.data_ptr() : nullptr,
-                        (float*)o.lse.data_ptr(), status_of(q), current_stream(q)),
+                        (float*)o.lse.data_ptr(), plan.defined() ? (int*)plan.data_ptr() : nullptr, status_of(q), current_stream(q)),
         "psgd_attention");
   return o;
 }
@@ -305,7 +312,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
         dq.zero_(), dk.zero_(), dv.zero_();
       } else {
         const Tensor q = usable(saved[0].detach()), k = usable(saved[1].detach()), v = usable(saved[2].detach()), offsets = saved[3].contiguous();
-        const Tensor g = usable(grads[0].to(out.scalar_type())), delta = at::empty({heads, tokens}, lse.options());
+        const Tensor plan = plan_of(offsets.size(0) - 1, tokens, q), g = usable(grads[0].to(out.scalar_type())), delta = at::empty({heads, tokens}, lse.options());
         long long strides[8];
         strides_of(q, strides);
         strides_of(k, strides + 2);
@@ -314,7 +321,8 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
         check(entry.attention_backward(q.const_data_ptr(), k.const_data_ptr(), v.const_data_ptr(), g.const_data_ptr(), strides, (const int*)offsets.const_data_ptr(),
                                        (int)(offsets.size(0) - 1), (int)tokens, (int)heads, (int)groups, (int)size, type_code(out.scalar_type()),
                                        ctx->saved_data["causal"].toBool(), (float)ctx->saved_data["scale"].toDouble(), out.const_data_ptr(), rest.const_data_ptr(),
-                                       (const float*)lse.const_data_ptr(), (float*)delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), status_of(q),
+                                       (const float*)lse.const_data_ptr(), (float*)delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                       plan.defined() ? (int*)plan.data_ptr() : nullptr, status_of(q),
                                        current_stream(q)),
               "psgd_attention_backward");
       }
@@ -375,16 +383,17 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
 }
 
 // ---- what Python hands over ---------------------------------------------------------------------
-// bind(error, token, token_grad, attention, attention_backward, adamw): addresses of the native library's entry points.
+// bind(error, token, token_grad, attention, attention_backward, adamw, attention_plan_ints): addresses of the native library's entry points.
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[6];
-  if (!PyArg_ParseTuple(args, "KKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5)) return nullptr;
+  unsigned long long a[7];
+  if (!PyArg_ParseTuple(args, "KKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6)) return nullptr;
   entry.error = (decltype(entry.error))a[0];
   entry.token = (decltype(entry.token))a[1];
   entry.token_grad = (decltype(entry.token_grad))a[2];
   entry.attention = (decltype(entry.attention))a[3];
   entry.attention_backward = (decltype(entry.attention_backward))a[4];
   entry.adamw = (decltype(entry.adamw))a[5];
+  entry.attention_plan_ints = (decltype(entry.attention_plan_ints))a[6];
   Py_RETURN_NONE;
 }
 // status(device, host address, device address): the status word of a device.
@@ -414,7 +423,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods,
 PyMODINIT_FUNC PyInit__operators() {
   PyObject* m = PyModule_Create(&module);
   // what this was compiled for, which the loader compares (csrc/build.py, scan_target)
-  if (m != nullptr && (PyModule_AddStringConstant(m, "target", PSGD_SCAN_TARGET) != 0 || PyModule_AddIntConstant(m, "entry_points", 6) != 0)) {
+  if (m != nullptr && (PyModule_AddStringConstant(m, "target", PSGD_SCAN_TARGET) != 0 || PyModule_AddIntConstant(m, "entry_points", 7) != 0)) {
     Py_DECREF(m);
     return nullptr;
   }

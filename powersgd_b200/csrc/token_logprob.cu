@@ -159,7 +159,7 @@ __device__ __forceinline__ LpSum lp_join(const LpSum& x, const LpSum& y, float k
 // A key orders by value, then by the lower index: the bits of the number as an unsigned integer in the order of the numbers, and
 // the complement of the index.
 __device__ __forceinline__ uint32_t lp_order(float v) {
-  const uint32_t b = __float_as_uint(v);
+  const uint32_t b = __float_as_uint(v + 0.f);   // (the two zeros are equal)
   return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
 }
 __device__ __forceinline__ float lp_value(uint32_t order) {

@@ -77,8 +77,9 @@ f64 = C.c_double
 _OPTIONAL = {
     "psgd_adamw_item_bytes": (i32, []),
     "psgd_adamw_step": (i32, [C.c_char_p, i32, i32, i32, f64, vp, f64, f64, f64, f64, f64, f64, C.c_uint, vp, vp]),
-    "psgd_attention": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp]),
-    "psgd_attention_backward": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
+    "psgd_attention_plan_ints": (i64, [i32, i32]),
+    "psgd_attention": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp]),
+    "psgd_attention_backward": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
     "psgd_token_logprob_max_top": (i32, []),
     "psgd_token_logprob": (i32, [vp, i32, i64, i32, i64, vp, i32, i64, f32, i32, vp, vp, vp, vp, vp, vp]),
     "psgd_token_logprob_grad": (i32, [vp, i32, i64, i32, i64, vp, i64, vp, i32, i64, f32, i32, vp, vp, vp, vp, vp, vp, vp]),

@@ -107,6 +107,12 @@ def _strides(*tensors) -> ctypes.Array:
     return (ctypes.c_longlong * len(out))(*out)
 
 
+def _plan(sequences: int, tokens: int, device: torch.device) -> Optional[torch.Tensor]:
+    """Scratch for the order of the tiles, where there are many sequences."""
+    ints = native.lib().psgd_attention_plan_ints(sequences, tokens)
+    return torch.empty(ints, dtype=torch.int32, device=device) if ints else None
+
+
 def _forward(q, k, v, offsets, causal, scale, gradient: bool):
     """The output, and for a backward pass the logarithms of the sums and what rounding took from the output."""
     if not _native(q):
@@ -118,11 +124,12 @@ def _forward(q, k, v, offsets, causal, scale, gradient: bool):
         return out.zero_(), None, None
     lse = torch.empty((heads, tokens), dtype=torch.float32, device=q.device)
     rest = torch.empty_like(out) if gradient else None
-    q, k, v, offsets = _usable(q), _usable(k), _usable(v), offsets.contiguous()
+    q, k, v, offsets, plan = _usable(q), _usable(k), _usable(v), offsets.contiguous(), _plan(sequences, tokens, q.device)
     with native.on_device(q.device) as stream:
         code = native.lib().psgd_attention(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), _strides(q, k, v), offsets.data_ptr(), sequences, tokens, heads, k.shape[1], size, DTYPES[q.dtype],
-            causal, scale, out.data_ptr(), rest.data_ptr() if gradient else None, lse.data_ptr(), _status(q.device), stream,
+            causal, scale, out.data_ptr(), rest.data_ptr() if gradient else None, lse.data_ptr(), None if plan is None else plan.data_ptr(),
+            _status(q.device), stream,
         )
     native.check(code, "psgd_attention")
     return out, lse, rest
@@ -139,12 +146,12 @@ def _backward(q, k, v, offsets, out, lse, rest, grad, causal, scale):
     if tokens == 0 or sequences == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
     delta = torch.empty((heads, tokens), dtype=torch.float32, device=q.device)
-    q, k, v, grad, offsets = _usable(q), _usable(k), _usable(v), _usable(grad), offsets.contiguous()
+    q, k, v, grad, offsets, plan = _usable(q), _usable(k), _usable(v), _usable(grad), offsets.contiguous(), _plan(sequences, tokens, q.device)
     with native.on_device(q.device) as stream:
         code = native.lib().psgd_attention_backward(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), grad.data_ptr(), _strides(q, k, v, grad), offsets.data_ptr(), sequences, tokens, heads, groups, size,
             DTYPES[q.dtype], causal, scale, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-            _status(q.device), stream,
+            None if plan is None else plan.data_ptr(), _status(q.device), stream,
         )
     native.check(code, "psgd_attention_backward")
     return dq, dk, dv

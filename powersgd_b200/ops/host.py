@@ -8,7 +8,8 @@ import os
 from ..csrc.build import operators_lib, scan_target
 from . import native
 
-ENTRY_POINTS = ("psgd_last_error", "psgd_token_logprob", "psgd_token_logprob_grad", "psgd_attention", "psgd_attention_backward", "psgd_adamw_step")
+ENTRY_POINTS = ("psgd_last_error", "psgd_token_logprob", "psgd_token_logprob_grad", "psgd_attention", "psgd_attention_backward", "psgd_adamw_step",
+                "psgd_attention_plan_ints")
 
 
 def _load():

@@ -60,8 +60,8 @@ def check(logits, targets, top, ignore_index, temperature) -> None:
         raise ValueError(f"token_log_probs: logits on {logits.device}, targets on {targets.device}")
     if not 0 <= top <= min(MOST_TOP, vocab):
         raise ValueError(f"token_log_probs: top = {top}; 0 to {min(MOST_TOP, vocab)} for a vocabulary of {vocab}")
-    if not (math.isfinite(temperature) and temperature > 0):
-        raise ValueError(f"token_log_probs: temperature {temperature}")
+    if not 2.0**-100 <= temperature <= 2.0**100:
+        raise ValueError(f"token_log_probs: temperature {temperature}; 2^-100 to 2^100")
     if not -(2**63) <= ignore_index < 2**63:
         raise ValueError(f"token_log_probs: ignore_index {ignore_index}")
 

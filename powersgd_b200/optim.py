@@ -168,8 +168,11 @@ class AdamW(torch.optim.Optimizer):
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         for i, p in zip(saved, params_in_optimizer(self)):
             for name, value in state_dict["state"].get(i, {}).items():
-                if isinstance(value, torch.Tensor):
-                    self.state[p][name] = value.to(p.device, copy=True)
+                if name == "step":      # (a number in old states)
+                    self.state[p][name] = torch.as_tensor(value, dtype=torch.float32).detach().reshape(()).to(p.device, copy=True)
+                elif isinstance(value, torch.Tensor):   # (torch.optim has moments of the parameter's type)
+                    dtype = torch.float32 if name in ("exp_avg", "exp_avg_sq") and value.dtype in (torch.bfloat16, torch.float16) else value.dtype
+                    self.state[p][name] = value.to(p.device, dtype, copy=True)
         for group in self.param_groups:
             if group.get("amsgrad") or group.get("maximize"):
                 raise ValueError("AdamW: a state of torch.optim.AdamW with amsgrad or maximize does not carry over")

@@ -89,6 +89,20 @@ def test_checkpoint_continues_the_run(bits, dtype):
     assert c.state_dict()["param_groups"] == b.state_dict()["param_groups"]
 
 
+def test_states_of_torch_in_other_types():
+    ours, theirs = _params((7, 9), dtype=torch.bfloat16), _params((7, 9), dtype=torch.bfloat16)
+    a, b = AdamW(ours, lr=1e-2), torch.optim.AdamW(theirs, lr=1e-2)
+    _grads(theirs, 0)
+    b.step()
+    state = copy.deepcopy(b.state_dict())
+    assert state["state"][0]["exp_avg"].dtype == torch.bfloat16
+    state["state"][0]["step"] = 1
+    a.load_state_dict(state)
+    _grads(ours, 1)
+    a.step()
+    assert a.state[ours[0]]["exp_avg"].dtype == torch.float32 and a.state[ours[0]]["step"] == 2
+
+
 def test_parameters_without_gradient_and_other_layouts():
     params = _params((6, 4), (8,), (3, 5, 2, 2))
     params[2].data = params[2].data.contiguous(memory_format=torch.channels_last)

@@ -100,6 +100,21 @@ def test_long_and_many(causal, size):
         _check(q, k, v, g, _offsets(lengths), causal=causal, scale=0.2)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("size", [32, 128])
+def test_more_sequences_than_lanes(size, causal):
+    """Their order is written down first."""
+    gen = torch.Generator().manual_seed(5)
+    for lengths in ([1] * 33, [0] * 40 + [129] + [5] * 20, torch.randint(0, 400, (70,), generator=gen).tolist(), torch.randint(0, 6, (900,), generator=gen).tolist()):
+        q, k, v, g = _inputs(sum(lengths) + 3, 2, 1, size, torch.bfloat16, seed=4)
+        got = _check(q, k, v, g, _offsets(lengths), causal=causal)
+        assert all((x[sum(lengths):] == 0).all() for x in got)
+    q, k, v, _ = _inputs(300, 2, 1, size, torch.bfloat16)
+    bad = torch.tensor([0, 250, 20, 300] * 20, device="cuda", dtype=torch.int32)     # overlapping: not defined, but inside
+    packed_attention(q, k, v, bad)
+    torch.cuda.synchronize()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_large_scores(dtype):
     q, k, v, g = _inputs(700, 2, 1, 64, dtype, scale=0.5)

@@ -66,7 +66,7 @@ def test_nothing_to_do():
 
 @pytest.mark.parametrize("change, error", [
     (dict(logits=torch.zeros(3, 8, dtype=torch.int32)), TypeError), (dict(targets=torch.zeros(3)), TypeError), (dict(targets=torch.zeros(4, dtype=torch.int64)), ValueError),
-    (dict(top=9), ValueError), (dict(top=-1), ValueError), (dict(temperature=0.0), ValueError), (dict(temperature=math.inf), ValueError),
+    (dict(top=9), ValueError), (dict(top=-1), ValueError), (dict(temperature=0.0), ValueError), (dict(temperature=math.inf), ValueError), (dict(temperature=1e-40), ValueError),
     (dict(logits=torch.zeros(3, 0)), ValueError), (dict(logits=torch.zeros(3, 64), top=33), ValueError), (dict(ignore_index=2**63), ValueError),
 ])
 def test_refusals(change, error):

@@ -163,6 +163,14 @@ def test_orders_of_the_largest(kind, rows, vocab):
         _check(z.to("cuda", dtype).expand(rows, vocab).contiguous(), torch.full((rows,), vocab // 2, device="cuda"), top=32, entropy=True, gradients=("top",))
 
 
+def test_zeros_of_both_signs_are_equal():
+    for rows, vocab in ((1, 40), (3, 5000)):
+        z = torch.zeros(rows, vocab, device="cuda")
+        z[:, ::2] = -0.0
+        r = token_log_probs(z, torch.zeros(rows, dtype=torch.int64, device="cuda"), top=5)
+        assert (r.top_tokens == torch.arange(5, device="cuda")).all()
+
+
 def test_streams_and_graphs():
     gen = torch.Generator(device="cuda").manual_seed(1)
     z = torch.randn(64, 5003, generator=gen, device="cuda", requires_grad=True)
