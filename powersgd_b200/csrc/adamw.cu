@@ -5,7 +5,8 @@
 //
 // in float32 whatever the type of p and g; p is rounded to its type once. A step moves 28 bytes per float32
 // parameter (p, m, v in and out, g in), 16.1 with moments in 8 bits, and computes some tens of operations: the
-// memory bounds it. A block takes 4096 elements of one tensor, found by a search in the list that the launch
+// memory bounds it in 32 bits (355 M float32 parameters 1455 us, 6.8 TB/s; 31.8 M 138 us) and the instructions of the rounding in 8
+// (1160 us, 4.9 TB/s; bfloat16 parameters take as long). A block takes 4096 elements of one tensor, found by a search in the list that the launch
 // carries in its own arguments: nothing is uploaded, and a recorded launch keeps its list.
 //
 // The number of steps of a tensor, t, lives in device memory, so that a replayed graph counts on. Every block reads

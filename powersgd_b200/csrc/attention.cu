@@ -21,6 +21,10 @@
 // A row of a tile that belongs to another sequence, or lies behind the last one, may hold anything: before it is multiplied with anything
 // but scores that are replaced, its row in shared memory is cleared.
 //
+// Heads of 64, four sequences of 4096: 690 TFLOP/s forward, 560 to 600 backward (counted as five products); heads of 128 1080 and 630; GPT-2
+// medium's step over documents of 24 to 1024, 49 GFLOP, 39 + 112 us. Bound by the chains' latencies (see above), for long sequences of heads of 128 by the
+// tensor cores.
+//
 // Blocks are dealt out with the longest first: the device finds the n-th tile in the order of its distance from the
 // sequence's beginning (causal: of its work), from the offsets alone.
 //

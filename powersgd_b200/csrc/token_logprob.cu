@@ -12,6 +12,9 @@
 // The forward pass reads a row once: every thread keeps a running maximum, the sum of exponentials below it and
 // the sum of e d, and scales the two when the maximum moves. The gradient is computed elementwise from the row's
 // two statistics.
+//
+// What bounds it is HBM: 8192 x 50257 bfloat16 logits take 136 us forward (6.1 TB/s) and 247 us backward (6.7 TB/s, a read and a write),
+// 1920 x 33278 float32 ones 42 us (6.1 TB/s). One exponential per element is a third of what the special function units give in that time.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
