@@ -182,7 +182,8 @@ PyObject* step_fits(PyObject*, PyObject* args) {
   });
 }
 
-// adam_items(params, state, names, first_block): the list of an AdamW step (PsgdAdamTensor, csrc/adamw.cu), see ops/scan.py.
+// adam_items(params, state, names, first_block): the list of an AdamW step (PsgdAdamTensor, csrc/adamw.cu), see ops/scan.py. A list that is
+// answered is going to be stepped: autograd is told that the parameters change.
 struct AdamItem {
   uint64_t p, g, m, v, m_scale, v_scale, step;
   int64_t n;
@@ -198,7 +199,9 @@ PyObject* adam_items(PyObject*, PyObject* args) {
     const bool narrow = keys.size() == 5;   // step, two moments, their scales
     if (!narrow && keys.size() != 3) Py_RETURN_NONE;
     std::vector<AdamItem> items;
+    std::vector<const at::Tensor*> stepped;
     items.reserve(params.size());
+    stepped.reserve(params.size());
     int device = -1;
     at::ScalarType type = at::kFloat;
     for (Py_ssize_t i = 0; i < params.size(); ++i) {
@@ -235,10 +238,13 @@ PyObject* adam_items(PyObject*, PyObject* args) {
         if (!fits) Py_RETURN_NONE;
       }
       auto at_of = [](const at::Tensor* x) { return x == nullptr ? (uint64_t)0 : (uint64_t)x->data_ptr(); };
+      stepped.push_back(p);
       items.push_back({at_of(p), (uint64_t)g.data_ptr(), at_of(t[1]), at_of(t[2]), at_of(t[3]), at_of(t[4]), at_of(t[0]), n, (uint32_t)block0, 0u});
     }
     const int code = type == at::kFloat ? 0 : type == at::kBFloat16 ? 1 : type == at::kHalf ? 2 : -1;
     if (code < 0) Py_RETURN_NONE;
+    for (const at::Tensor* p : stepped)   // (the step writes behind autograd's back)
+      if (!p->is_inference()) p->unsafeGetTensorImpl()->bump_version();
     return Py_BuildValue("(y#niiL)", reinterpret_cast<const char*>(items.data()), (Py_ssize_t)(items.size() * sizeof(AdamItem)),
                          (Py_ssize_t)items.size(), device, code, block);
   });

@@ -114,6 +114,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mo
             raise ValueError("adamw_step: a ticket is needed on CUDA")
         launch(items.tobytes(), len(params), device, DTYPES[params[0].dtype], bits=bits, lr=lr, beta1=beta1, beta2=beta2, eps=eps,
                weight_decay=weight_decay, seed=seed, ticket=ticket)
+        torch.autograd.graph.increment_version([p for p in params if not p.is_inference()])   # (torch operations do so themselves)
         return
     lr = float(lr)
     for i, p in enumerate(params):

@@ -93,5 +93,5 @@ def adam_items(params, state, names, first_block: int):
     """The list of an AdamW step (`adamw.ITEM`s as bytes) for the parameters that have a gradient, as `(items, count, device index,
     type, end)`; `names`: step and the moments as the state of a parameter has them; `end`: the block of random
     numbers behind the last parameter. None where anything is not as the kernel takes it, or has no state yet: the caller then asks
-    one by one."""
+    one by one. With a list, autograd knows the parameters to have changed."""
     return _native.adam_items(params, state, names, first_block) if _native is not None else None

@@ -260,3 +260,16 @@ def test_refusals():
     with pytest.raises(ValueError, match="ticket"):
         adamw.adamw_step([p], [p.grad], [[torch.zeros(8, device="cuda")], [torch.zeros(8, device="cuda")]], [torch.zeros((), device="cuda")], bits=32, lr=0.1,
                          beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_step_between_forward_and_backward_is_noticed(bits):
+    """The first step goes one by one through Python, the second by the list."""
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = AdamW([p], state_bits=bits)
+    for _ in range(2):
+        p.grad = torch.ones_like(p)
+        loss = p.square().sum()
+        opt.step()
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            loss.backward()
