@@ -119,7 +119,7 @@ class AdamW(torch.optim.Optimizer):
                 device = torch.device("cuda", device)
                 ticket = self._ticket(device)
                 if torch.cuda.is_current_stream_capturing():
-                    self._keep(group["params"], [self.state[p] for p in group["params"] if p.grad is not None], ticket)
+                    self._keep(group, group["params"], [self.state[p] for p in group["params"] if p.grad is not None], ticket)
                 beta1, beta2 = group["betas"]
                 _adamw.launch(items, count, device, dtype, bits=bits, lr=group["lr"], beta1=beta1, beta2=beta2, eps=group["eps"],
                               weight_decay=group["weight_decay"], seed=group["seed"], ticket=ticket)
@@ -142,7 +142,7 @@ class AdamW(torch.optim.Optimizer):
             if device.type == "cuda" and native.use_for_cuda():
                 ticket = self._ticket(device)
                 if torch.cuda.is_current_stream_capturing():
-                    self._keep(params, states, ticket)
+                    self._keep(group, params, states, ticket)
             missing = [name for name in ("step", *names) if any(name not in s for s in states)]
             if missing:
                 raise ValueError(f"AdamW: the state has no {missing[0]}; it belongs to moments of another number of bits than {bits}")
@@ -158,9 +158,9 @@ class AdamW(torch.optim.Optimizer):
                 ticket = self._tickets[device] = torch.zeros(1, dtype=torch.int32, device=device)
         return ticket
 
-    def _keep(self, params, states, ticket: torch.Tensor) -> None:
-        """What the graph that is being recorded refers to stays, whatever is loaded later."""
-        keep_with_graph(self._held, *params, *[t for s in states for t in s.values()], ticket)
+    def _keep(self, group: dict, params, states, ticket: torch.Tensor) -> None:
+        """What the graph that is being recorded refers to stays, whatever is loaded or set later."""
+        keep_with_graph(self._held, *params, *[t for s in states for t in s.values()], ticket, group["lr"])
 
     def load_state_dict(self, state_dict: dict) -> None:
         """As in `torch.optim`, except that moments and numbers of steps keep their own types."""

@@ -273,3 +273,18 @@ def test_a_step_between_forward_and_backward_is_noticed(bits):
         opt.step()
         with pytest.raises(RuntimeError, match="modified by an inplace"):
             loss.backward()
+
+
+def test_a_recorded_step_keeps_its_learning_rate():
+    """A group's learning rate is replaced by another one: the recorded step goes on with the tensor that it was recorded with."""
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = AdamW([p], lr=torch.tensor(LR, device="cuda"), weight_decay=0.0)
+    p.grad = torch.ones_like(p)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.param_groups[0]["lr"] = 0.5
+    others = [torch.full((), 7.0, device="cuda") for _ in range(64)]     # (would take the place of a tensor that is gone)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (p.detach() - (1 - LR)).abs().max() < 1e-6 and len(others) == 64   # first step: lr m / sqrt(v), both corrected; 1e-8 / |g| less
