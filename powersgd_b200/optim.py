@@ -48,8 +48,8 @@ class AdamW(torch.optim.Optimizer):
     scale per 256 elements (`ops/adamw.py`), rounded by random bits that follow from `seed` and the number of steps,
     so that a run can be repeated. A gradient that is infinite or no number spoils the moments of its 256 elements.
 
-    Parameters are float32, bfloat16 or float16 tensors that lie in one piece (any order of dimensions). The arithmetic
-    is float32. A step may be recorded in a CUDA graph: the number of steps is counted on the device; a learning rate
+    Parameters are float32, bfloat16 or float16 tensors that lie in one piece (any order of dimensions), each in memory of its own. The
+    arithmetic is float32. A step may be recorded in a CUDA graph: the number of steps is counted on the device; a learning rate
     that is to change between replays is given as a float32 tensor on the GPU. The optimizer outlives the graph.
     On the CPU the same step runs in torch operations.
     """
@@ -98,6 +98,16 @@ class AdamW(torch.optim.Optimizer):
         for i, p in enumerate(group["params"]):
             if p.dtype not in _adamw.DTYPES:
                 raise TypeError(f"AdamW: parameter {i} is {p.dtype}; float32, bfloat16 and float16 are supported")
+        # one launch steps all of a group at once: none may lie in another's memory
+        taken = {}
+        for i, p in enumerate(group["params"]):
+            if p.numel() and p.device.type in ("cpu", "cuda") and _adamw.in_one_piece(p):
+                taken.setdefault(p.device, []).append((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size(), i))
+        for pieces in taken.values():
+            pieces.sort()
+            for (_, end, i), (start, _, j) in zip(pieces, pieces[1:]):
+                if start < end:
+                    raise ValueError(f"AdamW: parameters {min(i, j)} and {max(i, j)} share memory")
 
     def step(self, closure=None):
         loss = None

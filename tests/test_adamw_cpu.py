@@ -159,3 +159,12 @@ def test_refused_tensors():
         q = torch.nn.Parameter(torch.zeros(4))
         with pytest.warns(UserWarning):
             AdamW([q, q])
+
+
+def test_parameters_in_the_same_memory_are_refused():
+    x = torch.zeros(4, 6)
+    for a, b in ((x, x), (x, x[1:3]), (x[2:], x[:3]), (x, x.view(6, 4))):
+        with pytest.raises(ValueError, match="0 and 1 share memory"):
+            AdamW([torch.nn.Parameter(a), torch.nn.Parameter(b)])
+    opt = AdamW([torch.nn.Parameter(x[:2]), torch.nn.Parameter(x[2:]), torch.nn.Parameter(x[:0]), torch.nn.Parameter(torch.zeros(4, 6))])
+    assert len(opt.param_groups) == 1
