@@ -93,7 +93,8 @@ class GPT2(nn.Module):
 
     def forward(self, tokens: torch.Tensor, offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Logits of [batch, time] tokens, or of [rows] tokens of packed documents (`offsets`: int32, see `packed_attention`; on the GPU
-        under bf16 or fp16 autocast). A document's positions begin at zero; rows that belong to no document give logits of no meaning."""
+        under bf16 or fp16 autocast). A document's positions begin at zero, and from n_positions on are the
+        last one (lengths are not known to the host, which could refuse them); rows that belong to no document give logits of no meaning."""
         if offsets is not None and self.cfg.dropout and self.training:
             raise ValueError("GPT2: packed documents are trained on without dropout")
         if tokens.dim() != (2 if offsets is None else 1):

@@ -288,3 +288,19 @@ def test_a_recorded_step_keeps_its_learning_rate():
     graph.replay()
     torch.cuda.synchronize()
     assert (p.detach() - (1 - LR)).abs().max() < 1e-6 and len(others) == 64   # first step: lr m / sqrt(v), both corrected; 1e-8 / |g| less
+
+
+def test_more_elements_than_thirty_two_bits_count():
+    """A tensor of more than 2^31 elements: its end is stepped as the same elements by themselves are."""
+    n, tail = 2**31 + 5000, 4096 + 904      # the tail begins a block of 256
+    whole = torch.nn.Parameter(torch.empty(n, device="cuda", dtype=torch.bfloat16).normal_())
+    part = torch.nn.Parameter(whole.detach()[-tail:].clone())
+    gradient = torch.empty(n, device="cuda", dtype=torch.bfloat16).normal_()
+    for p in (whole, part):
+        p.grad = gradient[-p.numel():].clone() if p is part else gradient
+        AdamW([p], lr=LR).step()
+    assert torch.equal(whole.detach()[-tail:], part.detach())
+    before = whole.detach()[:10].clone()
+    AdamW([whole], lr=LR, state_bits=8).step()
+    AdamW([part], lr=LR, state_bits=8).step()      # first step: the update uses the moments before they are rounded
+    assert torch.equal(whole.detach()[-tail:], part.detach()) and not torch.equal(before, whole.detach()[:10])

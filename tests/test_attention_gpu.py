@@ -227,3 +227,20 @@ def test_refusals():
     q, k, v, _ = _inputs(10, 2, 2, 64, torch.bfloat16)
     with pytest.raises(ValueError, match="tensors on"):
         packed_attention(q, k, v, _offsets([10]).cpu())
+
+
+@pytest.mark.parametrize("heads, size", [(16, 128), (32, 64)])
+def test_more_elements_than_thirty_two_bits_count(heads, size):
+    """Rows that begin behind 2^31 elements: the same as those rows by themselves."""
+    tokens = 2**20 + 5000
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, g = (torch.empty(tokens, heads, size, device="cuda", dtype=torch.bfloat16).normal_(generator=gen) for _ in range(2))
+    k, v = (torch.empty(tokens, heads, size, device="cuda", dtype=torch.bfloat16).normal_(generator=gen) for _ in range(2))
+    lengths = [128] * (2**13) + [3000, 2000]
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = packed_attention(*leaves, _offsets(lengths))
+    got = (out, *torch.autograd.grad(out, leaves, g))
+    last = [x.detach()[-5000:].clone().requires_grad_() for x in (q, k, v)]
+    want = packed_attention(*last, _offsets([3000, 2000]))
+    for a, b in zip(got, (want, *torch.autograd.grad(want, last, g[-5000:]))):
+        assert torch.equal(a.detach()[-5000:], b.detach())

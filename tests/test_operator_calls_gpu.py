@@ -138,3 +138,30 @@ def test_a_wait_that_ran_out_is_told(monkeypatch):
         with pytest.raises(RuntimeError, match="ran out"):
             attention.packed_attention(x, x, x, offsets)
         attention.packed_attention(x, x, x, offsets)
+
+
+def test_gradients_of_some(monkeypatch):
+    """Only some inputs want a gradient; one tensor is all three of them."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q, k, v = (torch.randn(200, 2, 64, generator=gen, device="cuda").bfloat16() for _ in range(3))
+    offsets = torch.tensor([0, 70, 200], device="cuda", dtype=torch.int32)
+
+    def call():
+        out = []
+        whole = [x.detach().requires_grad_() for x in (q, k, v)]
+        want = torch.autograd.grad(attention.packed_attention(*whole, offsets).float().square().sum(), whole)
+        for i in range(3):
+            given = [x.detach().requires_grad_() if i == j else x for j, x in enumerate((q, k, v))]
+            got, = torch.autograd.grad(attention.packed_attention(*given, offsets).float().square().sum(), given[i])
+            assert torch.equal(got, want[i])
+            out.append(got)
+        apart = [q.detach().requires_grad_() for _ in range(3)]
+        parts = torch.autograd.grad(attention.packed_attention(*apart, offsets).float().square().sum(), apart)
+        same = q.detach().requires_grad_()
+        got, = torch.autograd.grad(attention.packed_attention(same, same, same, offsets).float().square().sum(), same)
+        # sums of three, rounded at each addition, in any order: each rounding is half a step of a partial sum
+        size = sum(x.double().abs() for x in parts)
+        assert ((got.double() - sum(x.double() for x in parts)).abs() <= 2 * 2.0**-8 * size).all()
+        return out + [got]
+
+    _same(*_both(monkeypatch, attention, call))

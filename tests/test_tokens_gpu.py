@@ -198,3 +198,17 @@ def test_streams_and_graphs():
     got = [x.detach().clone() for x in got]
     assert not torch.equal(got[0], want[0])
     assert all(torch.equal(a, b) for a, b in zip([x.detach() for x in call()], got))   # (the same rows at the same addresses: the same order of sums)
+
+
+def test_more_elements_than_thirty_two_bits_count():
+    """Rows that begin behind 2^31 elements: the same as those rows by themselves."""
+    rows, vocab = 43000, 50257     # 2^31 = 42730.2 x 50257
+    z = torch.empty(rows, vocab, device="cuda", dtype=torch.bfloat16).normal_(generator=torch.Generator(device="cuda").manual_seed(0)).requires_grad_()
+    t = torch.arange(rows, device="cuda") % vocab
+    r = token_log_probs(z, t, top=3, entropy=True)
+    grad, = torch.autograd.grad(r.log_probs.sum() + r.entropy.sum(), z)
+    last = z.detach()[-300:].clone().requires_grad_()
+    want = token_log_probs(last, t[-300:], top=3, entropy=True)
+    for a, b in zip(r, want):
+        assert torch.equal(a[-300:], b)
+    assert torch.equal(grad[-300:], torch.autograd.grad(want.log_probs.sum() + want.entropy.sum(), last)[0])
