@@ -406,7 +406,7 @@ int aw_launch(const AwHyper& h, const PsgdAdamTensor* list, int count, int bits,
     }
     a.count = n;
     done += n;
-    if (chunks == 0) continue;
+    if (chunks == 0) chunks = 1;   // (tensors without elements make steps too: the one block counts them)
     const int grid = (int)(chunks < AW_PER_SM * 148 ? chunks : AW_PER_SM * 148);
     const int code = bits == 32 ? psgd_launch(psgd_adamw_kernel<T, MOST>, (int)chunks, AW_THREADS, 0, stream, 0, a)
                                 : psgd_launch(psgd_adamw8_kernel<T, MOST>, grid, AW_THREADS, 0, stream, 0, a);

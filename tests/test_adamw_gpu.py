@@ -304,3 +304,15 @@ def test_more_elements_than_thirty_two_bits_count():
     AdamW([whole], lr=LR, state_bits=8).step()
     AdamW([part], lr=LR, state_bits=8).step()      # first step: the update uses the moments before they are rounded
     assert torch.equal(whole.detach()[-tail:], part.detach()) and not torch.equal(before, whole.detach()[:10])
+
+
+@pytest.mark.parametrize("device", ["cuda", "cpu"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_without_elements_make_steps(bits, device):
+    params = [torch.nn.Parameter(torch.zeros(0, 4, device=device)) for _ in range(2)]
+    opt = AdamW(params, state_bits=bits)
+    for _ in range(3):
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        opt.step()
+    assert [float(opt.state[p]["step"]) for p in params] == [3, 3]
