@@ -209,6 +209,13 @@ def test_more_elements_than_thirty_two_bits_count():
     grad, = torch.autograd.grad(r.log_probs.sum() + r.entropy.sum(), z)
     last = z.detach()[-300:].clone().requires_grad_()
     want = token_log_probs(last, t[-300:], top=3, entropy=True)
-    for a, b in zip(r, want):
-        assert torch.equal(a[-300:], b)
-    assert torch.equal(grad[-300:], torch.autograd.grad(want.log_probs.sum() + want.entropy.sum(), last)[0])
+    # Not bit for bit: the 42700th row begins 8 bytes behind a 16-byte boundary and its copy on one, so that threads sum other elements.
+    # A sum of 197 terms in a thread and 8 levels above: 205 x 2^-24 of s, an exponential 2^-22 and its argument 16 x 2^-24 off: for two
+    # such sums 2 (205 + 4 + 16) 2^-24 < 2.7e-5; the rest of log p (of 14) 2^-20. In H what is off by 2.7e-5 has a weight of |d| <= 14.
+    # A gradient is p (< 2e-3) times what is off by less than both together, 5e-4, and is rounded once on either side.
+    off = 2.7e-5 + 2.0**-20
+    for a, b, atol in zip(r[:3], want[:3], (off, 15 * off, off)):
+        assert ((a[-300:] - b).abs() <= atol).all()
+    assert torch.equal(r.top_tokens[-300:], want.top_tokens)
+    expected = torch.autograd.grad(want.log_probs.sum() + want.entropy.sum(), last)[0].double()
+    assert ((grad[-300:].double() - expected).abs() <= 1e-6 + 2.0**-7 * expected.abs()).all()
