@@ -131,7 +131,8 @@ __device__ bool at_find(const AtArgs& a, int rows, int index, bool from_end, AtP
     else hi = mid;
   }
   // the sequence that has more than `lo` pieces as the index says
-  const int from = __fns(__ballot_sync(0xffffffffu, mine > lo), 0, index - above(lo + 1) + 1);
+  const unsigned deep = __ballot_sync(0xffffffffu, mine > lo);
+  const int nth = index - above(lo + 1), from = __ffs(__ballot_sync(0xffffffffu, mine > lo && __popc(deep & ((1u << lane) - 1)) == nth)) - 1;
   out.start = __shfl_sync(0xffffffffu, begin, from);
   out.length = __shfl_sync(0xffffffffu, length, from);
   out.piece = from_end ? __shfl_sync(0xffffffffu, mine, from) - 1 - lo : lo;
@@ -551,38 +552,42 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
 // ---- backward ----------------------------------------------------------------------------------
 constexpr int AB_MOST_SPLIT = 8;      // blocks of a cluster
 constexpr int AB_ENOUGH = 4 * 148;    // with so many blocks the heads of a group stay in one
-// CHAINS of four warps each take the steps in turn; then a warp that loads and one that issues the products. One chain where two blocks fit an SM,
-// two where one does.
-__host__ __device__ constexpr int ab_threads(int chains) { return 128 * chains + 64; }
+// CHAINS of eight warps each take the steps in turn; then a warp that loads and one that issues the products. One chain where two blocks fit an SM,
+// two where one does. Two threads share a row of a tile, AB_WIDE columns each.
+__host__ __device__ constexpr int ab_threads(int chains) { return 256 * chains + 64; }
+constexpr int AB_WIDE = AT_STEP / 2;
+constexpr int AB_GAP = AB_WIDE / 2;   // columns: each thread's 16-bit numbers take the first half of its own place
 // Tiles that pass come in pairs (K and V, or Q and dO).
 __host__ __device__ constexpr int ab_stages(int panels) { return panels == 1 ? 3 : 4; }
-__host__ __device__ constexpr size_t ab_shared(int panels) { return 1024 + (size_t)panels * (2 + ab_stages(panels)) * UMMA_PANEL; }
+constexpr int AB_ONES = 2 * AT_TILE * 16, AB_STATS = 2 * 2 * AT_STEP * 16;   // bytes: rows of 16 elements, see umma_add_columns
+// `more`: bytes besides the tiles.
+__host__ __device__ constexpr size_t ab_shared(int panels, int more) { return 1024 + (size_t)panels * (2 + ab_stages(panels)) * UMMA_PANEL + more; }
 
 template <int CHAINS, int STAGES>
 struct AbBars {
   uint64_t fixed, full[STAGES], empty[STAGES], s[CHAINS], dp[CHAINS], p[CHAINS], ds[CHAINS], done;
-  __device__ __forceinline__ void init() {
-    psgd_mbar_init(&fixed, 1);
+  __device__ __forceinline__ void init(int of_fixed, int of_full) {
+    psgd_mbar_init(&fixed, of_fixed);
     for (int i = 0; i < STAGES; ++i) {
-      psgd_mbar_init(&full[i], 1);
+      psgd_mbar_init(&full[i], of_full);
       psgd_mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < CHAINS; ++i) {
       psgd_mbar_init(&s[i], 1);
       psgd_mbar_init(&dp[i], 1);
-      psgd_mbar_init(&p[i], 4);
-      psgd_mbar_init(&ds[i], 4);
+      psgd_mbar_init(&p[i], 8);
+      psgd_mbar_init(&ds[i], 8);
     }
     psgd_mbar_init(&done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
 };
 
-// 64 exponentials 2^(scale2 s - at) of a row.
+// Exponentials 2^(scale2 s - at) of a row.
 __device__ __forceinline__ void ab_exponentials(float* s, float scale2, float at) {
   const float2 factor = make_float2(scale2, scale2), minus = make_float2(-at, -at);
 #pragma unroll
-  for (int c = 0; c < AT_STEP; c += 2) {
+  for (int c = 0; c < AB_WIDE; c += 2) {
     const float2 x = fma2(make_float2(s[c], s[c + 1]), factor, minus);
     s[c] = at_exp2(x.x);
     s[c + 1] = at_exp2(x.y);
@@ -595,7 +600,7 @@ template <typename T, int PANELS>
 __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention_dq_kernel(const __grid_constant__ AtArgs a) {
   constexpr int TILE_BYTES = PANELS * UMMA_PANEL, HALF = TILE_BYTES / 2, CHAINS = PANELS, STAGES = ab_stages(PANELS);
   constexpr int DQ = 2 * AT_STEP * CHAINS, COLUMNS = 256 * CHAINS;   // tensor memory; chain c has its scores at 128 c, slopes behind
-  constexpr int LOADER = 4 * CHAINS, ISSUER = LOADER + 1;
+  constexpr int LOADER = 8 * CHAINS, ISSUER = LOADER + 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = base;
@@ -620,7 +625,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
   }
   if (warp == LOADER && lane < 4) tma_prefetch_map(lane == 0 ? &a.q : lane == 1 ? &a.g : lane == 2 ? &a.k : &a.v);
   if (tid == 32) {
-    bars.init();
+    bars.init(1, 1);
     s_abort = 0;
   }
   if (warp == ISSUER) tmem_alloc(&s_tmem, COLUMNS);
@@ -697,90 +702,98 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       ok = ok && wait(&bars.ds[chain], parity);
       if (!ok) break;
       umma_fence_after();
-      umma_weights_by_rows<0, 4, AT_STEP>(tmem + DQ, tmem + chain * 128 + AT_STEP, ring_at + j % STAGES * TILE_BYTES, q_shape, j > 0);
+      umma_weights_by_rows<0, 4, AT_STEP, AB_GAP>(tmem + DQ, tmem + chain * 128 + AT_STEP, ring_at + j % STAGES * TILE_BYTES, q_shape, j > 0);
       umma_arrive(&bars.empty[j % STAGES]);
       if (j + CHAINS < steps) slopes(j + CHAINS);
       if (j == steps - 1) umma_arrive(&bars.done);
     }
   } else {
-    const int chain = warp >> 2, row = tid & 127, q = q0 + row;
+    const int chain = warp >> 3, half = (warp >> 2) & 1, row = tid & 127, q = q0 + row;
     const bool held = q < length;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + chain * 128, dp_at = s_at + AT_STEP;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + chain * 128 + half * AB_WIDE, dp_at = s_at + AT_STEP;
     const long long stat = (long long)head * a.tokens + start + q;
-    // delta of the row, for the keys' pass too. It is a small difference of large sums, and what it is off by moves a whole row of
+    // delta of the rows, for the keys' pass too. It is a small difference of large sums, and what it is off by moves a whole row of
     // dS one way: it takes the output unrounded, in two parts. (With the rounded one dQ and dK were off by 1.7 times their own
-    // rounding, so by 1.4.)
-    float delta = 0.f;
+    // rounding, so by 1.4.) Eight lanes to a row of 64: a row to a thread took 5000 cycles, since every load touched 32 lines.
     const float lse = held ? a.lse[stat] : 0.f;
-    if (held && chain == 0) {
-      const long long at = ((long long)(start + q) * a.heads + head) * a.size;
-      const T* o = (const T*)a.out + at;
-      const T* o_rest = (const T*)a.rest + at;
-      const T* g = (const T*)a.grad + (long long)(start + q) * a.grad_row + (long long)head * a.grad_head;
-#pragma unroll 4
-      for (int c = 0; c < a.size; c += 8) {
-        const uint4 x = *reinterpret_cast<const uint4*>(o + c), y = *reinterpret_cast<const uint4*>(g + c), z = *reinterpret_cast<const uint4*>(o_rest + c);
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, zs[4] = {z.x, z.y, z.z, z.w};
+    {
+      constexpr int ROWS = AT_TILE / (8 * CHAINS), LOADS = ROWS / 4 * PANELS;    // rows of a warp
+      uint4 x[LOADS], y[LOADS], z[LOADS];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 u = unpack2<T>(xs[i]), v = unpack2<T>(ys[i]), w = unpack2<T>(zs[i]);
-          delta = fmaf(u.x + w.x, v.x, delta);
-          delta = fmaf(u.y + w.y, v.y, delta);
+      for (int i = 0; i < LOADS; ++i) {    // all on their way before the first is used
+        const int r = warp * ROWS + i / PANELS * 4 + (lane >> 3), c = i % PANELS * 64 + (lane & 7) * 8;
+        const bool in = q0 + r < length && c < a.size;
+        const long long at = ((long long)(start + q0 + r) * a.heads + head) * a.size + c;
+        x[i] = y[i] = z[i] = make_uint4(0, 0, 0, 0);
+        if (in) x[i] = *reinterpret_cast<const uint4*>((const T*)a.out + at);
+        if (in) y[i] = *reinterpret_cast<const uint4*>((const T*)a.grad + (long long)(start + q0 + r) * a.grad_row + (long long)head * a.grad_head + c);
+        if (in) z[i] = *reinterpret_cast<const uint4*>((const T*)a.rest + at);
+      }
+      float sums[ROWS / 4];
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w}, zs[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
+        if (i % PANELS == 0) sums[i / PANELS] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 u = unpack2<T>(xs[e]), v = unpack2<T>(ys[e]), w = unpack2<T>(zs[e]);
+          sums[i / PANELS] = fmaf(u.x + w.x, v.x, sums[i / PANELS]);
+          sums[i / PANELS] = fmaf(u.y + w.y, v.y, sums[i / PANELS]);
         }
       }
-      a.delta[stat] = delta;
+#pragma unroll
+      for (int i = 0; i < ROWS / 4; ++i) {
+#pragma unroll
+        for (int by = 4; by > 0; by >>= 1) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], by);
+        if ((lane & 7) == 0) s_delta[warp * ROWS + i * 4 + (lane >> 3)] = sums[i];
+      }
     }
-    if (CHAINS == 2) {
-      if (chain == 0) s_delta[row] = delta;
-      asm volatile("bar.sync 1, 256;" ::: "memory");
-      delta = s_delta[row];
-    }
-    const int limit = a.causal ? q : length - 1;    // last key that counts
+    asm volatile("bar.sync 1, %0;" ::"n"(256 * CHAINS) : "memory");
+    const float delta = s_delta[row];
+    if (held && warp < 4) a.delta[stat] = delta;
+    const int limit = (a.causal ? q : length - 1) - half * AB_WIDE;    // last key that counts, from this thread's first on
     bool ok = true;
     for (int j = chain; j < steps; j += CHAINS) {
       const uint32_t parity = (j / CHAINS) & 1;
       ok = wait(&bars.s[chain], parity);
       if (!ok) break;
       umma_fence_after();
-      float p[AT_STEP];
+      float p[AB_WIDE];
       tmem_load32(s_at, p);
-      tmem_load32(s_at + 32, p + 32);
-      tmem_load_wait<AT_STEP>(p);
+      tmem_load_wait<AB_WIDE>(p);
       at_arrive(&bars.p[chain]);
       ab_exponentials(p, a.scale2, lse);
       if ((j + 1) * AT_STEP > (a.causal ? q0 + 1 : length)) {     // some keys do not count for some rows
         const int last = limit - j * AT_STEP;
 #pragma unroll
-        for (int c = 0; c < AT_STEP; ++c)
+        for (int c = 0; c < AB_WIDE; ++c)
           if (c > last) p[c] = 0.f;
       }
       ok = wait(&bars.dp[chain], parity);
       if (!ok) break;
       umma_fence_after();
       const float2 minus = make_float2(-delta, -delta);
-      float d[AT_STEP];
+      float d[AB_WIDE];
       tmem_load32(dp_at, d);
-      tmem_load32(dp_at + 32, d + 32);
-      tmem_load_wait<AT_STEP>(d);
+      tmem_load_wait<AB_WIDE>(d);
+      uint32_t w[16];
 #pragma unroll
-      for (int c = 0; c < AT_STEP; c += 32) {
-        uint32_t w[16];
-#pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const float2 x = mul2(make_float2(p[c + i], p[c + i + 1]), add2(make_float2(d[c + i], d[c + i + 1]), minus));
-          w[i / 2] = pack2<T>(x.x, x.y);
-        }
-        tmem_store16(dp_at + c / 2, w);
+      for (int i = 0; i < AB_WIDE; i += 2) {
+        const float2 x = mul2(make_float2(p[i], p[i + 1]), add2(make_float2(d[i], d[i + 1]), minus));
+        w[i / 2] = pack2<T>(x.x, x.y);
       }
+      tmem_store16(dp_at, w);
       tmem_store_wait();
       at_arrive(&bars.ds[chain]);
     }
     if (ok) ok = wait(&bars.done, 0);
     if (ok) {
       umma_fence_after();
-      const int first = q0 + warp * 32;
-      if (chain == 0) at_write_rows<T, PANELS>(tmem + lanes + DQ, a.scale, s_q + warp * 4096, (T*)a.dq + ((long long)(start + first) * a.heads + head) * a.size, (T*)nullptr,
-                               (long long)a.heads * a.size, length - first, a.size);
+      const int first = q0 + (warp & 3) * 32, panel = CHAINS == 2 ? half : 0;     // heads of more than 64: half of them each
+      if (chain == 0 && half < PANELS)
+        at_write_rows<T, 1>(tmem + lanes + DQ + panel * 64, a.scale, s_q + (panel * 4 + (warp & 3)) * 4096,
+                            (T*)a.dq + ((long long)(start + first) * a.heads + head) * a.size + panel * 64, (T*)nullptr, (long long)a.heads * a.size, length - first,
+                            a.size - panel * 64);
     }
   }
   umma_fence_before();
@@ -799,19 +812,23 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
 // of a step and S^T of the chain's next are multiplied while dS^T is formed, dK and the next dP^T while the next exponentials are
 // taken. Where few tiles of keys share many query heads, the heads are dealt out over a cluster of blocks (`split`), whose sums are
 // added in shared memory, in the order of their rank.
+// What is subtracted from a column of S^T and dP^T, the logarithm of its sum and its delta, is a 32-bit number in three parts of eight bits: one more
+// step of the products, with ones. (As numbers that every thread reads they took more of shared memory's time than all operands
+// together, since a row of threads reads one word at a time.)
 template <typename T, int PANELS>
 __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention_dkv_kernel(const __grid_constant__ AtArgs a) {
   constexpr int CHAINS = PANELS;
   constexpr int TILE_BYTES = PANELS * UMMA_PANEL, HALF = TILE_BYTES / 2, STAGES = ab_stages(PANELS);
   constexpr int DV = 2 * AT_STEP * CHAINS, DK = DV + 64 * PANELS, COLUMNS = 256 * CHAINS;   // tensor memory; chain c has its scores at 128 c, slopes behind
-  constexpr int LOADER = 4 * CHAINS, ISSUER = LOADER + 1;
+  constexpr int LOADER = 8 * CHAINS, ISSUER = LOADER + 1;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_k = base;
   uint8_t* s_v = base + TILE_BYTES;
   uint8_t* s_ring = base + 2 * TILE_BYTES;   // stage: Q, dO
+  uint8_t* s_ones = s_ring + STAGES * TILE_BYTES;
+  uint8_t* s_stats = s_ones + AB_ONES;       // stage: logarithms, deltas
   __shared__ __align__(8) AbBars<CHAINS, STAGES> bars;
-  __shared__ __align__(16) float s_stats[CHAINS][3][2 * AT_STEP];   // of a chain's i-th step in place i % 3 (see below): logarithms, then deltas
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_found;
   __shared__ AtPiece s_piece;
@@ -829,10 +846,14 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
   }
   if (warp == LOADER && lane < 4) tma_prefetch_map(lane == 0 ? &a.q : lane == 1 ? &a.g : lane == 2 ? &a.k : &a.v);
   if (tid == 32) {
-    bars.init();
+    bars.init(1, 2);
     s_abort = 0;
   }
   if (warp == ISSUER) tmem_alloc(&s_tmem, COLUMNS);
+  // three ones to a row, zeros, and room for three parts of each statistic, zeros
+  for (int i = tid; i < (AB_ONES + STAGES * AB_STATS) / 16; i += ab_threads(CHAINS))
+    reinterpret_cast<uint4*>(s_ones)[i] = i < AT_TILE ? make_uint4(0x3F803F80u, 0x3F80u, 0, 0) : make_uint4(0, 0, 0, 0);
+  psgd_fence_async_shared();
   umma_fence_before();
   __syncthreads();
   umma_fence_after();
@@ -870,23 +891,52 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
         at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_k), &a.k, head, start + k0, &bars.fixed);
         at_load_tile<PANELS, AT_TILE>(psgd_smem_u32(s_v), &a.v, head, start + k0, &bars.fixed);
       }
-      Step step = {head0, first * AT_STEP};
+      Step step = {head0, first * AT_STEP}, later = step;
+      const float per_log = -1.f / a.scale2;
+      float x[4];      // of queries `lane` and `lane` + 32 of a step: minus the logarithm of the sum, as the products are scaled, and minus delta
+      auto statistics = [&](const Step& at) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const bool in = at.row + lane + 32 * h < length;
+          const long long from = (long long)at.head * a.tokens + start + at.row + lane + 32 * h;
+          x[2 * h] = in ? a.lse[from] * per_log : 0.f;
+          x[2 * h + 1] = in ? -a.delta[from] : 0.f;
+        }
+      };
       for (int i = 0; i < steps; ++i, next(step, 1)) {
         const int slot = i % STAGES;
         if (!wait(&bars.empty[slot], ((i / STAGES) & 1) ^ 1)) break;
-        if (lane != 0) continue;
-        psgd_mbar_expect_tx(&bars.full[slot], 2 * HALF);
-        const uint32_t at = psgd_smem_u32(s_ring + slot * TILE_BYTES);
-        at_load_tile<PANELS, AT_STEP>(at, &a.q, step.head, start + step.row, &bars.full[slot]);
-        at_load_tile<PANELS, AT_STEP>(at + HALF, &a.g, step.head, start + step.row, &bars.full[slot]);
+        if (lane == 0) {
+          psgd_mbar_expect_tx(&bars.full[slot], 2 * HALF);
+          const uint32_t at = psgd_smem_u32(s_ring + slot * TILE_BYTES);
+          at_load_tile<PANELS, AT_STEP>(at, &a.q, step.head, start + step.row, &bars.full[slot]);
+          at_load_tile<PANELS, AT_STEP>(at + HALF, &a.g, step.head, start + step.row, &bars.full[slot]);
+        }
+        if (i == 0) {
+          psgd_wait_for_predecessor();   // delta is complete
+          statistics(step);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float high = __bfloat162float(__float2bfloat16_rn(x[e])), low = x[e] - high, middle = __bfloat162float(__float2bfloat16_rn(low));
+          *reinterpret_cast<uint4*>(s_stats + slot * AB_STATS + (e & 1) * (AB_STATS / 2) + (lane + 32 * (e >> 1)) * 16) =
+              make_uint4(pack2<__nv_bfloat16>(high, middle), pack2<__nv_bfloat16>(low - middle, 0.f), 0, 0);
+        }
+        psgd_fence_async_shared();
+        __syncwarp();
+        if (lane == 0) psgd_mbar_arrive(&bars.full[slot]);
+        next(later, 1);
+        if (i + 1 < steps) statistics(later);
       }
-      psgd_wait_for_predecessor();
     }
+    psgd_wait_for_predecessor();   // (nobody behind this grid may begin before the one before it has ended)
   } else if (warp == ISSUER) {
     const int k_steps = (a.size + 15) / 16;
     constexpr uint32_t S_SHAPE = umma_shape(AtType<T>::value, false, AT_STEP);
     const uint32_t o_shape = umma_shape(AtType<T>::value, true, k_steps * 16);
     const uint32_t k_at = warp_uniform(psgd_smem_u32(s_k)), v_at = k_at + TILE_BYTES, ring_at = k_at + 2 * TILE_BYTES;
+    const uint32_t ones_at = ring_at + STAGES * TILE_BYTES, stats_at = ones_at + AB_ONES;
+    constexpr uint32_t ONE_SHAPE = umma_shape(AtType<__nv_bfloat16>::value, false, AT_STEP);
     bool ok = wait(&bars.fixed, 0);
     int have = -1;
     Step step = {head0, first * AT_STEP};     // the one behind `have`
@@ -907,11 +957,13 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
     auto scores = [&](int i) {
       if (!there(i)) return;
       umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem + i % CHAINS * 128, k_at, ring_at + i % STAGES * TILE_BYTES, S_SHAPE, k_steps);
+      umma_add_columns<AT_TILE, AT_STEP>(tmem + i % CHAINS * 128, ones_at, stats_at + i % STAGES * AB_STATS, ONE_SHAPE);
       umma_arrive(&bars.s[i % CHAINS]);
     };
     auto slopes = [&](int i) {
       if (!there(i)) return;
       umma_rows_by_rows<4 * PANELS, AT_STEP>(tmem + i % CHAINS * 128 + AT_STEP, v_at, ring_at + i % STAGES * TILE_BYTES + HALF, S_SHAPE, k_steps);
+      umma_add_columns<AT_TILE, AT_STEP>(tmem + i % CHAINS * 128 + AT_STEP, ones_at, stats_at + i % STAGES * AB_STATS + AB_STATS / 2, ONE_SHAPE);
       umma_arrive(&bars.dp[i % CHAINS]);
     };
     for (int i = 0; i < CHAINS && i < steps && ok; ++i) {
@@ -924,126 +976,87 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       ok = wait(&bars.p[chain], parity);
       if (!ok) break;
       umma_fence_after();
-      umma_weights_by_rows<0, 4, AT_STEP>(tmem + DV, tmem + chain * 128, stage + HALF, o_shape, i > 0);
+      umma_weights_by_rows<0, 4, AT_STEP, AB_GAP>(tmem + DV, tmem + chain * 128, stage + HALF, o_shape, i > 0);
       if (i + CHAINS < steps) scores(i + CHAINS);
       ok = ok && wait(&bars.ds[chain], parity);
       if (!ok) break;
       umma_fence_after();
-      umma_weights_by_rows<0, 4, AT_STEP>(tmem + DK, tmem + chain * 128 + AT_STEP, stage, o_shape, i > 0);
+      umma_weights_by_rows<0, 4, AT_STEP, AB_GAP>(tmem + DK, tmem + chain * 128 + AT_STEP, stage, o_shape, i > 0);
       umma_arrive(&bars.empty[i % STAGES]);
       if (i + CHAINS < steps) slopes(i + CHAINS);
       if (i == steps - 1) umma_arrive(&bars.done);
     }
-    psgd_wait_for_predecessor();
   } else {
-    const int chain = warp >> 2, row = tid & 127, key = k0 + row;
-    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + chain * 128, dp_at = s_at + AT_STEP;
-    psgd_wait_for_predecessor();   // delta is complete
-    const float* statistics = (row < AT_STEP ? a.lse : a.delta) + start + row % AT_STEP;
-    auto statistic = [&](const Step& at) {   // of query row % 64 of a step, negative: logarithm of the sum, or delta
-      return at.row + row % AT_STEP < length ? -statistics[(long long)at.head * a.tokens + at.row] : 0.f;
-    };
-    float (*stats)[2 * AT_STEP] = s_stats[chain];
-    Step step = {head0, first * AT_STEP}, later;
+    const int chain = warp >> 3, half = (warp >> 2) & 1, row = tid & 127, key = k0 + row;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + chain * 128 + half * AB_WIDE, dp_at = s_at + AT_STEP;
+    Step step = {head0, first * AT_STEP};
     next(step, chain);
-    if (chain < steps) stats[0][row] = statistic(step);
-    later = step;
-    asm volatile("bar.sync %0, 128;" ::"r"(1 + chain) : "memory");
     bool ok = true;
     int mine = 0;                   // steps of this chain so far
-    for (int i = chain; i < steps; i += CHAINS, ++mine) {
-      const int q0 = step.row;
-      next(later, CHAINS);
-      const float ahead = i + CHAINS < steps ? statistic(later) : 0.f;
-      step = later;
-      const float* now = stats[mine % 3];
-      // The statistics of a step were written before the arrivals for the one before. A warp may be behind by the second half of a step, no
-      // more: two places would not do, three do.
-      ok = (mine == 0 || wait(&bars.p[chain], (mine - 1) & 1)) && wait(&bars.s[chain], mine & 1);
+    for (int i = chain; i < steps; i += CHAINS, ++mine, next(step, CHAINS)) {
+      const int q0 = step.row + half * AB_WIDE;      // this thread's first query
+      ok = wait(&bars.s[chain], mine & 1);
       if (!ok) break;
       umma_fence_after();
-      float p[AT_STEP];
+      float p[AB_WIDE];
       tmem_load32(s_at, p);
-      tmem_load32(s_at + 32, p + 32);
-      tmem_load_wait<AT_STEP>(p);
-      const float2 factor = make_float2(a.scale2, a.scale2);
+      tmem_load_wait<AB_WIDE>(p);
 #pragma unroll
-      for (int c = 0; c < AT_STEP; c += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(now + c);
-#pragma unroll
-        for (int h = 0; h < 4; h += 2) {
-          const float2 y = fma2(make_float2(p[c + h], p[c + h + 1]), factor, h ? make_float2(x.z, x.w) : make_float2(x.x, x.y));
-          p[c + h] = at_exp2(y.x);
-          p[c + h + 1] = at_exp2(y.y);
-        }
+      for (int c = 0; c < AB_WIDE; c += 2) {
+        const float2 y = mul2(make_float2(p[c], p[c + 1]), make_float2(a.scale2, a.scale2));
+        p[c] = at_exp2(y.x);
+        p[c + 1] = at_exp2(y.y);
       }
       if (a.causal && q0 < k0 + AT_TILE) {     // some queries come before some keys
         const int from = key - q0;
 #pragma unroll
-        for (int c = 0; c < AT_STEP; ++c)
+        for (int c = 0; c < AB_WIDE; ++c)
           if (c < from) p[c] = 0.f;
       }
       // (Queries behind the sequence have rows of zeros and deltas of zero: their weights are multiplied by zeros, their slopes are zeros.)
+      uint32_t w[16];
 #pragma unroll
-      for (int c = 0; c < AT_STEP; c += 32) {
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) w[e / 2] = pack2<T>(p[c + e], p[c + e + 1]);
-        tmem_store16(s_at + c / 2, w);
-      }
-      stats[(mine + 1) % 3][row] = ahead;
+      for (int e = 0; e < AB_WIDE; e += 2) w[e / 2] = pack2<T>(p[e], p[e + 1]);
+      tmem_store16(s_at, w);
       tmem_store_wait();
       at_arrive(&bars.p[chain]);
       ok = wait(&bars.dp[chain], mine & 1);
       if (!ok) break;
       umma_fence_after();
-      float d[AT_STEP];
+      float d[AB_WIDE];
       tmem_load32(dp_at, d);
-      tmem_load32(dp_at + 32, d + 32);
-      tmem_load_wait<AT_STEP>(d);
+      tmem_load_wait<AB_WIDE>(d);
 #pragma unroll
-      for (int c = 0; c < AT_STEP; c += 32) {
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 32; e += 4) {
-          const float4 x = *reinterpret_cast<const float4*>(now + AT_STEP + c + e);
-#pragma unroll
-          for (int h = 0; h < 4; h += 2) {
-            const int at = c + e + h;
-            const float2 f = mul2(make_float2(p[at], p[at + 1]), add2(make_float2(d[at], d[at + 1]), h ? make_float2(x.z, x.w) : make_float2(x.x, x.y)));
-            w[(e + h) / 2] = pack2<T>(f.x, f.y);
-          }
-        }
-        tmem_store16(dp_at + c / 2, w);
+      for (int e = 0; e < AB_WIDE; e += 2) {
+        const float2 f = mul2(make_float2(p[e], p[e + 1]), make_float2(d[e], d[e + 1]));
+        w[e / 2] = pack2<T>(f.x, f.y);
       }
+      tmem_store16(dp_at, w);
       tmem_store_wait();
       at_arrive(&bars.ds[chain]);
     }
     if (ok) ok = wait(&bars.done, 0);
     if (ok) {
       umma_fence_after();
-      // dV by the first chain, dK by the last
+      // dV and dK by four warps each; heads of more than 64 by the eight of a chain
+      const int which = CHAINS == 2 ? chain : half, panel = CHAINS == 2 ? half : 0;
+      const uint32_t at = tmem + lanes + (which == 0 ? DV : DK) + panel * 64;
+      if (a.split == 1) {
+        const int first_row = k0 + (warp & 3) * 32;
+        at_write_rows<T, 1>(at, which == 0 ? 1.f : a.scale, (which == 0 ? s_v : s_k) + (panel * 4 + (warp & 3)) * 4096,
+                            (T*)(which == 0 ? a.dv : a.dk) + ((long long)(start + first_row) * kv_heads + head) * a.size + panel * 64, (T*)nullptr,
+                            (long long)kv_heads * a.size, length - first_row, a.size - panel * 64);
+      } else {
+        // this block's share: [dV, dK][128 rows][64 PANELS] float32, groups of four elements where no two lanes meet in a bank
+        float* share = reinterpret_cast<float*>(base) + (which * AT_TILE + row) * 64 * PANELS;
 #pragma unroll
-      for (int which = 0; which < 2; ++which) {
-        if (CHAINS == 2 && which != chain) continue;
-        const uint32_t at = tmem + lanes + (which == 0 ? DV : DK);
-        if (a.split == 1) {
-          const int first_row = k0 + (warp & 3) * 32;
-          at_write_rows<T, PANELS>(at, which == 0 ? 1.f : a.scale, (which == 0 ? s_v : s_k) + (warp & 3) * 4096,
-                                   (T*)(which == 0 ? a.dv : a.dk) + ((long long)(start + first_row) * kv_heads + head) * a.size, (T*)nullptr,
-                                   (long long)kv_heads * a.size, length - first_row, a.size);
-        } else {
-          // this block's share: [dV, dK][128 rows][64 PANELS] float32, groups of four elements where no two lanes meet in a bank
-          float* share = reinterpret_cast<float*>(base) + (which * AT_TILE + row) * 64 * PANELS;
+        for (int c = 0; c < 64; c += 32) {
+          float f[32];
+          tmem_load32(at + c, f);
+          tmem_load_wait<32>(f);
 #pragma unroll
-          for (int c = 0; c < PANELS * 64; c += 32) {
-            float f[32];
-            tmem_load32(at + c, f);
-            tmem_load_wait<32>(f);
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(share + ((c + e) ^ ((row & 7) << 2))) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-          }
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(share + ((panel * 64 + c + e) ^ ((row & 7) << 2))) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
         }
       }
     }
@@ -1173,16 +1186,16 @@ int at_forward(const AtArgs& a, cudaStream_t stream) {
 template <typename T, int PANELS>
 int at_backward(AtArgs a, cudaStream_t stream) {
   static unsigned long long q_devices = 0, kv_devices = 0;
-  if (const int code = psgd_allow_shared((const void*)psgd_attention_dq_kernel<T, PANELS>, ab_shared(PANELS), q_devices)) return code;
-  if (const int code = psgd_allow_shared((const void*)psgd_attention_dkv_kernel<T, PANELS>, ab_shared(PANELS), kv_devices)) return code;
+  if (const int code = psgd_allow_shared((const void*)psgd_attention_dq_kernel<T, PANELS>, ab_shared(PANELS, 0), q_devices)) return code;
+  if (const int code = psgd_allow_shared((const void*)psgd_attention_dkv_kernel<T, PANELS>, ab_shared(PANELS, AB_ONES + ab_stages(PANELS) * AB_STATS), kv_devices)) return code;
   // (delta comes from the first)
-  if (const int code = psgd_launch(psgd_attention_dq_kernel<T, PANELS>, a.blocks * a.heads, ab_threads(PANELS), ab_shared(PANELS), stream, 0, a)) return code;
+  if (const int code = psgd_launch(psgd_attention_dq_kernel<T, PANELS>, a.blocks * a.heads, ab_threads(PANELS), ab_shared(PANELS, 0), stream, 0, a)) return code;
   const int kv_heads = a.heads / a.group;
   a.split = 1;
   for (int split = 2; split <= AB_MOST_SPLIT && split <= a.group && (long long)a.blocks * kv_heads * a.split < AB_ENOUGH; ++split)
     if (a.group % split == 0) a.split = split;
   if ((long long)a.blocks * kv_heads * a.split > 0x7fffffffll) a.split = 1;
-  return psgd_launch_clusters(psgd_attention_dkv_kernel<T, PANELS>, a.blocks * kv_heads * a.split, ab_threads(PANELS), ab_shared(PANELS), stream, 1,
+  return psgd_launch_clusters(psgd_attention_dkv_kernel<T, PANELS>, a.blocks * kv_heads * a.split, ab_threads(PANELS), ab_shared(PANELS, AB_ONES + ab_stages(PANELS) * AB_STATS), stream, 1,
                               a.split, a);
 }
 

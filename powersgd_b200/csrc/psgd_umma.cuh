@@ -64,12 +64,20 @@ __device__ __forceinline__ void umma_rows_by_rows(uint32_t d, uint32_t a, uint32
     umma_ss(d, ta + (((s >> 2) * UMMA_PANEL + (s & 3) * 32) >> 4), tb + (((s >> 2) * B_ROWS * 128 + (s & 3) * 32) >> 4), shape, s > 0);
   }
 }
-// D[128 x n] (+)= A B over rows [16 FROM, 16 TO) of B: A in tensor memory, eight columns for every 16 of K; B_ROWS rows of B are K.
-template <int FROM, int TO, int B_ROWS>
+// D[128 x n] (+)= A B over rows [16 FROM, 16 TO) of B: A in tensor memory, eight columns for every 16 of K and GAP columns between those for
+// every 32; B_ROWS rows of B are K.
+template <int FROM, int TO, int B_ROWS, int GAP = 0>
 __device__ __forceinline__ void umma_weights_by_rows(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, bool accumulate) {
   const uint64_t tb = umma_tile(b, B_ROWS * 128);
 #pragma unroll
-  for (int s = FROM; s < TO; ++s) umma_ts(d, a + s * 8, tb + (s * 2048 >> 4), shape, accumulate || s > 0);
+  for (int s = FROM; s < TO; ++s) umma_ts(d, a + s * 8 + s / 2 * GAP, tb + (s * 2048 >> 4), shape, accumulate || s > 0);
+}
+// D[128 x n] += A B^T over 16 elements. Both lie without a swizzle: elements 0 to 7 of all rows, 16 bytes to a row, then elements 8 to 15.
+template <int A_ROWS, int B_ROWS>
+__device__ __forceinline__ void umma_add_columns(uint32_t d, uint32_t a, uint32_t b, uint32_t shape) {
+  // (eight rows, 128 bytes, are one unit; the next rows' follows it, the next elements' is a whole column of them further)
+  auto tile = [](uint32_t saddr, int rows) { return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)(rows * 16 >> 4) << 16) | ((uint64_t)(128 >> 4) << 32) | (1ull << 46); };
+  umma_ss(d, tile(a, A_ROWS), tile(b, B_ROWS), shape, true);
 }
 
 // 32 columns of the 32 lanes of this warp. A wait must follow before the registers are used.

@@ -30,7 +30,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     [sequences + 1], on the tensors' device, never decreasing: sequence s has the rows offsets[s] to offsets[s + 1], and may have none.
     It is read by the kernels and not by the host: a call neither waits nor checks it, values outside [0, tokens] are taken for the
     nearer end, and what sequences that overlap give is not defined. Rows that belong to no sequence give zeros, whatever they
-    hold. `scale`: 1 / sqrt(size) unless given.
+    hold. `scale`: 1 / sqrt(size) unless given; 2^-100 to 2^100.
 
     Differentiable (once) in q, k and v, whose gradients have the shapes of these; the result and the gradients are the same
     in every run. Tensors may be views, as parts of one projection are: rows and heads that do not begin on 16-byte boundaries, or
@@ -64,8 +64,8 @@ def check(q, k, v, offsets, scale) -> None:
         raise ValueError(f"packed_attention: tensors on {q.device}, {k.device}, {v.device} and {offsets.device}")
     if q.shape[0] >= 2**31 - 2**16:
         raise ValueError(f"packed_attention: {q.shape[0]} tokens")
-    if scale is not None and not (math.isfinite(scale) and scale > 0):
-        raise ValueError(f"packed_attention: scale {scale}")
+    if scale is not None and not 2.0**-100 <= scale <= 2.0**100:
+        raise ValueError(f"packed_attention: scale {scale}; 2^-100 to 2^100")
 
 
 def _native(t: torch.Tensor) -> bool:

@@ -71,3 +71,10 @@ def test_refusals(change, error):
     call.update(change)
     with pytest.raises(error):
         packed_attention(call.pop("q"), call.pop("k"), call.pop("v"), call.pop("offsets"), **call)
+
+
+@pytest.mark.parametrize("scale", [0.0, -1.0, 2.0**-101, 2.0**101, math.inf, math.nan])
+def test_refused_scales(scale):
+    x = torch.zeros(3, 1, 8)
+    with pytest.raises(ValueError, match="scale"):
+        packed_attention(x, x, x, torch.tensor([0, 3], dtype=torch.int32), scale=scale)

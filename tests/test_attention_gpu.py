@@ -244,3 +244,10 @@ def test_more_elements_than_thirty_two_bits_count(heads, size):
     want = packed_attention(*last, _offsets([3000, 2000]))
     for a, b in zip(got, (want, *torch.autograd.grad(want, last, g[-5000:]))):
         assert torch.equal(a.detach()[-5000:], b.detach())
+
+
+@pytest.mark.parametrize("scale", [2.0**-100, 2.0**-60, 2.0**-12])
+def test_small_scales(scale):
+    """Scores that hardly differ: the output is near the mean of the values, dV near that of the gradients."""
+    q, k, v, g = _inputs(200, 2, 1, 64, torch.bfloat16)
+    _check(q, k, v, g, _offsets([200]), False, scale=scale)
