@@ -557,6 +557,11 @@ constexpr int AB_ENOUGH = 4 * 148;    // with so many blocks the heads of a grou
 __host__ __device__ constexpr int ab_threads(int chains) { return 256 * chains + 64; }
 constexpr int AB_WIDE = AT_STEP / 2;
 constexpr int AB_GAP = AB_WIDE / 2;   // columns: each thread's 16-bit numbers take the first half of its own place
+// In sequences up to this long dS goes into the products in two parts, what rounding took from it in the second half of its place. Few terms leave more of
+// their roundings in a sum: dQ and dK were 1.45 to 1.54 times as far from 64 bits as results that are only rounded, 1.05 to 1.15 times so. (Longer
+// sequences: 1.45. There the second products would cost 10 to 20 %: documents of 24 to 1024 forward and backward 137.7 / 147.1 us, 4 x 4096
+// heads of 128 backward 1080 / 1310; here they are not seen, 7 sequences up to 64 15.7 / 15.8.)
+constexpr int AB_FINE = AT_TILE;
 // Tiles that pass come in pairs (K and V, or Q and dO).
 __host__ __device__ constexpr int ab_stages(int panels) { return panels == 1 ? 3 : 4; }
 constexpr int AB_ONES = 2 * AT_TILE * 16, AB_STATS = 2 * 2 * AT_STEP * 16;   // bytes: rows of 16 elements, see umma_add_columns
@@ -592,6 +597,17 @@ __device__ __forceinline__ void ab_exponentials(float* s, float scale2, float at
     s[c] = at_exp2(x.x);
     s[c + 1] = at_exp2(x.y);
   }
+}
+
+// What rounding took from `x`, as rounded in `w`.
+template <typename T>
+__device__ __forceinline__ void ab_store_rest(uint32_t at, const float* x, uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < AB_WIDE; i += 2) {
+    const float2 back = unpack2<T>(w[i / 2]);
+    w[i / 2] = pack2<T>(x[i] - back.x, x[i + 1] - back.y);
+  }
+  tmem_store16(at, w);
 }
 
 // dQ: tensor memory holds, per chain, S and dP (64 columns each; dS takes the first half of dP's place), and dQ. S of a chain's next step is
@@ -703,6 +719,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       if (!ok) break;
       umma_fence_after();
       umma_weights_by_rows<0, 4, AT_STEP, AB_GAP>(tmem + DQ, tmem + chain * 128 + AT_STEP, ring_at + j % STAGES * TILE_BYTES, q_shape, j > 0);
+      if (length <= AB_FINE) umma_weights_by_rows<0, 4, AT_STEP, AB_GAP>(tmem + DQ, tmem + chain * 128 + AT_STEP + AB_GAP, ring_at + j % STAGES * TILE_BYTES, q_shape, true);
       umma_arrive(&bars.empty[j % STAGES]);
       if (j + CHAINS < steps) slopes(j + CHAINS);
       if (j == steps - 1) umma_arrive(&bars.done);
@@ -781,8 +798,11 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       for (int i = 0; i < AB_WIDE; i += 2) {
         const float2 x = mul2(make_float2(p[i], p[i + 1]), add2(make_float2(d[i], d[i + 1]), minus));
         w[i / 2] = pack2<T>(x.x, x.y);
+        d[i] = x.x;
+        d[i + 1] = x.y;
       }
       tmem_store16(dp_at, w);
+      if (length <= AB_FINE) ab_store_rest<T>(dp_at + AB_GAP, d, w);
       tmem_store_wait();
       at_arrive(&bars.ds[chain]);
     }
@@ -982,6 +1002,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       if (!ok) break;
       umma_fence_after();
       umma_weights_by_rows<0, 4, AT_STEP, AB_GAP>(tmem + DK, tmem + chain * 128 + AT_STEP, stage, o_shape, i > 0);
+      if (length <= AB_FINE) umma_weights_by_rows<0, 4, AT_STEP, AB_GAP>(tmem + DK, tmem + chain * 128 + AT_STEP + AB_GAP, stage, o_shape, true);
       umma_arrive(&bars.empty[i % STAGES]);
       if (i + CHAINS < steps) slopes(i + CHAINS);
       if (i == steps - 1) umma_arrive(&bars.done);
@@ -1030,8 +1051,11 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       for (int e = 0; e < AB_WIDE; e += 2) {
         const float2 f = mul2(make_float2(p[e], p[e + 1]), make_float2(d[e], d[e + 1]));
         w[e / 2] = pack2<T>(f.x, f.y);
+        d[e] = f.x;
+        d[e + 1] = f.y;
       }
       tmem_store16(dp_at, w);
+      if (length <= AB_FINE) ab_store_rest<T>(dp_at + AB_GAP, d, w);
       tmem_store_wait();
       at_arrive(&bars.ds[chain]);
     }

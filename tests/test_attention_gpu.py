@@ -251,3 +251,31 @@ def test_small_scales(scale):
     """Scores that hardly differ: the output is near the mean of the values, dV near that of the gradients."""
     q, k, v, g = _inputs(200, 2, 1, 64, torch.bfloat16)
     _check(q, k, v, g, _offsets([200]), False, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("length, size", [(2, 16), (64, 16), (128, 64), (128, 80), (16, 128)])
+def test_short_sequences_lose_little(length, size, dtype):
+    """With queries (or keys) of zeros and a power of two of keys the weights are exact: what is left is one rounding of dQ (of dK) and that of dS in
+    two 16-bit parts, u^2 < 2^-15 of it (float16: what is lost below its smallest step, 2^-25, besides)."""
+    u = torch.finfo(dtype).eps / 2
+    heads, tokens = 2, 4 * length
+    offsets = _offsets([length] * 4)
+    for zero in ("q", "k"):
+        q, k, v, g = _inputs(tokens, heads, heads, size, dtype, seed=length)
+        (q if zero == "q" else k).zero_()
+        leaves = [x.requires_grad_() for x in (q, k, v)]
+        got = torch.autograd.grad(packed_attention(*leaves, offsets, causal=False), leaves, g)[0 if zero == "q" else 1]
+        Q, K, V, G, got = (x.detach().double().view(4, length, heads, size).transpose(1, 2) for x in (q, k, v, g, got))
+        O = V.mean(2, keepdim=True)
+        dP = G @ V.transpose(2, 3)
+        dS = (dP - (G * O).sum(3, keepdim=True)) / length
+        off = 2.0**-15 * dS.abs() + (2.0**-15 * (G.abs() * O.abs()).sum(3, keepdim=True) + 2.0**-17 * (G.abs() @ V.abs().transpose(2, 3))) / length
+        off = off + (2.0**-25 if dtype == torch.float16 else 0.0)
+        c = 1 / math.sqrt(size)
+        if zero == "q":
+            want, bound = dS @ K * c, off @ K.abs() * c
+        else:
+            want, bound = dS.transpose(2, 3) @ Q * c, off.transpose(2, 3) @ Q.abs() * c
+        bound = bound + u * (want.abs() + bound) + (2.0**-25 if dtype == torch.float16 else 0.0)
+        assert ((got - want).abs() <= bound).all()
