@@ -9,10 +9,11 @@
 // logarithm of the sum are float32; P and dS are rounded to 16 bits as operands of the second products, as the tensor
 // core takes them, and results are rounded once.
 //
-// Rows of Q, K, V and dO come by TMA, and the scores never leave tensor memory and registers: a thread owns a row of a tile
-// (a lane of tensor memory), so that a row's maximum and sum need no exchange between lanes, and P and dS go back to tensor
-// memory as the A operand of the second products. A step's chain (products, into registers, exponentials, back, products) is
-// much longer than the work of any one unit in it, so two chains run on every SM: two blocks, or two tiles of one.
+// Rows of Q, K, V and dO come by TMA, and the scores never leave tensor memory and registers: in the forward pass a thread owns a row of a
+// tile (a lane of tensor memory), so that a row's maximum and sum need no exchange between lanes; in the backward pass, which
+// needs neither, two threads share it. P and dS go back to tensor memory as the A operand of the second products. A step's chain
+// (products, into registers, exponentials, back, products) is much longer than the work of any one unit in it, so two chains run on
+// every SM: two blocks, or two tiles of one.
 //   forward   tiles of 128 queries, walking over tiles of 128 keys.
 //   dQ        tiles of 128 queries, walking over tiles of 64 keys.
 //   dK, dV    tiles of 128 keys, walking over tiles of 64 queries of all heads of the group, transposed: lanes are
@@ -21,9 +22,9 @@
 // A row of a tile that belongs to another sequence, or lies behind the last one, may hold anything: before it is multiplied with anything
 // but scores that are replaced, its row in shared memory is cleared.
 //
-// Heads of 64, four sequences of 4096: 690 TFLOP/s forward, 560 to 600 backward (counted as five products); heads of 128 1080 and 630; GPT-2
-// medium's step over documents of 24 to 1024, 49 GFLOP, 39 + 112 us. Bound by the chains' latencies (see above), for long sequences of heads of 128 by the
-// tensor cores.
+// Heads of 64, four sequences of 4096: 690 TFLOP/s forward, 570 to 630 backward (counted as five products); heads of 128 1000 to 1080 and 635; GPT-2
+// medium's step over documents of 24 to 1024, 49 GFLOP, 38 + 99 us. Bound by the chains: with two of them the tensor cores are 42 to 64 % busy
+// in the backward pass, the special functions 45 to 57 %, instructions are issued in 44 to 51 % of all cycles.
 //
 // Blocks are dealt out with the longest first: the device finds the n-th tile in the order of its distance from the
 // sequence's beginning (causal: of its work), from the offsets alone.
