@@ -23,8 +23,8 @@
 // but scores that are replaced, its row in shared memory is cleared.
 //
 // Heads of 64, four sequences of 4096: 690 TFLOP/s forward, 570 to 630 backward (counted as five products); heads of 128 1000 to 1080 and 635; GPT-2
-// medium's step over documents of 24 to 1024, 49 GFLOP, 38 + 99 us. Bound by the chains: with two of them the tensor cores are 42 to 64 % busy
-// in the backward pass, the special functions 45 to 57 %, instructions are issued in 44 to 51 % of all cycles.
+// medium's step over documents of 24 to 1024, 49 GFLOP, 38 + 99 us. Bound by the chains: with two of them the tensor cores are 43 to 55 % busy
+// in the backward pass, the special functions 51 to 58 % (heads of 64), instructions are issued in 42 to 45 % of all cycles.
 //
 // Blocks are dealt out with the longest first: the device finds the n-th tile in the order of its distance from the
 // sequence's beginning (causal: of its work), from the offsets alone.
