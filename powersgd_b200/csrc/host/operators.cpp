@@ -100,7 +100,7 @@ struct Tokens {
 Tokens token_forward(const Tensor& logits, const Tensor& targets, int64_t top, bool entropy, int64_t ignore_index, double temperature) {
   const c10::cuda::CUDAGuard guard(logits.device());
   int64_t stride;
-  const Tensor z = as_rows(logits.detach(), stride), t = targets.contiguous();
+  const Tensor z = as_rows(logits, stride), t = targets.contiguous();
   const int64_t n = targets.numel(), vocab = logits.sizes().back();
   const auto f32 = z.options().dtype(at::kFloat);
   Tokens o;
@@ -153,7 +153,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
       if (!g.defined() && !g_entropy.defined() && !g_top.defined()) return variable_list(6);
       const c10::cuda::CUDAGuard guard(logits.device());
       int64_t stride;
-      const Tensor z = as_rows(logits.detach(), stride), t = targets.contiguous();
+      const Tensor z = as_rows(logits, stride), t = targets.contiguous();
       const int64_t n = targets.numel(), vocab = logits.sizes().back(), size = z.element_size();
       // each row as far from a 16-byte boundary as that of the logits, see _grad_like in ops/tokens.py
       const int64_t lead = (int64_t)((uintptr_t)z.const_data_ptr() % 16) / size, between = n > 1 ? (stride - vocab) % (16 / size) : 0, pitch = vocab + between;
@@ -278,7 +278,7 @@ Attended attention_forward(const Tensor& q0, const Tensor& k0, const Tensor& v0,
   }
   o.lse = at::empty({heads, tokens}, q0.options().dtype(at::kFloat));
   if (gradient) o.rest = at::empty({tokens, heads, size}, q0.options());
-  const Tensor q = usable(q0.detach()), k = usable(k0.detach()), v = usable(v0.detach()), offsets = offsets0.contiguous(), plan = plan_of(sequences, tokens, q);
+  const Tensor q = usable(q0), k = usable(k0), v = usable(v0), offsets = offsets0.contiguous(), plan = plan_of(sequences, tokens, q);
   long long strides[6];
   strides_of(q, strides);
   strides_of(k, strides + 2);
@@ -311,8 +311,8 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
       if (!lse.defined()) {
         dq.zero_(), dk.zero_(), dv.zero_();
       } else {
-        const Tensor q = usable(saved[0].detach()), k = usable(saved[1].detach()), v = usable(saved[2].detach()), offsets = saved[3].contiguous();
-        const Tensor plan = plan_of(offsets.size(0) - 1, tokens, q), g = usable(grads[0].to(out.scalar_type())), delta = at::empty({heads, tokens}, lse.options());
+        const Tensor q = usable(saved[0]), k = usable(saved[1]), v = usable(saved[2]), offsets = saved[3].contiguous();
+        const Tensor plan = plan_of(offsets.size(0) - 1, tokens, q), g = usable(grads[0]), delta = at::empty({heads, tokens}, lse.options());
         long long strides[8];
         strides_of(q, strides);
         strides_of(k, strides + 2);
