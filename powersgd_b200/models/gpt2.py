@@ -7,7 +7,8 @@ independent of the sequence length, so no sequence parallelism is involved.
 
 Documents of different lengths are trained on without padding, packed one behind another: `model.loss(tokens, targets,
 offsets)` with the rows of document i from offsets[i] to offsets[i + 1]. Attention then is `packed_attention` and the
-loss `token_log_probs`; both keep off the host, so that the lengths may change from step to step of a recorded graph.
+loss `token_log_probs`; both keep off the host, so that the lengths may change from step to step of a recorded graph. (A backward pass is recorded
+while no earlier loss of the same parameters is alive: PyTorch would run the ends of it on that loss's stream.)
 """
 from __future__ import annotations
 
