@@ -332,6 +332,8 @@ __global__ void __launch_bounds__(THREADS) psgd_token_logprob_kernel(const __gri
     }
     return;
   }
+  // Said here and waited for behind the row: all CTAs of the cluster run, so that the shared memory of the first may be written.
+  if (parts > 1) asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   const bool known = target >= 0 && target < a.vocab;
   float z_target = 0.f;
   if (part == 0 && tid == 0 && known) z_target = V::one(z + target);   // on its way while the row is read
@@ -410,6 +412,7 @@ __global__ void __launch_bounds__(THREADS) psgd_token_logprob_kernel(const __gri
   }
   if (lane == 0) s_sum[warp] = t;
   __syncthreads();
+  if (parts > 1) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   if (tid == 0) {
     for (int w = 1; w < WARPS; ++w) t = lp_join<ENT>(t, s_sum[w], a.k);
     if (parts > 1) *cluster.map_shared_rank(&s_parts[part], 0) = t;

@@ -1,0 +1,33 @@
+"""token_log_probs on the GPU where it can go wrong, against float64. Bounds as in test_tokens_gpu.py."""
+import math
+
+import pytest
+import torch
+
+from powersgd_b200.ops.tokens import token_log_probs
+
+pytestmark = pytest.mark.gpu
+
+
+def _logits(rows, vocab, dtype, seed=0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(rows, vocab, generator=gen, device="cuda") * 2).to(dtype), torch.randint(0, vocab, (rows,), generator=gen, device="cuda")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows, vocab", [(1, 4096), (1, 8192), (3, 8195), (1, 32768), (5, 32771), (36, 32768), (37, 50257), (147, 8192)])
+def test_rows_shared_by_blocks(rows, vocab, dtype):
+    """Few rows: two, four or eight blocks to a row, which bring their parts together in the shared memory of the first. Some rows are ignored: their
+    blocks leave at once."""
+    z, t = _logits(rows, vocab, dtype)
+    log_p = torch.log_softmax(z.double(), 1)
+    at = log_p.gather(1, t[:, None])[:, 0]
+    base = (vocab / 64 + 24) * 2.0**-24 + 2.0**-22 + 16 * 2.0**-22      # log p of a row's mean: below 16
+    best = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :7]
+    for _ in range(20):
+        plain, both = token_log_probs(z, t), token_log_probs(z, t, top=7, entropy=True)
+        for r in (plain, both):
+            assert ((r.log_probs.double() - at).abs() <= base + at.abs() * 2.0**-22).all()
+        assert torch.equal(both.top_tokens, best)
+    ignored = torch.where(torch.arange(rows, device="cuda") % 2 == 0, t, torch.full_like(t, -100))
+    assert torch.equal(token_log_probs(z, ignored).log_probs, torch.where(ignored == -100, 0.0, plain.log_probs))
