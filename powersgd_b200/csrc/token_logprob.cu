@@ -286,7 +286,8 @@ __device__ __forceinline__ void lp_select(const T* z, int lead, int v0, int v1, 
       const bool valid = v < v1;
       uint4 r = make_uint4(0, 0, 0, 0);
       if (valid) r = zv[v];
-      const unsigned long long seen = *(volatile unsigned long long*)&s_least;
+      // (one lane's reading for all: others raise it meanwhile, and lanes that held different bounds would part in front of votes of the whole warp)
+      const unsigned long long seen = __shfl_sync(0xffffffffu, *(volatile unsigned long long*)&s_least, 0);
       if (seen > list.least) list.least = seen;
       if (!__any_sync(0xffffffffu, valid && lp_order(V::largest(r)) >= (uint32_t)(list.least >> 32))) continue;
       float f[V::N];

@@ -31,3 +31,17 @@ def test_rows_shared_by_blocks(rows, vocab, dtype):
         assert torch.equal(both.top_tokens, best)
     ignored = torch.where(torch.arange(rows, device="cuda") % 2 == 0, t, torch.full_like(t, -100))
     assert torch.equal(token_log_probs(z, ignored).log_probs, torch.where(ignored == -100, 0.0, plain.log_probs))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("rows, vocab", [(4, 700), (3, 5003), (300, 8191), (2, 50257)])
+def test_more_equal_logits_than_candidates(rows, vocab, dtype):
+    """Every warp then keeps a list, under a bound that all warps of the block raise; the last round of vectors is a partial one."""
+    gen = torch.Generator(device="cuda").manual_seed(vocab)
+    z = torch.randint(0, 3, (rows, vocab), generator=gen, device="cuda").to(dtype)
+    z[:, vocab // 2:] += (torch.arange(vocab - vocab // 2, device="cuda") // 600).to(dtype) / 8      # bounds that rise as the row is read
+    t = torch.zeros(rows, device="cuda", dtype=torch.int64)
+    for top in (1, 20, 32):
+        want = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :top]
+        for _ in range(10):
+            assert torch.equal(token_log_probs(z, t, top=top).top_tokens, want)
