@@ -143,20 +143,24 @@ __device__ bool at_find(const AtArgs& a, int rows, int index, bool from_end, AtP
 // The same order written down, for more sequences than 32: block `level` has the pieces of that level. Their places follow those of all higher levels,
 // in the order of their sequences. (A block that asked for itself as above, in turns of 32 sequences, would read all offsets again for every
 // question: with thousands of sequences that is more than its work.)
+// Counts are of 64 bits: of lists that go down, where long sequences overlap again and again, the pieces may be more than 2^31, of which
+// those that the grid has room for are written down.
 constexpr int AT_PLAN_THREADS = 256;
 __global__ void __launch_bounds__(AT_PLAN_THREADS) psgd_attention_plan_kernel(const int* offsets, int sequences, int tokens, int rows, int capacity, int* plan) {
+  __shared__ long long s_wide[AT_PLAN_THREADS / 32];
   __shared__ int s_sum[AT_PLAN_THREADS / 32];
   const int level = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto sum = [&](int x) {        // over the block
-    x = (int)__reduce_add_sync(0xffffffffu, (unsigned)x);
+  auto sum = [&](long long x) {  // over the block
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
     __syncthreads();
-    if (lane == 0) s_sum[warp] = x;
+    if (lane == 0) s_wide[warp] = x;
     __syncthreads();
-    int all = 0;
-    for (int w = 0; w < AT_PLAN_THREADS / 32; ++w) all += s_sum[w];
+    long long all = 0;
+    for (int w = 0; w < AT_PLAN_THREADS / 32; ++w) all += s_wide[w];
     return all;
   };
-  int higher = 0, here = 0, total = 0;
+  long long higher = 0, here = 0, total = 0;
   for (int s = threadIdx.x; s < sequences; s += AT_PLAN_THREADS) {
     const int n = (max(at_bound(offsets, s + 1, tokens) - at_bound(offsets, s, tokens), 0) + rows - 1) / rows;
     higher += max(n - level - 1, 0);
@@ -167,11 +171,11 @@ __global__ void __launch_bounds__(AT_PLAN_THREADS) psgd_attention_plan_kernel(co
   here = sum(here);
   if (level == 0) {
     total = sum(total);
-    if (threadIdx.x == 0) plan[0] = min(total, capacity);
+    if (threadIdx.x == 0) plan[0] = (int)min(total, (long long)capacity);
   }
-  if (here == 0) return;
-  int at = higher;
-  for (int s0 = 0; s0 < sequences; s0 += AT_PLAN_THREADS) {
+  if (here == 0 || higher >= capacity) return;
+  long long at = higher;
+  for (int s0 = 0; s0 < sequences && at < capacity; s0 += AT_PLAN_THREADS) {
     const int s = s0 + threadIdx.x;
     int begin = 0, length = 0;
     if (s < sequences) {
@@ -188,7 +192,7 @@ __global__ void __launch_bounds__(AT_PLAN_THREADS) psgd_attention_plan_kernel(co
       before += w < warp ? s_sum[w] : 0;
       all += s_sum[w];
     }
-    const int place = at + before;
+    const long long place = at + before;
     if (has && place < capacity) {
       int* x = plan + 1 + 3 * place;
       x[0] = begin;

@@ -352,7 +352,7 @@ PyObject* packed_attention(PyObject*, PyObject* args) {
     if (entry.attention == nullptr || q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || q.size(0) != k.size(0) || q.size(2) != k.size(2) || k.size(1) < 1 ||
         q.size(1) < 1 || q.size(1) % k.size(1) != 0 || q.size(2) < 8 || q.size(2) > 128 || q.size(2) % 8 != 0 || (type != at::kBFloat16 && type != at::kHalf) ||
         k.scalar_type() != type || v.scalar_type() != type || offsets.scalar_type() != at::kInt || offsets.dim() != 1 || offsets.size(0) < 1 ||
-        q.size(0) >= (1ll << 31) - (1 << 16) || !(scale == 0 || (scale >= 0x1p-100 && scale <= 0x1p100)) || q.get_device() >= MOST_DEVICES)
+        offsets.size(0) > (1ll << 31) - (1 << 16) || q.size(0) >= (1ll << 31) - (1 << 16) || !(scale == 0 || (scale >= 0x1p-100 && scale <= 0x1p100)) || q.get_device() >= MOST_DEVICES)
       Py_RETURN_NONE;
     const Status& status = statuses[q.get_device()];
     if (status.host == nullptr || *status.host != 0) Py_RETURN_NONE;

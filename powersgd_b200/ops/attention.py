@@ -64,6 +64,8 @@ def check(q, k, v, offsets, scale) -> None:
         raise ValueError(f"packed_attention: tensors on {q.device}, {k.device}, {v.device} and {offsets.device}")
     if q.shape[0] >= 2**31 - 2**16:
         raise ValueError(f"packed_attention: {q.shape[0]} tokens")
+    if offsets.shape[0] > 2**31 - 2**16:
+        raise ValueError(f"packed_attention: {offsets.shape[0] - 1} sequences")
     if scale is not None and not 2.0**-100 <= scale <= 2.0**100:
         raise ValueError(f"packed_attention: scale {scale}; 2^-100 to 2^100")
 

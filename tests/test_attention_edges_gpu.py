@@ -1,0 +1,33 @@
+"""packed_attention on the GPU where it can go wrong."""
+import math
+
+import pytest
+import torch
+
+from powersgd_b200.ops.attention import packed_attention
+
+pytestmark = pytest.mark.gpu
+
+
+def _offsets(lengths, first=0):
+    return torch.tensor([first + sum(lengths[:i]) for i in range(len(lengths) + 1)], device="cuda", dtype=torch.int32)
+
+
+def _inputs(tokens, heads, groups, size, dtype, seed=0, scale=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    make = lambda n: (torch.randn(tokens, n, size, generator=gen, device="cuda") * scale).to(dtype)  # noqa: E731
+    return make(heads), make(groups), make(groups), make(heads)
+
+
+def test_offsets_that_go_down_again_and_again():
+    """2^24 and more sequences of 128 tiles each over the same rows: their tiles, more than 2^31, are counted without overflow, and what the grid
+    has no room for is left. What such offsets give is not defined, but nothing is written elsewhere."""
+    tokens, turns = 2**14, 2**24 + 2**21
+    offsets = torch.zeros(2 * turns, device="cuda", dtype=torch.int32)
+    offsets[1::2] = tokens
+    whole = torch.zeros(3, tokens, 1, 16, device="cuda", dtype=torch.bfloat16)
+    q, k, v = whole.unbind(0)
+    guard = torch.full((2**26,), 7, device="cuda", dtype=torch.int32)
+    packed_attention(q, k, v, offsets)
+    torch.cuda.synchronize()
+    assert (guard == 7).all() and (whole == 0).all()
