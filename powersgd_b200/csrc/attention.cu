@@ -78,7 +78,8 @@ __device__ __forceinline__ float at_max3(float x, float y, float z) {
 }
 
 // 2^x in plain arithmetic: x = n + f with |f| <= 1/2 by rounding, a polynomial of degree 4 in f with the least maximal relative error
-// (2.8e-6; fitted with value 1 at 0), n added to the exponent. Below -127 the result is zero.
+// (2.8e-6; fitted with value 1 at 0), n added to the exponent. Below -127 the result is zero, and of what is no number it is any: a row that
+// holds such a score has a maximum that is none, and the exponentials beside this one say so.
 constexpr int AT_POLY = 2;   // of 16 exponentials, those that are taken so: the special function unit has 16 results per cycle and SM
 __device__ __forceinline__ float2 at_exp2_poly(float2 x) {
   const float2 magic = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f), minus = make_float2(-1.f, -1.f);
@@ -477,7 +478,7 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
         for (int i = 0; i < 4; ++i) most[i] = at_max3(most[i], s[c + i], s[c + i + 4]);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], s[AT_TILE - 4 + i]);
+      for (int i = 0; i < 4; ++i) most[i] = at_max3(most[i], s[AT_TILE - 4 + i], s[AT_TILE - 4 + i]);
       const float largest = at_max3(at_max3(most[0], most[1], most[2]), most[3], most[3]);
       if (j == 0) {
         m = largest;

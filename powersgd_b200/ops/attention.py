@@ -34,7 +34,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
     Differentiable (once) in q, k and v, whose gradients have the shapes of these; the result and the gradients are the same
     in every run. Tensors may be views, as parts of one projection are: rows and heads that do not begin on 16-byte boundaries, or
-    elements that do not lie side by side, are copied first. Under float16 a gradient beyond its range becomes infinite."""
+    elements that do not lie side by side, are copied first. Under float16 a gradient beyond its range becomes infinite. Positions that
+    see a score which is no number give NaN; where a row of q, k, v or a gradient is not finite, any other of its sequence may."""
     if operators is not None and (scale is None or scale > 0):
         out = operators.packed_attention(q, k, v, offsets, causal, 0.0 if scale is None else scale)
         if out is not None:

@@ -31,3 +31,24 @@ def test_offsets_that_go_down_again_and_again():
     packed_attention(q, k, v, offsets)
     torch.cuda.synchronize()
     assert (guard == 7).all() and (whole == 0).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("size", [64, 128])
+def test_scores_that_are_no_numbers(size, bad, causal):
+    """One key of a sequence: positions that see a score of NaN (or +inf, whose softmax is none) give NaN, as the form in torch operations does,
+    wherever in a tile the key lies."""
+    for place in (0, 1, 2, 16, 17, 40, 123, 124, 127, 128, 130, 250):
+        q, k, v, _ = _inputs(300, 2, 1, size, torch.bfloat16, seed=place)
+        k[20 + place] = bad if math.isnan(bad) else k[20 + place]
+        if math.isinf(bad):
+            k[20 + place, 0, 3] = bad
+        offsets = torch.tensor([0, 20, 280, 300], device="cuda", dtype=torch.int32)
+        got = packed_attention(q, k, v, offsets, causal=causal)
+        want = packed_attention(*(x.cpu().float() for x in (q, k, v)), offsets.cpu(), causal=causal)
+        assert torch.equal(got.isnan().cpu(), want.isnan()), place
+        fine = ~want.isnan()
+        assert want.isnan().any() and fine.any()
+        # a weight is off by 2^-8 of itself and 2^-12 (its score), the output by half a step
+        assert ((got.cpu().float() - want)[fine].abs() <= 2.0**-7 * v.abs().max().item()).all()
