@@ -484,8 +484,8 @@ __global__ void __launch_bounds__(af_threads(TILES), 3 - TILES) psgd_attention_k
         m = largest;
       } else {
         // The sums stay relative to an older maximum while exponents stay below 2^8: accumulators are rescaled only when it moves by
-        // more (and where it is no number).
-        const bool moves = !((largest - m) * a.scale2 <= 8.f);
+        // more (and where it is no number; not where all scores so far are -inf, which are no distance apart).
+        const bool moves = !((largest - m) * a.scale2 <= 8.f) && largest != -INFINITY;
         if (__any_sync(0xffffffffu, moves)) {
           ok = wait(&bar_o[t], (j - 1) & 1);
           if (!ok) break;

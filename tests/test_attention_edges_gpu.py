@@ -50,5 +50,19 @@ def test_scores_that_are_no_numbers(size, bad, causal):
         assert torch.equal(got.isnan().cpu(), want.isnan()), place
         fine = ~want.isnan()
         assert want.isnan().any() and fine.any()
-        # a weight is off by 2^-8 of itself and 2^-12 (its score), the output by half a step
-        assert ((got.cpu().float() - want)[fine].abs() <= 2.0**-7 * v.abs().max().item()).all()
+        # a weight is off by 2^-8 of itself and 2^-12 (its score), the output by half a step, 2^-8
+        assert ((got.cpu().float() - want)[fine].abs() <= (2.0**-7 + 2.0**-11) * v.abs().max().item()).all()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("until", [128, 150, 256, 300])
+def test_scores_of_minus_infinity_come_first(until, size, causal):
+    """Keys whose scores are -inf have no weight, also where whole tiles of them come before all others."""
+    q, k, v, _ = _inputs(500, 2, 1, size, torch.bfloat16, seed=until)
+    q[..., 3] = q[..., 3].abs() + 0.25
+    k[:until, :, 3] = -math.inf
+    got = packed_attention(q, k, v, _offsets([500]), causal=causal)
+    want = packed_attention(*(x.cpu().float() for x in (q, k, v)), _offsets([500]).cpu(), causal=causal)
+    assert torch.equal(got.isnan().cpu(), want.isnan()) and want[until:].isfinite().all()
+    assert ((got.cpu().float() - want)[until:].abs() <= (2.0**-7 + 2.0**-11) * v.abs().max().item()).all()
