@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(LG_THREADS) psgd_token_logprob_grad_kernel(con
   const float m = st.x, log_s = st.y;
   const bool empty = m == -INFINITY && log_s == 0.f;
   float g = a.g_log_prob && !ignored ? a.g_log_prob[row] : 0.f;
-  if (!ignored && (target < 0 || target >= a.vocab)) g = NAN;
+  if (a.g_log_prob && !ignored && (target < 0 || target >= a.vocab)) g = NAN;   // (entropy and alternatives do not depend on the target)
   float all = g;
   if (TOP)
     for (int j = 0; j < a.top; ++j) all += a.g_top[row * a.top + j];

@@ -33,7 +33,7 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0
 
     `logits`: float32, bfloat16 or float16, [*targets.shape, vocabulary]; `targets`: int64 or int32.
     A target equal to `ignore_index` has log probability zero and no gradient; entropy and alternatives are those of its row all
-    the same. A target outside the vocabulary has log probability NaN: nothing is read for it. Masked tokens have logits of
+    the same. A target outside the vocabulary has log probability NaN, whose gradient is NaN too: nothing is read for it. Masked tokens have logits of
     -inf; a row that has only those is no distribution: log probability -inf, entropy zero, no gradient. A row that
     holds +inf or NaN gives NaN, and any tokens. Returned statistics are float32."""
     out = operators.token_log_probs(logits, targets, top, entropy, ignore_index, temperature) if operators is not None else None
@@ -217,7 +217,7 @@ def _backward_torch(logits, targets, stats, entropy, tokens, g, g_entropy, g_top
     at_target = zero
     if g is not None:
         at_target = torch.where(ignored, zero, g.reshape(-1, 1).to(zero.dtype))
-    at_target = torch.where(known | ignored, at_target, torch.full_like(zero, math.nan))
+        at_target = torch.where(known | ignored, at_target, torch.full_like(zero, math.nan))   # (entropy and alternatives do not depend on the target)
     all_of = all_of + at_target
     if g_top is not None:
         g_top = g_top.reshape(p.shape[0], -1).to(zero.dtype)

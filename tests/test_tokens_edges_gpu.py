@@ -45,3 +45,28 @@ def test_more_equal_logits_than_candidates(rows, vocab, dtype):
         want = torch.sort(z, dim=1, descending=True, stable=True).indices[:, :top]
         for _ in range(10):
             assert torch.equal(token_log_probs(z, t, top=top).top_tokens, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("vocab", [40, 5003])
+def test_entropy_and_alternatives_do_not_depend_on_the_target(vocab, dtype):
+    """Their gradients with targets outside the vocabulary: the same as with any other, and those of 64 bits. p is off by 2^-20 of itself and
+    2^-21 for each unit of its logarithm (below 16 where it counts), the gradient by half a step of its type."""
+    z, _ = _logits(6, vocab, dtype)
+    z.requires_grad_()
+    t = torch.tensor([-1, vocab, 3, -100, vocab + 5, -7], device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    gh, gt = torch.randn(6, generator=gen, device="cuda"), torch.randn(6, 4, generator=gen, device="cuda")
+    log_p = torch.log_softmax(z.detach().double(), 1)
+    p = log_p.exp()
+    h = torch.special.entr(p).sum(1, keepdim=True)
+    best = torch.sort(z.detach(), dim=1, descending=True, stable=True).indices[:, :4]
+    for which, g, want, size in (("entropy", gh, gh[:, None].double() * (torch.special.entr(p) - p * h), gh[:, None].double().abs() * (torch.special.entr(p) + p * h)),
+                                 ("top_log_probs", gt, torch.zeros_like(p).scatter_(1, best, gt.double()) - p * gt.double().sum(1, keepdim=True),
+                                  torch.zeros_like(p).scatter_(1, best, gt.double().abs()) + p * gt.double().abs().sum(1, keepdim=True))):
+        got, = torch.autograd.grad(getattr(token_log_probs(z, t, top=4, entropy=True), which), z, g)
+        other, = torch.autograd.grad(getattr(token_log_probs(z, torch.zeros_like(t), top=4, entropy=True), which), z, g)
+        assert torch.equal(got, other)
+        least = 2.0**-25 if dtype == torch.float16 else 1e-36
+        bound = size * (2.0**-17 + (vocab / 64 + 24) * 2.0**-22) + want.abs() * torch.finfo(dtype).eps / 2 * 1.01 + least
+        assert ((got.double() - want).abs() <= bound).all()
