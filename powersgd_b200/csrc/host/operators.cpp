@@ -59,6 +59,12 @@ const Tensor* plain(PyObject* object) {
   return &t;
 }
 
+// Does the tensor carry a tangent of forward-mode differentiation? Results here would lose it.
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+void refuse_tangents(const variable_list& grads, const char* what) {
+  for (const Tensor& g : grads) TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(g), what, ": forward-mode differentiation is not supported");
+}
+
 void* current_stream(const Tensor& t) { return (void*)c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 // What a backward pass returns cannot be differentiated again: asking for it raises.
@@ -141,6 +147,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents(grads, "token_log_probs");
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &targets = saved[1], &stats = saved[2], &entropy = saved[3], &tokens = saved[4];
     Tensor grad;
@@ -218,7 +225,7 @@ PyObject* token_log_probs(PyObject*, PyObject* args) {
     const auto index = targets->scalar_type();
     if (!logits->is_cuda() || logits->device() != targets->device() || type_code(logits->scalar_type()) < 0 || (index != at::kLong && index != at::kInt) || vocab < 1 ||
         vocab >= (1ll << 31) - (1 << 16) || logits->sizes().slice(0, logits->dim() - 1) != targets->sizes() || top < 0 || top > 32 || top > vocab ||
-        !(temperature >= 0x1p-100 && temperature <= 0x1p100))
+        !(temperature >= 0x1p-100 && temperature <= 0x1p100) || has_tangent(*logits))
       Py_RETURN_NONE;
     Tensor out[4];
     if (at::GradMode::is_enabled() && logits->requires_grad()) {
@@ -300,6 +307,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents(grads, "packed_attention");
     const auto saved = ctx->get_saved_variables();
     variable_list result(6);
     {
@@ -352,7 +360,8 @@ PyObject* packed_attention(PyObject*, PyObject* args) {
     if (entry.attention == nullptr || q.dim() != 3 || k.dim() != 3 || k.sizes() != v.sizes() || q.size(0) != k.size(0) || q.size(2) != k.size(2) || k.size(1) < 1 ||
         q.size(1) < 1 || q.size(1) % k.size(1) != 0 || q.size(2) < 8 || q.size(2) > 128 || q.size(2) % 8 != 0 || (type != at::kBFloat16 && type != at::kHalf) ||
         k.scalar_type() != type || v.scalar_type() != type || offsets.scalar_type() != at::kInt || offsets.dim() != 1 || offsets.size(0) < 1 ||
-        offsets.size(0) > (1ll << 31) - (1 << 16) || q.size(0) >= (1ll << 31) - (1 << 16) || !(scale == 0 || (scale >= 0x1p-100 && scale <= 0x1p100)) || q.get_device() >= MOST_DEVICES)
+        offsets.size(0) > (1ll << 31) - (1 << 16) || q.size(0) >= (1ll << 31) - (1 << 16) || !(scale == 0 || (scale >= 0x1p-100 && scale <= 0x1p100)) || q.get_device() >= MOST_DEVICES ||
+        has_tangent(q) || has_tangent(k) || has_tangent(v))
       Py_RETURN_NONE;
     const Status& status = statuses[q.get_device()];
     if (status.host == nullptr || *status.host != 0) Py_RETURN_NONE;

@@ -32,7 +32,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     nearer end, and what sequences that overlap give is not defined. Rows that belong to no sequence give zeros, whatever they
     hold. `scale`: 1 / sqrt(size) unless given; 2^-100 to 2^100.
 
-    Differentiable (once) in q, k and v, whose gradients have the shapes of these; the result and the gradients are the same
+    Differentiable (once, backwards) in q, k and v, whose gradients have the shapes of these; the result and the gradients are the same
     in every run. Tensors may be views, as parts of one projection are: rows and heads that do not begin on 16-byte boundaries, or
     elements that do not lie side by side, are copied first. Under float16 a gradient beyond its range becomes infinite. Positions that
     see a score which is no number give NaN; where a row of q, k, v or a gradient is not finite, any other of its sequence may."""
@@ -69,6 +69,7 @@ def check(q, k, v, offsets, scale) -> None:
         raise ValueError(f"packed_attention: {offsets.shape[0] - 1} sequences")
     if scale is not None and not 2.0**-100 <= scale <= 2.0**100:
         raise ValueError(f"packed_attention: scale {scale}; 2^-100 to 2^100")
+    native.refuse_tangents("packed_attention", q, k, v)
 
 
 def _native(t: torch.Tensor) -> bool:
@@ -171,6 +172,7 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        native.refuse_tangents("packed_attention", grad)
         q, k, v, offsets, out, lse, rest = ctx.saved_tensors
         return (*_backward(q, k, v, offsets, out, lse, rest, grad, ctx.causal, ctx.scale), None, None, None)
 

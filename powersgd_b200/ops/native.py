@@ -13,6 +13,7 @@ import os
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # PSGD_B200_LIB points at another build of the same library (e.g. one with development counters)
@@ -74,6 +75,12 @@ def check(code: int, what: str) -> None:
     if code != 0:
         msg = lib().psgd_last_error()
         raise RuntimeError(f"{what} failed (code {code}): {msg.decode() if msg else ''}")
+
+
+def refuse_tangents(what: str, *tensors) -> None:
+    """For operators whose results would lose the tangents of forward-mode differentiation without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{what}: forward-mode differentiation is not supported")
 
 
 class on_device:

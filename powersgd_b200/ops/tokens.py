@@ -29,7 +29,7 @@ class TokenLogProbs(NamedTuple):
 def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0, entropy: bool = False, ignore_index: int = -100,
                     temperature: float = 1.0) -> TokenLogProbs:
     """Of the distribution softmax(logits / temperature) over the last dimension: the log probability of each target, the entropy (in nats),
-    and the `top` (at most 32) most likely tokens with their log probabilities. All but the tokens are differentiable (once).
+    and the `top` (at most 32) most likely tokens with their log probabilities. All but the tokens are differentiable (once, backwards).
 
     `logits`: float32, bfloat16 or float16, [*targets.shape, vocabulary]; `targets`: int64 or int32.
     A target equal to `ignore_index` has log probability zero and no gradient; entropy and alternatives are those of its row all
@@ -64,6 +64,7 @@ def check(logits, targets, top, ignore_index, temperature) -> None:
         raise ValueError(f"token_log_probs: temperature {temperature}; 2^-100 to 2^100")
     if not -(2**63) <= ignore_index < 2**63:
         raise ValueError(f"token_log_probs: ignore_index {ignore_index}")
+    native.refuse_tangents("token_log_probs", logits)
 
 
 def _rows(logits: torch.Tensor) -> torch.Tensor:
@@ -161,6 +162,7 @@ class _TokenLogProbs(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g, g_entropy, g_top, _):
+        native.refuse_tangents("token_log_probs", g, g_entropy, g_top)
         logits, targets, stats, entropy, tokens = ctx.saved_tensors
         if g is None and g_entropy is None and g_top is None:
             return (None,) * 6

@@ -1,0 +1,27 @@
+"""Calls of token_log_probs, packed_attention and AdamW on the GPU that go through the extension (csrc/host/operators.cpp) or through Python: both
+refuse, raise and answer alike."""
+import pytest
+import torch
+from test_operator_edges_cpu import _tangent_calls
+
+from powersgd_b200.ops import attention, host, tokens
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=["extension", "python"])
+def form(request, monkeypatch):
+    if request.param == "python":
+        monkeypatch.setattr(tokens, "operators", None)
+        monkeypatch.setattr(attention, "operators", None)
+    else:
+        assert host.operators is not None
+        x = torch.zeros(1, 1, 8, device="cuda", dtype=torch.bfloat16)
+        attention.packed_attention(x, x, x, torch.tensor([0, 1], device="cuda", dtype=torch.int32))   # (a device's first call goes through Python)
+    return request.param
+
+
+def test_tangents_are_refused(form):
+    for call in _tangent_calls("cuda"):
+        with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|jvp|setup_context"):
+            call()

@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from powersgd_b200.ops.attention import packed_attention
 from powersgd_b200.ops.tokens import token_log_probs
 
 
@@ -18,3 +19,44 @@ def test_entropy_and_alternatives_do_not_depend_on_the_target(which):
     r = token_log_probs(z, t, entropy=True)     # its own gradient does
     grad, = torch.autograd.grad(r.log_probs.sum() + r.entropy.sum(), z)
     assert grad[:2].isnan().all() and grad[2:].isfinite().all()
+
+
+def _tangent_calls(device):
+    """Calls of both operators with a tangent at one input, or at the gradient that is handed in."""
+    import torch.autograd.forward_ad as fw
+
+    z, t = torch.randn(3, 8, device=device), torch.tensor([0, 5, -100], device=device)
+    x = torch.randn(6, 2, 8, device=device).bfloat16()
+    offsets = torch.tensor([0, 2, 6], dtype=torch.int32, device=device)
+    tokens = lambda z: token_log_probs(z, t, top=2, entropy=True)[:3]  # noqa: E731
+    places = [lambda y: packed_attention(y, x, x, offsets), lambda y: packed_attention(x, y, x, offsets), lambda y: packed_attention(x, x, y, offsets)]
+    calls = []
+    for f, at in [(tokens, z), *((f, x) for f in places)]:
+        def jvp(f=f, at=at):
+            torch.func.jvp(f, (at,), (torch.ones_like(at),))
+
+        def dual(f=f, at=at, grad=False):
+            with fw.dual_level():
+                f(fw.make_dual(at.clone().requires_grad_() if grad else at, torch.ones_like(at)))
+
+        def unrecorded(dual=dual):
+            with torch.no_grad():
+                dual()
+
+        def handed_in(f=f, at=at):
+            leaf = at.clone().requires_grad_()
+            out = f(leaf)
+            out = out if isinstance(out, torch.Tensor) else out[0]
+            with fw.dual_level():
+                torch.autograd.grad(out, leaf, fw.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+        calls += [jvp, dual, lambda dual=dual: dual(grad=True), unrecorded, handed_in]
+    calls.append(lambda: torch.func.jacfwd(lambda z: token_log_probs(z, t).log_probs)(z))
+    return calls
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation would find results without tangents, which it takes for zeros."""
+    for call in _tangent_calls("cpu"):
+        with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|jvp|setup_context"):
+            call()
