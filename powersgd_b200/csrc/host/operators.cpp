@@ -17,6 +17,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <cstdint>
@@ -225,7 +226,7 @@ PyObject* token_log_probs(PyObject*, PyObject* args) {
     const auto index = targets->scalar_type();
     if (!logits->is_cuda() || logits->device() != targets->device() || type_code(logits->scalar_type()) < 0 || (index != at::kLong && index != at::kInt) || vocab < 1 ||
         vocab >= (1ll << 31) - (1 << 16) || logits->sizes().slice(0, logits->dim() - 1) != targets->sizes() || top < 0 || top > 32 || top > vocab ||
-        !(temperature >= 0x1p-100 && temperature <= 0x1p100) || has_tangent(*logits))
+        !(temperature >= 0x1p-100 && temperature <= 0x1p100) || has_tangent(*logits) || torch::jit::tracer::isTracing())
       Py_RETURN_NONE;
     Tensor out[4];
     if (at::GradMode::is_enabled() && logits->requires_grad()) {
@@ -361,7 +362,7 @@ PyObject* packed_attention(PyObject*, PyObject* args) {
         q.size(1) < 1 || q.size(1) % k.size(1) != 0 || q.size(2) < 8 || q.size(2) > 128 || q.size(2) % 8 != 0 || (type != at::kBFloat16 && type != at::kHalf) ||
         k.scalar_type() != type || v.scalar_type() != type || offsets.scalar_type() != at::kInt || offsets.dim() != 1 || offsets.size(0) < 1 ||
         offsets.size(0) > (1ll << 31) - (1 << 16) || q.size(0) >= (1ll << 31) - (1 << 16) || !(scale == 0 || (scale >= 0x1p-100 && scale <= 0x1p100)) || q.get_device() >= MOST_DEVICES ||
-        has_tangent(q) || has_tangent(k) || has_tangent(v))
+        has_tangent(q) || has_tangent(k) || has_tangent(v) || torch::jit::tracer::isTracing())
       Py_RETURN_NONE;
     const Status& status = statuses[q.get_device()];
     if (status.host == nullptr || *status.host != 0) Py_RETURN_NONE;

@@ -48,6 +48,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
 
 def check(q, k, v, offsets, scale) -> None:
+    native.refuse_tracing("packed_attention", q)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together; [tokens, heads, size] is expected")
     heads, groups, size = q.shape[1], k.shape[1], q.shape[2]

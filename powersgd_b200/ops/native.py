@@ -83,6 +83,12 @@ def refuse_tangents(what: str, *tensors) -> None:
         raise NotImplementedError(f"{what}: forward-mode differentiation is not supported")
 
 
+def refuse_tracing(what: str, t: torch.Tensor) -> None:
+    """torch.jit.trace writes down operations of PyTorch: of a native call it would see an empty result and no kernel."""
+    if t.is_cuda and use_for_cuda() and torch._C._get_tracing_state() is not None:
+        raise NotImplementedError(f"{what}: torch.jit.trace does not see native calls")
+
+
 class on_device:
     """`with on_device(device) as stream`: launches for tensors of `device` (an index is given), on its current stream."""
 

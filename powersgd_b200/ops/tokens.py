@@ -47,6 +47,7 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0
 
 
 def check(logits, targets, top, ignore_index, temperature) -> None:
+    native.refuse_tracing("token_log_probs", logits)
     if logits.dtype not in DTYPES and not (logits.dtype == torch.float64 and not logits.is_cuda):
         raise TypeError(f"token_log_probs: logits are {logits.dtype}; float32, bfloat16 and float16 are supported")
     if targets.dtype not in (torch.int64, torch.int32):

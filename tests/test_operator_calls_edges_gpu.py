@@ -25,3 +25,14 @@ def test_tangents_are_refused(form):
     for call in _tangent_calls("cuda"):
         with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|jvp|setup_context"):
             call()
+
+
+@pytest.mark.parametrize("gradient", [False, True])
+def test_tracing_is_refused(form, gradient):
+    """A trace would hold an empty tensor and no kernel."""
+    z, t = torch.randn(3, 8, device="cuda", requires_grad=gradient), torch.tensor([0, 5, -100], device="cuda")
+    x = torch.randn(6, 2, 8, device="cuda").bfloat16().requires_grad_(gradient)
+    offsets = torch.tensor([0, 2, 6], dtype=torch.int32, device="cuda")
+    for f, args in ((lambda z, t: tokens.token_log_probs(z, t).log_probs, (z, t)), (lambda x, o: attention.packed_attention(x, x, x, o), (x, offsets))):
+        with pytest.raises(NotImplementedError, match="jit.trace"):
+            torch.jit.trace(f, args)
