@@ -14,6 +14,7 @@
 #include <ATen/TensorSubclassLikeUtils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -21,7 +22,6 @@
 
 #include <cmath>
 #include <cstdint>
-#include <exception>
 
 namespace {
 
@@ -199,14 +199,12 @@ PyObject* wrap(const Tensor& t) {
   return THPVariable_Wrap(t);
 }
 
+// No C++ exception leaves the module: each becomes the Python exception that PyTorch's own calls raise for it.
 template <class F>
-PyObject* guarded(F body) {   // no C++ exception leaves the module
-  try {
-    return body();
-  } catch (const std::exception& e) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, e.what());
-    return nullptr;
-  }
+PyObject* guarded(F body) {
+  HANDLE_TH_ERRORS
+  return body();
+  END_HANDLE_TH_ERRORS
 }
 
 // token_log_probs(logits, targets, top, entropy, ignore_index, temperature): the four results, or None.

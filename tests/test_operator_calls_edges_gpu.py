@@ -36,3 +36,13 @@ def test_tracing_is_refused(form, gradient):
     for f, args in ((lambda z, t: tokens.token_log_probs(z, t).log_probs, (z, t)), (lambda x, o: attention.packed_attention(x, x, x, o), (x, offsets))):
         with pytest.raises(NotImplementedError, match="jit.trace"):
             torch.jit.trace(f, args)
+
+
+def test_requests_for_too_much_memory_are_told_as_such(form):
+    """Copies and results beyond any GPU's memory: torch.OutOfMemoryError, which programs catch, through either form."""
+    z = torch.zeros(1, 50257, device="cuda", dtype=torch.bfloat16).expand(2**23, 50257)
+    with pytest.raises(torch.OutOfMemoryError):
+        tokens.token_log_probs(z, torch.zeros(2**23, device="cuda", dtype=torch.int32))
+    x = torch.zeros(1, 1, 128, device="cuda", dtype=torch.bfloat16).expand(2**20, 2**13, 128)
+    with pytest.raises(torch.OutOfMemoryError):
+        attention.packed_attention(x, x[:, :1], x[:, :1], torch.tensor([0, 5], device="cuda", dtype=torch.int32))
