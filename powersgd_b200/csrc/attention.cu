@@ -58,6 +58,10 @@ struct AtArgs {
   const void* rest;              // what rounding took from the output, likewise; null where no gradient will be asked for
   const void* grad;              // the gradient of the output, as `g` addresses it
   long long grad_row, grad_head; // its strides
+  const void* value;             // V likewise
+  long long value_row, value_head;
+  int* lengths_v;                // [key heads, tokens], float16: at the first row of each tile an exponent of its longest row of V, see below
+  int* lengths_g;                // [heads, tokens], likewise of dO
   float* lse;                    // [heads, tokens]: log2 of the sum of exponentials, scaled scores
   float* delta;                  // [heads, tokens]
   void *dq, *dk, *dv;
@@ -616,6 +620,96 @@ __device__ __forceinline__ void ab_store_rest(uint32_t at, const float* x, uint3
   tmem_store16(at, w);
 }
 
+// Powers of two, float16. dS is small wherever gradients are: a weight of 1 / 4096 and a gradient of 2^-10 make 2^-19, of which float16, whose normal
+// numbers end at 2^-14, holds five bits. So dS is multiplied with a power of two before it is rounded, which the last scaling takes back:
+//   |dS| <= |P| (|dP| + |delta|) <= 2 |dO_i| max_j |V_j|,
+// and the largest power is taken that keeps this below 2^14. In dQ each row has its own; dK sums over rows, which share that of the longest dO
+// of all that see the tile's keys. (One power for all inputs would have to keep the largest gradients finite.) It rides on operations that
+// are there: in dQ a sum becomes a fused one; in dK, dV it is added to exponents, so that the weights have it too, and only
+// where it is below one are slopes multiplied with it. Rows of what is no number have no say: whatever they touch is none either. bfloat16 has the
+// range of float32 and needs none of this.
+template <typename T>
+constexpr bool AB_SHIFTS = AtType<T>::value == 0;
+constexpr int AB_ROOM = 13;           // 2^(shift + exponents of both lengths + 1) <= 2^14
+constexpr int AB_MOST_SHIFT = 14;     // (weights times 2^14 are finite, and a scale of 2^-100 times 2^-14 is a normal number)
+// The least e for which a vector is shorter than 2^e, from the square of its length; of what is not finite as of zeros.
+__device__ __forceinline__ int ab_exponent(float square) {
+  const int b = (int)(__float_as_uint(square) >> 23 & 0xFF);
+  return b == 0xFF ? -63 : (b - 125) >> 1;
+}
+__device__ __forceinline__ float ab_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ float ab_square(uint4 x, float square) {   // (of eight float16)
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = unpack2<__half>(w[j]);
+    square = fmaf(f.x, f.x, fmaf(f.y, f.y, square));
+  }
+  return square;
+}
+// What the longest rows of V leave of AB_ROOM, and where asked those of dO of the heads that share them, in the tiles from `from` on. A warp asks.
+__device__ __forceinline__ int ab_room(const AtArgs& a, int kv_head, int start, int length, bool gradients, int from) {
+  const int tiles = (length + AT_TILE - 1) / AT_TILE, heads = gradients ? a.group : 0;
+  const int* v = a.lengths_v + (long long)kv_head * a.tokens + start;
+  const int* g = a.lengths_g + (long long)kv_head * a.group * a.tokens + start;
+  int of_v = -63, of_g = -63;
+  for (int i = (int)(threadIdx.x & 31); i < tiles; i += 32) {
+    const int at = i * AT_TILE;
+    of_v = max(of_v, v[at]);
+    if (i < from) continue;
+#pragma unroll 4
+    for (int h = 0; h < heads; ++h) of_g = max(of_g, g[(long long)h * a.tokens + at]);
+  }
+  of_v = __reduce_max_sync(0xffffffffu, of_v);
+  return AB_ROOM - of_v - (gradients ? __reduce_max_sync(0xffffffffu, of_g) : 0);
+}
+
+// Exponents of the rows of V; those of dO come from the pass over the queries, which begins beside this one. (3357 rows of 4 heads of 80: 3.5 us, of which
+// 2.3 are seen; the whole of it, with the weights' powers, takes 131 to 135 us of forward and backward pass.)
+constexpr int AN_THREADS = 256;
+__global__ void __launch_bounds__(AN_THREADS) psgd_attention_lengths_kernel(const __grid_constant__ AtArgs a) {
+  __shared__ int s_most[AN_THREADS / 32], s_found;
+  __shared__ AtPiece s_piece;
+  psgd_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, kv_heads = a.heads / a.group;
+  const int head = blockIdx.x % kv_heads, index = blockIdx.x / kv_heads;
+  if (tid < 32) {
+    AtPiece piece = {0, 0, 0, 0, 0};
+    const bool found = at_find(a, AT_TILE, index, false, piece);
+    if (lane == 0) {
+      s_piece = piece;
+      s_found = found;
+    }
+  }
+  __syncthreads();
+  if (!s_found) return;
+  constexpr int LOADS = AT_TILE / (AN_THREADS / 16);       // 16 lanes to a row
+  const long long row0 = s_piece.start + (long long)s_piece.piece * AT_TILE;
+  const int rows = min(AT_TILE, s_piece.length - s_piece.piece * AT_TILE), c = tid % 16 * 8;
+  const __half* v = (const __half*)a.value + head * a.value_head + row0 * a.value_row + c;
+  uint4 x[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int r = tid / 16 + i * (AN_THREADS / 16);
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (r < rows && c < a.size) x[i] = *reinterpret_cast<const uint4*>(v + r * a.value_row);
+  }
+  int e = -63;
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    float square = ab_square(x[i], 0.f);
+#pragma unroll
+    for (int by = 8; by > 0; by >>= 1) square += __shfl_xor_sync(0xffffffffu, square, by);
+    e = max(e, ab_exponent(square));
+  }
+  e = __reduce_max_sync(0xffffffffu, e);
+  if (lane == 0) s_most[tid / 32] = e;
+  __syncthreads();
+  if (tid != 0) return;
+  for (int w = 1; w < AN_THREADS / 32; ++w) e = max(e, s_most[w]);
+  a.lengths_v[(long long)head * a.tokens + row0] = e;
+}
+
 // dQ: tensor memory holds, per chain, S and dP (64 columns each; dS takes the first half of dP's place), and dQ. S of a chain's next step is
 // multiplied as soon as this one is in registers, its dP behind dQ of this one.
 template <typename T, int PANELS>
@@ -630,6 +724,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
   uint8_t* s_ring = base + 2 * TILE_BYTES;   // stage: K, V
   __shared__ __align__(8) AbBars<CHAINS, STAGES> bars;
   __shared__ float s_delta[AT_TILE];
+  __shared__ int s_exponent[AB_SHIFTS<T> ? AT_TILE : 1], s_room;      // float16: of the rows of dO; AB_ROOM without the longest row of V
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort, s_found;
   __shared__ AtPiece s_piece;
@@ -656,6 +751,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
   umma_fence_after();
   at_clear_outside<T>(a, s_piece, (T*)a.dq, a.heads, head, index);
   if (!s_found) {
+    if (AB_SHIFTS<T>) psgd_wait_for_predecessor();
     if (warp == ISSUER) tmem_free(s_tmem, COLUMNS);
     return;
   }
@@ -674,11 +770,19 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       for (int j = 0; j < steps; ++j) {
         const int slot = j % STAGES;
         if (!wait(&bars.empty[slot], ((j / STAGES) & 1) ^ 1)) break;
-        if (lane != 0) continue;
-        psgd_mbar_expect_tx(&bars.full[slot], 2 * HALF);
-        const uint32_t at = psgd_smem_u32(s_ring + slot * TILE_BYTES);
-        at_load_tile<PANELS, AT_STEP>(at, &a.k, head / a.group, start + j * AT_STEP, &bars.full[slot]);
-        at_load_tile<PANELS, AT_STEP>(at + HALF, &a.v, head / a.group, start + j * AT_STEP, &bars.full[slot]);
+        if (lane == 0) {
+          psgd_mbar_expect_tx(&bars.full[slot], 2 * HALF);
+          const uint32_t at = psgd_smem_u32(s_ring + slot * TILE_BYTES);
+          at_load_tile<PANELS, AT_STEP>(at, &a.k, head / a.group, start + j * AT_STEP, &bars.full[slot]);
+          at_load_tile<PANELS, AT_STEP>(at + HALF, &a.v, head / a.group, start + j * AT_STEP, &bars.full[slot]);
+        }
+        if (AB_SHIFTS<T> && j == min(STAGES, steps) - 1) {   // nothing has been waited for yet
+          psgd_wait_for_predecessor();
+          const int room = ab_room(a, head / a.group, start, length, false, 0);
+          if (lane == 0) s_room = room;
+          __syncwarp();
+          asm volatile("bar.arrive 1, %0;" ::"n"(256 * CHAINS + 32) : "memory");
+        }
       }
     }
   } else if (warp == ISSUER) {
@@ -752,11 +856,12 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
         if (in) y[i] = *reinterpret_cast<const uint4*>((const T*)a.grad + (long long)(start + q0 + r) * a.grad_row + (long long)head * a.grad_head + c);
         if (in) z[i] = *reinterpret_cast<const uint4*>((const T*)a.rest + at);
       }
-      float sums[ROWS / 4];
+      float sums[ROWS / 4], squares[ROWS / 4];
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
         const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w}, ys[4] = {y[i].x, y[i].y, y[i].z, y[i].w}, zs[4] = {z[i].x, z[i].y, z[i].z, z[i].w};
-        if (i % PANELS == 0) sums[i / PANELS] = 0.f;
+        if (i % PANELS == 0) sums[i / PANELS] = squares[i / PANELS] = 0.f;
+        if (AB_SHIFTS<T>) squares[i / PANELS] = ab_square(y[i], squares[i / PANELS]);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float2 u = unpack2<T>(xs[e]), v = unpack2<T>(ys[e]), w = unpack2<T>(zs[e]);
@@ -769,10 +874,19 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
 #pragma unroll
         for (int by = 4; by > 0; by >>= 1) sums[i] += __shfl_xor_sync(0xffffffffu, sums[i], by);
         if ((lane & 7) == 0) s_delta[warp * ROWS + i * 4 + (lane >> 3)] = sums[i];
+        if (AB_SHIFTS<T>) {
+#pragma unroll
+          for (int by = 4; by > 0; by >>= 1) squares[i] += __shfl_xor_sync(0xffffffffu, squares[i], by);
+          if ((lane & 7) == 0) s_exponent[warp * ROWS + i * 4 + (lane >> 3)] = ab_exponent(squares[i]);
+        }
       }
     }
-    asm volatile("bar.sync 1, %0;" ::"n"(256 * CHAINS) : "memory");
-    const float delta = s_delta[row];
+    asm volatile("bar.sync 1, %0;" ::"n"(256 * CHAINS + (AB_SHIFTS<T> ? 32 : 0)) : "memory");
+    const float delta = s_delta[row], power = AB_SHIFTS<T> ? ab_power(min(s_room - s_exponent[row], AB_MOST_SHIFT)) : 1.f;
+    if (AB_SHIFTS<T> && warp == 0) {
+      const int e = __reduce_max_sync(0xffffffffu, max(max(s_exponent[lane], s_exponent[lane + 32]), max(s_exponent[lane + 64], s_exponent[lane + 96])));
+      if (lane == 0) a.lengths_g[(long long)head * a.tokens + start + q0] = e;
+    }
     if (held && warp < 4) a.delta[stat] = delta;
     const int limit = (a.causal ? q : length - 1) - half * AB_WIDE;    // last key that counts, from this thread's first on
     bool ok = true;
@@ -795,14 +909,15 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       ok = wait(&bars.dp[chain], parity);
       if (!ok) break;
       umma_fence_after();
-      const float2 minus = make_float2(-delta, -delta);
+      const float2 times = make_float2(power, power), minus = make_float2(-delta * power, -delta * power);
       float d[AB_WIDE];
       tmem_load32(dp_at, d);
       tmem_load_wait<AB_WIDE>(d);
       uint32_t w[16];
 #pragma unroll
       for (int i = 0; i < AB_WIDE; i += 2) {
-        const float2 x = mul2(make_float2(p[i], p[i + 1]), add2(make_float2(d[i], d[i + 1]), minus));
+        const float2 slope = make_float2(d[i], d[i + 1]);
+        const float2 x = mul2(make_float2(p[i], p[i + 1]), AB_SHIFTS<T> ? fma2(slope, times, minus) : add2(slope, minus));
         w[i / 2] = pack2<T>(x.x, x.y);
         d[i] = x.x;
         d[i + 1] = x.y;
@@ -817,7 +932,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       umma_fence_after();
       const int first = q0 + (warp & 3) * 32, panel = CHAINS == 2 ? half : 0;     // heads of more than 64: half of them each
       if (chain == 0 && half < PANELS)
-        at_write_rows<T, 1>(tmem + lanes + DQ + panel * 64, a.scale, s_q + (panel * 4 + (warp & 3)) * 4096,
+        at_write_rows<T, 1>(tmem + lanes + DQ + panel * 64, a.scale / power, s_q + (panel * 4 + (warp & 3)) * 4096,
                             (T*)a.dq + ((long long)(start + first) * a.heads + head) * a.size + panel * 64, (T*)nullptr, (long long)a.heads * a.size, length - first,
                             a.size - panel * 64);
     }
@@ -856,7 +971,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
   uint8_t* s_stats = s_ones + AB_ONES;       // stage: logarithms, deltas
   __shared__ __align__(8) AbBars<CHAINS, STAGES> bars;
   __shared__ uint32_t s_tmem;
-  __shared__ int s_abort, s_found;
+  __shared__ int s_abort, s_found, s_shift;
   __shared__ AtPiece s_piece;
 
   const int tid = threadIdx.x, warp = warp_uniform(tid >> 5), lane = tid & 31;
@@ -1020,6 +1135,15 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
     next(step, chain);
     bool ok = true;
     int mine = 0;                   // steps of this chain so far
+    if (AB_SHIFTS<T>) {
+      if (warp == 0) {              // (beside the warp that loads, which waits for the statistics)
+        psgd_wait_for_predecessor();
+        const int room = ab_room(a, head, start, length, true, first * AT_STEP / AT_TILE);
+        if (lane == 0) s_shift = min(room, AB_MOST_SHIFT);
+      }
+      asm volatile("bar.sync 1, %0;" ::"n"(256 * CHAINS) : "memory");
+    }
+    const int shift = AB_SHIFTS<T> ? s_shift : 0, lift = max(shift, 0);     // of dS, of P
     for (int i = chain; i < steps; i += CHAINS, ++mine, next(step, CHAINS)) {
       const int q0 = step.row + half * AB_WIDE;      // this thread's first query
       ok = wait(&bars.s[chain], mine & 1);
@@ -1030,7 +1154,8 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       tmem_load_wait<AB_WIDE>(p);
 #pragma unroll
       for (int c = 0; c < AB_WIDE; c += 2) {
-        const float2 y = mul2(make_float2(p[c], p[c + 1]), make_float2(a.scale2, a.scale2));
+        const float2 x = make_float2(p[c], p[c + 1]), factor = make_float2(a.scale2, a.scale2);
+        const float2 y = AB_SHIFTS<T> ? fma2(x, factor, make_float2((float)lift, (float)lift)) : mul2(x, factor);
         p[c] = at_exp2(y.x);
         p[c + 1] = at_exp2(y.y);
       }
@@ -1044,6 +1169,11 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       uint32_t w[16];
 #pragma unroll
       for (int e = 0; e < AB_WIDE; e += 2) w[e / 2] = pack2<T>(p[e], p[e + 1]);
+      if (AB_SHIFTS<T> && shift < lift) {
+        const float less = ab_power(shift - lift);
+#pragma unroll
+        for (int e = 0; e < AB_WIDE; ++e) p[e] *= less;
+      }
       tmem_store16(s_at, w);
       tmem_store_wait();
       at_arrive(&bars.p[chain]);
@@ -1073,7 +1203,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       const uint32_t at = tmem + lanes + (which == 0 ? DV : DK) + panel * 64;
       if (a.split == 1) {
         const int first_row = k0 + (warp & 3) * 32;
-        at_write_rows<T, 1>(at, which == 0 ? 1.f : a.scale, (which == 0 ? s_v : s_k) + (panel * 4 + (warp & 3)) * 4096,
+        at_write_rows<T, 1>(at, which == 0 ? 1.f / ab_power(lift) : a.scale / ab_power(shift), (which == 0 ? s_v : s_k) + (panel * 4 + (warp & 3)) * 4096,
                             (T*)(which == 0 ? a.dv : a.dk) + ((long long)(start + first_row) * kv_heads + head) * a.size + panel * 64, (T*)nullptr,
                             (long long)kv_heads * a.size, length - first_row, a.size - panel * 64);
       } else {
@@ -1119,7 +1249,8 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
         sum.z += x.z;
         sum.w += x.w;
       }
-      const float f = which == 0 ? 1.f : a.scale;
+      const int shift = AB_SHIFTS<T> ? s_shift : 0;      // (the same in all blocks)
+      const float f = which == 0 ? 1.f / ab_power(max(shift, 0)) : a.scale / ab_power(shift);
       T* out = (T*)(which == 0 ? a.dv : a.dk) + ((long long)(start + k0 + r) * kv_heads + head) * a.size + c;
       *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(sum.x * f, sum.y * f), pack2<T>(sum.z * f, sum.w * f));
     }
@@ -1218,8 +1349,11 @@ int at_backward(AtArgs a, cudaStream_t stream) {
   static unsigned long long q_devices = 0, kv_devices = 0;
   if (const int code = psgd_allow_shared((const void*)psgd_attention_dq_kernel<T, PANELS>, ab_shared(PANELS, 0), q_devices)) return code;
   if (const int code = psgd_allow_shared((const void*)psgd_attention_dkv_kernel<T, PANELS>, ab_shared(PANELS, AB_ONES + ab_stages(PANELS) * AB_STATS), kv_devices)) return code;
+  if constexpr (AB_SHIFTS<T>) {
+    if (const int code = psgd_launch(psgd_attention_lengths_kernel, a.blocks * (a.heads / a.group), AN_THREADS, 0, stream, 0, a)) return code;
+  }
   // (delta comes from the first)
-  if (const int code = psgd_launch(psgd_attention_dq_kernel<T, PANELS>, a.blocks * a.heads, ab_threads(PANELS), ab_shared(PANELS, 0), stream, 0, a)) return code;
+  if (const int code = psgd_launch(psgd_attention_dq_kernel<T, PANELS>, a.blocks * a.heads, ab_threads(PANELS), ab_shared(PANELS, 0), stream, AB_SHIFTS<T>, a)) return code;
   const int kv_heads = a.heads / a.group;
   a.split = 1;
   for (int split = 2; split <= AB_MOST_SPLIT && split <= a.group && (long long)a.blocks * kv_heads * a.split < AB_ENOUGH; ++split)
@@ -1249,7 +1383,7 @@ PSGD_API int psgd_attention(const void* q, const void* k, const void* v, const l
   return size <= 64 ? at_forward<__half, 1>(a, stream) : at_forward<__half, 2>(a, stream);
 }
 
-// strides: those of q, k, v and of the output's gradient. delta: scratch, [heads, tokens]. dq, dk, dv are contiguous.
+// strides: those of q, k, v and of the output's gradient. delta: scratch, [2 heads + key heads, tokens] words. dq, dk, dv are contiguous.
 PSGD_API int psgd_attention_backward(const void* q, const void* k, const void* v, const void* grad, const long long* strides, const int* offsets, int sequences,
                                      int tokens, int heads, int kv_heads, int size, int dtype, int causal, float scale, const void* out, const void* rest, const float* lse,
                                      float* delta, void* dq, void* dk, void* dv, int* plan, int* status, cudaStream_t stream) {
@@ -1263,6 +1397,11 @@ PSGD_API int psgd_attention_backward(const void* q, const void* k, const void* v
   a.grad_head = strides[7];
   a.lse = (float*)lse;
   a.delta = delta;
+  a.lengths_g = (int*)(delta + (long long)heads * tokens);
+  a.lengths_v = a.lengths_g + (long long)heads * tokens;
+  a.value = v;
+  a.value_row = strides[4];
+  a.value_head = strides[5];
   a.dq = dq;
   a.dk = dk;
   a.dv = dv;

@@ -150,7 +150,7 @@ def _backward(q, k, v, offsets, out, lse, rest, grad, causal, scale):
     dv = torch.empty_like(dk)
     if tokens == 0 or sequences == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    delta = torch.empty((heads, tokens), dtype=torch.float32, device=q.device)
+    delta = torch.empty((2 * heads + groups, tokens), dtype=torch.float32, device=q.device)   # scratch
     q, k, v, grad, offsets, plan = _usable(q), _usable(k), _usable(v), _usable(grad), offsets.contiguous(), _plan(sequences, tokens, q.device)
     with native.on_device(q.device) as stream:
         code = native.lib().psgd_attention_backward(
