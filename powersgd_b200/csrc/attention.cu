@@ -625,8 +625,9 @@ __device__ __forceinline__ void ab_store_rest(uint32_t at, const float* x, uint3
 //   |dS| <= |P| (|dP| + |delta|) <= 2 |dO_i| max_j |V_j|,
 // and the largest power is taken that keeps this below 2^14. In dQ each row has its own; dK sums over rows, which share that of the longest dO
 // of all that see the tile's keys. (One power for all inputs would have to keep the largest gradients finite.) It rides on operations that
-// are there: in dQ a sum becomes a fused one; in dK, dV it is added to exponents, so that the weights have it too, and only
-// where it is below one are slopes multiplied with it. Rows of what is no number have no say: whatever they touch is none either. bfloat16 has the
+// are there: in dQ a sum becomes a fused one; in dK, dV it is added to exponents, so that the weights have it too. Those are small in long
+// sequences, 1 / length as a rule: their power is at least the one that brings this to 2^-10, and where it is above that of dS what dS is made of
+// is multiplied with the difference. Rows of what is no number have no say: whatever they touch is none either. bfloat16 has the
 // range of float32 and needs none of this.
 template <typename T>
 constexpr bool AB_SHIFTS = AtType<T>::value == 0;
@@ -638,6 +639,7 @@ __device__ __forceinline__ int ab_exponent(float square) {
   return b == 0xFF ? -63 : (b - 125) >> 1;
 }
 __device__ __forceinline__ float ab_power(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ int ab_lift(int shift, int length) { return max(max(shift, 0), min(22 - __clz(length), AB_MOST_SHIFT)); }   // of P
 __device__ __forceinline__ float ab_square(uint4 x, float square) {   // (of eight float16)
   const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
@@ -1143,7 +1145,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
       }
       asm volatile("bar.sync 1, %0;" ::"n"(256 * CHAINS) : "memory");
     }
-    const int shift = AB_SHIFTS<T> ? s_shift : 0, lift = max(shift, 0);     // of dS, of P
+    const int shift = AB_SHIFTS<T> ? s_shift : 0, lift = AB_SHIFTS<T> ? ab_lift(shift, length) : 0;     // of dS, of P
     for (int i = chain; i < steps; i += CHAINS, ++mine, next(step, CHAINS)) {
       const int q0 = step.row + half * AB_WIDE;      // this thread's first query
       ok = wait(&bars.s[chain], mine & 1);
@@ -1250,7 +1252,7 @@ __global__ void __launch_bounds__(ab_threads(PANELS), 3 - PANELS) psgd_attention
         sum.w += x.w;
       }
       const int shift = AB_SHIFTS<T> ? s_shift : 0;      // (the same in all blocks)
-      const float f = which == 0 ? 1.f / ab_power(max(shift, 0)) : a.scale / ab_power(shift);
+      const float f = which == 0 ? 1.f / ab_power(AB_SHIFTS<T> ? ab_lift(shift, length) : 0) : a.scale / ab_power(shift);
       T* out = (T*)(which == 0 ? a.dv : a.dk) + ((long long)(start + k0 + r) * kv_heads + head) * a.size + c;
       *reinterpret_cast<uint2*>(out) = make_uint2(pack2<T>(sum.x * f, sum.y * f), pack2<T>(sum.z * f, sum.w * f));
     }

@@ -163,3 +163,20 @@ def test_half_precision_rows_that_are_no_numbers(bad):
     v[650] = bad
     got = dq()
     assert torch.equal(got[:512], want[:512]) and torch.equal(got[700:], want[700:])     # (tiles of 128 queries, see the call's notes)
+
+
+@pytest.mark.parametrize("size, heads, groups", [(16, 1, 1), (128, 2, 1)])
+@pytest.mark.parametrize("length, gradients", [(3 * 2**16 + 5, 64.0), (20000, 64.0), (20000, 0.001), (5, 64.0)])
+def test_half_precision_weights_of_long_sequences(length, gradients, size, heads, groups):
+    """Queries of zeros: all weights are 1 / length, dV is the mean of the gradients. A weight and the result are rounded, 2^-11 each; scores add 2^-12. The
+    tensor cores add 16 terms at a time to a sum in 32 bits and may cut what does not fit, 2^-23 of it. All terms are equal and all cuts go one way: n / 16 of
+    them, of a sum that is half of the last one on average, make n 2^-28 (twice 196613 terms are 2^-9.4)."""
+    q, k, v, _ = _inputs(length, heads, groups, size, torch.float16)
+    q.zero_()
+    g = torch.full_like(q, gradients)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = packed_attention(*leaves, _offsets([length]), causal=False)
+    dv, = torch.autograd.grad(out, leaves[2:], g)
+    want = g[0, 0, 0].double() * heads / groups
+    off = 2.0**-10 + 2.0**-12 + length * heads / groups * 2.0**-28
+    assert ((dv.double() - want).abs() <= off * want).all(), ((dv.double() - want).abs().max() / want).item()
