@@ -92,6 +92,8 @@ int64_t row_stride(const Tensor& t) {
   if (stride < 0) return vocab;   // one row
   return stride >= vocab ? stride : -1;
 }
+// The numbers that a tensor stands for, in memory: some only say that what they refer to is to be negated, or that all of it is zero.
+Tensor in_memory(const Tensor& t) { return t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.resolve_neg(); }
 // `t`, or a contiguous copy where its rows do not lie as the kernels take them.
 Tensor as_rows(const Tensor& t, int64_t& stride) {
   stride = row_stride(t);
@@ -177,7 +179,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
         grad = at::empty({lead + n * pitch}, z.options()).as_strided(logits.sizes(), strides, lead);
       }
       if (n > 0) {
-        auto f32 = [](const Tensor& x) { return x.defined() ? x.to(at::kFloat).contiguous() : x; };
+        auto f32 = [](const Tensor& x) { return x.defined() ? in_memory(x).to(at::kFloat).contiguous() : x; };
         auto at_of = [](const Tensor& x) { return x.defined() ? (const float*)x.const_data_ptr() : nullptr; };
         g = f32(g), g_entropy = f32(g_entropy), g_top = f32(g_top);
         check(entry.token_grad(z.const_data_ptr(), type_code(z.scalar_type()), n, (int)vocab, stride, grad.data_ptr(), pitch, t.const_data_ptr(),
@@ -319,7 +321,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
         dq.zero_(), dk.zero_(), dv.zero_();
       } else {
         const Tensor q = usable(saved[0]), k = usable(saved[1]), v = usable(saved[2]), offsets = saved[3].contiguous();
-        const Tensor plan = plan_of(offsets.size(0) - 1, tokens, q), g = usable(grads[0]), delta = at::empty({2 * heads + groups, tokens}, lse.options());
+        const Tensor plan = plan_of(offsets.size(0) - 1, tokens, q), g = usable(in_memory(grads[0])), delta = at::empty({2 * heads + groups, tokens}, lse.options());
         long long strides[8];
         strides_of(q, strides);
         strides_of(k, strides + 2);

@@ -217,7 +217,7 @@ PyObject* adam_items(PyObject*, PyObject* args) {
         type = p->scalar_type();
       }
       if (!p->is_cuda() || p->get_device() != device || p->scalar_type() != type || !p->is_non_overlapping_and_dense()) Py_RETURN_NONE;
-      if (g.layout() != at::kStrided || !g.unsafeGetTensorImpl()->has_storage() || at::isTensorSubclassLike(g)) Py_RETURN_NONE;
+      if (g.layout() != at::kStrided || !g.unsafeGetTensorImpl()->has_storage() || at::isTensorSubclassLike(g) || g.is_neg() || g._is_zerotensor()) Py_RETURN_NONE;
       if (g.scalar_type() != type || !g.is_cuda() || g.get_device() != device || !same_layout(g, *p)) Py_RETURN_NONE;
       PyObject* own = PyDict_GetItemWithError(state, params[i]);
       if (own == nullptr || !PyDict_Check(own)) {

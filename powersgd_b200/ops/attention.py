@@ -96,6 +96,7 @@ def _status(device: torch.device):
 
 def _usable(t: torch.Tensor) -> torch.Tensor:
     """As the kernels address it: elements of a head side by side, rows and heads on 16-byte boundaries and apart. A copy if need be."""
+    t = native.in_memory(t)
     tokens, heads, size = t.shape
     row, head, one = t.stride()
     if (one == 1 or size == 1) and t.data_ptr() % 16 == 0 and (tokens == 1 or (row % 8 == 0 and row >= size)) and (heads == 1 or (head % 8 == 0 and head >= size)):

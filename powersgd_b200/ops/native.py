@@ -89,6 +89,12 @@ def refuse_tracing(what: str, t: torch.Tensor) -> None:
         raise NotImplementedError(f"{what}: torch.jit.trace does not see native calls")
 
 
+def in_memory(t: torch.Tensor) -> torch.Tensor:
+    """The numbers that a tensor stands for: some only say that what they refer to is to be negated (the imaginary part of a conjugate),
+    or that all of it is zero. Kernels read memory."""
+    return torch.zeros_like(t) if t._is_zerotensor() else t.resolve_neg()
+
+
 class on_device:
     """`with on_device(device) as stream`: launches for tensors of `device` (an index is given), on its current stream."""
 

@@ -70,7 +70,7 @@ def check(logits, targets, top, ignore_index, temperature) -> None:
 
 def _rows(logits: torch.Tensor) -> torch.Tensor:
     """The logits as [rows, vocabulary] with elements of a row side by side and rows apart: a view where they lie so, else a copy."""
-    vocab = logits.shape[-1]
+    logits, vocab = native.in_memory(logits), logits.shape[-1]
     if logits.is_contiguous():
         return logits.view(-1, vocab)
     if logits.stride(-1) == 1 or vocab == 1:
@@ -117,7 +117,7 @@ def _backward(logits, targets, stats, entropy, tokens, g, g_entropy, g_top, igno
     n, vocab = z.shape
     grad, rows = _grad_like(logits, z)
     if n:
-        g, g_entropy, g_top = (None if x is None else x.contiguous() for x in (g, g_entropy, g_top))
+        g, g_entropy, g_top = (None if x is None else native.in_memory(x).contiguous() for x in (g, g_entropy, g_top))
         at = lambda x: None if x is None else x.data_ptr()  # noqa: E731
         with native.on_device(logits.device) as stream:
             code = native.lib().psgd_token_logprob_grad(

@@ -142,6 +142,8 @@ class AdamW(torch.optim.Optimizer):
                     with outside_capture(p.device) if p.is_cuda else _nothing():
                         state.update(_adamw.new_state(p, bits))
                 g = p.grad
+                if g.layout == torch.strided:
+                    g = native.in_memory(g)
                 if g.layout == torch.strided and g.dtype == p.dtype and not _adamw.laid_like(g, p):
                     g = torch.empty_like(p, memory_format=torch.preserve_format).copy_(g)
                 lists.setdefault((p.device, p.dtype), []).append((p, g, state, at))

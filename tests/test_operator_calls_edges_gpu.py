@@ -4,7 +4,8 @@ import pytest
 import torch
 from test_operator_edges_cpu import _tangent_calls
 
-from powersgd_b200.ops import attention, host, tokens
+from powersgd_b200 import AdamW
+from powersgd_b200.ops import attention, host, scan, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -46,3 +47,52 @@ def test_requests_for_too_much_memory_are_told_as_such(form):
     x = torch.zeros(1, 1, 128, device="cuda", dtype=torch.bfloat16).expand(2**20, 2**13, 128)
     with pytest.raises(torch.OutOfMemoryError):
         attention.packed_attention(x, x[:, :1], x[:, :1], torch.tensor([0, 5], device="cuda", dtype=torch.int32))
+
+
+def _negated(x):
+    """-x as a tensor that only says so, as the imaginary part of a conjugate does."""
+    assert torch.complex(x, x).conj().imag.is_neg()
+    return torch._neg_view(x)
+
+
+def test_tensors_that_only_say_that_they_are_negated(form):
+    z, t = torch.randn(3, 80, device="cuda"), torch.tensor([0, 5, -100], device="cuda")
+
+    def both(z, g):
+        leaf = z.detach().requires_grad_()
+        r = tokens.token_log_probs(leaf, t, entropy=True)
+        return [r.log_probs, r.entropy, *torch.autograd.grad((r.log_probs, r.entropy), leaf, (g, g))]
+
+    g = torch.randn(3, device="cuda")
+    for got in (both(_negated(z), g), both((-z).requires_grad_(), _negated(-g))):
+        assert all(torch.equal(a, b) for a, b in zip(both(-z, g), got))
+    zero = torch._efficientzerotensor((3,), device="cuda")
+    assert (both(z, zero)[2] == 0).all()
+
+    x, g = torch.randn(6, 2, 8, device="cuda").half(), torch.randn(6, 2, 8, device="cuda").half()
+    offsets = torch.tensor([0, 2, 6], dtype=torch.int32, device="cuda")
+
+    def grads(x, g):
+        leaf = x.detach().requires_grad_()
+        out = attention.packed_attention(leaf, leaf, leaf, offsets)
+        return [out, *torch.autograd.grad(out, leaf, g)]
+
+    for got in (grads(torch._neg_view(x), g), grads(-x, torch._neg_view(-g))):
+        assert all(torch.equal(a, b) for a, b in zip(grads(-x, g), got))
+    assert (grads(x, torch._efficientzerotensor(x.shape, device="cuda", dtype=x.dtype))[1] == 0).all()
+
+
+@pytest.mark.parametrize("listed", [True, False])
+def test_gradients_that_only_say_that_they_are_negated(listed, monkeypatch):
+    if not listed:
+        monkeypatch.setattr(scan, "_native", None)
+    start, g = torch.randn(300, device="cuda"), torch.randn(300, device="cuda")
+    results = []
+    for grad in (-g, _negated(g)):
+        p = torch.nn.Parameter(start.clone())
+        optimizer = AdamW([p], lr=0.1)
+        for _ in range(2):      # the first step makes the state
+            p.grad = grad
+            optimizer.step()
+        results.append(p.detach())
+    assert torch.equal(*results)
