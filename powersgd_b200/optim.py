@@ -175,9 +175,13 @@ class AdamW(torch.optim.Optimizer):
         keep_with_graph(self._held, *params, *[t for s in states for t in s.values()], ticket, group["lr"])
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As in `torch.optim`, except that moments and numbers of steps keep their own types."""
-        super().load_state_dict(state_dict)
+        """As in `torch.optim`, except that moments and numbers of steps keep their own types. What is refused changes nothing."""
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for group, own in zip(state_dict["param_groups"], self.param_groups):
+            if group.get("amsgrad") or group.get("maximize"):
+                raise ValueError("AdamW: a state of torch.optim.AdamW with amsgrad or maximize does not carry over")
+            self._check({**self.defaults, **group, "params": own["params"]})
+        super().load_state_dict(state_dict)
         for i, p in zip(saved, params_in_optimizer(self)):
             for name, value in state_dict["state"].get(i, {}).items():
                 if name == "step":      # (a number in old states)
@@ -186,11 +190,8 @@ class AdamW(torch.optim.Optimizer):
                     dtype = torch.float32 if name in ("exp_avg", "exp_avg_sq") and value.dtype in (torch.bfloat16, torch.float16) else value.dtype
                     self.state[p][name] = value.to(p.device, dtype, copy=True)
         for group in self.param_groups:
-            if group.get("amsgrad") or group.get("maximize"):
-                raise ValueError("AdamW: a state of torch.optim.AdamW with amsgrad or maximize does not carry over")
             for name, value in self.defaults.items():   # what a state of torch.optim.AdamW does not have
                 group.setdefault(name, value)
-            self._check(group)
 
 
 class _nothing:

@@ -1,7 +1,10 @@
 """token_log_probs, packed_attention and AdamW where they can go wrong, in their forms on the CPU."""
+import copy
+
 import pytest
 import torch
 
+from powersgd_b200 import AdamW
 from powersgd_b200.ops.attention import packed_attention
 from powersgd_b200.ops.tokens import token_log_probs
 
@@ -60,3 +63,25 @@ def test_tangents_are_refused():
     for call in _tangent_calls("cpu"):
         with pytest.raises((NotImplementedError, RuntimeError), match="forward-mode|jvp|setup_context"):
             call()
+
+
+@pytest.mark.parametrize("change, error", [(dict(amsgrad=True), ValueError), (dict(maximize=True), ValueError), (dict(lr=-1.0), ValueError),
+                                           (dict(betas=(0.9, 1.0)), ValueError), (dict(state_bits=16), ValueError), (dict(seed=-1), ValueError)])
+def test_a_state_that_is_refused_changes_nothing(change, error):
+    def optimizer(lr):
+        p = [torch.nn.Parameter(torch.ones(5)), torch.nn.Parameter(torch.ones(3))]
+        opt = AdamW([dict(params=p[:1]), dict(params=p[1:], lr=0.5)], lr=lr)
+        for x in p:
+            x.grad = torch.full_like(x, lr)
+        opt.step()
+        return opt
+
+    a, state = optimizer(0.1), copy.deepcopy(optimizer(0.2).state_dict())
+    before = copy.deepcopy(a.state_dict())
+    state["param_groups"][1].update(change)
+    with pytest.raises(error):
+        a.load_state_dict(state)
+    after = a.state_dict()
+    assert after["param_groups"] == before["param_groups"]
+    for i, moments in before["state"].items():
+        assert all(torch.equal(x, after["state"][i][name]) for name, x in moments.items())
