@@ -67,6 +67,15 @@ def laid_like(t: torch.Tensor, p: torch.Tensor) -> bool:
     return t.shape == p.shape and all(n == 1 or a == b for n, a, b in zip(p.shape, t.stride(), p.stride()))
 
 
+def lay_like(state: dict, p: torch.Tensor) -> None:
+    """Moments in 32 bits in the order of their parameter's dimensions, which may have changed (a model that became channels_last, a state
+    saved before it did). Recorded graphs keep what they refer to."""
+    for name in state_names(32):
+        t = state.get(name)
+        if t is not None and t.shape == p.shape and not laid_like(t, p):
+            state[name] = torch.empty_like(p, dtype=t.dtype, memory_format=torch.preserve_format).copy_(t)
+
+
 def check_lists(params, grads, moments, steps, bits: int) -> None:
     names = state_names(bits)
     for i, p in enumerate(params):
@@ -84,7 +93,8 @@ def check_lists(params, grads, moments, steps, bits: int) -> None:
             dtype = torch.float32 if bits == 32 or scale else torch.float8_e4m3fn
             fits = t.numel() == blocks_of(p.numel()) and t.is_contiguous() if scale else laid_like(t, p)
             if t.dtype != dtype or t.device != p.device or not fits:
-                raise ValueError(f"AdamW: {name} of parameter {i} is {t.dtype} {tuple(t.shape)} on {t.device}; expected {dtype} for {tuple(p.shape)} on {p.device}")
+                raise ValueError(f"AdamW: {name} of parameter {i} is {t.dtype} {tuple(t.shape)}, strides {t.stride()}, on {t.device}; expected {dtype} for "
+                                 f"{tuple(p.shape)}, strides {p.stride()}, on {p.device}")
         if steps[i].dtype != torch.float32 or steps[i].numel() != 1 or steps[i].device != p.device:
             raise ValueError(f"AdamW: the number of steps of parameter {i} must be one float32 on {p.device}")
 

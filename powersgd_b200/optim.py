@@ -141,6 +141,8 @@ class AdamW(torch.optim.Optimizer):
                 if not state:
                     with outside_capture(p.device) if p.is_cuda else _nothing():
                         state.update(_adamw.new_state(p, bits))
+                elif bits == 32 and not (p.is_cuda and torch.cuda.is_current_stream_capturing()):
+                    _adamw.lay_like(state, p)
                 g = p.grad
                 if g.layout == torch.strided:
                     g = native.in_memory(g)
@@ -175,7 +177,8 @@ class AdamW(torch.optim.Optimizer):
         keep_with_graph(self._held, *params, *[t for s in states for t in s.values()], ticket, group["lr"])
 
     def load_state_dict(self, state_dict: dict) -> None:
-        """As in `torch.optim`, except that moments and numbers of steps keep their own types. What is refused changes nothing."""
+        """As in `torch.optim`, except that moments and numbers of steps keep their own types. What is refused changes nothing. Moments in 32 bits
+        take the order of dimensions that their parameter has; those in 8 bits share scales in the order that they were saved in and keep it."""
         saved = [i for group in state_dict["param_groups"] for i in group["params"]]
         for group, own in zip(state_dict["param_groups"], self.param_groups):
             if group.get("amsgrad") or group.get("maximize"):

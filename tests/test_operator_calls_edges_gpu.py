@@ -2,7 +2,7 @@
 refuse, raise and answer alike."""
 import pytest
 import torch
-from test_operator_edges_cpu import _tangent_calls
+from test_operator_edges_cpu import _tangent_calls, check_orders_of_dimensions
 
 from powersgd_b200 import AdamW
 from powersgd_b200.ops import attention, host, scan, tokens
@@ -96,3 +96,7 @@ def test_gradients_that_only_say_that_they_are_negated(listed, monkeypatch):
             optimizer.step()
         results.append(p.detach())
     assert torch.equal(*results)
+
+
+def test_orders_of_dimensions():
+    check_orders_of_dimensions("cuda")

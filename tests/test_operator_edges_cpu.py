@@ -85,3 +85,38 @@ def test_a_state_that_is_refused_changes_nothing(change, error):
     assert after["param_groups"] == before["param_groups"]
     for i, moments in before["state"].items():
         assert all(torch.equal(x, after["state"][i][name]) for name, x in moments.items())
+
+
+def check_orders_of_dimensions(device):
+    """A parameter whose order of dimensions changes after steps were made, and a state that was saved before it did: the same steps as
+    those of torch. In 8 bits, where elements share scales in the order of memory, the step is refused."""
+    torch.manual_seed(0)
+    start = torch.randn(6, 4, 3, 3, device=device)
+    grads = [torch.randn(6, 4, 3, 3, device=device) for _ in range(4)]
+    last = torch.channels_last
+
+    def steps(make, change):
+        p = torch.nn.Parameter(start.clone())
+        opt = make([p])
+        for i, g in enumerate(grads):
+            if i == 2 and change == "data":
+                p.data = p.data.contiguous(memory_format=last)
+            if i == 2 and change == "load":
+                state, q = copy.deepcopy(opt.state_dict()), torch.nn.Parameter(p.detach().contiguous(memory_format=last))
+                p, opt = q, make([q])
+                opt.load_state_dict(state)
+            p.grad = g.clone()
+            opt.step()
+        return p.detach(), opt
+
+    want, _ = steps(lambda p: torch.optim.AdamW(p, lr=0.1, foreach=False), "none")
+    for change in ("data", "load"):
+        got, opt = steps(lambda p: AdamW(p, lr=0.1), change)
+        torch.testing.assert_close(got, want, rtol=1e-5, atol=1e-6)
+        assert next(iter(opt.state.values()))["exp_avg"].is_contiguous(memory_format=last)
+        with pytest.raises(ValueError, match="strides"):
+            steps(lambda p: AdamW(p, lr=0.1, state_bits=8), change)
+
+
+def test_orders_of_dimensions():
+    check_orders_of_dimensions("cpu")
