@@ -104,7 +104,7 @@ class GPT2(nn.Module):
         pos = torch.arange(t, device=tokens.device, dtype=torch.int64 if offsets is None else torch.int32)
         if offsets is not None:
             document = torch.searchsorted(offsets[1:].contiguous(), pos, right=True, out_int32=True)
-            pos = (pos - offsets[document]).clamp(0, self.cfg.n_positions - 1)
+            pos = (pos - offsets[document].clamp_min(0)).clamp(0, self.cfg.n_positions - 1)   # (below zero attention begins at zero too)
         x = self.wte(tokens) + self.wpe(pos)
         for block in self.h:
             x = block(x) if offsets is None else block(x, offsets)

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from powersgd_b200 import AdamW
+from powersgd_b200.models import GPT2, GPT2Config
 from powersgd_b200.ops.attention import packed_attention
 from powersgd_b200.ops.tokens import token_log_probs
 
@@ -120,3 +121,12 @@ def check_orders_of_dimensions(device):
 
 def test_orders_of_dimensions():
     check_orders_of_dimensions("cpu")
+
+
+def test_positions_of_documents_with_offsets_outside():
+    """Offsets outside the rows are taken for the nearer end, by attention and by positions."""
+    torch.manual_seed(0)
+    model, tokens = GPT2(GPT2Config.tiny()), torch.randint(0, 512, (30,))
+    for bad, good in (([-5, 9, 30], [0, 9, 30]), ([-9, -3, 20, 99], [0, 0, 20, 30]), ([4, 12, 40], [4, 12, 30])):
+        bad, good = (torch.tensor(x, dtype=torch.int32) for x in (bad, good))
+        assert torch.equal(model(tokens, bad), model(tokens, good))
