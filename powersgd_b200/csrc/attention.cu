@@ -1349,6 +1349,10 @@ int at_forward(const AtArgs& a, cudaStream_t stream) {
 template <typename T, int PANELS>
 int at_backward(AtArgs a, cudaStream_t stream) {
   static unsigned long long q_devices = 0, kv_devices = 0;
+  // A block of the keys' pass holds its tensor memory while it waits for the queries' pass to end, whose blocks may have begun without theirs: as many as
+  // fit beside one of them must leave it enough.
+  constexpr size_t SM_SHARED = 228 * 1024, OF_Q = ab_shared(PANELS, 0), OF_KV = ab_shared(PANELS, AB_ONES + ab_stages(PANELS) * AB_STATS);
+  static_assert(((SM_SHARED - OF_Q) / OF_KV + 1) * 256 * PANELS <= 512, "tensor memory");
   if (const int code = psgd_allow_shared((const void*)psgd_attention_dq_kernel<T, PANELS>, ab_shared(PANELS, 0), q_devices)) return code;
   if (const int code = psgd_allow_shared((const void*)psgd_attention_dkv_kernel<T, PANELS>, ab_shared(PANELS, AB_ONES + ab_stages(PANELS) * AB_STATS), kv_devices)) return code;
   if constexpr (AB_SHIFTS<T>) {

@@ -94,6 +94,13 @@ def _status(device: torch.device):
     return word[1]
 
 
+def check_waits() -> None:
+    """Raises RuntimeError if a wait inside an attention kernel has run out, on any device, in what has ended by now. Every call of `packed_attention`
+    asks this of the calls before it; a program asks it behind its last call and behind replays of a graph, once these have ended."""
+    for device in list(_statuses):
+        _status(device)
+
+
 def _usable(t: torch.Tensor) -> torch.Tensor:
     """As the kernels address it: elements of a head side by side, rows and heads on 16-byte boundaries and apart. A copy if need be."""
     t = native.in_memory(t)

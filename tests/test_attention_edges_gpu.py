@@ -180,3 +180,38 @@ def test_half_precision_weights_of_long_sequences(length, gradients, size, heads
     want = g[0, 0, 0].double() * heads / groups
     off = 2.0**-10 + 2.0**-12 + length * heads / groups * 2.0**-28
     assert ((dv.double() - want).abs() <= off * want).all(), ((dv.double() - want).abs().max() / want).item()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths, heads, groups, size", [([700, 300, 24], 4, 2, 64), ([700, 300, 24], 8, 1, 128), ([20] * 40 + [224], 4, 4, 64), ([64] * 16, 2, 1, 16)])
+def test_graphs_and_repeats(lengths, heads, groups, size, dtype):
+    """The same bits in every run, beside other calls on another stream, and from a graph whose offsets change."""
+    q, k, v, g = _inputs(1024, heads, groups, size, dtype)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    offsets = _offsets(lengths)
+
+    def call():
+        out = packed_attention(*leaves, offsets)
+        return (out.detach(), *torch.autograd.grad(out, leaves, g))
+
+    want = [x.clone() for x in call()]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    others = []
+    for _ in range(30):
+        with torch.cuda.stream(side):
+            others.append(call())
+        got = call()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    side.synchronize()
+    assert all(torch.equal(a, b) for other in others for a, b in zip(want, other))
+    del others, got
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call()
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    reverse = _offsets(lengths[::-1])
+    offsets.copy_(reverse)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(call(), got))

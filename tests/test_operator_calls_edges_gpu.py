@@ -100,3 +100,15 @@ def test_gradients_that_only_say_that_they_are_negated(listed, monkeypatch):
 
 def test_orders_of_dimensions():
     check_orders_of_dimensions("cuda")
+
+
+def test_a_wait_that_ran_out_is_told_behind_the_last_call(form):
+    """The status word that kernels write is set from the host."""
+    x = torch.zeros(4, 1, 8, device="cuda", dtype=torch.bfloat16)
+    attention.packed_attention(x, x, x, torch.tensor([0, 4], device="cuda", dtype=torch.int32))
+    torch.cuda.synchronize()
+    attention.check_waits()
+    attention._statuses[x.device][0][0] = 3
+    with pytest.raises(RuntimeError, match="ran out"):
+        attention.check_waits()
+    attention.check_waits()
