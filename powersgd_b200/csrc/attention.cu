@@ -19,6 +19,7 @@
 //   dK, dV    tiles of 128 keys, walking over tiles of 64 queries of all heads of the group, transposed: lanes are
 //             keys, so that P^T and dS^T are A operands as they come. Nothing is added with atomics: the same inputs
 //             give the same bits. The price is that S and dP are computed twice (seven products instead of five).
+// float16: weights and dS are multiplied with powers of two in the backward pass, so that small ones keep their bits.
 // A row of a tile that belongs to another sequence, or lies behind the last one, may hold anything: before it is multiplied with anything
 // but scores that are replaced, its row in shared memory is cleared.
 //
@@ -1389,7 +1390,7 @@ PSGD_API int psgd_attention(const void* q, const void* k, const void* v, const l
   return size <= 64 ? at_forward<__half, 1>(a, stream) : at_forward<__half, 2>(a, stream);
 }
 
-// strides: those of q, k, v and of the output's gradient. delta: scratch, [2 heads + key heads, tokens] words. dq, dk, dv are contiguous.
+// strides: those of q, k, v and of the output's gradient. delta: scratch, [heads, tokens] words, float16 [2 heads + key heads, tokens]. dq, dk, dv are contiguous.
 PSGD_API int psgd_attention_backward(const void* q, const void* k, const void* v, const void* grad, const long long* strides, const int* offsets, int sequences,
                                      int tokens, int heads, int kv_heads, int size, int dtype, int causal, float scale, const void* out, const void* rest, const float* lse,
                                      float* delta, void* dq, void* dk, void* dv, int* plan, int* status, cudaStream_t stream) {
@@ -1403,8 +1404,10 @@ PSGD_API int psgd_attention_backward(const void* q, const void* k, const void* v
   a.grad_head = strides[7];
   a.lse = (float*)lse;
   a.delta = delta;
-  a.lengths_g = (int*)(delta + (long long)heads * tokens);
-  a.lengths_v = a.lengths_g + (long long)heads * tokens;
+  if (dtype != 1) {
+    a.lengths_g = (int*)(delta + (long long)heads * tokens);
+    a.lengths_v = a.lengths_g + (long long)heads * tokens;
+  }
   a.value = v;
   a.value_row = strides[4];
   a.value_head = strides[5];

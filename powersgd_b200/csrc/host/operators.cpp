@@ -321,7 +321,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
         dq.zero_(), dk.zero_(), dv.zero_();
       } else {
         const Tensor q = usable(saved[0]), k = usable(saved[1]), v = usable(saved[2]), offsets = saved[3].contiguous();
-        const Tensor plan = plan_of(offsets.size(0) - 1, tokens, q), g = usable(in_memory(grads[0])), delta = at::empty({2 * heads + groups, tokens}, lse.options());
+        const Tensor plan = plan_of(offsets.size(0) - 1, tokens, q), g = usable(in_memory(grads[0])), delta = at::empty({out.scalar_type() == at::kHalf ? 2 * heads + groups : heads, tokens}, lse.options());
         long long strides[8];
         strides_of(q, strides);
         strides_of(k, strides + 2);

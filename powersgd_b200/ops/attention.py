@@ -32,7 +32,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     nearer end, and what sequences that overlap give is not defined. Rows that belong to no sequence give zeros, whatever they
     hold. `scale`: 1 / sqrt(size) unless given; 2^-100 to 2^100.
 
-    Differentiable (once, backwards) in q, k and v, whose gradients have the shapes of these; the result and the gradients are the same
+    Differentiable (once, backwards) in q, k and v, whose gradients have the shapes of these; all three are computed where one is asked for. Until
+    then a second tensor as large as the output is kept, what rounding took from it. The result and the gradients are the same
     in every run. Tensors may be views, as parts of one projection are: rows and heads that do not begin on 16-byte boundaries, or
     elements that do not lie side by side, are copied first. Under float16 a gradient beyond its range becomes infinite. Positions that
     see a score which is no number give NaN; where a row of q, k, v or a gradient is not finite, any other of its sequence may."""
@@ -158,7 +159,7 @@ def _backward(q, k, v, offsets, out, lse, rest, grad, causal, scale):
     dv = torch.empty_like(dk)
     if tokens == 0 or sequences == 0:
         return dq.zero_(), dk.zero_(), dv.zero_()
-    delta = torch.empty((2 * heads + groups, tokens), dtype=torch.float32, device=q.device)   # scratch
+    delta = torch.empty((2 * heads + groups if q.dtype == torch.float16 else heads, tokens), dtype=torch.float32, device=q.device)   # scratch
     q, k, v, grad, offsets, plan = _usable(q), _usable(k), _usable(v), _usable(grad), offsets.contiguous(), _plan(sequences, tokens, q.device)
     with native.on_device(q.device) as stream:
         code = native.lib().psgd_attention_backward(
