@@ -5,8 +5,8 @@
 //
 // in float32 whatever the type of p and g; p is rounded to its type once. A step moves 28 bytes per float32
 // parameter (p, m, v in and out, g in), 16.1 with moments in 8 bits, and computes some tens of operations: the
-// memory bounds it in 32 bits (355 M float32 parameters 1455 us, 6.8 TB/s; 31.8 M 138 us) and the instructions of the rounding in 8
-// (1160 us, 4.9 TB/s; bfloat16 parameters take as long). A block takes 4096 elements of one tensor, found by a search in the list that the launch
+// memory bounds it in 32 bits (355 M float32 parameters 1444 us, 6.9 TB/s; 31.8 M 135 us, as bfloat16 110 us, 6.4 TB/s). In 8 it is the
+// rounding: issue is 62 to 75 % busy, the rest waits for loads (1099 us, 5.2 TB/s; bfloat16 parameters take as long). A block takes 4096 elements of one tensor, found by a search in the list that the launch
 // carries in its own arguments: nothing is uploaded, and a recorded launch keeps its list.
 //
 // The number of steps of a tensor, t, lives in device memory, so that a replayed graph counts on. Every block reads
@@ -261,8 +261,8 @@ __device__ __forceinline__ float aw_scale(uint32_t bits, float& inv) {
 }
 
 // A warp holds a block of 256: elements 4 lane + j and 128 + 4 lane + j. A block of threads takes every gridDim.x-th chunk of the list: what it needs
-// to know of a tensor it finds out once for most of its chunks. (355 M float32 parameters: 1310 us so, 2131 with a chunk to a block;
-// with 32-bit moments, where there is little to compute, it is the other way round, 1660 and 1459.)
+// to know of a tensor it finds out once for most of its chunks. (A step of 355 M float32 parameters: 1256 us so, 2087 with a chunk to a
+// block; 6.3 M bfloat16 ones 34 and 41. With 32-bit moments, where there is little to compute, it was the other way round, 1660 and 1459.)
 template <typename T, int MOST>
 __global__ void __launch_bounds__(AW_THREADS, AW_PER_SM) psgd_adamw8_kernel(const __grid_constant__ AwArgs<MOST> a) {
   constexpr int PER_WARP = AW_CHUNK / AW_THREADS / 8, APART = AW_THREADS / 32 * AW_BLOCK;

@@ -16,7 +16,9 @@ time: the input batch (copied into static buffers), the learning-rate table (ref
 pinned memory), the warm-start factors and the residuals. Steps that are structurally
 different run eagerly or get their own graph: the un-compressed warm-up phase, the first
 steps (cuDNN autotuning, lazy momentum buffers), and — for an odd `num_iters_per_step` — the
-two parities of the power iteration.
+two parities of the power iteration. With an optimizer whose update is not part of the fused
+sequence (anything but a plain `torch.optim.SGD`, `AdamW` among them) every step runs eagerly; a
+program may record one in a graph of its own.
 """
 from __future__ import annotations
 
