@@ -215,3 +215,17 @@ def test_graphs_and_repeats(lengths, heads, groups, size, dtype):
     offsets.copy_(reverse)
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(call(), got))
+
+
+def test_half_precision_more_elements_than_thirty_two_bits_count():
+    """Rows that begin behind 2^31 elements: the same as those rows by themselves."""
+    tokens = 2**20 + 5000
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q, g, k, v = (torch.empty(tokens, 16, 128, device="cuda", dtype=torch.float16).normal_(generator=gen) for _ in range(4))
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    out = packed_attention(*leaves, _offsets([128] * (2**13) + [3000, 2000]))
+    got = (out, *torch.autograd.grad(out, leaves, g))
+    last = [x.detach()[-5000:].clone().requires_grad_() for x in (q, k, v)]
+    want = packed_attention(*last, _offsets([3000, 2000]))
+    for a, b in zip(got, (want, *torch.autograd.grad(want, last, g[-5000:]))):
+        assert torch.equal(a.detach()[-5000:], b.detach())

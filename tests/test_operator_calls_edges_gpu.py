@@ -4,7 +4,8 @@ import pytest
 import torch
 from test_operator_edges_cpu import _tangent_calls, check_orders_of_dimensions
 
-from powersgd_b200 import AdamW
+from powersgd_b200 import AdamW, Config, PowerSGD
+from powersgd_b200.engine import TrainStep
 from powersgd_b200.ops import attention, host, scan, tokens
 
 pytestmark = pytest.mark.gpu
@@ -112,3 +113,23 @@ def test_a_wait_that_ran_out_is_told_behind_the_last_call(form):
     with pytest.raises(RuntimeError, match="ran out"):
         attention.check_waits()
     attention.check_waits()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_train_step_with_adamw(bits):
+    """Every step runs eagerly, on weights that became channels_last; moments in 32 bits may be older than that."""
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(torch.nn.Conv2d(3, 16, 3), torch.nn.ReLU(), torch.nn.Conv2d(16, 16, 3), torch.nn.AdaptiveAvgPool2d(1), torch.nn.Flatten(), torch.nn.Linear(16, 10)).cuda()
+    params = list(model.parameters())
+    optimizer = AdamW(params, lr=1e-2, state_bits=bits)
+    if bits == 32:
+        for p in params:
+            p.grad = torch.randn_like(p)
+        optimizer.step()
+        optimizer.zero_grad()
+    step = TrainStep(model, torch.nn.functional.cross_entropy, optimizer, PowerSGD(params, Config(rank=2, min_compression_rate=2, num_iters_per_step=2, start_compressing_after_num_steps=1)))
+    x, y = torch.randn(32, 3, 16, 16, device="cuda"), torch.randint(0, 10, (32,), device="cuda")
+    before = [p.detach().clone() for p in params]
+    assert all(step(x, y).isfinite() for _ in range(5)) and not step._graphs
+    assert all(p.isfinite().all() and not torch.equal(p, b) for p, b in zip(params, before))
+    assert all(optimizer.state[p]["step"] == (6 if bits == 32 else 5) for p in params)
