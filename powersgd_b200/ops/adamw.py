@@ -70,9 +70,10 @@ def laid_like(t: torch.Tensor, p: torch.Tensor) -> bool:
 def lay_like(state: dict, p: torch.Tensor) -> None:
     """Moments in 32 bits in the order of their parameter's dimensions, which may have changed (a model that became channels_last, a state
     saved before it did). Recorded graphs keep what they refer to."""
+    strides = p.stride()
     for name in state_names(32):
         t = state.get(name)
-        if t is not None and t.shape == p.shape and not laid_like(t, p):
+        if t is not None and t.stride() != strides and t.shape == p.shape and not laid_like(t, p) and not (p.is_cuda and torch.cuda.is_current_stream_capturing()):
             state[name] = torch.empty_like(p, dtype=t.dtype, memory_format=torch.preserve_format).copy_(t)
 
 

@@ -141,7 +141,7 @@ class AdamW(torch.optim.Optimizer):
                 if not state:
                     with outside_capture(p.device) if p.is_cuda else _nothing():
                         state.update(_adamw.new_state(p, bits))
-                elif bits == 32 and not (p.is_cuda and torch.cuda.is_current_stream_capturing()):
+                elif bits == 32:
                     _adamw.lay_like(state, p)
                 g = p.grad
                 if g.layout == torch.strided:
