@@ -114,7 +114,7 @@ __device__ bool at_find(const AtArgs& a, int rows, int index, bool from_end, AtP
     out.before = at_bound(a.offsets, 0, a.tokens);
     out.behind = max(at_bound(a.offsets, a.sequences, a.tokens), out.before);
     if (index >= a.plan[0]) return false;
-    const int* x = a.plan + 1 + 3 * index;
+    const int* x = a.plan + 1 + 3ll * index;
     out.start = x[0];
     out.length = x[1];
     out.piece = from_end ? (out.length + rows - 1) / rows - 1 - x[2] : x[2];
@@ -212,9 +212,9 @@ __global__ void __launch_bounds__(AT_PLAN_THREADS) psgd_attention_plan_kernel(co
 // Rows of a result that belong to no sequence: zeros. Dealt out over the blocks of a head.
 template <typename T>
 __device__ __forceinline__ void at_clear_outside(const AtArgs& a, const AtPiece& piece, T* out, int heads, int head, int block) {
-  const int outside = piece.before + a.tokens - piece.behind;
-  for (int i = block; i < outside; i += a.blocks) {
-    const int row = i < piece.before ? i : piece.behind + i - piece.before;
+  const unsigned outside = a.tokens - (piece.behind - piece.before), before = piece.before;      // (a row and a step behind it may pass 2^31)
+  for (unsigned i = block; i < outside; i += a.blocks) {
+    const int row = (int)(i < before ? i : i + (piece.behind - piece.before));
     T* p = out + ((long long)row * heads + head) * a.size;
     for (int e = threadIdx.x; e < a.size; e += blockDim.x) p[e] = T(0.f);
   }
