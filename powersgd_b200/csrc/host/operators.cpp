@@ -1,11 +1,11 @@
-// Calls of token_log_probs, packed_attention and AdamW from Python, as a CPython extension against PyTorch's C++ interface.
+// Calls of token_log_probs, packed_attention, AdamW and the gradients' norm from Python, as a CPython extension against PyTorch's C++ interface.
 //
 // Through Python and a foreign function call a forward pass took 25 us of the host, and a backward pass, whose node the autograd
 // engine runs on a thread of its own that must first get the interpreter lock, 80 us besides the engine's own 45: more than the kernels
 // of all but large inputs. Here the nodes are C++ ones.
 //
 // A call answers None for whatever is not plain (other types, layouts that must be refused, subclasses of Tensor): the caller then
-// goes through the Python form (ops/tokens.py, ops/attention.py), which checks, refuses and explains. Nothing is remembered
+// goes through the Python form (ops/tokens.py, ops/attention.py, ops/grad_norm.py), which checks, refuses and explains. Nothing is remembered
 // from one call for the next but the entry points of the native library and the status words that Python hands over.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -20,8 +20,11 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <utility>
+#include <vector>
 
 namespace {
 
@@ -41,6 +44,8 @@ struct Entry {
   int (*attention_backward)(const void*, const void*, const void*, const void*, const long long*, const int*, int, int, int, int, int, int, int, float,
                             const void*, const void*, const float*, float*, void*, void*, void*, int*, int*, void*) = nullptr;
   int (*adamw)(const void*, int, int, int, double, const float*, double, double, double, double, double, double, unsigned, int*, void*) = nullptr;
+  int (*grad_norm)(const void*, int, int, int, double, double*, void*, int, void*) = nullptr;
+  long long (*grad_norm_parts)(int) = nullptr;
 } entry;
 
 constexpr int MOST_DEVICES = 64;
@@ -392,11 +397,80 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   });
 }
 
+// ---- norm of gradients --------------------------------------------------------------------------
+struct NormItem {   // PsgdNormTensor, csrc/grad_norm.cu
+  uint64_t g;
+  int64_t n;
+  uint32_t type, piece_end;
+};
+
+// grad_norm(parameters, largest, clip, max_norm): the norm of their gradients, scaled where `clip`; or None.
+PyObject* grad_norm(PyObject*, PyObject* args) {
+  return guarded([&]() -> PyObject* {
+    PyObject* list;
+    int largest, clip;
+    double max_norm;
+    if (!PyArg_ParseTuple(args, "Oppd", &list, &largest, &clip, &max_norm)) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    if (entry.grad_norm == nullptr || !PyList_CheckExact(list)) Py_RETURN_NONE;
+    const Py_ssize_t count = PyList_GET_SIZE(list);
+    std::vector<NormItem> items;
+    std::vector<const Tensor*> grads;
+    items.reserve(count);
+    grads.reserve(count);
+    bool wide = false, sorted = true;
+    uint64_t end = 0;
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      PyObject* object = PyList_GET_ITEM(list, i);
+      if (!THPVariable_CheckExact(object)) Py_RETURN_NONE;
+      const Tensor& p = THPVariable_Unpack(object);
+      if (!p.defined() || at::isTensorSubclassLike(p)) Py_RETURN_NONE;
+      const Tensor& g = p.grad();
+      if (!g.defined()) continue;
+      if (g.layout() != at::kStrided || !g.unsafeGetTensorImpl()->has_storage() || at::isTensorSubclassLike(g) || g._is_zerotensor() || !g.is_cuda() || has_tangent(g) ||
+          !g.is_non_overlapping_and_dense() || (!grads.empty() && g.get_device() != grads[0]->get_device()))
+        Py_RETURN_NONE;
+      const int type = g.scalar_type() == at::kDouble ? 3 : type_code(g.scalar_type());
+      if (type < 0) Py_RETURN_NONE;
+      wide = wide || type == 3;
+      const uint64_t at = (uint64_t)g.const_data_ptr();
+      if (g.numel() > 0) {
+        sorted = sorted && at >= end;
+        end = at + (uint64_t)g.numel() * g.element_size();
+      }
+      items.push_back({at, g.numel(), (uint32_t)type, 0u});
+      grads.push_back(&g);
+    }
+    if (grads.empty() || items.size() >= (1u << 30) || torch::jit::tracer::isTracing()) Py_RETURN_NONE;
+    if (clip && !sorted) {   // none may lie in another's memory
+      std::vector<std::pair<uint64_t, uint64_t>> places;
+      places.reserve(items.size());
+      for (size_t i = 0; i < items.size(); ++i)
+        if (items[i].n > 0) places.emplace_back(items[i].g, items[i].g + (uint64_t)items[i].n * grads[i]->element_size());
+      std::sort(places.begin(), places.end());
+      for (size_t i = 1; i < places.size(); ++i)
+        if (places[i].first < places[i - 1].second) Py_RETURN_NONE;
+    }
+    const c10::cuda::CUDAGuard guard(grads[0]->device());
+    const at::NoGradGuard no_grad;
+    const auto f64 = at::TensorOptions().device(grads[0]->device()).dtype(at::kDouble);
+    const Tensor out = at::empty({}, f64.dtype(wide ? at::kDouble : at::kFloat)), parts = at::empty({entry.grad_norm_parts((int)items.size())}, f64);
+    check(entry.grad_norm(items.data(), (int)items.size(), largest, clip, max_norm, (double*)parts.data_ptr(), out.data_ptr(), wide, current_stream(out)), "psgd_grad_norm");
+    if (clip)   // (the kernel writes behind autograd's back)
+      for (const Tensor* g : grads)
+        if (!g->is_inference()) g->unsafeGetTensorImpl()->bump_version();
+    return wrap(out);
+  });
+}
+
 // ---- what Python hands over ---------------------------------------------------------------------
-// bind(error, token, token_grad, attention, attention_backward, adamw, attention_plan_ints): addresses of the native library's entry points.
+// bind(error, token, token_grad, attention, attention_backward, adamw, attention_plan_ints, grad_norm, grad_norm_parts): addresses of the native library's
+// entry points.
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[7];
-  if (!PyArg_ParseTuple(args, "KKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6)) return nullptr;
+  unsigned long long a[9];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7, a + 8)) return nullptr;
   entry.error = (decltype(entry.error))a[0];
   entry.token = (decltype(entry.token))a[1];
   entry.token_grad = (decltype(entry.token_grad))a[2];
@@ -404,6 +478,8 @@ PyObject* bind(PyObject*, PyObject* args) {
   entry.attention_backward = (decltype(entry.attention_backward))a[4];
   entry.adamw = (decltype(entry.adamw))a[5];
   entry.attention_plan_ints = (decltype(entry.attention_plan_ints))a[6];
+  entry.grad_norm = (decltype(entry.grad_norm))a[7];
+  entry.grad_norm_parts = (decltype(entry.grad_norm_parts))a[8];
   Py_RETURN_NONE;
 }
 // status(device, host address, device address): the status word of a device.
@@ -424,6 +500,7 @@ PyMethodDef methods[] = {
     {"token_log_probs", token_log_probs, METH_VARARGS, nullptr},
     {"packed_attention", packed_attention, METH_VARARGS, nullptr},
     {"adamw_step", adamw_step, METH_VARARGS, nullptr},
+    {"grad_norm", grad_norm, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -433,7 +510,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods,
 PyMODINIT_FUNC PyInit__operators() {
   PyObject* m = PyModule_Create(&module);
   // what this was compiled for, which the loader compares (csrc/build.py, scan_target)
-  if (m != nullptr && (PyModule_AddStringConstant(m, "target", PSGD_SCAN_TARGET) != 0 || PyModule_AddIntConstant(m, "entry_points", 7) != 0)) {
+  if (m != nullptr && (PyModule_AddStringConstant(m, "target", PSGD_SCAN_TARGET) != 0 || PyModule_AddIntConstant(m, "entry_points", 9) != 0)) {
     Py_DECREF(m);
     return nullptr;
   }

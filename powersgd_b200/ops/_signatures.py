@@ -77,6 +77,9 @@ f64 = C.c_double
 _OPTIONAL = {
     "psgd_adamw_item_bytes": (i32, []),
     "psgd_adamw_step": (i32, [C.c_char_p, i32, i32, i32, f64, vp, f64, f64, f64, f64, f64, f64, C.c_uint, vp, vp]),
+    "psgd_grad_norm_item_bytes": (i32, []),
+    "psgd_grad_norm_parts": (i64, [i32]),
+    "psgd_grad_norm": (i32, [C.c_char_p, i32, i32, i32, f64, vp, vp, i32, vp]),
     "psgd_attention_plan_ints": (i64, [i32, i32]),
     "psgd_attention": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp]),
     "psgd_attention_backward": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),
