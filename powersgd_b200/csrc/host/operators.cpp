@@ -1,11 +1,11 @@
-// Calls of token_log_probs, packed_attention, AdamW and the gradients' norm from Python, as a CPython extension against PyTorch's C++ interface.
+// Calls of token_log_probs, packed_attention, rotate_heads, AdamW and the gradients' norm from Python, as a CPython extension against PyTorch's C++ interface.
 //
 // Through Python and a foreign function call a forward pass took 25 us of the host, and a backward pass, whose node the autograd
 // engine runs on a thread of its own that must first get the interpreter lock, 80 us besides the engine's own 45: more than the kernels
 // of all but large inputs. Here the nodes are C++ ones.
 //
 // A call answers None for whatever is not plain (other types, layouts that must be refused, subclasses of Tensor): the caller then
-// goes through the Python form (ops/tokens.py, ops/attention.py, ops/grad_norm.py), which checks, refuses and explains. Nothing is remembered
+// goes through the Python form (ops/tokens.py, ops/attention.py, ops/rotary.py, ops/grad_norm.py), which checks, refuses and explains. Nothing is remembered
 // from one call for the next but the entry points of the native library and the status words that Python hands over.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
@@ -23,6 +23,8 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <optional>
+#include <string>
 #include <utility>
 #include <vector>
 
@@ -31,6 +33,25 @@ namespace {
 using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
+
+struct RotateCall {   // PsgdRotate, csrc/rotary.cu
+  const void* x;
+  const void* grad[3];
+  const void* weight[2];
+  const int* offsets;
+  const void* positions;
+  void* out[2];
+  void* dx;
+  void* dweight[2];
+  float* parts;
+  const void* frequencies;
+  long long x_row, x_head, grad_row[3], grad_head[3];
+  int rows, sequences, heads, keys, values, size, rotated, pairs;
+  int type, weight_type;
+  int wide, norm;
+  float eps;
+  int pad;
+};
 
 // ---- entry points of the native library ---------------------------------------------------------
 struct Entry {
@@ -46,6 +67,9 @@ struct Entry {
   int (*adamw)(const void*, int, int, int, double, const float*, double, double, double, double, double, double, unsigned, int*, void*) = nullptr;
   int (*grad_norm)(const void*, int, int, int, double, double*, void*, int, void*) = nullptr;
   long long (*grad_norm_parts)(int) = nullptr;
+  int (*rotate)(const RotateCall*, void*) = nullptr;
+  int (*rotate_grad)(const RotateCall*, void*) = nullptr;
+  long long (*rotate_parts)(int) = nullptr;
 } entry;
 
 constexpr int MOST_DEVICES = 64;
@@ -378,6 +402,166 @@ PyObject* packed_attention(PyObject*, PyObject* args) {
   });
 }
 
+// ---- heads normed and turned --------------------------------------------------------------------
+struct Turn {   // what a call says besides its tensors
+  int64_t heads, keys, rotated;
+  bool pairs;
+  double eps;   // below zero: no norm
+  std::string frequencies;
+};
+RotateCall rotate_call(const Tensor& x, const Turn& turn, const Tensor& q_weight, const Tensor& k_weight, const Tensor& offsets, const Tensor& positions) {
+  RotateCall c = {};
+  long long strides[2];
+  strides_of(x, strides);
+  c.x = x.const_data_ptr();
+  c.x_row = strides[0], c.x_head = strides[1];
+  const Tensor* weights[2] = {&q_weight, &k_weight};
+  for (int i = 0; i < 2; ++i) {
+    if (!weights[i]->defined()) continue;
+    c.weight[i] = weights[i]->const_data_ptr();
+    c.weight_type = type_code(weights[i]->scalar_type());
+  }
+  if (offsets.defined()) {
+    c.offsets = (const int*)offsets.const_data_ptr();
+    c.sequences = (int)offsets.size(0) - 1;
+  }
+  if (positions.defined()) {
+    c.positions = positions.const_data_ptr();
+    c.wide = positions.scalar_type() == at::kLong;
+  }
+  c.frequencies = turn.frequencies.data();
+  c.rows = (int)x.size(0), c.heads = (int)turn.heads, c.keys = (int)turn.keys, c.values = (int)(x.size(1) - turn.heads - turn.keys), c.size = (int)x.size(2);
+  c.rotated = (int)turn.rotated, c.pairs = turn.pairs;
+  c.type = type_code(x.scalar_type());
+  c.norm = turn.eps >= 0, c.eps = (float)turn.eps;
+  return c;
+}
+Tensor laid(const Tensor& t) { return t.defined() ? t.contiguous() : t; }
+
+// Queries, and keys and values of a projection (keys > 0); values are a view of x.
+variable_list rotate_forward(const Tensor& x0, const Turn& turn, const Tensor& q_weight, const Tensor& k_weight, const Tensor& offsets, const Tensor& positions) {
+  const c10::cuda::CUDAGuard guard(x0.device());
+  const int64_t rows = x0.size(0), size = x0.size(2);
+  const Tensor x = usable(x0), wq = laid(q_weight), wk = laid(k_weight), o = laid(offsets), p = laid(positions);
+  variable_list out = {at::empty({rows, turn.heads, size}, x.options())};
+  if (turn.keys > 0) {
+    out.push_back(at::empty({rows, turn.keys, size}, x.options()));
+    out.push_back(x0.narrow(1, turn.heads + turn.keys, x0.size(1) - turn.heads - turn.keys));
+  }
+  RotateCall c = rotate_call(x, turn, wq, wk, o, p);
+  c.out[0] = out[0].data_ptr();
+  if (turn.keys > 0) c.out[1] = out[1].data_ptr();
+  check(entry.rotate(&c, current_stream(x)), "psgd_rotate");
+  return out;
+}
+
+struct Rotate : torch::autograd::Function<Rotate> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const std::optional<Tensor>& q_weight, const std::optional<Tensor>& k_weight,
+                               const std::optional<Tensor>& offsets, const std::optional<Tensor>& positions, const Turn& turn) {
+    const Tensor wq = q_weight.value_or(Tensor()), wk = k_weight.value_or(Tensor()), o = offsets.value_or(Tensor()), p = positions.value_or(Tensor());
+    ctx->save_for_backward({x, wq, wk, o, p});
+    ctx->saved_data["heads"] = turn.heads;
+    ctx->saved_data["keys"] = turn.keys;
+    ctx->saved_data["rotated"] = turn.rotated;
+    ctx->saved_data["pairs"] = turn.pairs;
+    ctx->saved_data["eps"] = turn.eps;
+    ctx->saved_data["frequencies"] = turn.frequencies;
+    ctx->set_materialize_grads(false);
+    return rotate_forward(x, turn, wq, wk, o, p);
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    refuse_tangents(grads, "rotate_heads");
+    const auto saved = ctx->get_saved_variables();
+    variable_list result(6);
+    {
+      const at::NoGradGuard no_grad;
+      const Tensor x = usable(saved[0]), wq = laid(saved[1]), wk = laid(saved[2]), o = laid(saved[3]), p = laid(saved[4]);
+      const c10::cuda::CUDAGuard guard(x.device());
+      const Turn turn = {ctx->saved_data["heads"].toInt(), ctx->saved_data["keys"].toInt(), ctx->saved_data["rotated"].toInt(), ctx->saved_data["pairs"].toBool(),
+                         ctx->saved_data["eps"].toDouble(), ctx->saved_data["frequencies"].toStringRef()};
+      RotateCall c = rotate_call(x, turn, wq, wk, o, p);
+      Tensor g[3], parts;
+      for (size_t i = 0; i < grads.size(); ++i) {
+        if (!grads[i].defined()) continue;
+        g[i] = usable(in_memory(grads[i]));
+        long long strides[2];
+        strides_of(g[i], strides);
+        c.grad[i] = g[i].const_data_ptr();
+        c.grad_row[i] = strides[0], c.grad_head[i] = strides[1];
+      }
+      size_t edge = 0;   // of the inputs that are there
+      if (ctx->needs_input_grad(edge++)) {
+        result[0] = at::empty(x.sizes(), x.options());
+        c.dx = result[0].data_ptr();
+      }
+      for (int i = 0; i < 2; ++i) {
+        const Tensor& w = i ? wk : wq;
+        if (!w.defined() || !ctx->needs_input_grad(edge++)) continue;
+        result[1 + i] = c.rows ? at::empty(w.sizes(), w.options()) : at::zeros(w.sizes(), w.options());
+        c.dweight[i] = result[1 + i].data_ptr();
+      }
+      if (c.dweight[0] != nullptr || c.dweight[1] != nullptr) {
+        parts = at::empty({entry.rotate_parts(c.size)}, x.options().dtype(at::kFloat));
+        c.parts = (float*)parts.data_ptr();
+      }
+      check(entry.rotate_grad(&c, current_stream(x)), "psgd_rotate_grad");
+    }
+    return once(std::move(result));
+  }
+};
+
+// rotate(x, heads, keys, offsets, positions, q_weight, k_weight, eps, rotated, pairs, frequencies): the results as a tuple, or None. The caller has checked the
+// numbers; of the tensors everything but the shape of x is asked here.
+PyObject* rotate(PyObject*, PyObject* args) {
+  return guarded([&]() -> PyObject* {
+    PyObject *x_object, *objects[4];
+    long long heads, keys, rotated;
+    double eps;
+    int pairs;
+    const char* frequencies;
+    Py_ssize_t bytes;
+    if (!PyArg_ParseTuple(args, "OLLOOOOdLpy#", &x_object, &heads, &keys, objects, objects + 1, objects + 2, objects + 3, &eps, &rotated, &pairs, &frequencies, &bytes)) {
+      PyErr_Clear();
+      Py_RETURN_NONE;
+    }
+    const Tensor* xp = plain(x_object);
+    if (entry.rotate == nullptr || xp == nullptr) Py_RETURN_NONE;
+    const Tensor& x = *xp;
+    const auto type = x.scalar_type();
+    if (!x.is_cuda() || type_code(type) < 0 || x.dim() != 3 || heads < 1 || keys < 0 || x.size(1) < heads + keys || (keys == 0 && x.size(1) != heads) || x.size(2) < 8 ||
+        x.size(2) > 256 || x.size(2) % 8 != 0 || rotated < 0 || rotated > x.size(2) || rotated % 8 != 0 || bytes != rotated / 2 * 8 || x.size(0) >= (1ll << 31) - (1 << 16) ||
+        x.size(1) >= (1ll << 31) - (1 << 16) || has_tangent(x) || torch::jit::tracer::isTracing())
+      Py_RETURN_NONE;
+    Tensor t[4];
+    for (int i = 0; i < 4; ++i) {
+      if (objects[i] == Py_None) continue;
+      const Tensor* p = plain(objects[i]);
+      if (p == nullptr || p->device() != x.device() || p->dim() != 1) Py_RETURN_NONE;
+      t[i] = *p;
+    }
+    if (t[0].defined() && (t[0].scalar_type() != at::kInt || t[0].size(0) < 1 || t[0].size(0) > (1ll << 31) - (1 << 16) || t[1].defined())) Py_RETURN_NONE;
+    if (t[1].defined() && ((t[1].scalar_type() != at::kInt && t[1].scalar_type() != at::kLong) || t[1].size(0) != x.size(0))) Py_RETURN_NONE;
+    if (rotated > 0 && !t[0].defined() && !t[1].defined()) Py_RETURN_NONE;
+    for (int i = 2; i < 4; ++i)
+      if (t[i].defined() && (eps < 0 || t[i].size(0) != x.size(2) || (t[i].scalar_type() != at::kFloat && t[i].scalar_type() != type) || has_tangent(t[i]) ||
+                             (t[5 - i].defined() && t[i].scalar_type() != t[5 - i].scalar_type())))
+        Py_RETURN_NONE;
+    const Turn turn = {heads, keys, rotated, pairs != 0, eps, std::string(frequencies, (size_t)bytes)};
+    variable_list out;
+    const auto asks = [](const Tensor& w) { return w.defined() && w.requires_grad(); };
+    if (at::GradMode::is_enabled() && (x.requires_grad() || asks(t[2]) || asks(t[3]))) {
+      const auto given = [](const Tensor& w) { return w.defined() ? std::optional<Tensor>(w) : std::nullopt; };
+      out = Rotate::apply(x, given(t[2]), given(t[3]), given(t[0]), given(t[1]), turn);
+    } else {
+      out = rotate_forward(x, turn, t[2], t[3], t[0], t[1]);
+    }
+    PyObject* result = PyTuple_New((Py_ssize_t)out.size());
+    for (size_t i = 0; i < out.size() && result != nullptr; ++i) PyTuple_SET_ITEM(result, (Py_ssize_t)i, wrap(out[i]));
+    return result;
+  });
+}
+
 // ---- AdamW --------------------------------------------------------------------------------------
 // adamw_step(items, count, device, type, bits, lr, address of lr, betas and their logarithms, eps, decay, seed, ticket): the native step on the
 // device's current stream. Returns its code.
@@ -466,11 +650,11 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
 }
 
 // ---- what Python hands over ---------------------------------------------------------------------
-// bind(error, token, token_grad, attention, attention_backward, adamw, attention_plan_ints, grad_norm, grad_norm_parts): addresses of the native library's
-// entry points.
+// bind(error, token, token_grad, attention, attention_backward, adamw, attention_plan_ints, grad_norm, grad_norm_parts, rotate, rotate_grad, rotate_parts): addresses
+// of the native library's entry points.
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a[9];
-  if (!PyArg_ParseTuple(args, "KKKKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7, a + 8)) return nullptr;
+  unsigned long long a[12];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKK", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, a + 7, a + 8, a + 9, a + 10, a + 11)) return nullptr;
   entry.error = (decltype(entry.error))a[0];
   entry.token = (decltype(entry.token))a[1];
   entry.token_grad = (decltype(entry.token_grad))a[2];
@@ -480,6 +664,9 @@ PyObject* bind(PyObject*, PyObject* args) {
   entry.attention_plan_ints = (decltype(entry.attention_plan_ints))a[6];
   entry.grad_norm = (decltype(entry.grad_norm))a[7];
   entry.grad_norm_parts = (decltype(entry.grad_norm_parts))a[8];
+  entry.rotate = (decltype(entry.rotate))a[9];
+  entry.rotate_grad = (decltype(entry.rotate_grad))a[10];
+  entry.rotate_parts = (decltype(entry.rotate_parts))a[11];
   Py_RETURN_NONE;
 }
 // status(device, host address, device address): the status word of a device.
@@ -501,6 +688,7 @@ PyMethodDef methods[] = {
     {"packed_attention", packed_attention, METH_VARARGS, nullptr},
     {"adamw_step", adamw_step, METH_VARARGS, nullptr},
     {"grad_norm", grad_norm, METH_VARARGS, nullptr},
+    {"rotate", rotate, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
@@ -510,7 +698,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_operators", nullptr, -1, methods,
 PyMODINIT_FUNC PyInit__operators() {
   PyObject* m = PyModule_Create(&module);
   // what this was compiled for, which the loader compares (csrc/build.py, scan_target)
-  if (m != nullptr && (PyModule_AddStringConstant(m, "target", PSGD_SCAN_TARGET) != 0 || PyModule_AddIntConstant(m, "entry_points", 9) != 0)) {
+  if (m != nullptr && (PyModule_AddStringConstant(m, "target", PSGD_SCAN_TARGET) != 0 || PyModule_AddIntConstant(m, "entry_points", 12) != 0)) {
     Py_DECREF(m);
     return nullptr;
   }

@@ -80,6 +80,10 @@ _OPTIONAL = {
     "psgd_grad_norm_item_bytes": (i32, []),
     "psgd_grad_norm_parts": (i64, [i32]),
     "psgd_grad_norm": (i32, [C.c_char_p, i32, i32, i32, f64, vp, vp, i32, vp]),
+    "psgd_rotate_call_bytes": (i32, []),
+    "psgd_rotate_parts": (i64, [i32]),
+    "psgd_rotate": (i32, [vp, vp]),
+    "psgd_rotate_grad": (i32, [vp, vp]),
     "psgd_attention_plan_ints": (i64, [i32, i32]),
     "psgd_attention": (i32, [vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp]),
     "psgd_attention_backward": (i32, [vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, f32, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp]),

@@ -9,7 +9,7 @@ from ..csrc.build import operators_lib, scan_target
 from . import native
 
 ENTRY_POINTS = ("psgd_last_error", "psgd_token_logprob", "psgd_token_logprob_grad", "psgd_attention", "psgd_attention_backward", "psgd_adamw_step",
-                "psgd_attention_plan_ints", "psgd_grad_norm", "psgd_grad_norm_parts")
+                "psgd_attention_plan_ints", "psgd_grad_norm", "psgd_grad_norm_parts", "psgd_rotate", "psgd_rotate_grad", "psgd_rotate_parts")
 
 
 def _load():
