@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "psgd_common.cuh"
 
 // A call, as the caller fills it in (ops/rotary.py, host/operators.cpp). Strides are in elements, of rows and heads.
@@ -43,19 +45,57 @@ typedef struct {
 namespace {
 
 constexpr int RT_THREADS = 256, RT_WARPS = RT_THREADS / 32;
-constexpr int RT_MOST_SIZE = 256;
+constexpr int RT_MOST_SIZE = 256, RT_MOST_ANGLES = RT_MOST_SIZE / 2;
 constexpr int RT_SMS = 148;
-constexpr int RT_FORWARD_BLOCKS = 3, RT_BACKWARD_BLOCKS = 2;   // of an SM at a time
+#ifndef FB
+#define FB 4
+#define BB 2
+#define WF 1
+#define WB 1
+#endif
+constexpr int RT_FORWARD_BLOCKS = FB, RT_BACKWARD_BLOCKS = BB;   // of an SM at a time
+constexpr int RT_PART_BLOCKS = RT_SMS * RT_BACKWARD_BLOCKS;    // that add up gradients of weights
 constexpr float RT_DOWN = 0x1p-70f;                            // for heads whose squares leave the range
 
 struct RtArgs {
   PsgdRotate c;
   int lanes;                       // of a head: a power of two
-  int span, parts[2];              // heads of a warp's share of a row, shares of a row's queries and keys
-  unsigned long long frequency[RT_MOST_SIZE / 2];
+  int parts;                       // warps that share a row
+  float share;                     // 1 / size
+  unsigned long long frequency[RT_MOST_ANGLES];
 };
 
-// W elements of a type that lie side by side, on a multiple of 16 bytes (or of their size, if that is less).
+// Two float32 in one register of 64 bits. (As two of 32 bits, which ptxas has to move together before each operation, the kernels executed PLACEHOLDER
+// more instructions.)
+typedef unsigned long long RtPair;
+__device__ __forceinline__ RtPair rt_pair(float a, float b) {
+  RtPair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ RtPair rt_both(float x) { return rt_pair(x, x); }
+__device__ __forceinline__ float2 rt_floats(RtPair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ RtPair rt_mul(RtPair a, RtPair b) {
+  RtPair c;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(c) : "l"(a), "l"(b));
+  return c;
+}
+__device__ __forceinline__ RtPair rt_fma(RtPair a, RtPair b, RtPair c) {
+  RtPair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+// c - a b (scalars subtract for nothing)
+__device__ __forceinline__ RtPair rt_less(RtPair a, RtPair b, RtPair c) {
+  const float2 x = rt_floats(a), y = rt_floats(b), z = rt_floats(c);
+  return rt_pair(fmaf(-x.x, y.x, z.x), fmaf(-x.y, y.y, z.y));
+}
+
+// W elements of a type that lie side by side, on a multiple of 16 bytes (or of their size, if that is less), as W / 2 pairs.
 template <typename T, int W>
 struct RtVec;
 template <int W>
@@ -69,13 +109,16 @@ struct RtVec<float, W> {
 #pragma unroll
     for (int i = 0; i < W / 4; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ __forceinline__ void unpack(float* f) const {
+  __device__ __forceinline__ void unpack(RtPair* f) const {
 #pragma unroll
-    for (int i = 0; i < W / 4; ++i) f[4 * i] = v[i].x, f[4 * i + 1] = v[i].y, f[4 * i + 2] = v[i].z, f[4 * i + 3] = v[i].w;
+    for (int i = 0; i < W / 4; ++i) f[2 * i] = rt_pair(v[i].x, v[i].y), f[2 * i + 1] = rt_pair(v[i].z, v[i].w);
   }
-  static __device__ __forceinline__ void store(float* p, const float* f) {
+  static __device__ __forceinline__ void store(float* p, const RtPair* f) {
 #pragma unroll
-    for (int i = 0; i < W / 4; ++i) reinterpret_cast<float4*>(p)[i] = make_float4(f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]);
+    for (int i = 0; i < W / 4; ++i) {
+      const float2 a = rt_floats(f[2 * i]), b = rt_floats(f[2 * i + 1]);
+      reinterpret_cast<float4*>(p)[i] = make_float4(a.x, a.y, b.x, b.y);
+    }
   }
 };
 template <int N>
@@ -88,14 +131,17 @@ template <>
 struct RtWords<4> {
   typedef uint4 type;
 };
-__device__ __forceinline__ float2 rt_wide(uint32_t w, __nv_bfloat16) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
-__device__ __forceinline__ float2 rt_wide(uint32_t w, __half) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
-__device__ __forceinline__ uint32_t rt_narrow(float a, float b, __nv_bfloat16) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+__device__ __forceinline__ RtPair rt_wide(uint32_t w, __nv_bfloat16) { return rt_pair(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ RtPair rt_wide(uint32_t w, __half) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return rt_pair(f.x, f.y);
+}
+__device__ __forceinline__ uint32_t rt_narrow(float2 f, __nv_bfloat16) {
+  const __nv_bfloat162 h = __float22bfloat162_rn(f);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint32_t rt_narrow(float a, float b, __half) {
-  const __half2 h = __floats2half2_rn(a, b);
+__device__ __forceinline__ uint32_t rt_narrow(float2 f, __half) {
+  const __half2 h = __float22half2_rn(f);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <typename T, int W>
@@ -110,17 +156,14 @@ struct RtVec {
 #pragma unroll
     for (int i = 0; i < W / 2; ++i) w[i] = 0;
   }
-  __device__ __forceinline__ void unpack(float* f) const {
+  __device__ __forceinline__ void unpack(RtPair* f) const {
 #pragma unroll
-    for (int i = 0; i < W / 2; ++i) {
-      const float2 p = rt_wide(w[i], T());
-      f[2 * i] = p.x, f[2 * i + 1] = p.y;
-    }
+    for (int i = 0; i < W / 2; ++i) f[i] = rt_wide(w[i], T());
   }
-  static __device__ __forceinline__ void store(T* p, const float* f) {
+  static __device__ __forceinline__ void store(T* p, const RtPair* f) {
     RtVec o;
 #pragma unroll
-    for (int i = 0; i < W / 2; ++i) o.w[i] = rt_narrow(f[2 * i], f[2 * i + 1], T());
+    for (int i = 0; i < W / 2; ++i) o.w[i] = rt_narrow(rt_floats(f[i]), T());
     *reinterpret_cast<Words*>(p) = o.v;
   }
 };
@@ -153,30 +196,57 @@ __device__ __forceinline__ bool rt_position(const PsgdRotate& c, int row, int la
     lo += next;
   }
   const int mine = lane < n ? c.offsets[lo + lane] : 0x7fffffff;
-  lo += __popc(__ballot_sync(0xffffffffu, lane < n && mine <= row));
-  if (lo == 0 || lo > c.sequences) return false;
-  position = (unsigned long long)(row - max(c.offsets[lo - 1], 0));
+  const unsigned before = __ballot_sync(0xffffffffu, lane < n && mine <= row);
+  const int count = lo + __popc(before);
+  if (count == 0 || count > c.sequences) return false;
+  // (where the last one that is not behind the row was among these, a lane has it)
+  const int start = before ? __shfl_sync(0xffffffffu, mine, (__popc(before) - 1) & 31) : c.offsets[count - 1];
+  position = (unsigned long long)(row - max(start, 0));
   return true;
 }
 
-// Cosine and sine of a fraction of a turn (64 bits behind the point): the nearest quarter is taken out first.
+// Cosine and sine of a fraction of a turn (64 bits behind the point): the nearest quarter is taken out first. What is left, an eighth of a turn
+// at most, goes into the first terms of their series: what follows is below 2e-9 and 3e-10.
 __device__ __forceinline__ float2 rt_angle(unsigned long long turns) {
   const uint32_t high = (uint32_t)(turns >> 32);
   const uint32_t quarter = (high + 0x20000000u) >> 30;
-  const int rest = (int)(high - (quarter << 30));
-  float s, c;
-  sincospif(fmaf((float)rest, 0x1p-31f, (float)(uint32_t)turns * 0x1p-63f), &s, &c);
+  const float t = (float)(int)(high - (quarter << 30)) * 1.4629180792671596e-9f, u = t * t;   // 2 pi / 2^32
+  const float s = fmaf(t * u, fmaf(u, fmaf(u, fmaf(u, 1.f / 362880.f, -1.f / 5040.f), 1.f / 120.f), -1.f / 6.f), t);
+  const float c = fmaf(u, fmaf(u, fmaf(u, fmaf(u, fmaf(u, -1.f / 3628800.f, 1.f / 40320.f), -1.f / 720.f), 1.f / 24.f), -0.5f), 1.f);
   const float a = quarter & 1 ? s : c, b = quarter & 1 ? c : s;
   return make_float2((quarter + 1) & 2 ? -a : a, quarter & 2 ? -b : b);
 }
 
-// What does not change in a thread: its place in a head and the angles that its lane computes.
+// What a block has in shared memory besides sums.
+struct __align__(16) RtShared {
+  float cosine[RT_WARPS][RT_MOST_ANGLES], sine[RT_WARPS][RT_MOST_ANGLES];   // of the row that a warp has
+  float weight[2][RT_MOST_SIZE];
+  unsigned long long frequency[RT_MOST_ANGLES];
+  __device__ __forceinline__ void fill(const RtArgs& a) {
+    for (int i = threadIdx.x; i < a.c.rotated / 2; i += RT_THREADS) frequency[i] = a.frequency[i];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      for (int i = threadIdx.x; i < a.c.size; i += RT_THREADS) weight[k][i] = a.c.weight[k] != nullptr ? rt_weight(a.c.weight[k], a.c.weight_type, i) : 1.f;
+  }
+};
+
+// Eight (or four) floats on a 16-byte boundary of shared memory.
+template <int W>
+__device__ __forceinline__ void rt_get(const float* p, RtPair* f) {
+#pragma unroll
+  for (int i = 0; i < W / 4; ++i) {
+    const ulonglong2 v = reinterpret_cast<const ulonglong2*>(p)[i];
+    f[2 * i] = v.x, f[2 * i + 1] = v.y;
+  }
+}
+
+// A thread's place in a head: W elements from `lo` on and W from `hi` on, which hold W pairs.
 template <int W, bool PAIRS>
 struct RtPlace {
   int slot, heads;           // which of the heads that a warp takes at a time
-  int lo, hi, pair;          // its 2 W elements, and the first of its angles
+  int lo, hi, pair;          // and the first of its angles
   bool in, turned;
-  unsigned long long frequency[RT_MOST_SIZE / 64];
+  RtPair cosine[W / 2], sine[W / 2];
   __device__ __forceinline__ RtPlace(const RtArgs& a) {
     const int lane = threadIdx.x & 31, member = lane & (a.lanes - 1), half = a.c.rotated / 2;
     slot = lane / a.lanes;
@@ -193,140 +263,135 @@ struct RtPlace {
       lo = a.c.rotated + pair - half, hi = lo + (a.c.size - a.c.rotated) / 2;
       turned = false;
     }
-    turned = turned && in;
-#pragma unroll
-    for (int j = 0; j < RT_MOST_SIZE / 64; ++j) frequency[j] = lane + 32 * j < half ? a.frequency[lane + 32 * j] : 0ull;
+    if (!in) lo = hi = pair = 0, turned = false;   // (a lane without elements: zeros, whose weights are not its own)
   }
   // Cosines and sines of a row's angles, by way of the warp's shared memory.
-  __device__ __forceinline__ void angles(const RtArgs& a, unsigned long long position, float2* shared, float* cosine, float* sine) const {
-    const int lane = threadIdx.x & 31;
+  __device__ __forceinline__ void angles(const RtArgs& a, unsigned long long position, RtShared& shared) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __syncwarp();
+    for (int i = lane; i < a.c.rotated / 2; i += 32) {
+      const float2 t = rt_angle(position * shared.frequency[i]);
+      shared.cosine[warp][i] = t.x, shared.sine[warp][i] = t.y;
+    }
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < RT_MOST_SIZE / 64; ++j)
-      if (lane + 32 * j < a.c.rotated / 2) shared[lane + 32 * j] = rt_angle(position * frequency[j]);
-    __syncwarp();
-#pragma unroll
-    for (int e = 0; e < W; ++e) {
-      const float2 t = turned ? shared[pair + e] : make_float2(1.f, 0.f);
-      cosine[e] = t.x, sine[e] = t.y;
+    for (int e = 0; e < W / 2; ++e) cosine[e] = rt_both(1.f), sine[e] = rt_both(0.f);
+    if (turned) {
+      rt_get<W>(shared.cosine[warp] + pair, cosine);
+      rt_get<W>(shared.sine[warp] + pair, sine);
     }
   }
-  static __device__ __forceinline__ constexpr int first(int e) { return PAIRS ? 2 * e : e; }
-  static __device__ __forceinline__ constexpr int second(int e) { return PAIRS ? 2 * e + 1 : W + e; }
-  __device__ __forceinline__ int element(int i) const { return i < W ? lo + i : hi + i - W; }
+  // The 2 W elements turned, or turned back.
+  template <bool BACK>
+  __device__ __forceinline__ void turn(RtPair* v) const {
+    if (PAIRS) {
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        const float2 p = rt_floats(v[e]), cs = rt_floats(cosine[e / 2]), sn = rt_floats(sine[e / 2]);
+        const float c = e & 1 ? cs.y : cs.x, s = e & 1 ? sn.y : sn.x, t = BACK ? -s : s;
+        v[e] = rt_pair(fmaf(-p.y, t, p.x * c), fmaf(p.x, t, p.y * c));
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e) {
+        const RtPair p = v[e], q = v[W / 2 + e], pc = rt_mul(p, cosine[e]), qc = rt_mul(q, cosine[e]);
+        v[e] = BACK ? rt_fma(q, sine[e], pc) : rt_less(q, sine[e], pc);
+        v[W / 2 + e] = BACK ? rt_less(p, sine[e], qc) : rt_fma(p, sine[e], qc);
+      }
+    }
+  }
 };
 
 // Of the lanes of a head.
-__device__ __forceinline__ float rt_sum(float v, int lanes) {
-  for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+__device__ __forceinline__ float rt_sum(RtPair v2, int lanes) {
+  const float2 two = rt_floats(v2);
+  float v = two.x + two.y;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+    if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
-
-// A warp's next share: which of queries (0), keys (1) and values (2), of which row, from which head on.
-struct RtShare {
-  int kind, row, head, end;
-  __device__ __forceinline__ bool at(const RtArgs& a, long long u) {
-    const long long queries = (long long)a.c.rows * a.parts[0], keys = (long long)a.c.rows * a.parts[1];
-    kind = 0;
-    if (u >= queries) {
-      u -= queries;
-      kind = 1;
-      if (u >= keys) {
-        kind = 2;
-        row = (int)(u - keys);
-        return true;
-      }
-    }
-    const int parts = a.parts[kind], have = kind ? a.c.keys : a.c.heads;
-    row = parts == 1 ? (int)u : (int)(u / parts);
-    head = parts == 1 ? 0 : (int)(u - (long long)row * parts) * a.span;
-    end = min(head + a.span, have);
-    return true;
-  }
-};
+template <int W>
+__device__ __forceinline__ RtPair rt_dot(const RtPair* a, const RtPair* b) {
+  RtPair s = rt_mul(a[0], b[0]);
+#pragma unroll
+  for (int i = 1; i < W; ++i) s = rt_fma(a[i], b[i], s);
+  return s;
+}
 
 template <typename T, int W, bool PAIRS>
 __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_kernel(const __grid_constant__ RtArgs a) {
-  constexpr int U = 2;       // heads of a thread on their way
-  __shared__ float2 s_angles[RT_WARPS][RT_MOST_SIZE / 2];
+  __shared__ RtShared shared;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const RtPlace<W, PAIRS> place(a);
-  const long long shares = (long long)a.c.rows * (a.parts[0] + a.parts[1]);
-  const int size = a.c.size;
-  for (long long u = (long long)blockIdx.x * RT_WARPS + warp; u < shares; u += (long long)gridDim.x * RT_WARPS) {
-    RtShare share;
-    share.at(a, u);
-    const int have = share.kind ? a.c.keys : a.c.heads;
-    const T* x = (const T*)a.c.x + (long long)share.row * a.c.x_row + (share.kind ? (long long)a.c.heads * a.c.x_head : 0);
-    T* out = (T*)a.c.out[share.kind] + (long long)share.row * have * size;
-    RtVec<T, W> raw[U][2];
-    const auto load = [&](int head) {
+  RtPlace<W, PAIRS> place(a);
+  const int size = a.c.size, all = a.c.heads + a.c.keys, step = place.heads, steps = (all + step - 1) / step;
+  const long long u = (long long)blockIdx.x * RT_WARPS + warp;
+  int row = (int)u, first = 0, end = all;
+  if (a.parts > 1) {
+    row = (int)(u / a.parts);
+    const int part = (int)(u - (long long)row * a.parts);
+    first = steps * part / a.parts * step;
+    end = min(steps * (part + 1) / a.parts * step, all);
+  }
+  const bool live = row < a.c.rows;
+  const int apart = place.hi - place.lo;
+  // lanes that have no head, or none any more, read another one: their neighbours' sums need them
+  const T* x = (const T*)a.c.x + (long long)row * a.c.x_row + place.lo;
+  RtVec<T, W> raw[2];
+  const auto load = [&](int head) {
+    const T* p = x + min(head, end - 1) * a.c.x_head;
+    raw[0].load(p), raw[1].load(p + apart);
+  };
+  if (live) load(first + place.slot);
+  shared.fill(a);
+  __syncthreads();
+  if (!live) return;
+  T* queries = (T*)a.c.out[0] + (long long)row * a.c.heads * size + place.lo;
+  T* keys = (T*)a.c.out[1] + ((long long)row * a.c.keys - a.c.heads) * size + place.lo;
+  unsigned long long position;
+  if (!rt_position(a.c, row, lane, position)) {
+    RtPair zeros[W / 2];
 #pragma unroll
-      for (int j = 0; j < U; ++j) {
-        const int h = head + j * place.heads + place.slot;
-        if (place.in && h < share.end) {
-          raw[j][0].load(x + h * a.c.x_head + place.lo);
-          raw[j][1].load(x + h * a.c.x_head + place.hi);
-        } else {
-          raw[j][0].clear();
-          raw[j][1].clear();
+    for (int i = 0; i < W / 2; ++i) zeros[i] = 0;
+    for (int head = first + place.slot; place.in && head < end; head += step) {
+      T* to = (head < a.c.heads ? queries : keys) + head * size;
+      RtVec<T, W>::store(to, zeros);
+      RtVec<T, W>::store(to + apart, zeros);
+    }
+    return;
+  }
+  if (a.c.rotated > 0) place.angles(a, position, shared);
+  for (; first < end; first += step) {
+    RtPair f[W];
+    raw[0].unpack(f), raw[1].unpack(f + W / 2);
+    const int head = first + place.slot;
+    if (first + step < end) load(head + step);
+    if (a.c.norm) {
+      const RtPair squares = rt_dot<W>(f, f);
+      float s = rt_sum(place.in ? squares : 0, a.lanes), eps = a.c.eps;
+      const bool large = !(s < 0x1p126f);
+      if (sizeof(T) == 4 || std::is_same<T, __nv_bfloat16>::value) {
+        if (__any_sync(0xffffffffu, large)) {
+          const RtPair down = rt_both(large ? RT_DOWN : 1.f);
+#pragma unroll
+          for (int i = 0; i < W; ++i) f[i] = rt_mul(f[i], down);
+          const float t = rt_sum(place.in ? rt_dot<W>(f, f) : 0, a.lanes);
+          if (large) s = t, eps *= RT_DOWN * RT_DOWN;
         }
       }
-    };
-    load(share.head);
-    unsigned long long position;
-    const bool held = rt_position(a.c, share.row, lane, position);
-    float cosine[W], sine[W], w[2 * W];
-    place.angles(a, position, s_angles[warp], cosine, sine);
-    const void* weight = a.c.weight[share.kind];
+      const RtPair r = rt_both(rsqrtf(fmaf(s, a.share, eps)));
+      RtPair w[W];
+      const float* weight = shared.weight[head >= a.c.heads] + place.lo;
+      rt_get<W>(weight, w);
+      rt_get<W>(weight + apart, w + W / 2);
 #pragma unroll
-    for (int i = 0; i < 2 * W; ++i) w[i] = weight != nullptr && place.in ? rt_weight(weight, a.c.weight_type, place.element(i)) : 1.f;
-    for (int head = share.head;;) {
-#pragma unroll
-      for (int j = 0; j < U; ++j) {
-        float f[2 * W], z[2 * W];
-        raw[j][0].unpack(f);
-        raw[j][1].unpack(f + W);
-        float r = 1.f;
-        if (a.c.norm) {
-          float s = 0.f;
-#pragma unroll
-          for (int i = 0; i < 2 * W; ++i) s = fmaf(f[i], f[i], s);
-          s = rt_sum(s, a.lanes);
-          float eps = a.c.eps;
-          const bool large = !(s < 0x1p126f);
-          if (__any_sync(0xffffffffu, large)) {
-            float t = 0.f;
-#pragma unroll
-            for (int i = 0; i < 2 * W; ++i) {
-              if (large) f[i] *= RT_DOWN;
-              t = fmaf(f[i], f[i], t);
-            }
-            t = rt_sum(t, a.lanes);
-            if (large) s = t, eps *= RT_DOWN * RT_DOWN;
-          }
-          r = rsqrtf(s / (float)size + eps);
-        }
-#pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const int p = place.first(e), q = place.second(e);
-          const float ya = f[p] * w[p] * r, yb = f[q] * w[q] * r;
-          z[p] = ya * cosine[e] - yb * sine[e];
-          z[q] = yb * cosine[e] + ya * sine[e];
-        }
-        const int h = head + j * place.heads + place.slot;
-        if (place.in && h < share.end) {
-          if (!held) {
-#pragma unroll
-            for (int i = 0; i < 2 * W; ++i) z[i] = 0.f;
-          }
-          RtVec<T, W>::store(out + (long long)h * size + place.lo, z);
-          RtVec<T, W>::store(out + (long long)h * size + place.hi, z + W);
-        }
-      }
-      head += U * place.heads;
-      if (head >= share.end) break;
-      load(head);
+      for (int i = 0; i < W; ++i) f[i] = rt_mul(rt_mul(f[i], r), w[i]);
+    }
+    if (a.c.rotated > 0) place.template turn<false>(f);
+    if (place.in && head < end) {
+      T* to = (head < a.c.heads ? queries : keys) + head * size;
+      RtVec<T, W>::store(to, f);
+      RtVec<T, W>::store(to + apart, f + W / 2);
     }
   }
 }
@@ -334,135 +399,138 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
 template <typename T, int W, bool PAIRS>
 __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_grad_kernel(const __grid_constant__ RtArgs a) {
   psgd_launch_dependents();
-  __shared__ float2 s_angles[RT_WARPS][RT_MOST_SIZE / 2];
-  __shared__ float s_sums[2][RT_WARPS][RT_MOST_SIZE];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, size = a.c.size, all = a.c.heads + a.c.keys + a.c.values;
-  const RtPlace<W, PAIRS> place(a);
+  __shared__ RtShared shared;
+  __shared__ __align__(16) float s_sums[2][RT_WARPS][RT_MOST_SIZE];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, size = a.c.size, all = a.c.heads + a.c.keys + a.c.values, step = 32 / a.lanes;
+  RtPlace<W, PAIRS> place(a);
+  const int apart = place.hi - place.lo;
   const bool sums = a.c.parts != nullptr;
-  for (int i = lane; sums && i < 2 * size; i += 32) s_sums[i >= size][warp][i >= size ? i - size : i] = 0.f;
-  __syncwarp();
-  float acc[2 * W];
+  shared.fill(a);
+  if (sums)
+    for (int i = threadIdx.x; i < 2 * RT_WARPS * RT_MOST_SIZE; i += RT_THREADS) ((float*)s_sums)[i] = 0.f;
+  __syncthreads();
+  RtPair acc[W];
 #pragma unroll
-  for (int i = 0; i < 2 * W; ++i) acc[i] = 0.f;
-  // what the warp's threads have added up for one kind
+  for (int i = 0; i < W; ++i) acc[i] = 0;
+  // what the warp's threads have added up for one kind of heads
   const auto flush = [&](int kind) {
 #pragma unroll
-    for (int i = 0; i < 2 * W; ++i) {
-      for (int o = a.lanes; o < 32; o <<= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-      if (place.slot == 0 && place.in) s_sums[kind][warp][place.element(i)] = acc[i];
-      acc[i] = 0.f;
+    for (int i = 0; i < W; ++i) {
+      float2 v = rt_floats(acc[i]);
+      for (int o = a.lanes; o < 32; o <<= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+      }
+      if (place.slot == 0 && place.in) *reinterpret_cast<float2*>(&s_sums[kind][warp][(i < W / 2 ? place.lo : place.hi - W) + 2 * i]) = v;
+      acc[i] = 0;
     }
   };
-  const long long shares = (long long)a.c.rows * (a.parts[0] + a.parts[1] + (a.c.values && a.c.dx ? 1 : 0));
+  // shares of rows: all of the queries', then all of the keys' and the values', so that a warp adds up one kind of heads at a time
+  const uint32_t queries = (uint32_t)a.c.rows * (uint32_t)a.parts, shares = a.c.keys + a.c.values > 0 ? 2 * queries : queries, stride = gridDim.x * RT_WARPS;
   int kind = 0;
-  for (long long u = (long long)blockIdx.x * RT_WARPS + warp; u < shares; u += (long long)gridDim.x * RT_WARPS) {
-    RtShare share;
-    share.at(a, u);
-    if (share.kind != kind) {
-      if (sums && kind < 2) flush(kind);
-      kind = share.kind;
+  for (uint32_t u = blockIdx.x * RT_WARPS + warp; u < shares; u += stride) {
+    if (kind == 0 && u >= queries) {
+      if (sums) flush(0);
+      kind = 1;
     }
-    const T* g = (const T*)a.c.grad[kind];
-    if (g != nullptr) g += (long long)share.row * a.c.grad_row[kind];
-    T* dx = (T*)a.c.dx;
-    if (dx != nullptr) dx += ((long long)share.row * all + (kind == 0 ? 0 : kind == 1 ? a.c.heads : a.c.heads + a.c.keys)) * size;
-    if (kind == 2) {     // values pass by
+    const uint32_t v = kind ? u - queries : u;
+    const int row = a.parts == 1 ? (int)v : (int)(v / (uint32_t)a.parts), part = a.parts == 1 ? 0 : (int)(v - (uint32_t)row * (uint32_t)a.parts);
+    const int have = kind ? a.c.keys : a.c.heads, steps = (have + step - 1) / step;
+    int first = steps * part / a.parts * step;
+    const int end = min(steps * (part + 1) / a.parts * step, have);
+    T* dx_row = a.c.dx != nullptr ? (T*)a.c.dx + (long long)row * all * size : nullptr;
+    T* dx = dx_row + (kind ? a.c.heads * size : 0) + place.lo;
+    unsigned long long position;
+    if (!rt_position(a.c, row, lane, position)) {
+      RtPair zeros[W / 2];
+#pragma unroll
+      for (int i = 0; i < W / 2; ++i) zeros[i] = 0;
+      for (int head = first + place.slot; dx_row != nullptr && place.in && head < end; head += step) {
+        RtVec<T, W>::store(dx + head * size, zeros);
+        RtVec<T, W>::store(dx + head * size + apart, zeros);
+      }
+      first = end;
+    }
+    if (first < end) {
+      const T* x = (const T*)a.c.x + (long long)row * a.c.x_row + (kind ? a.c.heads * a.c.x_head : 0) + place.lo;
+      const bool given = a.c.grad[kind] != nullptr;
+      const T* g = (const T*)a.c.grad[kind] + (long long)row * a.c.grad_row[kind] + place.lo;
+      RtVec<T, W> raw[2], rawg[2];
+      const auto load = [&](int head) {    // (lanes that have no head any more read another one, with a gradient of zeros)
+        const T* p = x + min(head, end - 1) * a.c.x_head;
+        raw[0].load(p), raw[1].load(p + apart);
+        rawg[0].clear(), rawg[1].clear();
+        if (given && place.in && head < end) {
+          const T* q = g + head * a.c.grad_head[kind];
+          rawg[0].load(q), rawg[1].load(q + apart);
+        }
+      };
+      load(first + place.slot);
+      if (a.c.rotated > 0) place.angles(a, position, shared);
+      const float* weight = shared.weight[kind] + place.lo;
+      for (; first < end; first += step) {
+        RtPair f[W], d[W];
+        raw[0].unpack(f), raw[1].unpack(f + W / 2);
+        rawg[0].unpack(d), rawg[1].unpack(d + W / 2);
+        const int head = first + place.slot;
+        if (first + step < end) load(head + step);
+        if (a.c.rotated > 0) place.template turn<true>(d);
+        if (a.c.norm) {
+          const auto dots = [&](float& s, float& t) {
+            RtPair w[W], squares = rt_dot<W>(f, f);
+            rt_get<W>(weight, w);
+            rt_get<W>(weight + apart, w + W / 2);
+            RtPair along = rt_mul(rt_mul(d[0], w[0]), f[0]);
+#pragma unroll
+            for (int i = 1; i < W; ++i) along = rt_fma(rt_mul(d[i], w[i]), f[i], along);
+            s = rt_sum(place.in ? squares : 0, a.lanes);
+            t = rt_sum(along, a.lanes);
+          };
+          float s, t, eps = a.c.eps, down = 1.f;
+          dots(s, t);
+          if (sizeof(T) == 4 || std::is_same<T, __nv_bfloat16>::value) {
+            const bool large = !(s < 0x1p126f);
+            if (__any_sync(0xffffffffu, large)) {
+              const RtPair less = rt_both(large ? RT_DOWN : 1.f);
+#pragma unroll
+              for (int i = 0; i < W; ++i) f[i] = rt_mul(f[i], less);
+              dots(s, t);
+              if (large) eps *= RT_DOWN * RT_DOWN, down = RT_DOWN;
+            }
+          }
+          const float r = rsqrtf(fmaf(s, a.share, eps));
+          const RtPair r2 = rt_both(r), rd = rt_both(r * down), along = rt_both(-t * a.share * r * r * r * down);
+          RtPair w[W];
+          rt_get<W>(weight, w);
+          rt_get<W>(weight + apart, w + W / 2);
+          // dw += dy x r;  dx = dy w r - x r^3 mean(dy w x)
+#pragma unroll
+          for (int i = 0; i < W; ++i) {
+            if (sums) acc[i] = rt_fma(rt_mul(d[i], r2), f[i], acc[i]);
+            d[i] = rt_fma(f[i], along, rt_mul(rt_mul(d[i], w[i]), rd));
+          }
+        }
+        if (place.in && head < end && dx_row != nullptr) {
+          RtVec<T, W>::store(dx + head * size, d);
+          RtVec<T, W>::store(dx + head * size + apart, d + W / 2);
+        }
+      }
+    }
+    if (kind && dx_row != nullptr && a.c.values > 0) {     // values pass by
       constexpr int N = 16 / (int)sizeof(T);
       const int vectors = size / N;
-      for (int i = lane; i < a.c.values * vectors; i += 32) {
+      const T* gv = a.c.grad[2] != nullptr ? (const T*)a.c.grad[2] + (long long)row * a.c.grad_row[2] : nullptr;
+      T* to = dx_row + (long long)(a.c.heads + a.c.keys) * size;
+#pragma unroll 4
+      for (int i = part * 32 + lane; i < a.c.values * vectors; i += 32 * a.parts) {
         const int h = i / vectors, e = (i - h * vectors) * N;
-        *reinterpret_cast<uint4*>(dx + (long long)h * size + e) =
-            g != nullptr ? __ldcs(reinterpret_cast<const uint4*>(g + h * a.c.grad_head[2] + e)) : make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(to + (long long)h * size + e) = gv != nullptr ? __ldcs(reinterpret_cast<const uint4*>(gv + h * a.c.grad_head[2] + e)) : make_uint4(0, 0, 0, 0);
       }
-      continue;
     }
-    const T* x = (const T*)a.c.x + (long long)share.row * a.c.x_row + (kind ? (long long)a.c.heads * a.c.x_head : 0);
-    RtVec<T, W> raw[2], rawg[2];
-    const auto load = [&](int head) {
-      const int h = head + place.slot;
-      if (place.in && h < share.end) {
-        raw[0].load(x + h * a.c.x_head + place.lo);
-        raw[1].load(x + h * a.c.x_head + place.hi);
-      } else {
-        raw[0].clear(), raw[1].clear();
-      }
-      if (place.in && h < share.end && g != nullptr) {
-        rawg[0].load(g + h * a.c.grad_head[kind] + place.lo);
-        rawg[1].load(g + h * a.c.grad_head[kind] + place.hi);
-      } else {
-        rawg[0].clear(), rawg[1].clear();
-      }
-    };
-    load(share.head);
-    unsigned long long position;
-    const bool held = rt_position(a.c, share.row, lane, position);
-    float cosine[W], sine[W], w[2 * W];
-    place.angles(a, position, s_angles[warp], cosine, sine);
-    const void* weight = a.c.weight[kind];
-#pragma unroll
-    for (int i = 0; i < 2 * W; ++i) w[i] = weight != nullptr && place.in ? rt_weight(weight, a.c.weight_type, place.element(i)) : 1.f;
-    for (int head = share.head;;) {
-      float f[2 * W], z[2 * W], d[2 * W];
-      raw[0].unpack(f), raw[1].unpack(f + W);
-      rawg[0].unpack(z), rawg[1].unpack(z + W);
-      const int h = head + place.slot;
-      const bool mine = place.in && h < share.end;
-      head += place.heads;
-      const bool more = head < share.end;
-      if (more) load(head);
-#pragma unroll
-      for (int e = 0; e < W; ++e) {     // turned back
-        const int p = place.first(e), q = place.second(e);
-        d[p] = z[p] * cosine[e] + z[q] * sine[e];
-        d[q] = z[q] * cosine[e] - z[p] * sine[e];
-      }
-      float r = 1.f, t = 0.f, down = 1.f;
-      if (a.c.norm) {
-        float s = 0.f;
-#pragma unroll
-        for (int i = 0; i < 2 * W; ++i) {
-          s = fmaf(f[i], f[i], s);
-          t = fmaf(d[i] * w[i], f[i], t);
-        }
-        s = rt_sum(s, a.lanes);
-        t = rt_sum(t, a.lanes);
-        float eps = a.c.eps;
-        const bool large = !(s < 0x1p126f);
-        if (__any_sync(0xffffffffu, large)) {
-          float s1 = 0.f, t1 = 0.f;
-#pragma unroll
-          for (int i = 0; i < 2 * W; ++i) {
-            if (large) f[i] *= RT_DOWN;
-            s1 = fmaf(f[i], f[i], s1);
-            t1 = fmaf(d[i] * w[i], f[i], t1);
-          }
-          s1 = rt_sum(s1, a.lanes);
-          t1 = rt_sum(t1, a.lanes);
-          if (large) s = s1, t = t1, eps *= RT_DOWN * RT_DOWN, down = RT_DOWN;
-        }
-        r = rsqrtf(s / (float)size + eps);
-        t *= r / (float)size;         // mean(dn n)
-      }
-      if (mine && held) {
-#pragma unroll
-        for (int i = 0; i < 2 * W; ++i) {
-          const float n = f[i] * r;
-          acc[i] = fmaf(d[i], n, acc[i]);
-          z[i] = (d[i] * w[i] - n * t) * (r * down);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 2 * W; ++i) z[i] = 0.f;
-      }
-      if (mine && dx != nullptr) {
-        RtVec<T, W>::store(dx + (long long)h * size + place.lo, z);
-        RtVec<T, W>::store(dx + (long long)h * size + place.hi, z + W);
-      }
-      if (!more) break;
-    }
+    if (shares - u <= stride) break;   // (32 bits)
   }
   if (!sums) return;
-  if (kind < 2) flush(kind);
+  flush(kind);
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * size; i += RT_THREADS) {
     const int k = i >= size, e = k ? i - size : i;
@@ -473,19 +541,25 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   }
 }
 
-// Sums of the blocks' parts: 32 columns to a block, 8 threads to a column.
-__global__ void __launch_bounds__(RT_THREADS) psgd_rotate_weights_kernel(const float* parts, int blocks, int size, int type, void* queries, void* keys) {
+// Sums of the blocks' parts: 32 columns to a block, 32 threads to a column.
+constexpr int RT_SLICES = 32;
+__global__ void __launch_bounds__(32 * RT_SLICES) psgd_rotate_weights_kernel(const float* parts, int blocks, int size, int type, void* queries, void* keys) {
   psgd_wait_for_predecessor();
-  __shared__ float s_part[RT_WARPS][32];
+  __shared__ float s_part[RT_SLICES][32];
   const int column = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
   float v = 0.f;
-  if (column < 2 * size)
-    for (int b = slice; b < blocks; b += RT_WARPS) v += __ldcg(parts + (long long)b * 2 * size + column);
+  if (column < 2 * size) {
+#pragma unroll
+    for (int j = 0; j < (RT_PART_BLOCKS + RT_SLICES - 1) / RT_SLICES; ++j) {
+      const int b = j * RT_SLICES + slice;
+      v += b < blocks ? __ldcg(parts + (long long)b * 2 * size + column) : 0.f;
+    }
+  }
   s_part[slice][threadIdx.x & 31] = v;
   __syncthreads();
   if (slice != 0 || column >= 2 * size) return;
 #pragma unroll
-  for (int j = 1; j < RT_WARPS; ++j) v += s_part[j][threadIdx.x];
+  for (int j = 1; j < RT_SLICES; ++j) v += s_part[j][threadIdx.x];
   void* out = column < size ? queries : keys;
   const int e = column < size ? column : column - size;
   if (out == nullptr) return;
@@ -494,47 +568,44 @@ __global__ void __launch_bounds__(RT_THREADS) psgd_rotate_weights_kernel(const f
   else ((__half*)out)[e] = __float2half_rn(v);
 }
 
-// How a call is spread: 8 elements on either side of the pairs where they fit, shares of rows small enough that every SM has warps, where
-// there are few rows.
+// Where there are few rows, several warps share one, as long as each has heads (`heads` of a kind, `at_once` of which a warp takes in a step).
 template <int W>
-void rt_plan(RtArgs& a, int warps) {
+void rt_plan(RtArgs& a, int warps, int heads) {
   int lanes = 1;
   while (lanes * 2 * W < a.c.size) lanes *= 2;
   a.lanes = lanes;
-  const int least = 32 / lanes, most = a.c.heads > a.c.keys ? a.c.heads : a.c.keys;
-  int steps = (most + least - 1) / least;
-  const auto shares = [&](int span) { return (long long)a.c.rows * ((a.c.heads + span - 1) / span + (a.c.keys + span - 1) / span); };
-  while (steps > 1 && shares(steps * least) < warps) steps = (steps + 1) / 2;
-  a.span = steps * least;
-  a.parts[0] = (a.c.heads + a.span - 1) / a.span;
-  a.parts[1] = (a.c.keys + a.span - 1) / a.span;
+  a.share = 1.f / (float)a.c.size;
+  const int step = 32 / lanes, steps = (heads + step - 1) / step;
+  a.parts = 1;
+  while (a.parts < steps && (long long)a.c.rows * (a.parts + 1) <= warps) ++a.parts;
 }
 
 template <typename T, int W, bool PAIRS>
 int rt_forward(RtArgs& a, cudaStream_t stream) {
-  rt_plan<W>(a, RT_SMS * RT_FORWARD_BLOCKS * RT_WARPS);
-  const long long shares = (long long)a.c.rows * (a.parts[0] + a.parts[1]), blocks = (shares + RT_WARPS - 1) / RT_WARPS;
-  return psgd_launch(psgd_rotate_kernel<T, W, PAIRS>, (int)(blocks < RT_SMS * RT_FORWARD_BLOCKS ? blocks : RT_SMS * RT_FORWARD_BLOCKS), RT_THREADS, 0, stream, 0, a);
+  rt_plan<W>(a, RT_SMS * RT_FORWARD_BLOCKS * RT_WARPS, a.c.heads + a.c.keys);
+  const long long blocks = ((long long)a.c.rows * a.parts + RT_WARPS - 1) / RT_WARPS;
+  return psgd_launch(psgd_rotate_kernel<T, W, PAIRS>, (int)blocks, RT_THREADS, 0, stream, 0, a);
 }
 template <typename T, int W, bool PAIRS>
 int rt_backward(RtArgs& a, cudaStream_t stream) {
-  rt_plan<W>(a, RT_SMS * RT_BACKWARD_BLOCKS * RT_WARPS);
-  const long long shares = (long long)a.c.rows * (a.parts[0] + a.parts[1] + (a.c.values && a.c.dx ? 1 : 0)), blocks = (shares + RT_WARPS - 1) / RT_WARPS;
-  const int grid = (int)(blocks < RT_SMS * RT_BACKWARD_BLOCKS ? blocks : RT_SMS * RT_BACKWARD_BLOCKS);
+  rt_plan<W>(a, RT_PART_BLOCKS * RT_WARPS, a.c.heads > a.c.keys ? a.c.heads : a.c.keys);
+  const long long blocks = ((long long)a.c.rows * a.parts * (a.c.keys + a.c.values > 0 ? 2 : 1) + RT_WARPS - 1) / RT_WARPS;
+  const int grid = (int)(blocks < RT_PART_BLOCKS || a.c.parts == nullptr ? blocks : RT_PART_BLOCKS);
   if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS>, grid, RT_THREADS, 0, stream, 0, a)) return code;
   if (a.c.parts == nullptr) return 0;
-  return psgd_launch(psgd_rotate_weights_kernel, (2 * a.c.size + 31) / 32, RT_THREADS, 0, stream, 1, (const float*)a.c.parts, grid, a.c.size, a.c.weight_type, a.c.dweight[0],
+  return psgd_launch(psgd_rotate_weights_kernel, (2 * a.c.size + 31) / 32, 32 * RT_SLICES, 0, stream, 1, (const float*)a.c.parts, grid, a.c.size, a.c.weight_type, a.c.dweight[0],
                      a.c.dweight[1]);
 }
 
 template <typename T>
 int rt_dispatch(RtArgs& a, bool gradient, cudaStream_t stream) {
-  const bool wide = a.c.size % 16 == 0 && a.c.rotated % 16 == 0;
-  if (a.c.pairs) {
-    if (wide) return gradient ? rt_backward<T, 8, true>(a, stream) : rt_forward<T, 8, true>(a, stream);
-    return gradient ? rt_backward<T, 4, true>(a, stream) : rt_forward<T, 4, true>(a, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (a.c.size % 16 == 0 && a.c.rotated % 16 == 0 && (gradient ? WB : WF)) {
+      if (a.c.pairs) return gradient ? rt_backward<T, 8, true>(a, stream) : rt_forward<T, 8, true>(a, stream);
+      return gradient ? rt_backward<T, 8, false>(a, stream) : rt_forward<T, 8, false>(a, stream);
+    }
   }
-  if (wide) return gradient ? rt_backward<T, 8, false>(a, stream) : rt_forward<T, 8, false>(a, stream);
+  if (a.c.pairs) return gradient ? rt_backward<T, 4, true>(a, stream) : rt_forward<T, 4, true>(a, stream);
   return gradient ? rt_backward<T, 4, false>(a, stream) : rt_forward<T, 4, false>(a, stream);
 }
 
@@ -557,7 +628,7 @@ int rt_call(const PsgdRotate* call, bool gradient, cudaStream_t stream) {
 PSGD_API int psgd_rotate_call_bytes() { return (int)sizeof(PsgdRotate); }
 
 // Floats of scratch for the gradients of weights.
-PSGD_API long long psgd_rotate_parts(int size) { return (long long)RT_SMS * RT_BACKWARD_BLOCKS * 2 * size; }
+PSGD_API long long psgd_rotate_parts(int size) { return (long long)RT_PART_BLOCKS * 2 * size; }
 
 // `call`: host memory, read before the call returns. Rows that belong to no sequence give zeros.
 PSGD_API int psgd_rotate(const PsgdRotate* call, cudaStream_t stream) { return call->rows == 0 ? 0 : rt_call(call, false, stream); }
