@@ -52,7 +52,13 @@ constexpr int RT_SMS = 148;
 #define BB 2
 #define WF 1
 #define WB 1
+#define FS 3
+#define BS 3
 #endif
+constexpr int RT_FORWARD_STAGES = FS, RT_BACKWARD_STAGES = BS;   // steps of a warp whose inputs are on their way, and one more
+// Do the squares of a type leave the range of float32?
+template <typename T>
+constexpr bool RT_RANGE = !std::is_same<T, __half>::value;
 constexpr int RT_FORWARD_BLOCKS = FB, RT_BACKWARD_BLOCKS = BB;   // of an SM at a time
 constexpr int RT_PART_BLOCKS = RT_SMS * RT_BACKWARD_BLOCKS;    // that add up gradients of weights
 constexpr float RT_DOWN = 0x1p-70f;                            // for heads whose squares leave the range
@@ -101,13 +107,10 @@ struct RtVec;
 template <int W>
 struct RtVec<float, W> {
   float4 v[W / 4];
-  __device__ __forceinline__ void load(const float* p) {
+  static constexpr int BYTES = 4 * W;
+  __device__ __forceinline__ void get(const char* p) {
 #pragma unroll
-    for (int i = 0; i < W / 4; ++i) v[i] = __ldcs(reinterpret_cast<const float4*>(p) + i);
-  }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < W / 4; ++i) v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = 0; i < W / 4; ++i) v[i] = reinterpret_cast<const float4*>(p)[i];
   }
   __device__ __forceinline__ void unpack(RtPair* f) const {
 #pragma unroll
@@ -151,11 +154,8 @@ struct RtVec {
     Words v;
     uint32_t w[W / 2];
   };
-  __device__ __forceinline__ void load(const T* p) { v = __ldcs(reinterpret_cast<const Words*>(p)); }
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int i = 0; i < W / 2; ++i) w[i] = 0;
-  }
+  static constexpr int BYTES = 2 * W;
+  __device__ __forceinline__ void get(const char* p) { v = *reinterpret_cast<const Words*>(p); }
   __device__ __forceinline__ void unpack(RtPair* f) const {
 #pragma unroll
     for (int i = 0; i < W / 2; ++i) f[i] = rt_wide(w[i], T());
@@ -167,6 +167,17 @@ struct RtVec {
     *reinterpret_cast<Words*>(p) = o.v;
   }
 };
+
+// What is on its way to a thread's own places in shared memory: WORDS bytes each, zeros where `there` is false (nothing is read then).
+template <int BYTES>
+__device__ __forceinline__ void rt_fetch(void* to, const void* from, bool there) {
+  const uint32_t at = (uint32_t)__cvta_generic_to_shared(to);
+  if (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(at), "l"(from), "r"(there ? 16 : 0) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(at), "l"(from), "r"(there ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void rt_fetched() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LATER>
+__device__ __forceinline__ void rt_await() { asm volatile("cp.async.wait_group %0;" ::"n"(LATER) : "memory"); }
 
 __device__ __forceinline__ float rt_weight(const void* p, int type, int i) {
   if (type == 0) return ((const float*)p)[i];
@@ -321,94 +332,206 @@ __device__ __forceinline__ RtPair rt_dot(const RtPair* a, const RtPair* b) {
 
 template <typename T, int W, bool PAIRS>
 __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_kernel(const __grid_constant__ RtArgs a) {
+  typedef RtVec<T, W> Vec;
+  constexpr int HALF = RT_THREADS * Vec::BYTES, STAGE = 2 * HALF;     // of the ring
   __shared__ RtShared shared;
+  __shared__ __align__(16) char ring[RT_FORWARD_STAGES * STAGE];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   RtPlace<W, PAIRS> place(a);
-  const int size = a.c.size, all = a.c.heads + a.c.keys, step = place.heads, steps = (all + step - 1) / step;
-  const long long u = (long long)blockIdx.x * RT_WARPS + warp;
-  int row = (int)u, first = 0, end = all;
+  const int size = a.c.size, all = a.c.heads + a.c.keys, step = place.heads;
+  const uint32_t u = blockIdx.x * RT_WARPS + warp;
+  int row = (int)u, head = place.slot, end = all;
   if (a.parts > 1) {
-    row = (int)(u / a.parts);
-    const int part = (int)(u - (long long)row * a.parts);
-    first = steps * part / a.parts * step;
+    const int steps = (all + step - 1) / step;
+    row = (int)(u / (uint32_t)a.parts);
+    const int part = (int)(u - (uint32_t)row * (uint32_t)a.parts);
+    head += steps * part / a.parts * step;
     end = min(steps * (part + 1) / a.parts * step, all);
   }
   const bool live = row < a.c.rows;
-  const int apart = place.hi - place.lo;
-  // lanes that have no head, or none any more, read another one: their neighbours' sums need them
-  const T* x = (const T*)a.c.x + (long long)row * a.c.x_row + place.lo;
-  RtVec<T, W> raw[2];
-  const auto load = [&](int head) {
-    const T* p = x + min(head, end - 1) * a.c.x_head;
-    raw[0].load(p), raw[1].load(p + apart);
+  const int count = live ? (end - head + place.slot + step - 1) / step : 0, apart = place.hi - place.lo;
+  if (!place.in || !live) end = 0;
+  const long long x_step = step * a.c.x_head;
+  const T* x = (const T*)a.c.x + (long long)row * a.c.x_row + head * a.c.x_head + place.lo;
+  char* const mine = ring + threadIdx.x * Vec::BYTES;
+  int ahead = head, to = 0, from = 0;
+  const auto fetch = [&]() {      // (lanes without a head, or behind the last one, find zeros)
+    rt_fetch<Vec::BYTES>(mine + to, x, ahead < end);
+    rt_fetch<Vec::BYTES>(mine + to + HALF, x + apart, ahead < end);
+    rt_fetched();
+    ahead += step;
+    x += x_step;
+    to = to == (RT_FORWARD_STAGES - 1) * STAGE ? 0 : to + STAGE;
   };
-  if (live) load(first + place.slot);
+#pragma unroll
+  for (int i = 0; i < RT_FORWARD_STAGES - 1; ++i) fetch();
   shared.fill(a);
   __syncthreads();
-  if (!live) return;
-  T* queries = (T*)a.c.out[0] + (long long)row * a.c.heads * size + place.lo;
-  T* keys = (T*)a.c.out[1] + ((long long)row * a.c.keys - a.c.heads) * size + place.lo;
+  if (!live) {
+    rt_await<0>();
+    return;
+  }
+  const long long out_step = step * size, to_keys = ((T*)a.c.out[1] + ((long long)row * a.c.keys - a.c.heads) * size) - ((T*)a.c.out[0] + (long long)row * a.c.heads * size);
+  T* out = (T*)a.c.out[0] + ((long long)row * a.c.heads + head) * size + place.lo;     // (as if the keys lay behind the queries)
   unsigned long long position;
   if (!rt_position(a.c, row, lane, position)) {
     RtPair zeros[W / 2];
 #pragma unroll
     for (int i = 0; i < W / 2; ++i) zeros[i] = 0;
-    for (int head = first + place.slot; place.in && head < end; head += step) {
-      T* to = (head < a.c.heads ? queries : keys) + head * size;
-      RtVec<T, W>::store(to, zeros);
-      RtVec<T, W>::store(to + apart, zeros);
+    for (; head < end; head += step, out += out_step) {
+      T* o = head < a.c.heads ? out : out + to_keys;
+      Vec::store(o, zeros);
+      Vec::store(o + apart, zeros);
     }
+    rt_await<0>();
     return;
   }
   if (a.c.rotated > 0) place.angles(a, position, shared);
-  for (; first < end; first += step) {
+  const float* weight = shared.weight[0] + place.lo;
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    rt_await<RT_FORWARD_STAGES - 2>();
+    Vec raw[2];
+    raw[0].get(mine + from), raw[1].get(mine + from + HALF);
+    from = from == (RT_FORWARD_STAGES - 1) * STAGE ? 0 : from + STAGE;
     RtPair f[W];
     raw[0].unpack(f), raw[1].unpack(f + W / 2);
-    const int head = first + place.slot;
-    if (first + step < end) load(head + step);
+    fetch();     // to where the step before this one was read
+    const bool key = head >= a.c.heads;
     if (a.c.norm) {
-      const RtPair squares = rt_dot<W>(f, f);
-      float s = rt_sum(place.in ? squares : 0, a.lanes), eps = a.c.eps;
-      const bool large = !(s < 0x1p126f);
-      if (sizeof(T) == 4 || std::is_same<T, __nv_bfloat16>::value) {
+      float s = rt_sum(rt_dot<W>(f, f), a.lanes), eps = a.c.eps;
+      if (RT_RANGE<T>) {
+        const bool large = !(s < 0x1p126f);
         if (__any_sync(0xffffffffu, large)) {
           const RtPair down = rt_both(large ? RT_DOWN : 1.f);
 #pragma unroll
-          for (int i = 0; i < W; ++i) f[i] = rt_mul(f[i], down);
-          const float t = rt_sum(place.in ? rt_dot<W>(f, f) : 0, a.lanes);
+          for (int j = 0; j < W; ++j) f[j] = rt_mul(f[j], down);
+          const float t = rt_sum(rt_dot<W>(f, f), a.lanes);
           if (large) s = t, eps *= RT_DOWN * RT_DOWN;
         }
       }
       const RtPair r = rt_both(rsqrtf(fmaf(s, a.share, eps)));
       RtPair w[W];
-      const float* weight = shared.weight[head >= a.c.heads] + place.lo;
-      rt_get<W>(weight, w);
-      rt_get<W>(weight + apart, w + W / 2);
+      const float* own = weight + (key ? RT_MOST_SIZE : 0);
+      rt_get<W>(own, w);
+      rt_get<W>(own + apart, w + W / 2);
 #pragma unroll
-      for (int i = 0; i < W; ++i) f[i] = rt_mul(rt_mul(f[i], r), w[i]);
+      for (int j = 0; j < W; ++j) f[j] = rt_mul(rt_mul(f[j], r), w[j]);
     }
     if (a.c.rotated > 0) place.template turn<false>(f);
-    if (place.in && head < end) {
-      T* to = (head < a.c.heads ? queries : keys) + head * size;
-      RtVec<T, W>::store(to, f);
-      RtVec<T, W>::store(to + apart, f + W / 2);
+    if (head < end) {
+      T* o = key ? out + to_keys : out;
+      Vec::store(o, f);
+      Vec::store(o + apart, f + W / 2);
+    }
+    head += step;
+    out += out_step;
+  }
+  rt_await<0>();
+}
+
+// A warp's way through the shares of rows: all of the queries', then all of the keys', so that it adds up one kind of heads at a time.
+struct RtWay {
+  uint32_t u;
+  int kind, row, first, end;
+  __device__ __forceinline__ void share(const RtArgs& a, int step) {
+    const uint32_t queries = (uint32_t)a.c.rows * (uint32_t)a.parts;
+    kind = u >= queries;
+    const uint32_t v = kind ? u - queries : u;
+    const int have = kind ? a.c.keys : a.c.heads;
+    row = (int)v, first = 0, end = have;
+    if (a.parts > 1) {
+      const int steps = (have + step - 1) / step;
+      row = (int)(v / (uint32_t)a.parts);
+      const int part = (int)(v - (uint32_t)row * (uint32_t)a.parts);
+      first = steps * part / a.parts * step;
+      end = min(steps * (part + 1) / a.parts * step, have);
     }
   }
-}
+  // False behind the last share. (Shares may be empty: fewer keys than queries.)
+  __device__ __forceinline__ bool next(const RtArgs& a, uint32_t shares, uint32_t stride, int step) {
+    do {
+      if (shares - u <= stride) return false;     // (32 bits)
+      u += stride;
+      share(a, step);
+    } while (first >= end);
+    return true;
+  }
+};
 
 template <typename T, int W, bool PAIRS>
 __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_grad_kernel(const __grid_constant__ RtArgs a) {
   psgd_launch_dependents();
+  typedef RtVec<T, W> Vec;
+  constexpr int HALF = RT_THREADS * Vec::BYTES, STAGE = 4 * HALF;     // of the ring
+  extern __shared__ __align__(16) char ring[];
   __shared__ RtShared shared;
   __shared__ __align__(16) float s_sums[2][RT_WARPS][RT_MOST_SIZE];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, size = a.c.size, all = a.c.heads + a.c.keys + a.c.values, step = 32 / a.lanes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, size = a.c.size, all = a.c.heads + a.c.keys + a.c.values;
   RtPlace<W, PAIRS> place(a);
-  const int apart = place.hi - place.lo;
+  const int apart = place.hi - place.lo, step = place.heads;
+  const uint32_t shares = (uint32_t)a.c.rows * (uint32_t)a.parts * (a.c.keys > 0 ? 2u : 1u), stride = gridDim.x * RT_WARPS;
+  RtWay way;
+  way.u = blockIdx.x * RT_WARPS + warp;
+  bool more = way.u < shares;
+  if (more) {
+    way.share(a, step);
+    if (way.first >= way.end) more = way.next(a, shares, stride, step);
+  }
+  // what is fetched goes its way some steps ahead
+  RtWay ahead = way;
+  bool fetches = more, given = false;
+  const T *x = nullptr, *g = nullptr;
+  const long long x_step = step * a.c.x_head;
+  long long g_step = 0;
+  const auto open = [&]() {
+    x = (const T*)a.c.x + (long long)ahead.row * a.c.x_row + (ahead.first + place.slot + (ahead.kind ? a.c.heads : 0)) * a.c.x_head + place.lo;
+    g = (const T*)a.c.grad[ahead.kind];
+    given = g != nullptr;
+    g_step = step * a.c.grad_head[ahead.kind];
+    g = given ? g + (long long)ahead.row * a.c.grad_row[ahead.kind] + (ahead.first + place.slot) * a.c.grad_head[ahead.kind] + place.lo : x;
+  };
+  if (fetches) open();
+  char* const mine = ring + threadIdx.x * Vec::BYTES;
+  int to = 0, from = 0;
+  const auto fetch = [&]() {      // (lanes without a head, or behind the last one, find zeros)
+    if (fetches) {
+      const bool there = place.in && ahead.first + place.slot < ahead.end;
+      rt_fetch<Vec::BYTES>(mine + to, x, there);
+      rt_fetch<Vec::BYTES>(mine + to + HALF, x + apart, there);
+      rt_fetch<Vec::BYTES>(mine + to + 2 * HALF, g, there && given);
+      rt_fetch<Vec::BYTES>(mine + to + 3 * HALF, g + apart, there && given);
+      ahead.first += step;
+      x += x_step;
+      g += g_step;
+      if (ahead.first >= ahead.end) {
+        fetches = ahead.next(a, shares, stride, step);
+        if (fetches) open();
+      }
+    }
+    rt_fetched();
+    to = to == (RT_BACKWARD_STAGES - 1) * STAGE ? 0 : to + STAGE;
+  };
+#pragma unroll 1
+  for (int i = 0; i < RT_BACKWARD_STAGES - 1; ++i) fetch();
   const bool sums = a.c.parts != nullptr;
   shared.fill(a);
   if (sums)
     for (int i = threadIdx.x; i < 2 * RT_WARPS * RT_MOST_SIZE; i += RT_THREADS) ((float*)s_sums)[i] = 0.f;
   __syncthreads();
+  if (a.c.dx != nullptr && a.c.values > 0) {     // values pass by
+    constexpr int N = 16 / (int)sizeof(T);
+    const int vectors = size / N;
+    for (uint32_t row = blockIdx.x * RT_WARPS + warp; row < (uint32_t)a.c.rows; row += stride) {
+      const T* gv = a.c.grad[2] != nullptr ? (const T*)a.c.grad[2] + (long long)row * a.c.grad_row[2] : nullptr;
+      T* o = (T*)a.c.dx + ((long long)row * all + a.c.heads + a.c.keys) * size;
+#pragma unroll 4
+      for (int i = lane; i < a.c.values * vectors; i += 32) {
+        const int h = i / vectors, e = (i - h * vectors) * N;
+        *reinterpret_cast<uint4*>(o + h * size + e) = gv != nullptr ? __ldcs(reinterpret_cast<const uint4*>(gv + h * a.c.grad_head[2] + e)) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  }
   RtPair acc[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) acc[i] = 0;
@@ -425,110 +548,87 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
       acc[i] = 0;
     }
   };
-  // shares of rows: all of the queries', then all of the keys' and the values', so that a warp adds up one kind of heads at a time
-  const uint32_t queries = (uint32_t)a.c.rows * (uint32_t)a.parts, shares = a.c.keys + a.c.values > 0 ? 2 * queries : queries, stride = gridDim.x * RT_WARPS;
   int kind = 0;
-  for (uint32_t u = blockIdx.x * RT_WARPS + warp; u < shares; u += stride) {
-    if (kind == 0 && u >= queries) {
-      if (sums) flush(0);
-      kind = 1;
+  const int out_step = step * size;
+  while (more) {
+    if (way.kind != kind) {
+      if (sums) flush(kind);
+      kind = way.kind;
     }
-    const uint32_t v = kind ? u - queries : u;
-    const int row = a.parts == 1 ? (int)v : (int)(v / (uint32_t)a.parts), part = a.parts == 1 ? 0 : (int)(v - (uint32_t)row * (uint32_t)a.parts);
-    const int have = kind ? a.c.keys : a.c.heads, steps = (have + step - 1) / step;
-    int first = steps * part / a.parts * step;
-    const int end = min(steps * (part + 1) / a.parts * step, have);
-    T* dx_row = a.c.dx != nullptr ? (T*)a.c.dx + (long long)row * all * size : nullptr;
-    T* dx = dx_row + (kind ? a.c.heads * size : 0) + place.lo;
     unsigned long long position;
-    if (!rt_position(a.c, row, lane, position)) {
-      RtPair zeros[W / 2];
+    const bool held = rt_position(a.c, way.row, lane, position);
+    if (a.c.rotated > 0) place.angles(a, position, shared);
+    const float* weight = shared.weight[kind] + place.lo;
+    int head = way.first + place.slot;
+    const int count = (way.end - way.first + step - 1) / step, end = place.in && a.c.dx != nullptr ? way.end : 0;
+    T* dx = (T*)a.c.dx + ((long long)way.row * all + (kind ? a.c.heads : 0) + head) * size + place.lo;
+#pragma unroll 1
+    for (int i = 0; i < count; ++i) {
+      rt_await<RT_BACKWARD_STAGES - 2>();
+      RtPair f[W], d[W];
+      {
+        Vec raw[4];
 #pragma unroll
-      for (int i = 0; i < W / 2; ++i) zeros[i] = 0;
-      for (int head = first + place.slot; dx_row != nullptr && place.in && head < end; head += step) {
-        RtVec<T, W>::store(dx + head * size, zeros);
-        RtVec<T, W>::store(dx + head * size + apart, zeros);
-      }
-      first = end;
-    }
-    if (first < end) {
-      const T* x = (const T*)a.c.x + (long long)row * a.c.x_row + (kind ? a.c.heads * a.c.x_head : 0) + place.lo;
-      const bool given = a.c.grad[kind] != nullptr;
-      const T* g = (const T*)a.c.grad[kind] + (long long)row * a.c.grad_row[kind] + place.lo;
-      RtVec<T, W> raw[2], rawg[2];
-      const auto load = [&](int head) {    // (lanes that have no head any more read another one, with a gradient of zeros)
-        const T* p = x + min(head, end - 1) * a.c.x_head;
-        raw[0].load(p), raw[1].load(p + apart);
-        rawg[0].clear(), rawg[1].clear();
-        if (given && place.in && head < end) {
-          const T* q = g + head * a.c.grad_head[kind];
-          rawg[0].load(q), rawg[1].load(q + apart);
-        }
-      };
-      load(first + place.slot);
-      if (a.c.rotated > 0) place.angles(a, position, shared);
-      const float* weight = shared.weight[kind] + place.lo;
-      for (; first < end; first += step) {
-        RtPair f[W], d[W];
+        for (int j = 0; j < 4; ++j) raw[j].get(mine + from + j * HALF);
         raw[0].unpack(f), raw[1].unpack(f + W / 2);
-        rawg[0].unpack(d), rawg[1].unpack(d + W / 2);
-        const int head = first + place.slot;
-        if (first + step < end) load(head + step);
+        raw[2].unpack(d), raw[3].unpack(d + W / 2);
+      }
+      from = from == (RT_BACKWARD_STAGES - 1) * STAGE ? 0 : from + STAGE;
+      fetch();     // to where the step before this one was read
+      if (held) {
         if (a.c.rotated > 0) place.template turn<true>(d);
         if (a.c.norm) {
+          RtPair w[W];
+          rt_get<W>(weight, w);
+          rt_get<W>(weight + apart, w + W / 2);
           const auto dots = [&](float& s, float& t) {
-            RtPair w[W], squares = rt_dot<W>(f, f);
-            rt_get<W>(weight, w);
-            rt_get<W>(weight + apart, w + W / 2);
             RtPair along = rt_mul(rt_mul(d[0], w[0]), f[0]);
 #pragma unroll
-            for (int i = 1; i < W; ++i) along = rt_fma(rt_mul(d[i], w[i]), f[i], along);
-            s = rt_sum(place.in ? squares : 0, a.lanes);
-            t = rt_sum(along, a.lanes);
+            for (int j = 1; j < W; ++j) along = rt_fma(rt_mul(d[j], w[j]), f[j], along);
+            const float2 s2 = rt_floats(rt_dot<W>(f, f)), t2 = rt_floats(along);
+            s = s2.x + s2.y, t = t2.x + t2.y;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+              if (o >= a.lanes) break;
+              s += __shfl_xor_sync(0xffffffffu, s, o);
+              t += __shfl_xor_sync(0xffffffffu, t, o);
+            }
           };
           float s, t, eps = a.c.eps, down = 1.f;
           dots(s, t);
-          if (sizeof(T) == 4 || std::is_same<T, __nv_bfloat16>::value) {
+          if (RT_RANGE<T>) {
             const bool large = !(s < 0x1p126f);
             if (__any_sync(0xffffffffu, large)) {
               const RtPair less = rt_both(large ? RT_DOWN : 1.f);
 #pragma unroll
-              for (int i = 0; i < W; ++i) f[i] = rt_mul(f[i], less);
+              for (int j = 0; j < W; ++j) f[j] = rt_mul(f[j], less);
               dots(s, t);
               if (large) eps *= RT_DOWN * RT_DOWN, down = RT_DOWN;
             }
           }
           const float r = rsqrtf(fmaf(s, a.share, eps));
-          const RtPair r2 = rt_both(r), rd = rt_both(r * down), along = rt_both(-t * a.share * r * r * r * down);
-          RtPair w[W];
-          rt_get<W>(weight, w);
-          rt_get<W>(weight + apart, w + W / 2);
-          // dw += dy x r;  dx = dy w r - x r^3 mean(dy w x)
+          const RtPair r2 = rt_both(r), rd = rt_both(r * down), along = rt_both(-t * r * a.share);     // - mean(dn n)
 #pragma unroll
-          for (int i = 0; i < W; ++i) {
-            if (sums) acc[i] = rt_fma(rt_mul(d[i], r2), f[i], acc[i]);
-            d[i] = rt_fma(f[i], along, rt_mul(rt_mul(d[i], w[i]), rd));
+          for (int j = 0; j < W; ++j) {
+            const RtPair n = rt_mul(f[j], r2);
+            if (sums) acc[j] = rt_fma(d[j], n, acc[j]);
+            d[j] = rt_mul(rt_fma(n, along, rt_mul(d[j], w[j])), rd);
           }
         }
-        if (place.in && head < end && dx_row != nullptr) {
-          RtVec<T, W>::store(dx + head * size, d);
-          RtVec<T, W>::store(dx + head * size + apart, d + W / 2);
-        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < W; ++j) d[j] = 0;
       }
-    }
-    if (kind && dx_row != nullptr && a.c.values > 0) {     // values pass by
-      constexpr int N = 16 / (int)sizeof(T);
-      const int vectors = size / N;
-      const T* gv = a.c.grad[2] != nullptr ? (const T*)a.c.grad[2] + (long long)row * a.c.grad_row[2] : nullptr;
-      T* to = dx_row + (long long)(a.c.heads + a.c.keys) * size;
-#pragma unroll 4
-      for (int i = part * 32 + lane; i < a.c.values * vectors; i += 32 * a.parts) {
-        const int h = i / vectors, e = (i - h * vectors) * N;
-        *reinterpret_cast<uint4*>(to + (long long)h * size + e) = gv != nullptr ? __ldcs(reinterpret_cast<const uint4*>(gv + h * a.c.grad_head[2] + e)) : make_uint4(0, 0, 0, 0);
+      if (head < end) {
+        Vec::store(dx, d);
+        Vec::store(dx + apart, d + W / 2);
       }
+      head += step;
+      dx += out_step;
     }
-    if (shares - u <= stride) break;   // (32 bits)
+    more = way.next(a, shares, stride, step);
   }
+  rt_await<0>();
   if (!sums) return;
   flush(kind);
   __syncthreads();
@@ -589,9 +689,12 @@ int rt_forward(RtArgs& a, cudaStream_t stream) {
 template <typename T, int W, bool PAIRS>
 int rt_backward(RtArgs& a, cudaStream_t stream) {
   rt_plan<W>(a, RT_PART_BLOCKS * RT_WARPS, a.c.heads > a.c.keys ? a.c.heads : a.c.keys);
-  const long long blocks = ((long long)a.c.rows * a.parts * (a.c.keys + a.c.values > 0 ? 2 : 1) + RT_WARPS - 1) / RT_WARPS;
-  const int grid = (int)(blocks < RT_PART_BLOCKS || a.c.parts == nullptr ? blocks : RT_PART_BLOCKS);
-  if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS>, grid, RT_THREADS, 0, stream, 0, a)) return code;
+  const long long blocks = ((long long)a.c.rows * a.parts * (a.c.keys > 0 ? 2 : 1) + RT_WARPS - 1) / RT_WARPS;
+  const int grid = (int)(blocks < RT_PART_BLOCKS ? blocks : RT_PART_BLOCKS);
+  constexpr size_t ring = (size_t)RT_BACKWARD_STAGES * 4 * RT_THREADS * RtVec<T, W>::BYTES;
+  static unsigned long long devices = 0;
+  if (const int code = psgd_allow_shared((const void*)psgd_rotate_grad_kernel<T, W, PAIRS>, ring, devices)) return code;
+  if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS>, grid, RT_THREADS, ring, stream, 0, a)) return code;
   if (a.c.parts == nullptr) return 0;
   return psgd_launch(psgd_rotate_weights_kernel, (2 * a.c.size + 31) / 32, 32 * RT_SLICES, 0, stream, 1, (const float*)a.c.parts, grid, a.c.size, a.c.weight_type, a.c.dweight[0],
                      a.c.dweight[1]);

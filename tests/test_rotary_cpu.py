@@ -336,3 +336,24 @@ def test_gpt2_positions_matter_only_by_their_distance():
     a = model(tokens, torch.tensor([0, 12, 30], dtype=torch.int32))[12:]
     b = model(tokens[12:], torch.tensor([0, 18], dtype=torch.int32))
     torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-5)
+
+
+def check_small(device):
+    """Heads of zeros and of very small numbers under a small eps: r^3 would leave the range of float32."""
+    x = torch.zeros(3, 1, 16, device=device)
+    x[1, 0, 3], x[2] = 2.0**-60, 2.0**-50
+    w = torch.linspace(0.5, 2, 16, device=device).requires_grad_()
+    x.requires_grad_()
+    grad = torch.ones(3, 1, 16, device=device)
+    out = rotate_heads(x, positions=torch.zeros(3, dtype=torch.int32, device=device), weight=w, eps=2.0**-100)
+    dx, dw = torch.autograd.grad(out, (x, w), grad)
+    wide, ww = x.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    want = wide / (wide.square().mean(-1, keepdim=True) + 2.0**-100).sqrt() * ww
+    wants = torch.autograd.grad(want, (wide, ww), grad.double())
+    torch.testing.assert_close(out.double(), want, rtol=1e-5, atol=0)
+    torch.testing.assert_close(dw.double(), wants[1], rtol=1e-5, atol=0)
+    torch.testing.assert_close(dx.double(), wants[0], rtol=1e-4, atol=1e-5 * 2.0**50)    # differences of terms as large as w r, r up to 2^50
+
+
+def test_small():
+    check_small("cpu")

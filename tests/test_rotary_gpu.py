@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 from test_packed_training_cpu import _by_document, _documents
-from test_rotary_cpu import check, check_offsets, check_sizes_at_the_border, check_some_gradients, exact, places, refused, tangents, values
+from test_rotary_cpu import check, check_offsets, check_sizes_at_the_border, check_small, check_some_gradients, exact, places, refused, tangents, values
 
 from powersgd_b200 import AdamW, Config, PowerSGD, clip_grad_norm, optimizer_step
 from powersgd_b200.models import GPT2, GPT2Config
@@ -77,6 +77,10 @@ def test_offsets(form, dtype):
 
 def test_sizes_at_the_border(form):
     check_sizes_at_the_border("cuda")
+
+
+def test_small(form):
+    check_small("cuda")
 
 
 @pytest.mark.parametrize("dtype", TYPES)
