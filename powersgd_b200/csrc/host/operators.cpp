@@ -531,7 +531,7 @@ PyObject* rotate(PyObject*, PyObject* args) {
     const auto type = x.scalar_type();
     if (!x.is_cuda() || type_code(type) < 0 || x.dim() != 3 || heads < 1 || keys < 0 || x.size(1) < heads + keys || (keys == 0 && x.size(1) != heads) || x.size(2) < 8 ||
         x.size(2) > 256 || x.size(2) % 8 != 0 || rotated < 0 || rotated > x.size(2) || rotated % 8 != 0 || bytes != rotated / 2 * 8 || x.size(0) >= (1ll << 31) - (1 << 16) ||
-        x.size(1) > 1 << 16 || has_tangent(x) || torch::jit::tracer::isTracing())
+        x.size(1) > 4096 || has_tangent(x) || torch::jit::tracer::isTracing())
       Py_RETURN_NONE;
     Tensor t[4];
     for (int i = 0; i < 4; ++i) {

@@ -46,27 +46,27 @@ namespace {
 
 constexpr int RT_THREADS = 256, RT_WARPS = RT_THREADS / 32;
 constexpr int RT_MOST_SIZE = 256, RT_MOST_ANGLES = RT_MOST_SIZE / 2;
+constexpr int RT_MOST_HEADS = 4096;      // (so that no row is shared by more warps than RT_PART_BLOCKS have)
 constexpr int RT_SMS = 148;
 #ifndef FB
 #define FB 4
 #define BB 2
-#define WF 1
-#define WB 1
+#define RS 2
 #define FS 3
-#define BS 3
 #endif
-constexpr int RT_FORWARD_STAGES = FS, RT_BACKWARD_STAGES = BS;   // steps of a warp whose inputs are on their way, and one more
+constexpr int RT_FORWARD_BLOCKS = FB, RT_BACKWARD_BLOCKS = BB;   // of an SM at a time
+constexpr int RT_STEPS = RS;             // of a warp, gradients
+constexpr int RT_FORWARD_STAGES = FS;    // steps whose inputs are on their way or read
 // Do the squares of a type leave the range of float32?
 template <typename T>
 constexpr bool RT_RANGE = !std::is_same<T, __half>::value;
-constexpr int RT_FORWARD_BLOCKS = FB, RT_BACKWARD_BLOCKS = BB;   // of an SM at a time
 constexpr int RT_PART_BLOCKS = RT_SMS * RT_BACKWARD_BLOCKS;    // that add up gradients of weights
 constexpr float RT_DOWN = 0x1p-70f;                            // for heads whose squares leave the range
 
 struct RtArgs {
   PsgdRotate c;
   int lanes;                       // of a head: a power of two
-  int parts;                       // warps that share a row
+  int parts[2];                    // warps that share a row's queries, and its keys (a gradient); its queries and keys (forward)
   float share;                     // 1 / size
   unsigned long long frequency[RT_MOST_ANGLES];
 };
@@ -233,13 +233,17 @@ struct __align__(16) RtShared {
   float cosine[RT_WARPS][RT_MOST_ANGLES], sine[RT_WARPS][RT_MOST_ANGLES];   // of the row that a warp has
   float weight[2][RT_MOST_SIZE];
   unsigned long long frequency[RT_MOST_ANGLES];
-  __device__ __forceinline__ void fill(const RtArgs& a) {
-    for (int i = threadIdx.x; i < a.c.rotated / 2; i += RT_THREADS) frequency[i] = a.frequency[i];
+  __device__ __forceinline__ void fill(const RtArgs& a) {     // (a thread for each element)
+    const int i = threadIdx.x;
+    if (i < a.c.rotated / 2) frequency[i] = a.frequency[i];
+    if (i < a.c.size) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-      for (int i = threadIdx.x; i < a.c.size; i += RT_THREADS) weight[k][i] = a.c.weight[k] != nullptr ? rt_weight(a.c.weight[k], a.c.weight_type, i) : 1.f;
+      for (int k = 0; k < 2; ++k) weight[k][i] = a.c.weight[k] != nullptr ? rt_weight(a.c.weight[k], a.c.weight_type, i) : 1.f;
+    }
   }
 };
+static_assert(RT_MOST_HEADS / RT_STEPS + 2 <= RT_PART_BLOCKS * RT_WARPS, "a warp for each share of a row");
+static_assert(RT_THREADS >= RT_MOST_SIZE, "a thread for each element of a head");
 
 // Eight (or four) floats on a 16-byte boundary of shared memory.
 template <int W>
@@ -251,17 +255,18 @@ __device__ __forceinline__ void rt_get(const float* p, RtPair* f) {
   }
 }
 
-// A thread's place in a head: W elements from `lo` on and W from `hi` on, which hold W pairs.
-template <int W, bool PAIRS>
+// A thread's place in a head: W elements from `lo` on and W from `hi` on, which hold W pairs. LANES: of a head, 0: as the call says.
+template <int W, bool PAIRS, int LANES>
 struct RtPlace {
   int slot, heads;           // which of the heads that a warp takes at a time
   int lo, hi, pair;          // and the first of its angles
   bool in, turned;
   RtPair cosine[W / 2], sine[W / 2];
+  static __device__ __forceinline__ int lanes(const RtArgs& a) { return LANES ? LANES : a.lanes; }
   __device__ __forceinline__ RtPlace(const RtArgs& a) {
-    const int lane = threadIdx.x & 31, member = lane & (a.lanes - 1), half = a.c.rotated / 2;
-    slot = lane / a.lanes;
-    heads = 32 / a.lanes;
+    const int lane = threadIdx.x & 31, member = lane & (lanes(a) - 1), half = a.c.rotated / 2;
+    slot = lane / lanes(a);
+    heads = 32 / lanes(a);
     pair = member * W;
     in = 2 * pair < a.c.size;
     if (PAIRS) {
@@ -313,14 +318,18 @@ struct RtPlace {
   }
 };
 
-// Of the lanes of a head.
-__device__ __forceinline__ float rt_sum(RtPair v2, int lanes) {
-  const float2 two = rt_floats(v2);
-  float v = two.x + two.y;
+// Sums over the lanes of a head.
+template <int LANES>
+__device__ __forceinline__ void rt_sum(float& s, int lanes) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1)
-    if (o < lanes) v += __shfl_xor_sync(0xffffffffu, v, o);
-  return v;
+  for (int o = 1; o < (LANES ? LANES : 32); o <<= 1) {
+    if (!LANES && o >= lanes) break;
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+  }
+}
+__device__ __forceinline__ float rt_two(RtPair p) {
+  const float2 f = rt_floats(p);
+  return f.x + f.y;
 }
 template <int W>
 __device__ __forceinline__ RtPair rt_dot(const RtPair* a, const RtPair* b) {
@@ -330,23 +339,24 @@ __device__ __forceinline__ RtPair rt_dot(const RtPair* a, const RtPair* b) {
   return s;
 }
 
-template <typename T, int W, bool PAIRS>
+// A warp takes one row, or a share of it, its steps' inputs some steps ahead.
+template <typename T, int W, bool PAIRS, int LANES>
 __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_kernel(const __grid_constant__ RtArgs a) {
   typedef RtVec<T, W> Vec;
   constexpr int HALF = RT_THREADS * Vec::BYTES, STAGE = 2 * HALF;     // of the ring
   __shared__ RtShared shared;
   __shared__ __align__(16) char ring[RT_FORWARD_STAGES * STAGE];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  RtPlace<W, PAIRS> place(a);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = LANES ? LANES : a.lanes, parts = a.parts[0];
+  RtPlace<W, PAIRS, LANES> place(a);
   const int size = a.c.size, all = a.c.heads + a.c.keys, step = place.heads;
   const uint32_t u = blockIdx.x * RT_WARPS + warp;
   int row = (int)u, head = place.slot, end = all;
-  if (a.parts > 1) {
+  if (parts > 1) {
     const int steps = (all + step - 1) / step;
-    row = (int)(u / (uint32_t)a.parts);
-    const int part = (int)(u - (uint32_t)row * (uint32_t)a.parts);
-    head += steps * part / a.parts * step;
-    end = min(steps * (part + 1) / a.parts * step, all);
+    row = (int)(u / (uint32_t)parts);
+    const int part = (int)(u - (uint32_t)row * (uint32_t)parts);
+    head += steps * part / parts * step;
+    end = min(steps * (part + 1) / parts * step, all);
   }
   const bool live = row < a.c.rows;
   const int count = live ? (end - head + place.slot + step - 1) / step : 0, apart = place.hi - place.lo;
@@ -399,14 +409,16 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
     fetch();     // to where the step before this one was read
     const bool key = head >= a.c.heads;
     if (a.c.norm) {
-      float s = rt_sum(rt_dot<W>(f, f), a.lanes), eps = a.c.eps;
+      float s = rt_two(rt_dot<W>(f, f)), eps = a.c.eps;
+      rt_sum<LANES>(s, lanes);
       if (RT_RANGE<T>) {
         const bool large = !(s < 0x1p126f);
         if (__any_sync(0xffffffffu, large)) {
           const RtPair down = rt_both(large ? RT_DOWN : 1.f);
 #pragma unroll
           for (int j = 0; j < W; ++j) f[j] = rt_mul(f[j], down);
-          const float t = rt_sum(rt_dot<W>(f, f), a.lanes);
+          float t = rt_two(rt_dot<W>(f, f));
+          rt_sum<LANES>(t, lanes);
           if (large) s = t, eps *= RT_DOWN * RT_DOWN;
         }
       }
@@ -430,213 +442,152 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
   rt_await<0>();
 }
 
-// A warp's way through the shares of rows: all of the queries', then all of the keys', so that it adds up one kind of heads at a time.
-struct RtWay {
-  uint32_t u;
-  int kind, row, first, end;
-  __device__ __forceinline__ void share(const RtArgs& a, int step) {
-    const uint32_t queries = (uint32_t)a.c.rows * (uint32_t)a.parts;
-    kind = u >= queries;
-    const uint32_t v = kind ? u - queries : u;
-    const int have = kind ? a.c.keys : a.c.heads;
-    row = (int)v, first = 0, end = have;
-    if (a.parts > 1) {
-      const int steps = (have + step - 1) / step;
-      row = (int)(v / (uint32_t)a.parts);
-      const int part = (int)(v - (uint32_t)row * (uint32_t)a.parts);
-      first = steps * part / a.parts * step;
-      end = min(steps * (part + 1) / a.parts * step, have);
-    }
-  }
-  // False behind the last share. (Shares may be empty: fewer keys than queries.)
-  __device__ __forceinline__ bool next(const RtArgs& a, uint32_t shares, uint32_t stride, int step) {
-    do {
-      if (shares - u <= stride) return false;     // (32 bits)
-      u += stride;
-      share(a, step);
-    } while (first >= end);
-    return true;
-  }
-};
-
-template <typename T, int W, bool PAIRS>
+// Gradients: a warp has the same heads of every row that it comes to, RT_STEPS times what its lanes take at once, queries or keys, so that it adds up one weight's
+// gradient, and a share of the rows' values, which pass by. Each step has its place in shared memory, which, once read, is filled with the same
+// step of the warp's next row.
+template <typename T, int W, bool PAIRS, int LANES>
 __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_grad_kernel(const __grid_constant__ RtArgs a) {
   psgd_launch_dependents();
   typedef RtVec<T, W> Vec;
-  constexpr int HALF = RT_THREADS * Vec::BYTES, STAGE = 4 * HALF;     // of the ring
+  constexpr int HALF = RT_THREADS * Vec::BYTES, STEP = 4 * HALF, N = 16 / (int)sizeof(T);
   extern __shared__ __align__(16) char ring[];
   __shared__ RtShared shared;
-  __shared__ __align__(16) float s_sums[2][RT_WARPS][RT_MOST_SIZE];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, size = a.c.size, all = a.c.heads + a.c.keys + a.c.values;
-  RtPlace<W, PAIRS> place(a);
-  const int apart = place.hi - place.lo, step = place.heads;
-  const uint32_t shares = (uint32_t)a.c.rows * (uint32_t)a.parts * (a.c.keys > 0 ? 2u : 1u), stride = gridDim.x * RT_WARPS;
-  RtWay way;
-  way.u = blockIdx.x * RT_WARPS + warp;
-  bool more = way.u < shares;
-  if (more) {
-    way.share(a, step);
-    if (way.first >= way.end) more = way.next(a, shares, stride, step);
-  }
-  // what is fetched goes its way some steps ahead
-  RtWay ahead = way;
-  bool fetches = more, given = false;
-  const T *x = nullptr, *g = nullptr;
-  const long long x_step = step * a.c.x_head;
-  long long g_step = 0;
-  const auto open = [&]() {
-    x = (const T*)a.c.x + (long long)ahead.row * a.c.x_row + (ahead.first + place.slot + (ahead.kind ? a.c.heads : 0)) * a.c.x_head + place.lo;
-    g = (const T*)a.c.grad[ahead.kind];
-    given = g != nullptr;
-    g_step = step * a.c.grad_head[ahead.kind];
-    g = given ? g + (long long)ahead.row * a.c.grad_row[ahead.kind] + (ahead.first + place.slot) * a.c.grad_head[ahead.kind] + place.lo : x;
-  };
-  if (fetches) open();
+  __shared__ __align__(16) float s_sums[RT_WARPS][RT_MOST_SIZE];
+  __shared__ int s_kind[RT_WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, size = a.c.size, lanes = LANES ? LANES : a.lanes;
+  RtPlace<W, PAIRS, LANES> place(a);
+  const int apart = place.hi - place.lo, step = place.heads, parts = a.parts[0] + a.parts[1];
+  const int u = blockIdx.x * RT_WARPS + warp, stride = gridDim.x * RT_WARPS / parts, part = u % parts;
+  const int kind = part >= a.parts[0], own = kind ? part - a.parts[0] : part, have = kind ? a.c.keys : a.c.heads, steps = (have + step - 1) / step;
+  const int begin = steps * own / a.parts[kind], count = steps * (own + 1) / a.parts[kind] - begin, head = begin * step + place.slot;
+  int row = u / parts, ahead = row;
+  if (row >= stride) row = ahead = a.c.rows;       // (where the warps are no multiple of the parts)
+  const long long x_step = step * a.c.x_head, x_stride = stride * a.c.x_row, g_step = step * a.c.grad_head[kind], g_stride = stride * a.c.grad_row[kind];
+  const T* x = (const T*)a.c.x + (long long)row * a.c.x_row + (head + (kind ? a.c.heads : 0)) * a.c.x_head + place.lo;
+  const bool given = a.c.grad[kind] != nullptr;
+  const T* g = given ? (const T*)a.c.grad[kind] + (long long)row * a.c.grad_row[kind] + head * a.c.grad_head[kind] + place.lo : x;
   char* const mine = ring + threadIdx.x * Vec::BYTES;
-  int to = 0, from = 0;
-  const auto fetch = [&]() {      // (lanes without a head, or behind the last one, find zeros)
-    if (fetches) {
-      const bool there = place.in && ahead.first + place.slot < ahead.end;
-      rt_fetch<Vec::BYTES>(mine + to, x, there);
-      rt_fetch<Vec::BYTES>(mine + to + HALF, x + apart, there);
-      rt_fetch<Vec::BYTES>(mine + to + 2 * HALF, g, there && given);
-      rt_fetch<Vec::BYTES>(mine + to + 3 * HALF, g + apart, there && given);
-      ahead.first += step;
-      x += x_step;
-      g += g_step;
-      if (ahead.first >= ahead.end) {
-        fetches = ahead.next(a, shares, stride, step);
-        if (fetches) open();
-      }
+  const auto fetch = [&](int i) {      // (lanes without a head find zeros)
+    if (i < count && ahead < a.c.rows) {
+      const bool there = place.in && head + i * step < have;
+      rt_fetch<Vec::BYTES>(mine + i * STEP, x + i * x_step, there);
+      rt_fetch<Vec::BYTES>(mine + i * STEP + HALF, x + i * x_step + apart, there);
+      rt_fetch<Vec::BYTES>(mine + i * STEP + 2 * HALF, g + i * g_step, there && given);
+      rt_fetch<Vec::BYTES>(mine + i * STEP + 3 * HALF, g + i * g_step + apart, there && given);
     }
     rt_fetched();
-    to = to == (RT_BACKWARD_STAGES - 1) * STAGE ? 0 : to + STAGE;
   };
-#pragma unroll 1
-  for (int i = 0; i < RT_BACKWARD_STAGES - 1; ++i) fetch();
+#pragma unroll
+  for (int i = 0; i < RT_STEPS; ++i) fetch(i);
   const bool sums = a.c.parts != nullptr;
   shared.fill(a);
-  if (sums)
-    for (int i = threadIdx.x; i < 2 * RT_WARPS * RT_MOST_SIZE; i += RT_THREADS) ((float*)s_sums)[i] = 0.f;
   __syncthreads();
-  if (a.c.dx != nullptr && a.c.values > 0) {     // values pass by
-    constexpr int N = 16 / (int)sizeof(T);
-    const int vectors = size / N;
-    for (uint32_t row = blockIdx.x * RT_WARPS + warp; row < (uint32_t)a.c.rows; row += stride) {
-      const T* gv = a.c.grad[2] != nullptr ? (const T*)a.c.grad[2] + (long long)row * a.c.grad_row[2] : nullptr;
-      T* o = (T*)a.c.dx + ((long long)row * all + a.c.heads + a.c.keys) * size;
-#pragma unroll 4
-      for (int i = lane; i < a.c.values * vectors; i += 32) {
-        const int h = i / vectors, e = (i - h * vectors) * N;
-        *reinterpret_cast<uint4*>(o + h * size + e) = gv != nullptr ? __ldcs(reinterpret_cast<const uint4*>(gv + h * a.c.grad_head[2] + e)) : make_uint4(0, 0, 0, 0);
-      }
-    }
-  }
+  const int all = a.c.heads + a.c.keys + a.c.values, vectors = size / N, passing = a.c.dx != nullptr ? a.c.values * vectors : 0;
+  T* dx = (T*)a.c.dx + ((long long)row * all + (kind ? a.c.heads : 0) + head) * size + place.lo;
+  const long long dx_stride = (long long)stride * all * size;
+  const float* weight = shared.weight[kind] + place.lo;
   RtPair acc[W];
 #pragma unroll
   for (int i = 0; i < W; ++i) acc[i] = 0;
-  // what the warp's threads have added up for one kind of heads
-  const auto flush = [&](int kind) {
-#pragma unroll
-    for (int i = 0; i < W; ++i) {
-      float2 v = rt_floats(acc[i]);
-      for (int o = a.lanes; o < 32; o <<= 1) {
-        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+#pragma unroll 1
+  for (; row < a.c.rows; row = ahead) {
+    ahead = stride < a.c.rows - row ? row + stride : a.c.rows;
+    x += x_stride;
+    g += g_stride;
+    if (passing > 0) {
+      const T* gv = (const T*)a.c.grad[2];
+      T* o = (T*)a.c.dx + ((long long)row * all + a.c.heads + a.c.keys) * size;
+      if (gv != nullptr) gv += (long long)row * a.c.grad_row[2];
+#pragma unroll 2
+      for (int i = part * 32 + lane; i < passing; i += 32 * parts) {
+        const int h = i / vectors, e = (i - h * vectors) * N;
+        *reinterpret_cast<uint4*>(o + i * N) = gv != nullptr ? __ldcs(reinterpret_cast<const uint4*>(gv + h * a.c.grad_head[2] + e)) : make_uint4(0, 0, 0, 0);
       }
-      if (place.slot == 0 && place.in) *reinterpret_cast<float2*>(&s_sums[kind][warp][(i < W / 2 ? place.lo : place.hi - W) + 2 * i]) = v;
-      acc[i] = 0;
-    }
-  };
-  int kind = 0;
-  const int out_step = step * size;
-  while (more) {
-    if (way.kind != kind) {
-      if (sums) flush(kind);
-      kind = way.kind;
     }
     unsigned long long position;
-    const bool held = rt_position(a.c, way.row, lane, position);
+    const bool held = rt_position(a.c, row, lane, position);
     if (a.c.rotated > 0) place.angles(a, position, shared);
-    const float* weight = shared.weight[kind] + place.lo;
-    int head = way.first + place.slot;
-    const int count = (way.end - way.first + step - 1) / step, end = place.in && a.c.dx != nullptr ? way.end : 0;
-    T* dx = (T*)a.c.dx + ((long long)way.row * all + (kind ? a.c.heads : 0) + head) * size + place.lo;
-#pragma unroll 1
-    for (int i = 0; i < count; ++i) {
-      rt_await<RT_BACKWARD_STAGES - 2>();
-      RtPair f[W], d[W];
-      {
-        Vec raw[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) raw[j].get(mine + from + j * HALF);
-        raw[0].unpack(f), raw[1].unpack(f + W / 2);
-        raw[2].unpack(d), raw[3].unpack(d + W / 2);
-      }
-      from = from == (RT_BACKWARD_STAGES - 1) * STAGE ? 0 : from + STAGE;
-      fetch();     // to where the step before this one was read
-      if (held) {
-        if (a.c.rotated > 0) place.template turn<true>(d);
-        if (a.c.norm) {
-          RtPair w[W];
-          rt_get<W>(weight, w);
-          rt_get<W>(weight + apart, w + W / 2);
-          const auto dots = [&](float& s, float& t) {
-            RtPair along = rt_mul(rt_mul(d[0], w[0]), f[0]);
+    for (int i = 0; i < RT_STEPS; ++i) {
+      rt_await<RT_STEPS - 1>();
+      if (i < count) {
+        RtPair f[W], d[W];
+        {
+          Vec raw[4];
 #pragma unroll
-            for (int j = 1; j < W; ++j) along = rt_fma(rt_mul(d[j], w[j]), f[j], along);
-            const float2 s2 = rt_floats(rt_dot<W>(f, f)), t2 = rt_floats(along);
-            s = s2.x + s2.y, t = t2.x + t2.y;
+          for (int j = 0; j < 4; ++j) raw[j].get(mine + i * STEP + j * HALF);
+          raw[0].unpack(f), raw[1].unpack(f + W / 2);
+          raw[2].unpack(d), raw[3].unpack(d + W / 2);
+        }
+        fetch(i);
+        if (held) {
+          if (a.c.rotated > 0) place.template turn<true>(d);
+          if (a.c.norm) {
+            RtPair w[W];
+            rt_get<W>(weight, w);
+            rt_get<W>(weight + apart, w + W / 2);
+            const auto dots = [&](float& s, float& t) {
+              RtPair along = rt_mul(rt_mul(d[0], w[0]), f[0]);
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-              if (o >= a.lanes) break;
-              s += __shfl_xor_sync(0xffffffffu, s, o);
-              t += __shfl_xor_sync(0xffffffffu, t, o);
+              for (int j = 1; j < W; ++j) along = rt_fma(rt_mul(d[j], w[j]), f[j], along);
+              s = rt_two(rt_dot<W>(f, f)), t = rt_two(along);
+              rt_sum<LANES>(s, lanes);
+              rt_sum<LANES>(t, lanes);
+            };
+            float s, t, eps = a.c.eps, down = 1.f;
+            dots(s, t);
+            if (RT_RANGE<T>) {
+              const bool large = !(s < 0x1p126f);
+              if (__any_sync(0xffffffffu, large)) {
+                const RtPair less = rt_both(large ? RT_DOWN : 1.f);
+#pragma unroll
+                for (int j = 0; j < W; ++j) f[j] = rt_mul(f[j], less);
+                dots(s, t);
+                if (large) eps *= RT_DOWN * RT_DOWN, down = RT_DOWN;
+              }
             }
-          };
-          float s, t, eps = a.c.eps, down = 1.f;
-          dots(s, t);
-          if (RT_RANGE<T>) {
-            const bool large = !(s < 0x1p126f);
-            if (__any_sync(0xffffffffu, large)) {
-              const RtPair less = rt_both(large ? RT_DOWN : 1.f);
+            const float r = rsqrtf(fmaf(s, a.share, eps));
+            const RtPair r2 = rt_both(r), rd = rt_both(r * down), along = rt_both(-t * r * a.share);     // - mean(dn n)
 #pragma unroll
-              for (int j = 0; j < W; ++j) f[j] = rt_mul(f[j], less);
-              dots(s, t);
-              if (large) eps *= RT_DOWN * RT_DOWN, down = RT_DOWN;
+            for (int j = 0; j < W; ++j) {
+              const RtPair n = rt_mul(f[j], r2);
+              acc[j] = rt_fma(d[j], n, acc[j]);
+              d[j] = rt_mul(rt_fma(n, along, rt_mul(d[j], w[j])), rd);
             }
           }
-          const float r = rsqrtf(fmaf(s, a.share, eps));
-          const RtPair r2 = rt_both(r), rd = rt_both(r * down), along = rt_both(-t * r * a.share);     // - mean(dn n)
+        } else {
 #pragma unroll
-          for (int j = 0; j < W; ++j) {
-            const RtPair n = rt_mul(f[j], r2);
-            if (sums) acc[j] = rt_fma(d[j], n, acc[j]);
-            d[j] = rt_mul(rt_fma(n, along, rt_mul(d[j], w[j])), rd);
-          }
+          for (int j = 0; j < W; ++j) d[j] = 0;
+        }
+        if (place.in && a.c.dx != nullptr && head + i * step < have) {
+          T* o = dx + i * step * size;
+          Vec::store(o, d);
+          Vec::store(o + apart, d + W / 2);
         }
       } else {
-#pragma unroll
-        for (int j = 0; j < W; ++j) d[j] = 0;
+        rt_fetched();
       }
-      if (head < end) {
-        Vec::store(dx, d);
-        Vec::store(dx + apart, d + W / 2);
-      }
-      head += step;
-      dx += out_step;
     }
-    more = way.next(a, shares, stride, step);
+    dx += dx_stride;
   }
   rt_await<0>();
   if (!sums) return;
-  flush(kind);
+#pragma unroll
+  for (int i = 0; i < W; ++i) {
+    float2 v = rt_floats(acc[i]);
+    for (int o = lanes; o < 32; o <<= 1) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    }
+    if (place.slot == 0 && place.in) *reinterpret_cast<float2*>(&s_sums[warp][(i < W / 2 ? place.lo : place.hi - W) + 2 * i]) = v;
+  }
+  if (lane == 0) s_kind[warp] = kind;
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * size; i += RT_THREADS) {
     const int k = i >= size, e = k ? i - size : i;
     float v = 0.f;
 #pragma unroll
-    for (int j = 0; j < RT_WARPS; ++j) v += s_sums[k][j][e];
+    for (int j = 0; j < RT_WARPS; ++j) v += s_kind[j] == k ? s_sums[j][e] : 0.f;
     a.c.parts[(long long)blockIdx.x * 2 * size + i] = v;
   }
 }
@@ -668,53 +619,61 @@ __global__ void __launch_bounds__(32 * RT_SLICES) psgd_rotate_weights_kernel(con
   else ((__half*)out)[e] = __float2half_rn(v);
 }
 
-// Where there are few rows, several warps share one, as long as each has heads (`heads` of a kind, `at_once` of which a warp takes in a step).
-template <int W>
-void rt_plan(RtArgs& a, int warps, int heads) {
-  int lanes = 1;
-  while (lanes * 2 * W < a.c.size) lanes *= 2;
-  a.lanes = lanes;
-  a.share = 1.f / (float)a.c.size;
-  const int step = 32 / lanes, steps = (heads + step - 1) / step;
-  a.parts = 1;
-  while (a.parts < steps && (long long)a.c.rows * (a.parts + 1) <= warps) ++a.parts;
+// How many warps share `heads` of a row: as few as `most` steps to a warp allow, and more where there are few rows.
+inline int rt_parts(const RtArgs& a, int heads, int most, int warps) {
+  const int step = 32 / a.lanes, steps = (heads + step - 1) / step;
+  int parts = (steps + most - 1) / most;
+  while (parts < steps && (long long)a.c.rows * (parts + 1) <= warps) ++parts;
+  return parts;
 }
 
-template <typename T, int W, bool PAIRS>
+template <typename T, int W, bool PAIRS, int LANES>
 int rt_forward(RtArgs& a, cudaStream_t stream) {
-  rt_plan<W>(a, RT_SMS * RT_FORWARD_BLOCKS * RT_WARPS, a.c.heads + a.c.keys);
-  const long long blocks = ((long long)a.c.rows * a.parts + RT_WARPS - 1) / RT_WARPS;
-  return psgd_launch(psgd_rotate_kernel<T, W, PAIRS>, (int)blocks, RT_THREADS, 0, stream, 0, a);
+  a.parts[0] = rt_parts(a, a.c.heads + a.c.keys, RT_MOST_HEADS, RT_SMS * RT_FORWARD_BLOCKS * RT_WARPS);
+  const long long blocks = ((long long)a.c.rows * a.parts[0] + RT_WARPS - 1) / RT_WARPS;
+  return psgd_launch(psgd_rotate_kernel<T, W, PAIRS, LANES>, (int)blocks, RT_THREADS, 0, stream, 0, a);
 }
-template <typename T, int W, bool PAIRS>
+template <typename T, int W, bool PAIRS, int LANES>
 int rt_backward(RtArgs& a, cudaStream_t stream) {
-  rt_plan<W>(a, RT_PART_BLOCKS * RT_WARPS, a.c.heads > a.c.keys ? a.c.heads : a.c.keys);
-  const long long blocks = ((long long)a.c.rows * a.parts * (a.c.keys > 0 ? 2 : 1) + RT_WARPS - 1) / RT_WARPS;
+  a.parts[0] = rt_parts(a, a.c.heads, RT_STEPS, RT_PART_BLOCKS * RT_WARPS / 2);
+  a.parts[1] = a.c.keys > 0 ? rt_parts(a, a.c.keys, RT_STEPS, RT_PART_BLOCKS * RT_WARPS / 2) : 0;
+  const long long blocks = ((long long)a.c.rows * (a.parts[0] + a.parts[1]) + RT_WARPS - 1) / RT_WARPS;
   const int grid = (int)(blocks < RT_PART_BLOCKS ? blocks : RT_PART_BLOCKS);
-  constexpr size_t ring = (size_t)RT_BACKWARD_STAGES * 4 * RT_THREADS * RtVec<T, W>::BYTES;
+  constexpr size_t ring = (size_t)RT_STEPS * 4 * RT_THREADS * RtVec<T, W>::BYTES;
   static unsigned long long devices = 0;
-  if (const int code = psgd_allow_shared((const void*)psgd_rotate_grad_kernel<T, W, PAIRS>, ring, devices)) return code;
-  if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS>, grid, RT_THREADS, ring, stream, 0, a)) return code;
+  if (const int code = psgd_allow_shared((const void*)psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, ring, devices)) return code;
+  if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, grid, RT_THREADS, ring, stream, 0, a)) return code;
   if (a.c.parts == nullptr) return 0;
   return psgd_launch(psgd_rotate_weights_kernel, (2 * a.c.size + 31) / 32, 32 * RT_SLICES, 0, stream, 1, (const float*)a.c.parts, grid, a.c.size, a.c.weight_type, a.c.dweight[0],
                      a.c.dweight[1]);
 }
 
+template <typename T, int W, bool PAIRS, int LANES>
+int rt_launch(RtArgs& a, bool gradient, cudaStream_t stream) {
+  return gradient ? rt_backward<T, W, PAIRS, LANES>(a, stream) : rt_forward<T, W, PAIRS, LANES>(a, stream);
+}
+template <typename T, int W, bool PAIRS>
+int rt_lanes(RtArgs& a, bool gradient, cudaStream_t stream) {
+  a.lanes = 1;
+  while (a.lanes * 2 * W < a.c.size) a.lanes *= 2;
+  a.share = 1.f / (float)a.c.size;
+  if constexpr (W == 8) {
+    if (a.lanes == 4) return rt_launch<T, W, PAIRS, 4>(a, gradient, stream);
+    if (a.lanes == 8) return rt_launch<T, W, PAIRS, 8>(a, gradient, stream);
+  }
+  return rt_launch<T, W, PAIRS, 0>(a, gradient, stream);
+}
 template <typename T>
 int rt_dispatch(RtArgs& a, bool gradient, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    if (a.c.size % 16 == 0 && a.c.rotated % 16 == 0 && (gradient ? WB : WF)) {
-      if (a.c.pairs) return gradient ? rt_backward<T, 8, true>(a, stream) : rt_forward<T, 8, true>(a, stream);
-      return gradient ? rt_backward<T, 8, false>(a, stream) : rt_forward<T, 8, false>(a, stream);
-    }
+    if (a.c.size % 16 == 0 && a.c.rotated % 16 == 0) return a.c.pairs ? rt_lanes<T, 8, true>(a, gradient, stream) : rt_lanes<T, 8, false>(a, gradient, stream);
   }
-  if (a.c.pairs) return gradient ? rt_backward<T, 4, true>(a, stream) : rt_forward<T, 4, true>(a, stream);
-  return gradient ? rt_backward<T, 4, false>(a, stream) : rt_forward<T, 4, false>(a, stream);
+  return a.c.pairs ? rt_lanes<T, 4, true>(a, gradient, stream) : rt_lanes<T, 4, false>(a, gradient, stream);
 }
 
 int rt_call(const PsgdRotate* call, bool gradient, cudaStream_t stream) {
-  if (call->size < 8 || call->size > RT_MOST_SIZE || call->size % 8 || call->rotated < 0 || call->rotated > call->size || call->rotated % 8) {
-    psgd_set_error("psgd_rotate: heads of %d of which %d are turned", call->size, call->rotated);
+  if (call->heads + call->keys > RT_MOST_HEADS || call->size < 8 || call->size > RT_MOST_SIZE || call->size % 8 || call->rotated < 0 || call->rotated > call->size || call->rotated % 8) {
+    psgd_set_error("psgd_rotate: %d heads of %d of which %d are turned", call->heads + call->keys, call->size, call->rotated);
     return PSGD_BAD_ARGUMENT;
   }
   RtArgs a = {};

@@ -20,7 +20,7 @@ from .host import operators
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 MOST_SIZE = 256
-MOST_HEADS = 2**16
+MOST_HEADS = 4096
 
 
 class Call(ctypes.Structure):
@@ -38,7 +38,7 @@ def rotate_heads(x: torch.Tensor, *, offsets: Optional[torch.Tensor] = None, pos
     """Each head of `x` divided by the root of its mean square and multiplied with `weight`, and its first `rotated` elements turned pair by
     pair by position * base^(-2 i / rotated), i = 0 to rotated / 2 - 1.
 
-    `x`: [rows, heads, size], float32, bfloat16 or float16 on the GPU; size a multiple of 8 up to 256, heads up to 65536. `rotated`: a multiple of 8, all of the head
+    `x`: [rows, heads, size], float32, bfloat16 or float16 on the GPU; size a multiple of 8 up to 256, up to 4096 heads. `rotated`: a multiple of 8, all of the head
     unless given, or 0. Pairs are (i, i + rotated / 2), or (2 i, 2 i + 1) with `interleaved`. `eps` is added to the mean square, 2^-100 to 1; None: no
     norm. `weight`: [size], float32 or of the type of x; None: ones.
 

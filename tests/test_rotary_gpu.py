@@ -51,6 +51,14 @@ def test_many_rows(rows):
     check(values(rows, 6, 64, torch.bfloat16, "cuda"), 3, 2, lengths=lengths)
 
 
+@pytest.mark.parametrize("heads, keys, values_, size", [(4095, 1, 0, 8), (1, 4000, 95, 256), (2048, 2048, 0, 72)])
+@pytest.mark.parametrize("rows", [1, 3, 700])
+def test_many_heads(rows, heads, keys, values_, size):
+    """Rows that hundreds of warps share."""
+    rows = rows if size < 256 or rows < 100 else 70
+    check(values(rows, heads + keys + values_, size, torch.float32 if size == 256 else torch.bfloat16, "cuda"), heads, keys, lengths=[rows])
+
+
 @pytest.mark.parametrize("sequences", [1, 31, 32, 33, 1023, 1024, 1025, 33000])
 def test_where_sequences_begin(sequences):
     """Positions by themselves: a pair (1, 0) turned once around in 2^20 positions gives them back."""
