@@ -27,7 +27,10 @@ namespace {
 constexpr int GN_THREADS = 256;
 constexpr int GN_PIECE = 16384;                     // bytes
 constexpr int GN_VECTORS = GN_PIECE / 16 / GN_THREADS;
-constexpr int GN_BLOCKS = 148 * 6;                  // of a launch, at most
+constexpr int GN_PER_SM = 6;                        // blocks that run at a time
+constexpr int GN_BLOCKS = 148 * GN_PER_SM;          // of a launch, at most
+constexpr int GN_PER_SM_LARGE = 4;                  // for more pieces than GN_LARGE (355 M float32: 633 us and 656 with six; 31.8 M: 65 and 63)
+constexpr long long GN_LARGE = 32768;
 constexpr int GN_SHORT = 40, GN_LONG = 1200;        // tensors of a launch (28.8 KB of arguments; short lists are launched sooner)
 
 template <int MOST>
@@ -255,8 +258,11 @@ __device__ __forceinline__ int gn_find(const GnList<MOST>& a, uint32_t c, int lo
 }
 
 template <int KIND, int MOST>
-__global__ void __launch_bounds__(GN_THREADS, 6) psgd_grad_norm_kernel(const __grid_constant__ GnList<MOST> a, typename GnPart<KIND>::type* parts) {
+__global__ void __launch_bounds__(GN_THREADS, GN_PER_SM)
+    psgd_grad_norm_kernel(const __grid_constant__ GnList<MOST> a, typename GnPart<KIND>::type* parts, int* taken, int launches) {
   psgd_launch_dependents();
+  if (blockIdx.x == 0)
+    for (int i = threadIdx.x; i < launches; i += GN_THREADS) taken[i] = 0;
   GnSeen<KIND> seen;
   int which = -1;
   uint32_t first = 0, end = 0;
@@ -301,21 +307,26 @@ __global__ void __launch_bounds__(GN_THREADS) psgd_grad_norm_total_kernel(const 
   if (threadIdx.x == 0) gn_write(out, wide, norm);
 }
 
-// Pieces are taken in the reverse order: what was read last is still in L2.
+// Pieces are taken in the reverse order, as what was read last may still be in L2, by whichever block is ready: then those under way lie side by side. (355 M
+// float32 430 us, 500 with every 888th piece to a block, 530 with a stretch to each. Blocks for one piece each take 6 % less where they scale and
+// 100 us where there is nothing to scale.)
 template <int KIND, int MOST>
-__global__ void __launch_bounds__(GN_THREADS, 6)
-    psgd_grad_clip_kernel(const __grid_constant__ GnList<MOST> a, const typename GnPart<KIND>::type* parts, int count, double max_norm, void* out, int wide) {
+__global__ void __launch_bounds__(GN_THREADS, GN_PER_SM)
+    psgd_grad_clip_kernel(const __grid_constant__ GnList<MOST> a, const typename GnPart<KIND>::type* parts, int count, double max_norm, int* taken, void* out, int wide) {
   psgd_launch_dependents();
   psgd_wait_for_predecessor();
   const double norm = gn_total<KIND>(parts, count);
   if (blockIdx.x == 0 && threadIdx.x == 0 && out != nullptr) gn_write(out, wide, norm);
   const double factor = max_norm / (norm + 1e-6);
   if (factor >= 1.0) return;
+  __shared__ uint32_t s_next;
   const uint32_t pieces = a.t[a.count - 1].piece_end;
   int which = 0;
   uint32_t first = 1, end = 0;
-  for (uint32_t back = blockIdx.x; back < pieces; back += gridDim.x) {
+  for (uint32_t back = blockIdx.x; back < pieces;) {
     const uint32_t piece = pieces - 1 - back;
+    __syncthreads();
+    if (threadIdx.x == 0) s_next = gridDim.x + (uint32_t)atomicAdd(taken, 1);
     if (piece < first || piece >= end) {
       which = gn_find(a, piece, 0);
       first = which ? a.t[which - 1].piece_end : 0;
@@ -326,6 +337,8 @@ __global__ void __launch_bounds__(GN_THREADS, 6)
     else if (t.type == 1) gn_scale<__nv_bfloat16>(t, piece - first, factor);
     else if (t.type == 2) gn_scale<__half>(t, piece - first, factor);
     else gn_scale<double>(t, piece - first, factor);
+    __syncthreads();
+    back = s_next;
   }
 }
 
@@ -351,7 +364,8 @@ int gn_fill(GnList<MOST>& a, const PsgdNormTensor* list, int count, int& done, i
     a.t[a.count] = list[done];
     a.t[a.count++].piece_end = (uint32_t)pieces;
   }
-  grid = (int)(pieces < GN_BLOCKS ? pieces : GN_BLOCKS);
+  const int most = pieces > GN_LARGE ? 148 * GN_PER_SM_LARGE : GN_BLOCKS;
+  grid = (int)(pieces < most ? pieces : most);
   return 0;
 }
 
@@ -360,19 +374,21 @@ int gn_run(const PsgdNormTensor* list, int count, int clip, double max_norm, typ
   typedef const typename GnPart<KIND>::type* Parts;
   GnList<MOST> a;
   int grid = 0, have = 0, launches = 0;
+  const int most = (count + MOST - 1) / MOST;       // launches
+  int* taken = (int*)(parts + (size_t)most * GN_BLOCKS);
   for (int done = 0; done < count;) {
     if (const int code = gn_fill(a, list, count, done, grid)) return code;
     if (grid == 0) continue;
-    if (const int code = psgd_launch(psgd_grad_norm_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 0, a, parts + have)) return code;
+    if (const int code = psgd_launch(psgd_grad_norm_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 0, a, parts + have, taken, clip && launches == 0 ? most : 0)) return code;
     have += grid;
     ++launches;
   }
   if (!clip || launches == 0) return psgd_launch(psgd_grad_norm_total_kernel<KIND>, 1, GN_THREADS, 0, stream, launches > 0, (Parts)parts, have, out, wide);
-  if (launches == 1) return psgd_launch(psgd_grad_clip_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 1, a, (Parts)parts, have, max_norm, out, wide);
+  if (launches == 1) return psgd_launch(psgd_grad_clip_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 1, a, (Parts)parts, have, max_norm, taken, out, wide);
   for (int done = 0; done < count;) {
     if (const int code = gn_fill(a, list, count, done, grid)) return code;
     if (grid == 0) continue;
-    if (const int code = psgd_launch(psgd_grad_clip_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 1, a, (Parts)parts, have, max_norm, out, wide)) return code;
+    if (const int code = psgd_launch(psgd_grad_clip_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 1, a, (Parts)parts, have, max_norm, taken++, out, wide)) return code;
     out = nullptr;
   }
   return 0;
@@ -390,7 +406,7 @@ int gn_dispatch(const PsgdNormTensor* list, int count, int clip, double max_norm
 PSGD_API int psgd_grad_norm_item_bytes() { return (int)sizeof(PsgdNormTensor); }
 
 // Words of 8 bytes of scratch for a list of `count` tensors.
-PSGD_API long long psgd_grad_norm_parts(int count) { return (long long)GN_BLOCKS * (count <= GN_SHORT ? 1 : (count + GN_LONG - 1) / GN_LONG); }
+PSGD_API long long psgd_grad_norm_parts(int count) { return (GN_BLOCKS + 1ll) * (count <= GN_SHORT ? 1 : (count + GN_LONG - 1) / GN_LONG); }
 
 // `list`: host memory, read before the call returns. `largest`: the largest magnitude instead of the root of the sum of squares. `clip`: gradients are
 // scaled where max_norm / (norm + 1e-6) is not at least one. `out`: the norm before that, float, or double where `wide`.
