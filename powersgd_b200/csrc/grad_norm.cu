@@ -9,8 +9,11 @@
 // Two launches: sums of blocks, which a second one adds up again in every block, always in the same order. The list travels in
 // the launches' own arguments, so nothing is uploaded and a recorded graph keeps it. A block takes pieces of 16 KiB that begin on
 // 16-byte boundaries, wherever a tensor begins: only what a piece's first and last 16 bytes hold of other tensors is left out.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <utility>
 
 #include "psgd_common.cuh"
 
@@ -24,6 +27,8 @@ typedef struct {
 
 namespace {
 
+namespace cg = cooperative_groups;
+
 constexpr int GN_THREADS = 256;
 constexpr int GN_PIECE = 16384;                     // bytes
 constexpr int GN_VECTORS = GN_PIECE / 16 / GN_THREADS;
@@ -31,6 +36,8 @@ constexpr int GN_PER_SM = 6;                        // blocks that run at a time
 constexpr int GN_BLOCKS = 148 * GN_PER_SM;          // of a launch, at most
 constexpr int GN_PER_SM_LARGE = 4;                  // for more pieces than GN_LARGE (355 M float32: 633 us and 656 with six; 31.8 M: 65 and 63)
 constexpr long long GN_LARGE = 32768;
+constexpr int GN_CLUSTER = 8, GN_HELD = 8;          // blocks of a short list's one launch, pieces that each holds
+constexpr int GN_SMALL_THREADS = GN_PIECE / 16;
 constexpr int GN_SHORT = 40, GN_LONG = 1200;        // tensors of a launch (28.8 KB of arguments; short lists are launched sooner)
 
 template <int MOST>
@@ -342,6 +349,120 @@ __global__ void __launch_bounds__(GN_THREADS, GN_PER_SM)
   }
 }
 
+// Short lists in one launch: a cluster of blocks holds all of it in registers, a vector of 16 bytes to a thread and piece. What of a vector
+// belongs to other tensors is zero here and is not written back.
+template <typename T>
+__device__ __forceinline__ uint4 gn_fetch(const GnPiece<T>& p) {
+  constexpr int N = GnType<T>::N;
+  const int i = threadIdx.x * N;
+  if (i >= p.lo && i + N <= p.hi) return *reinterpret_cast<const uint4*>(p.base + i);
+  union {
+    uint4 v;
+    T t[N];
+  } raw;
+  raw.v = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (i + j >= p.lo && i + j < p.hi) raw.t[j] = p.base[i + j];
+  return raw.v;
+}
+template <typename T, int KIND>
+__device__ __forceinline__ void gn_take(const uint4& raw, GnSeen<KIND>& seen) {
+  typename GnWide<T>::type f[GnType<T>::N];
+  GnType<T>::unpack(raw, f);
+#pragma unroll
+  for (int j = 0; j < GnType<T>::N; ++j) seen.take(f[j]);
+}
+template <typename T>
+__device__ __forceinline__ void gn_put_back(const GnPiece<T>& p, const uint4& held, double factor) {
+  typedef typename GnWide<T>::type F;
+  constexpr int N = GnType<T>::N;
+  const int i = threadIdx.x * N;
+  const F c = (F)factor;
+  F f[N];
+  GnType<T>::unpack(held, f);
+#pragma unroll
+  for (int j = 0; j < N; ++j) f[j] *= c;
+  union {
+    uint4 v;
+    T t[N];
+  } raw;
+  raw.v = GnType<T>::pack(f);
+  if (i >= p.lo && i + N <= p.hi) {
+    *reinterpret_cast<uint4*>(p.base + i) = raw.v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (i + j >= p.lo && i + j < p.hi) p.base[i + j] = raw.t[j];
+  }
+}
+
+// (A perceptron's 0.8 MB: 8.5 us to a program that calls it again and again, 11.4 in two launches, which the host takes longer to make;
+// replayed in a graph 5.6 and 4.2.)
+template <int KIND, int MOST>
+__global__ void __launch_bounds__(GN_SMALL_THREADS, 1)
+    psgd_grad_small_kernel(const __grid_constant__ GnList<MOST> a, int clip, double max_norm, void* out, int wide) {
+  typedef GnPart<KIND> P;
+  __shared__ typename P::type s_warps[GN_SMALL_THREADS / 32], s_parts[GN_CLUSTER];
+  __shared__ int s_which[GN_HELD];
+  cg::cluster_group cluster = cg::this_cluster();
+  auto running = cluster.barrier_arrive();
+  const uint32_t pieces = a.t[a.count - 1].piece_end, rank = blockIdx.x;      // (the grid is one cluster)
+  if (threadIdx.x < GN_HELD) s_which[threadIdx.x] = rank + threadIdx.x * GN_CLUSTER < pieces ? gn_find(a, rank + threadIdx.x * GN_CLUSTER, 0) : -1;
+  __syncthreads();
+  uint4 raw[GN_HELD];
+#pragma unroll
+  for (int i = 0; i < GN_HELD; ++i) {
+    const int which = s_which[i];
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (which < 0) continue;
+    const PsgdNormTensor& t = a.t[which];
+    const uint32_t at = rank + i * GN_CLUSTER - (which ? a.t[which - 1].piece_end : 0);
+    raw[i] = t.type == 0 ? gn_fetch(GnPiece<float>(t, at)) : t.type == 1 ? gn_fetch(GnPiece<__nv_bfloat16>(t, at)) : t.type == 2 ? gn_fetch(GnPiece<__half>(t, at)) : gn_fetch(GnPiece<double>(t, at));
+  }
+  GnSeen<KIND> seen;
+#pragma unroll
+  for (int i = 0; i < GN_HELD; ++i) {
+    if (s_which[i] < 0) continue;
+    const uint32_t type = a.t[s_which[i]].type;
+    if (type == 0) gn_take<float>(raw[i], seen);
+    else if (type == 1) gn_take<__nv_bfloat16>(raw[i], seen);
+    else if (type == 2) gn_take<__half>(raw[i], seen);
+    else gn_take<double>(raw[i], seen);
+  }
+  typename P::type v = seen.all();
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = P::join(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if ((threadIdx.x & 31) == 0) s_warps[threadIdx.x >> 5] = v;
+  __syncthreads();
+  cluster.barrier_wait(std::move(running));        // all blocks run: their shared memory is there
+  if (threadIdx.x < 32) {
+    v = s_warps[threadIdx.x];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = P::join(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if (threadIdx.x < GN_CLUSTER) cluster.map_shared_rank(s_parts, threadIdx.x)[rank] = v;
+  }
+  cluster.sync();
+  v = s_parts[0];
+#pragma unroll
+  for (int i = 1; i < GN_CLUSTER; ++i) v = P::join(v, s_parts[i]);
+  const double norm = P::norm(v);
+  if (rank == 0 && threadIdx.x == 0) gn_write(out, wide, norm);
+  const double factor = max_norm / (norm + 1e-6);
+  if (!clip || factor >= 1.0) return;
+#pragma unroll
+  for (int i = 0; i < GN_HELD; ++i) {
+    const int which = s_which[i];
+    if (which < 0) continue;
+    const PsgdNormTensor& t = a.t[which];
+    const uint32_t at = rank + i * GN_CLUSTER - (which ? a.t[which - 1].piece_end : 0);
+    if (t.type == 0) gn_put_back(GnPiece<float>(t, at), raw[i], factor);
+    else if (t.type == 1) gn_put_back(GnPiece<__nv_bfloat16>(t, at), raw[i], factor);
+    else if (t.type == 2) gn_put_back(GnPiece<__half>(t, at), raw[i], factor);
+    else gn_put_back(GnPiece<double>(t, at), raw[i], factor);
+  }
+}
+
 inline long long gn_pieces(const PsgdNormTensor& t) {
   if (t.n <= 0) return 0;
   const long long width = t.type == 0 ? 4 : t.type == 3 ? 8 : 2, lead = (long long)((uintptr_t)t.g & 15u);
@@ -379,6 +500,8 @@ int gn_run(const PsgdNormTensor* list, int count, int clip, double max_norm, typ
   for (int done = 0; done < count;) {
     if (const int code = gn_fill(a, list, count, done, grid)) return code;
     if (grid == 0) continue;
+    if (launches == 0 && done == count && a.t[a.count - 1].piece_end <= GN_CLUSTER * GN_HELD)
+      return psgd_launch_clusters(psgd_grad_small_kernel<KIND, MOST>, GN_CLUSTER, GN_SMALL_THREADS, 0, stream, 0, GN_CLUSTER, a, clip, max_norm, out, wide);
     if (const int code = psgd_launch(psgd_grad_norm_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 0, a, parts + have, taken, clip && launches == 0 ? most : 0)) return code;
     have += grid;
     ++launches;

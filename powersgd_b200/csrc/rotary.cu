@@ -56,6 +56,7 @@ constexpr int RT_SMS = 148;
 #endif
 constexpr int RT_FORWARD_BLOCKS = FB, RT_BACKWARD_BLOCKS = BB;   // of an SM at a time
 constexpr int RT_STEPS = RS;             // of a warp, gradients
+constexpr int RT_PASSING = 2;            // vectors of values of a thread that pass by with them
 constexpr int RT_FORWARD_STAGES = FS;    // steps whose inputs are on their way or read
 // Do the squares of a type leave the range of float32?
 template <typename T>
@@ -71,8 +72,7 @@ struct RtArgs {
   unsigned long long frequency[RT_MOST_ANGLES];
 };
 
-// Two float32 in one register of 64 bits. (As two of 32 bits, which ptxas has to move together before each operation, the kernels executed PLACEHOLDER
-// more instructions.)
+// Two float32 in one register of 64 bits, so that they need not be moved together before each operation.
 typedef unsigned long long RtPair;
 __device__ __forceinline__ RtPair rt_pair(float a, float b) {
   RtPair p;
@@ -185,36 +185,50 @@ __device__ __forceinline__ float rt_weight(const void* p, int type, int i) {
   return __half2float(((const __half*)p)[i]);
 }
 
-// Position of a row; false where it belongs to no sequence. A whole warp asks. How many offsets are not behind the row: 32 of them at a time,
-// evenly apart, which leave a 32nd of the list. (Whatever the list holds, indices stay inside it.)
-__device__ __forceinline__ bool rt_position(const PsgdRotate& c, int row, int lane, unsigned long long& position) {
-  position = 0;
-  if (c.offsets == nullptr) {
-    if (c.positions != nullptr) position = c.wide ? ((const unsigned long long*)c.positions)[row] : (unsigned long long)(long long)((const int*)c.positions)[row];
+// Where the rows' positions come from. A whole warp asks. How many offsets are not behind the row: 32 of them at a time, evenly apart, which leave a 32nd
+// of the list. (Whatever the list holds, indices stay inside it.) The last 32, or a short list, are a lane's each.
+struct RtPositions {
+  int held;       // a short list's
+  bool few;
+  __device__ __forceinline__ RtPositions(const PsgdRotate& c) {
+    const int lane = threadIdx.x & 31;
+    few = c.offsets != nullptr && c.sequences < 32;
+    held = few && lane <= c.sequences ? c.offsets[lane] : 0x7fffffff;
+  }
+  // False where the row belongs to no sequence.
+  __device__ __forceinline__ bool of(const PsgdRotate& c, int row, unsigned long long& position) const {
+    const int lane = threadIdx.x & 31;
+    position = 0;
+    if (c.offsets == nullptr) {
+      if (c.positions != nullptr) position = c.wide ? ((const unsigned long long*)c.positions)[row] : (unsigned long long)(long long)((const int*)c.positions)[row];
+      return true;
+    }
+    int lo = 0, mine = held;
+    if (!few) {
+      int n = c.sequences + 1;
+      while (n > 32) {
+        const int step = (n + 31) >> 5;
+        const bool in = lane * step < n;
+        const int before = __popc(__ballot_sync(0xffffffffu, in && c.offsets[in ? lo + lane * step : lo] <= row));
+        if (before == 0) {                      // (the first of these is behind the row, and so are all)
+          n = 0;
+          break;
+        }
+        const int next = (before - 1) * step + 1;
+        n = min(step, n - (before - 1) * step) - 1;
+        lo += next;
+      }
+      mine = lane < n ? c.offsets[lo + lane] : 0x7fffffff;
+    }
+    const unsigned before = __ballot_sync(0xffffffffu, mine <= row);
+    const int count = lo + __popc(before);
+    if (count == 0 || count > c.sequences) return false;
+    // (where the last one that is not behind the row was among these, a lane has it)
+    const int start = before ? __shfl_sync(0xffffffffu, mine, (__popc(before) - 1) & 31) : c.offsets[count - 1];
+    position = (unsigned long long)(row - max(start, 0));
     return true;
   }
-  int lo = 0, n = c.sequences + 1;
-  while (n > 32) {
-    const int step = (n + 31) >> 5;
-    const bool in = lane * step < n;
-    const int before = __popc(__ballot_sync(0xffffffffu, in && c.offsets[in ? lo + lane * step : lo] <= row));
-    if (before == 0) {                      // (the first of these is behind the row, and so are all)
-      n = 0;
-      break;
-    }
-    const int next = (before - 1) * step + 1;
-    n = min(step, n - (before - 1) * step) - 1;
-    lo += next;
-  }
-  const int mine = lane < n ? c.offsets[lo + lane] : 0x7fffffff;
-  const unsigned before = __ballot_sync(0xffffffffu, lane < n && mine <= row);
-  const int count = lo + __popc(before);
-  if (count == 0 || count > c.sequences) return false;
-  // (where the last one that is not behind the row was among these, a lane has it)
-  const int start = before ? __shfl_sync(0xffffffffu, mine, (__popc(before) - 1) & 31) : c.offsets[count - 1];
-  position = (unsigned long long)(row - max(start, 0));
-  return true;
-}
+};
 
 // Cosine and sine of a fraction of a turn (64 bits behind the point): the nearest quarter is taken out first. What is left, an eighth of a turn
 // at most, goes into the first terms of their series: what follows is below 2e-9 and 3e-10.
@@ -234,7 +248,8 @@ struct __align__(16) RtShared {
   float weight[2][RT_MOST_SIZE];
   unsigned long long frequency[RT_MOST_ANGLES];
   __device__ __forceinline__ void fill(const RtArgs& a) {     // (a thread for each element)
-    const int i = threadIdx.x;
+    const int i = threadIdx.x, warp = i >> 5;
+    for (int j = a.c.rotated / 2 + (i & 31); j < a.c.size / 2; j += 32) cosine[warp][j] = 1.f, sine[warp][j] = 0.f;   // pairs that are not turned
     if (i < a.c.rotated / 2) frequency[i] = a.frequency[i];
     if (i < a.c.size) {
 #pragma unroll
@@ -271,7 +286,7 @@ struct RtPlace {
     in = 2 * pair < a.c.size;
     if (PAIRS) {
       lo = 2 * pair, hi = lo + W;
-      turned = lo < a.c.rotated;
+      turned = true;
     } else if (pair < half) {
       lo = pair, hi = pair + half;
       turned = true;
@@ -346,7 +361,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
   constexpr int HALF = RT_THREADS * Vec::BYTES, STAGE = 2 * HALF;     // of the ring
   __shared__ RtShared shared;
   __shared__ __align__(16) char ring[RT_FORWARD_STAGES * STAGE];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, lanes = LANES ? LANES : a.lanes, parts = a.parts[0];
+  const int warp = threadIdx.x >> 5, lanes = LANES ? LANES : a.lanes, parts = a.parts[0];
   RtPlace<W, PAIRS, LANES> place(a);
   const int size = a.c.size, all = a.c.heads + a.c.keys, step = place.heads;
   const uint32_t u = blockIdx.x * RT_WARPS + warp;
@@ -384,7 +399,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
   const long long out_step = step * size, to_keys = ((T*)a.c.out[1] + ((long long)row * a.c.keys - a.c.heads) * size) - ((T*)a.c.out[0] + (long long)row * a.c.heads * size);
   T* out = (T*)a.c.out[0] + ((long long)row * a.c.heads + head) * size + place.lo;     // (as if the keys lay behind the queries)
   unsigned long long position;
-  if (!rt_position(a.c, row, lane, position)) {
+  if (!RtPositions(a.c).of(a.c, row, position)) {
     RtPair zeros[W / 2];
 #pragma unroll
     for (int i = 0; i < W / 2; ++i) zeros[i] = 0;
@@ -467,7 +482,24 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   const bool given = a.c.grad[kind] != nullptr;
   const T* g = given ? (const T*)a.c.grad[kind] + (long long)row * a.c.grad_row[kind] + head * a.c.grad_head[kind] + place.lo : x;
   char* const mine = ring + threadIdx.x * Vec::BYTES;
+  // values: 16 bytes at a time, RT_PASSING of them by way of shared memory as well
+  const int all = a.c.heads + a.c.keys + a.c.values, vectors = size / N, passing = a.c.dx != nullptr ? a.c.values * vectors : 0;
+  char* const values = ring + RT_STEPS * STEP + threadIdx.x * 16;
+  const bool valued = a.c.grad[2] != nullptr;
+  const T* gv = valued ? (const T*)a.c.grad[2] + (long long)row * a.c.grad_row[2] : x;
+  long long passed[RT_PASSING];
+#pragma unroll
+  for (int j = 0; j < RT_PASSING; ++j) {
+    const int i = (j * parts + part) * 32 + lane, h = i / vectors;
+    passed[j] = h * a.c.grad_head[2] + (i - h * vectors) * N;
+  }
+  const long long gv_stride = valued ? stride * a.c.grad_row[2] : 0;
   const auto fetch = [&](int i) {      // (lanes without a head find zeros)
+    if (i == 0 && ahead < a.c.rows) {
+#pragma unroll
+      for (int j = 0; j < RT_PASSING; ++j)
+        if ((j * parts + part) * 32 + lane < passing) rt_fetch<16>(values + j * RT_THREADS * 16, gv + passed[j], valued);
+    }
     if (i < count && ahead < a.c.rows) {
       const bool there = place.in && head + i * step < have;
       rt_fetch<Vec::BYTES>(mine + i * STEP, x + i * x_step, there);
@@ -482,7 +514,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   const bool sums = a.c.parts != nullptr;
   shared.fill(a);
   __syncthreads();
-  const int all = a.c.heads + a.c.keys + a.c.values, vectors = size / N, passing = a.c.dx != nullptr ? a.c.values * vectors : 0;
+  const RtPositions positions(a.c);
   T* dx = (T*)a.c.dx + ((long long)row * all + (kind ? a.c.heads : 0) + head) * size + place.lo;
   const long long dx_stride = (long long)stride * all * size;
   const float* weight = shared.weight[kind] + place.lo;
@@ -494,22 +526,26 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
     ahead = stride < a.c.rows - row ? row + stride : a.c.rows;
     x += x_stride;
     g += g_stride;
-    if (passing > 0) {
-      const T* gv = (const T*)a.c.grad[2];
-      T* o = (T*)a.c.dx + ((long long)row * all + a.c.heads + a.c.keys) * size;
-      if (gv != nullptr) gv += (long long)row * a.c.grad_row[2];
-#pragma unroll 2
-      for (int i = part * 32 + lane; i < passing; i += 32 * parts) {
-        const int h = i / vectors, e = (i - h * vectors) * N;
-        *reinterpret_cast<uint4*>(o + i * N) = gv != nullptr ? __ldcs(reinterpret_cast<const uint4*>(gv + h * a.c.grad_head[2] + e)) : make_uint4(0, 0, 0, 0);
-      }
-    }
+    gv += gv_stride;
     unsigned long long position;
-    const bool held = rt_position(a.c, row, lane, position);
+    const bool held = positions.of(a.c, row, position);
     if (a.c.rotated > 0) place.angles(a, position, shared);
 #pragma unroll
     for (int i = 0; i < RT_STEPS; ++i) {
       rt_await<RT_STEPS - 1>();
+      if (i == 0 && passing > 0) {     // values pass by
+        T* o = (T*)a.c.dx + ((long long)row * all + a.c.heads + a.c.keys) * size;
+#pragma unroll
+        for (int j = 0; j < RT_PASSING; ++j) {
+          const int e = (j * parts + part) * 32 + lane;
+          if (e < passing) *reinterpret_cast<uint4*>(o + e * N) = *reinterpret_cast<const uint4*>(values + j * RT_THREADS * 16);
+        }
+        for (int e = (RT_PASSING * parts + part) * 32 + lane; e < passing; e += 32 * parts) {
+          const int h = e / vectors;
+          *reinterpret_cast<uint4*>(o + e * N) =
+              valued ? __ldcs(reinterpret_cast<const uint4*>(gv - gv_stride + h * a.c.grad_head[2] + (e - h * vectors) * N)) : make_uint4(0, 0, 0, 0);
+        }
+      }
       if (i < count) {
         RtPair f[W], d[W];
         {
@@ -639,7 +675,7 @@ int rt_backward(RtArgs& a, cudaStream_t stream) {
   a.parts[1] = a.c.keys > 0 ? rt_parts(a, a.c.keys, RT_STEPS, RT_PART_BLOCKS * RT_WARPS / 2) : 0;
   const long long blocks = ((long long)a.c.rows * (a.parts[0] + a.parts[1]) + RT_WARPS - 1) / RT_WARPS;
   const int grid = (int)(blocks < RT_PART_BLOCKS ? blocks : RT_PART_BLOCKS);
-  constexpr size_t ring = (size_t)RT_STEPS * 4 * RT_THREADS * RtVec<T, W>::BYTES;
+  constexpr size_t ring = (size_t)RT_THREADS * (RT_STEPS * 4 * RtVec<T, W>::BYTES + RT_PASSING * 16);
   static unsigned long long devices = 0;
   if (const int code = psgd_allow_shared((const void*)psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, ring, devices)) return code;
   if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, grid, RT_THREADS, ring, stream, 0, a)) return code;
@@ -666,7 +702,7 @@ int rt_lanes(RtArgs& a, bool gradient, cudaStream_t stream) {
 template <typename T>
 int rt_dispatch(RtArgs& a, bool gradient, cudaStream_t stream) {
   if constexpr (sizeof(T) == 2) {
-    if (a.c.size % 16 == 0 && a.c.rotated % 16 == 0) return a.c.pairs ? rt_lanes<T, 8, true>(a, gradient, stream) : rt_lanes<T, 8, false>(a, gradient, stream);
+    if (a.c.size % 16 == 0 && (a.c.pairs || a.c.rotated % 16 == 0)) return a.c.pairs ? rt_lanes<T, 8, true>(a, gradient, stream) : rt_lanes<T, 8, false>(a, gradient, stream);
   }
   return a.c.pairs ? rt_lanes<T, 4, true>(a, gradient, stream) : rt_lanes<T, 4, false>(a, gradient, stream);
 }

@@ -63,14 +63,17 @@ def _listed(parameters) -> List[torch.Tensor]:
     return [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
 
 
-@torch.no_grad()
 def _norm(parameters: List[torch.Tensor], largest: bool, max_norm) -> torch.Tensor:
     """The norm; gradients are scaled unless `max_norm` is None."""
-    what = "grad_norm" if max_norm is None else "clip_grad_norm"
     if operators is not None:
         out = operators.grad_norm(parameters, largest, max_norm is not None, 0.0 if max_norm is None else max_norm)
         if out is not None:
             return out
+    with torch.no_grad():
+        return _norm_checked("grad_norm" if max_norm is None else "clip_grad_norm", parameters, largest, max_norm)
+
+
+def _norm_checked(what: str, parameters: List[torch.Tensor], largest: bool, max_norm) -> torch.Tensor:
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.zeros((), device=parameters[0].device if parameters else None)
