@@ -48,16 +48,10 @@ constexpr int RT_THREADS = 256, RT_WARPS = RT_THREADS / 32;
 constexpr int RT_MOST_SIZE = 256, RT_MOST_ANGLES = RT_MOST_SIZE / 2;
 constexpr int RT_MOST_HEADS = 4096;      // (so that no row is shared by more warps than RT_PART_BLOCKS have)
 constexpr int RT_SMS = 148;
-#ifndef FB
-#define FB 4
-#define BB 2
-#define RS 2
-#define FS 3
-#endif
-constexpr int RT_FORWARD_BLOCKS = FB, RT_BACKWARD_BLOCKS = BB;   // of an SM at a time
-constexpr int RT_STEPS = RS;             // of a warp, gradients
+constexpr int RT_FORWARD_BLOCKS = 4, RT_BACKWARD_BLOCKS = 2;      // of an SM at a time
+constexpr int RT_FORWARD_STAGES = 3;     // steps whose inputs are on their way or read
+constexpr int RT_STEPS = 2;              // of a warp, gradients
 constexpr int RT_PASSING = 2;            // vectors of values of a thread that pass by with them
-constexpr int RT_FORWARD_STAGES = FS;    // steps whose inputs are on their way or read
 // Do the squares of a type leave the range of float32?
 template <typename T>
 constexpr bool RT_RANGE = !std::is_same<T, __half>::value;
