@@ -241,14 +241,20 @@ struct __align__(16) RtShared {
   float cosine[RT_WARPS][RT_MOST_ANGLES], sine[RT_WARPS][RT_MOST_ANGLES];   // of the row that a warp has
   float weight[2][RT_MOST_SIZE];
   unsigned long long frequency[RT_MOST_ANGLES];
-  __device__ __forceinline__ void fill(const RtArgs& a) {     // (a thread for each element)
+  // A thread for each element: `begin`, a barrier, what takes angles, `end`, a barrier, what takes weights. (The weights are on their way meanwhile.)
+  __device__ __forceinline__ float2 begin(const RtArgs& a) {
     const int i = threadIdx.x, warp = i >> 5;
-    for (int j = a.c.rotated / 2 + (i & 31); j < a.c.size / 2; j += 32) cosine[warp][j] = 1.f, sine[warp][j] = 0.f;   // pairs that are not turned
-    if (i < a.c.rotated / 2) frequency[i] = a.frequency[i];
+    float2 own = make_float2(1.f, 1.f);
     if (i < a.c.size) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) weight[k][i] = a.c.weight[k] != nullptr ? rt_weight(a.c.weight[k], a.c.weight_type, i) : 1.f;
+      if (a.c.weight[0] != nullptr) own.x = rt_weight(a.c.weight[0], a.c.weight_type, i);
+      if (a.c.weight[1] != nullptr) own.y = rt_weight(a.c.weight[1], a.c.weight_type, i);
     }
+    if (i < a.c.rotated / 2) frequency[i] = a.frequency[i];
+    for (int j = a.c.rotated / 2 + (i & 31); j < a.c.size / 2; j += 32) cosine[warp][j] = 1.f, sine[warp][j] = 0.f;   // pairs that are not turned
+    return own;
+  }
+  __device__ __forceinline__ void end(const RtArgs& a, float2 own) {
+    if (threadIdx.x < a.c.size) weight[0][threadIdx.x] = own.x, weight[1][threadIdx.x] = own.y;
   }
 };
 static_assert(RT_MOST_HEADS / RT_STEPS + 2 <= RT_PART_BLOCKS * RT_WARPS, "a warp for each share of a row");
@@ -384,7 +390,12 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
   };
 #pragma unroll
   for (int i = 0; i < RT_FORWARD_STAGES - 1; ++i) fetch();
-  shared.fill(a);
+  const float2 own = shared.begin(a);
+  __syncthreads();
+  unsigned long long position = 0;
+  const bool held = live && RtPositions(a.c).of(a.c, row, position);
+  if (held && a.c.rotated > 0) place.angles(a, position, shared);
+  shared.end(a, own);
   __syncthreads();
   if (!live) {
     rt_await<0>();
@@ -392,8 +403,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
   }
   const long long out_step = step * size, to_keys = ((T*)a.c.out[1] + ((long long)row * a.c.keys - a.c.heads) * size) - ((T*)a.c.out[0] + (long long)row * a.c.heads * size);
   T* out = (T*)a.c.out[0] + ((long long)row * a.c.heads + head) * size + place.lo;     // (as if the keys lay behind the queries)
-  unsigned long long position;
-  if (!RtPositions(a.c).of(a.c, row, position)) {
+  if (!held) {
     RtPair zeros[W / 2];
 #pragma unroll
     for (int i = 0; i < W / 2; ++i) zeros[i] = 0;
@@ -405,7 +415,6 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
     rt_await<0>();
     return;
   }
-  if (a.c.rotated > 0) place.angles(a, position, shared);
   const float* weight = shared.weight[0] + place.lo;
 #pragma unroll 1
   for (int i = 0; i < count; ++i) {
@@ -433,9 +442,9 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
       }
       const RtPair r = rt_both(rsqrtf(fmaf(s, a.share, eps)));
       RtPair w[W];
-      const float* own = weight + (key ? RT_MOST_SIZE : 0);
-      rt_get<W>(own, w);
-      rt_get<W>(own + apart, w + W / 2);
+      const float* of = weight + (key ? RT_MOST_SIZE : 0);
+      rt_get<W>(of, w);
+      rt_get<W>(of + apart, w + W / 2);
 #pragma unroll
       for (int j = 0; j < W; ++j) f[j] = rt_mul(rt_mul(f[j], r), w[j]);
     }
@@ -506,7 +515,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
 #pragma unroll
   for (int i = 0; i < RT_STEPS; ++i) fetch(i);
   const bool sums = a.c.parts != nullptr;
-  shared.fill(a);
+  shared.end(a, shared.begin(a));
   __syncthreads();
   const RtPositions positions(a.c);
   T* dx = (T*)a.c.dx + ((long long)row * all + (kind ? a.c.heads : 0) + head) * size + place.lo;

@@ -26,7 +26,7 @@ from typing import Callable, Dict, Optional
 
 import torch
 
-from .ops.grad_norm import clip_grad_norm
+from .ops.grad_norm import clip_for_step
 from .optim import optimizer_step
 from .utils import same_layout
 
@@ -162,7 +162,7 @@ class TrainStep:
 
     def _clip(self) -> None:
         if self.grad_clip is not None:
-            clip_grad_norm(self._params(), self.grad_clip)   # no host synchronisation, capturable
+            clip_for_step(self._params(), self.grad_clip)   # no host synchronisation, capturable
 
     def _params(self):
         return [p for g in self.optimizer.param_groups for p in g["params"]]

@@ -53,6 +53,18 @@ def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_
     return _norm(listed, largest, max_norm)
 
 
+def clip_for_step(parameters: Iterable[torch.Tensor], max_norm: float) -> torch.Tensor:
+    """What a training loop of this package clips with: `clip_grad_norm` on the GPU. Gradients on the CPU, and lists that it refuses (complex
+    gradients, several devices), go to the library, which refuses sparse ones too."""
+    listed = _listed(parameters)
+    if any(p.is_cuda for p in listed):
+        try:
+            return clip_grad_norm(listed, max_norm)
+        except (TypeError, ValueError):     # (nothing was changed)
+            pass
+    return torch.nn.utils.clip_grad_norm_(listed, max_norm)
+
+
 def _largest(what: str, norm_type: float) -> bool:
     if norm_type not in (2, math.inf):
         raise ValueError(f"{what}: norm_type {norm_type}; 2 and infinity are supported")

@@ -15,7 +15,7 @@ from typing import Dict, Iterable, List
 import torch
 
 from ...models.lstm import RNNModel
-from ...ops.grad_norm import clip_grad_norm
+from ...ops.grad_norm import clip_for_step
 from ...utils import MeanAccumulator
 from .utils import _world, zipf_tokens
 
@@ -115,7 +115,7 @@ class LanguageModelingTask:
             loss.backward()
         with self._timer("batch.evaluate", float(self._epoch)):
             metrics = self.evaluate_prediction(prediction, batch.y)
-        clip_grad_norm(self._model.parameters(), rnn_clip)
+        clip_for_step(self._model.parameters(), rnn_clip)
         return loss.detach(), [p.grad for p in self._model.parameters()], metrics
 
     def evaluate_prediction(self, output, target) -> Dict[str, torch.Tensor]:

@@ -190,6 +190,19 @@ def test_train_step_clips(graph):
         torch.testing.assert_close(p, q, rtol=1e-4, atol=1e-5)   # float32 sums in other orders through eight steps
 
 
+def test_lists_that_are_refused_are_clipped_by_the_library():
+    from powersgd_b200.ops.grad_norm import clip_for_step
+
+    def lists():
+        complex_, cpu = torch.nn.Parameter(torch.zeros(4, dtype=torch.complex64, device="cuda")), make([(4, 6)], TYPES[:1])[0]
+        complex_.grad = torch.ones(4, dtype=torch.complex64, device="cuda")
+        return [*make([(4, 6)], TYPES[:1], "cuda"), cpu], [*make([(4, 6)], TYPES[:1], "cuda"), complex_], [cpu]
+
+    for ours, theirs in zip(lists(), lists()):
+        assert torch.equal(clip_for_step(iter(ours), 0.1), torch.nn.utils.clip_grad_norm_(theirs, 0.1))
+        assert all(torch.equal(p.grad, q.grad) for p, q in zip(ours, theirs))
+
+
 @pytest.mark.parametrize("bits", [8, 32])
 def test_with_adamw_behind_an_aggregator(bits):
     torch.manual_seed(0)
