@@ -43,7 +43,7 @@ struct RotateCall {   // PsgdRotate, csrc/rotary.cu
   void* out[2];
   void* dx;
   void* dweight[2];
-  float* parts;
+  double* parts;
   const void* frequencies;
   long long x_row, x_head, grad_row[3], grad_head[3];
   int rows, sequences, heads, keys, values, size, rotated, pairs;
@@ -502,8 +502,8 @@ struct Rotate : torch::autograd::Function<Rotate> {
         c.dweight[i] = result[1 + i].data_ptr();
       }
       if (c.dweight[0] != nullptr || c.dweight[1] != nullptr) {
-        parts = at::empty({entry.rotate_parts(c.size)}, x.options().dtype(at::kFloat));
-        c.parts = (float*)parts.data_ptr();
+        parts = at::empty({entry.rotate_parts(c.size)}, x.options().dtype(at::kDouble));
+        c.parts = (double*)parts.data_ptr();
       }
       check(entry.rotate_grad(&c, current_stream(x)), "psgd_rotate_grad");
     }

@@ -31,7 +31,7 @@ typedef struct {
   void* out[2];                    // queries and keys, contiguous
   void* dx;                        // like x, contiguous, or null
   void* dweight[2];                // of the weights' type, or null
-  float* parts;                    // scratch for these: psgd_rotate_parts floats
+  double* parts;                   // scratch for these: psgd_rotate_parts numbers
   const unsigned long long* frequencies;   // host memory: rotated / 2 fractions of a turn per position
   long long x_row, x_head, grad_row[3], grad_head[3];
   int rows, sequences, heads, keys, values, size, rotated, pairs;
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   constexpr int HALF = RT_THREADS * Vec::BYTES, STEP = 4 * HALF, N = 16 / (int)sizeof(T);
   extern __shared__ __align__(16) char ring[];
   __shared__ RtShared shared;
-  __shared__ __align__(16) float s_sums[RT_WARPS][RT_MOST_SIZE];
+  __shared__ __align__(16) double s_sums[RT_WARPS][RT_MOST_SIZE];
   __shared__ int s_kind[RT_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, size = a.c.size, lanes = LANES ? LANES : a.lanes;
   RtPlace<W, PAIRS, LANES> place(a);
@@ -611,38 +611,40 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   }
   rt_await<0>();
   if (!sums) return;
+  // (a thread's sum of some tens of products is one of 32 bits; from here on 64: with 32 all the way a weight's gradient was 2e-7 off, now 1e-7)
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    float2 v = rt_floats(acc[i]);
+    const float2 own = rt_floats(acc[i]);
+    double2 v = make_double2(own.x, own.y);
     for (int o = lanes; o < 32; o <<= 1) {
       v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
       v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
     }
-    if (place.slot == 0 && place.in) *reinterpret_cast<float2*>(&s_sums[warp][(i < W / 2 ? place.lo : place.hi - W) + 2 * i]) = v;
+    if (place.slot == 0 && place.in) *reinterpret_cast<double2*>(&s_sums[warp][(i < W / 2 ? place.lo : place.hi - W) + 2 * i]) = v;
   }
   if (lane == 0) s_kind[warp] = kind;
   __syncthreads();
   for (int i = threadIdx.x; i < 2 * size; i += RT_THREADS) {
     const int k = i >= size, e = k ? i - size : i;
-    float v = 0.f;
+    double v = 0.0;
 #pragma unroll
-    for (int j = 0; j < RT_WARPS; ++j) v += s_kind[j] == k ? s_sums[j][e] : 0.f;
+    for (int j = 0; j < RT_WARPS; ++j) v += s_kind[j] == k ? s_sums[j][e] : 0.0;
     a.c.parts[(long long)blockIdx.x * 2 * size + i] = v;
   }
 }
 
 // Sums of the blocks' parts: 32 columns to a block, 32 threads to a column.
 constexpr int RT_SLICES = 32;
-__global__ void __launch_bounds__(32 * RT_SLICES) psgd_rotate_weights_kernel(const float* parts, int blocks, int size, int type, void* queries, void* keys) {
+__global__ void __launch_bounds__(32 * RT_SLICES) psgd_rotate_weights_kernel(const double* parts, int blocks, int size, int type, void* queries, void* keys) {
   psgd_wait_for_predecessor();
-  __shared__ float s_part[RT_SLICES][32];
+  __shared__ double s_part[RT_SLICES][32];
   const int column = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
-  float v = 0.f;
+  double v = 0.0;
   if (column < 2 * size) {
 #pragma unroll
     for (int j = 0; j < (RT_PART_BLOCKS + RT_SLICES - 1) / RT_SLICES; ++j) {
       const int b = j * RT_SLICES + slice;
-      v += b < blocks ? __ldcg(parts + (long long)b * 2 * size + column) : 0.f;
+      v += b < blocks ? __ldcg(parts + (long long)b * 2 * size + column) : 0.0;
     }
   }
   s_part[slice][threadIdx.x & 31] = v;
@@ -653,9 +655,9 @@ __global__ void __launch_bounds__(32 * RT_SLICES) psgd_rotate_weights_kernel(con
   void* out = column < size ? queries : keys;
   const int e = column < size ? column : column - size;
   if (out == nullptr) return;
-  if (type == 0) ((float*)out)[e] = v;
-  else if (type == 1) ((__nv_bfloat16*)out)[e] = __float2bfloat16_rn(v);
-  else ((__half*)out)[e] = __float2half_rn(v);
+  if (type == 0) ((float*)out)[e] = (float)v;
+  else if (type == 1) ((__nv_bfloat16*)out)[e] = __float2bfloat16_rn((float)v);
+  else ((__half*)out)[e] = __float2half_rn((float)v);
 }
 
 // How many warps share `heads` of a row: as few as `most` steps to a warp allow, and more where there are few rows.
@@ -683,7 +685,7 @@ int rt_backward(RtArgs& a, cudaStream_t stream) {
   if (const int code = psgd_allow_shared((const void*)psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, ring, devices)) return code;
   if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, grid, RT_THREADS, ring, stream, 0, a)) return code;
   if (a.c.parts == nullptr) return 0;
-  return psgd_launch(psgd_rotate_weights_kernel, (2 * a.c.size + 31) / 32, 32 * RT_SLICES, 0, stream, 1, (const float*)a.c.parts, grid, a.c.size, a.c.weight_type, a.c.dweight[0],
+  return psgd_launch(psgd_rotate_weights_kernel, (2 * a.c.size + 31) / 32, 32 * RT_SLICES, 0, stream, 1, (const double*)a.c.parts, grid, a.c.size, a.c.weight_type, a.c.dweight[0],
                      a.c.dweight[1]);
 }
 
@@ -728,7 +730,7 @@ int rt_call(const PsgdRotate* call, bool gradient, cudaStream_t stream) {
 
 PSGD_API int psgd_rotate_call_bytes() { return (int)sizeof(PsgdRotate); }
 
-// Floats of scratch for the gradients of weights.
+// Numbers of 64 bits, scratch for the gradients of weights.
 PSGD_API long long psgd_rotate_parts(int size) { return (long long)RT_PART_BLOCKS * 2 * size; }
 
 // `call`: host memory, read before the call returns. Rows that belong to no sequence give zeros.

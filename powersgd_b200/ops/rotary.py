@@ -187,7 +187,7 @@ def _backward(x, q_weight, k_weight, offsets, positions, grads, needs, heads, ke
         if w is not None and needs[1 + i]:
             dweights[i] = torch.empty_like(w) if x.shape[0] else torch.zeros_like(w)
             call.dweight[i] = dweights[i].data_ptr()
-            parts = torch.empty(native.lib().psgd_rotate_parts(x.shape[2]), dtype=torch.float32, device=x.device) if parts is None else parts
+            parts = torch.empty(native.lib().psgd_rotate_parts(x.shape[2]), dtype=torch.float64, device=x.device) if parts is None else parts
             call.parts = parts.data_ptr()
     with native.on_device(x.device) as stream:
         code = native.lib().psgd_rotate_grad(ctypes.byref(call), stream)
