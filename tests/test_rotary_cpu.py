@@ -294,14 +294,44 @@ def test_tangents_and_second_derivatives_are_refused():
         g.sum().backward()
 
 
-def test_no_rows_and_no_values():
+def check_no_rows_and_no_values(device):
     for rows in (0, 1):
-        x = torch.randn(rows, 4, 16, requires_grad=True)
-        w = torch.ones(16, requires_grad=True)
-        q, k, v = rotate_projection(x, 3, 1, positions=torch.arange(rows), q_weight=w, k_weight=w)
+        x = torch.randn(rows, 4, 16, device=device, requires_grad=True)
+        w = torch.ones(16, device=device, requires_grad=True)
+        q, k, v = rotate_projection(x, 3, 1, positions=torch.arange(rows, device=device), q_weight=w, k_weight=w)
         assert v.shape == (rows, 0, 16)
         dx, dw = torch.autograd.grad((q.sum() + k.sum()), (x, w))
         assert dx.shape == x.shape and (rows or (dw == 0).all())
+        assert rotate_heads(x.detach(), offsets=torch.zeros(1, dtype=torch.int32, device=device)).shape == (rows, 4, 16)
+
+
+def test_no_rows_and_no_values():
+    check_no_rows_and_no_values("cpu")
+
+
+def check_one_weight(device):
+    """Only one of the weights is given, or learns; the other's heads are the same as without it."""
+    x, at = values(9, 6, 16, torch.float32, device), torch.arange(9, device=device)
+    w = [torch.linspace(0.5, 2, 16, device=device), torch.linspace(2, 0.5, 16, device=device)]
+    grads = [torch.randn(9, 2, 16, device=device) for _ in range(3)]
+
+    def call(learns, given=(True, True)):
+        leaves = [t.clone().requires_grad_(i in learns) if g else None for i, (t, g) in enumerate(zip(w, given))]
+        out = rotate_projection(x, 2, 2, positions=at, q_weight=leaves[0], k_weight=leaves[1])
+        return out, torch.autograd.grad(out, [leaves[i] for i in learns], grads) if learns else ()
+
+    both = call((0, 1))
+    for i in (0, 1):
+        assert torch.equal(call((i,))[1][0], both[1][i])
+        out, grad = call((i,), given=(i == 0, i == 1))
+        assert torch.equal(out[i], both[0][i]) and torch.equal(grad[0], both[1][i])
+        assert torch.equal(out[1 - i], rotate_heads(x[:, 2 - 2 * i : 4 - 2 * i], positions=at))
+    with torch.inference_mode():
+        assert all(torch.equal(a, b) for a, b in zip(call(())[0], both[0]))
+
+
+def test_one_weight():
+    check_one_weight("cpu")
 
 
 @pytest.mark.parametrize("rotary, qk_norm", [(True, False), (False, True), (True, True)])

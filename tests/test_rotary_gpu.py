@@ -6,7 +6,8 @@ import math
 import pytest
 import torch
 from test_packed_training_cpu import _by_document, _documents
-from test_rotary_cpu import check, check_offsets, check_sizes_at_the_border, check_small, check_some_gradients, exact, places, refused, tangents, values
+from test_rotary_cpu import (check, check_no_rows_and_no_values, check_offsets, check_one_weight, check_sizes_at_the_border, check_small, check_some_gradients, exact,
+                             places, refused, tangents, values)
 
 from powersgd_b200 import AdamW, Config, PowerSGD, clip_grad_norm, optimizer_step
 from powersgd_b200.models import GPT2, GPT2Config
@@ -89,6 +90,11 @@ def test_sizes_at_the_border(form):
 
 def test_small(form):
     check_small("cuda")
+
+
+def test_no_rows_no_values_one_weight(form):
+    check_no_rows_and_no_values("cuda")
+    check_one_weight("cuda")
 
 
 @pytest.mark.parametrize("dtype", TYPES)
