@@ -10,10 +10,15 @@
 // Everything is held in 32 bits; results are rounded to their type once. An angle is a fraction of a turn: the position times the frequency in turns,
 // a number of 64 bits behind the point, whose whole turns fall off by themselves. So it is as exact for far positions as for near ones.
 //
-// A row is a warp's: its lanes find where the row's sequence begins (32 offsets at a time), compute one angle each, hand them round in
+// Forward, a row is a warp's: its lanes find where the row's sequence begins (32 offsets at a time), compute one angle each, hand them round in
 // shared memory, and then take 2 W elements of a head each, W on either side of the pairs, so that a pair lies in one thread. Where there are few
-// rows, several warps share one. All heads of a row turn by the same angles: a sine and a cosine for heads * d / (R / 2) elements.
-// Sums of weight gradients go from threads to warps to blocks to one more launch, always in the same order.
+// rows, several warps share one. All heads of a row turn by the same angles: a sine and a cosine for heads * d / (R / 2) elements. Backward, a warp
+// has the same heads of every row that it comes to, queries or keys, whose weight's gradient it adds up. The sums go from threads to warps to blocks
+// to one more launch, always in the same order. Inputs come by asynchronous copies into a thread's own places in shared memory, some steps ahead.
+//
+// 8192 rows of 16 + 16 heads of 64, bfloat16: forward 14.1 us (67 MB, 4.8 TB/s); backward, with 16 heads of values, 25.9 us (134 MB, 5.2 TB/s) and 2 for the
+// weights. 14336 rows of 32 + 8 heads of 128: forward 49 us (294 MB, 6.0 TB/s). Besides HBM it is the instructions, some 4 to an element and pass, and
+// waiting for shuffles and shared memory: issue is 59 and 58 % busy in the first two.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
