@@ -40,7 +40,7 @@ constexpr int GN_PER_SM = 6;                        // blocks that run at a time
 constexpr int GN_BLOCKS = 148 * GN_PER_SM;          // of a launch, at most
 constexpr int GN_PER_SM_LARGE = 4;                  // for more pieces than GN_LARGE (355 M float32: 633 us and 656 with six; 31.8 M: 65 and 63)
 constexpr long long GN_LARGE = 32768;
-constexpr int GN_CLUSTER = 8, GN_HELD = 8;          // blocks of a short list's one launch, pieces that each holds
+constexpr int GN_CLUSTER = 16, GN_HELD = 4;         // blocks of a short list's one launch, pieces that each holds
 constexpr int GN_SMALL_THREADS = GN_PIECE / 16;
 constexpr int GN_SHORT = 40, GN_LONG = 1200;        // tensors of a launch (28.8 KB of arguments; short lists are launched sooner)
 
@@ -403,8 +403,8 @@ __device__ __forceinline__ void gn_put_back(const GnPiece<T>& p, const uint4& he
   }
 }
 
-// (A perceptron's 0.8 MB: 8.5 us to a program that calls it again and again, 11.4 in two launches, which the host takes longer to make;
-// replayed in a graph 5.6 and 4.2.)
+// (A perceptron's 0.8 MB: 7.1 us to a program that calls it again and again, 8.2 with clusters of 8, 11.4 in two launches, which the host takes longer
+// to make. A megabyte: 7.4, 10.3 and 11.)
 template <int KIND, int MOST>
 __global__ void __launch_bounds__(GN_SMALL_THREADS, 1)
     psgd_grad_small_kernel(const __grid_constant__ GnList<MOST> a, int clip, double max_norm, void* out, int wide) {
@@ -496,6 +496,17 @@ int gn_fill(GnList<MOST>& a, const PsgdNormTensor* list, int count, int& done, i
   return 0;
 }
 
+// Clusters of more than 8 blocks are asked for once per device (one bit each).
+inline int gn_allow_cluster(const void* kernel, unsigned long long& devices) {
+  int device = 0;
+  PSGD_CUDA_OK(cudaGetDevice(&device));
+  const unsigned long long bit = 1ull << (device & 63);
+  if (device < 64 && (__atomic_load_n(&devices, __ATOMIC_RELAXED) & bit) != 0) return 0;
+  PSGD_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  if (device < 64) __atomic_fetch_or(&devices, bit, __ATOMIC_RELAXED);
+  return 0;
+}
+
 template <int KIND, int MOST>
 int gn_run(const PsgdNormTensor* list, int count, int clip, double max_norm, typename GnPart<KIND>::type* parts, void* out, int wide, cudaStream_t stream) {
   typedef const typename GnPart<KIND>::type* Parts;
@@ -506,8 +517,11 @@ int gn_run(const PsgdNormTensor* list, int count, int clip, double max_norm, typ
   for (int done = 0; done < count;) {
     if (const int code = gn_fill(a, list, count, done, grid)) return code;
     if (grid == 0) continue;
-    if (launches == 0 && done == count && a.t[a.count - 1].piece_end <= GN_CLUSTER * GN_HELD)
+    if (launches == 0 && done == count && a.t[a.count - 1].piece_end <= GN_CLUSTER * GN_HELD) {
+      static unsigned long long devices = 0;
+      if (const int code = gn_allow_cluster((const void*)psgd_grad_small_kernel<KIND, MOST>, devices)) return code;
       return psgd_launch_clusters(psgd_grad_small_kernel<KIND, MOST>, GN_CLUSTER, GN_SMALL_THREADS, 0, stream, 0, GN_CLUSTER, a, clip, max_norm, out, wide);
+    }
     if (const int code = psgd_launch(psgd_grad_norm_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 0, a, parts + have, taken, clip && launches == 0 ? most : 0)) return code;
     have += grid;
     ++launches;
