@@ -527,7 +527,7 @@ int gn_run(const PsgdNormTensor* list, int count, int clip, double max_norm, typ
     ++launches;
   }
   if (!clip || launches == 0) return psgd_launch(psgd_grad_norm_total_kernel<KIND>, 1, GN_THREADS, 0, stream, launches > 0, (Parts)parts, have, out, wide);
-  if (launches == 1) return psgd_launch(psgd_grad_clip_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 1, a, (Parts)parts, have, max_norm, taken, out, wide);
+  if (count <= MOST) return psgd_launch(psgd_grad_clip_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 1, a, (Parts)parts, have, max_norm, taken, out, wide);
   for (int done = 0; done < count;) {
     if (const int code = gn_fill(a, list, count, done, grid)) return code;
     if (grid == 0) continue;

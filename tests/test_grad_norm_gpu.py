@@ -35,6 +35,13 @@ def test_long_lists(count, dtypes):
     check(make([(i % 37, i % 11 + 1) for i in range(count)], dtypes, "cuda"), 0.4)
 
 
+@pytest.mark.parametrize("full, empty", [(40, 3), (1200, 1), (1200, 1300), (2400, 1), (3, 1300)])
+@pytest.mark.parametrize("behind", [True, False])
+def test_tensors_without_elements(full, empty, behind):
+    shapes = [[(0,)] * empty, [(70, 100)] * full]
+    check(make(sum(shapes[::-1] if behind else shapes, []), [torch.float32], "cuda"), 0.4)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_ends_of_pieces(dtype):
     """Tensors that end around a piece's end, begin anywhere and lie right behind one another; what is between them stays."""
