@@ -23,14 +23,14 @@ ITEM = np.dtype([("g", "u8"), ("n", "i8"), ("type", "u4"), ("piece_end", "u4")])
 
 def grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:
     """The norm of all gradients of `parameters` as if they were one vector: the root of the sum of squares, or the largest magnitude
-    (`norm_type` infinity). See `clip_grad_norm`."""
+    (`norm_type` infinity). See `clip_grad_norm`; a parameter that is listed twice counts twice, and gradients may lie in each other's memory."""
     return _norm(_listed(parameters), _largest("grad_norm", norm_type), None)
 
 
 def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                    error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the gradients of `parameters` by max_norm / (norm + 1e-6) where that is below one, and returns their norm before that: a tensor without
-    dimensions on their device, float32 (float64 where a gradient is), zero where there are none. As `torch.nn.utils.clip_grad_norm_`, in two launches for the
+    dimensions on their device, float32 (float64 where a gradient is), zero where there are none. As `torch.nn.utils.clip_grad_norm_`, in one launch or two for the
     whole list and without waiting for the GPU.
 
     Gradients are dense, float32, bfloat16, float16 or float64, in one list if need be, of one device, and none lies in another's

@@ -156,17 +156,27 @@ def test_refusals():
     check_refusals("cpu")
 
 
-def layouts(device, dtype=torch.float32):
+def layouts(device):
     """Gradients in other orders of dimensions, with gaps, negated views and zeros that have no memory."""
     params = []
     for g in (torch.randn(6, 10, device=device).t(), torch.randn(8, 6, 3, 3, device=device).contiguous(memory_format=torch.channels_last), torch.randn(20, 30, device=device)[::2, 3:17],
-              torch._neg_view(torch.randn(50, device=device)), torch.randn(101, device=device)[1:]):
-        if not g._is_view() or g.is_neg() or dtype == torch.float32:
-            g = g.to(dtype) if not g.is_neg() else g
+              torch._neg_view(torch.randn(50, device=device)), torch.randn(101, device=device)[1:], torch._efficientzerotensor((5,), device=device)):
         p = torch.nn.Parameter(torch.zeros(g.shape, device=device, dtype=g.dtype))
         p.grad = g
         params.append(p)
     return params
+
+
+def check_counted_twice(device):
+    p = make([(300,)], TYPES[:1], device)[0]
+    twin = torch.nn.Parameter(torch.zeros(100, device=device))
+    twin.grad = p.grad[50:150]
+    norm = exact([p, p, twin], 2)
+    assert abs(grad_norm([p, p, twin]).item() - norm) <= norm * 2.0**-23
+
+
+def test_counted_twice():
+    check_counted_twice("cpu")
 
 
 def test_layouts():

@@ -3,7 +3,7 @@ import math
 
 import pytest
 import torch
-from test_grad_norm_cpu import SHAPES, TYPES, check, check_refusals, exact, layouts, make
+from test_grad_norm_cpu import SHAPES, TYPES, check, check_counted_twice, check_refusals, exact, layouts, make
 
 from powersgd_b200 import AdamW, AllReduce, Config, PowerSGD, clip_grad_norm, grad_norm, optimizer_step
 from powersgd_b200.engine import TrainStep
@@ -69,6 +69,7 @@ def test_layouts(form):
 
 def test_refusals(form):
     check_refusals("cuda")
+    check_counted_twice("cuda")
 
 
 @pytest.mark.parametrize("norm_type", [2.0, math.inf])
