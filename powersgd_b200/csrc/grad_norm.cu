@@ -403,8 +403,8 @@ __device__ __forceinline__ void gn_put_back(const GnPiece<T>& p, const uint4& he
   }
 }
 
-// (A perceptron's 0.8 MB: 7.1 us to a program that calls it again and again, 8.2 with clusters of 8, 11.4 in two launches, which the host takes longer
-// to make. A megabyte: 7.4, 10.3 and 11.)
+// (A perceptron's 0.8 MB: 6.8 us to a program that calls it again and again, 8 with clusters of 8, 11.4 in two launches, which the host takes longer
+// to make. A megabyte: 6.8, 10 and 11. A few KB: 4.7.)
 template <int KIND, int MOST>
 __global__ void __launch_bounds__(GN_SMALL_THREADS, 1)
     psgd_grad_small_kernel(const __grid_constant__ GnList<MOST> a, int clip, double max_norm, void* out, int wide) {
@@ -517,7 +517,7 @@ int gn_run(const PsgdNormTensor* list, int count, int clip, double max_norm, typ
   for (int done = 0; done < count;) {
     if (const int code = gn_fill(a, list, count, done, grid)) return code;
     if (grid == 0) continue;
-    if (launches == 0 && done == count && a.t[a.count - 1].piece_end <= GN_CLUSTER * GN_HELD) {
+    if (launches == 0 && done == count && a.t[a.count - 1].piece_end <= GN_CLUSTER * GN_HELD) {     // (`parts` is null)
       static unsigned long long devices = 0;
       if (const int code = gn_allow_cluster((const void*)psgd_grad_small_kernel<KIND, MOST>, devices)) return code;
       return psgd_launch_clusters(psgd_grad_small_kernel<KIND, MOST>, GN_CLUSTER, GN_SMALL_THREADS, 0, stream, 0, GN_CLUSTER, a, clip, max_norm, out, wide);
@@ -548,8 +548,14 @@ int gn_dispatch(const PsgdNormTensor* list, int count, int clip, double max_norm
 
 PSGD_API int psgd_grad_norm_item_bytes() { return (int)sizeof(PsgdNormTensor); }
 
-// Words of 8 bytes of scratch for a list of `count` tensors.
-PSGD_API long long psgd_grad_norm_parts(int count) { return (GN_BLOCKS + 1ll) * (count <= GN_SHORT ? 1 : (count + GN_LONG - 1) / GN_LONG); }
+// Words of 8 bytes of scratch that a list asks for: none where one launch holds it.
+PSGD_API long long psgd_grad_norm_parts(const void* list, int count) {
+  const PsgdNormTensor* t = (const PsgdNormTensor*)list;
+  long long pieces = 0;
+  for (int i = 0; i < count && pieces <= GN_CLUSTER * GN_HELD; ++i) pieces += gn_pieces(t[i]);
+  if (pieces <= GN_CLUSTER * GN_HELD) return 0;
+  return (GN_BLOCKS + 1ll) * (count <= GN_SHORT ? 1 : (count + GN_LONG - 1) / GN_LONG);
+}
 
 // `list`: host memory, read before the call returns. `largest`: the largest magnitude instead of the root of the sum of squares. `clip`: gradients are
 // scaled where max_norm / (norm + 1e-6) is not at least one. `out`: the norm before that, float, or double where `wide`.

@@ -66,7 +66,7 @@ struct Entry {
                             const void*, const void*, const float*, float*, void*, void*, void*, int*, int*, void*) = nullptr;
   int (*adamw)(const void*, int, int, int, double, const float*, double, double, double, double, double, double, unsigned, int*, void*) = nullptr;
   int (*grad_norm)(const void*, int, int, int, double, double*, void*, int, void*) = nullptr;
-  long long (*grad_norm_parts)(int) = nullptr;
+  long long (*grad_norm_parts)(const void*, int) = nullptr;
   int (*rotate)(const RotateCall*, void*) = nullptr;
   int (*rotate_grad)(const RotateCall*, void*) = nullptr;
   long long (*rotate_parts)(int) = nullptr;
@@ -640,8 +640,9 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
     const c10::cuda::CUDAGuard guard(grads[0]->device());
     const at::NoGradGuard no_grad;
     const auto f64 = at::TensorOptions().device(grads[0]->device()).dtype(at::kDouble);
-    const Tensor out = at::empty({}, f64.dtype(wide ? at::kDouble : at::kFloat)), parts = at::empty({entry.grad_norm_parts((int)items.size())}, f64);
-    check(entry.grad_norm(items.data(), (int)items.size(), largest, clip, max_norm, (double*)parts.data_ptr(), out.data_ptr(), wide, current_stream(out)), "psgd_grad_norm");
+    const long long words = entry.grad_norm_parts(items.data(), (int)items.size());
+    const Tensor out = at::empty({}, f64.dtype(wide ? at::kDouble : at::kFloat)), parts = words ? at::empty({words}, f64) : Tensor();
+    check(entry.grad_norm(items.data(), (int)items.size(), largest, clip, max_norm, words ? (double*)parts.data_ptr() : nullptr, out.data_ptr(), wide, current_stream(out)), "psgd_grad_norm");
     if (clip)   // (the kernel writes behind autograd's back)
       for (const Tensor* g : grads)
         if (!g->is_inference()) g->unsafeGetTensorImpl()->bump_version();

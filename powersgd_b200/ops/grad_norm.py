@@ -108,11 +108,11 @@ def _norm_checked(what: str, parameters: List[torch.Tensor], largest: bool, max_
     items["g"] = np.frombuffer(scan.addresses(laid), dtype=np.uint64)
     items["n"] = [g.numel() for g in laid]
     items["type"] = [DTYPES[g.dtype] for g in laid]
-    device, wide = grads[0].device, any(g.dtype == torch.float64 for g in grads)
+    device, wide, listed = grads[0].device, any(g.dtype == torch.float64 for g in grads), items.tobytes()
     out = torch.empty((), dtype=torch.float64 if wide else torch.float32, device=device)
-    parts = torch.empty(native.lib().psgd_grad_norm_parts(len(laid)), dtype=torch.float64, device=device)
+    parts = torch.empty(native.lib().psgd_grad_norm_parts(listed, len(laid)), dtype=torch.float64, device=device)
     with native.on_device(device) as stream:
-        code = native.lib().psgd_grad_norm(items.tobytes(), len(laid), largest, max_norm is not None, 0.0 if max_norm is None else max_norm, parts.data_ptr(), out.data_ptr(),
+        code = native.lib().psgd_grad_norm(listed, len(laid), largest, max_norm is not None, 0.0 if max_norm is None else max_norm, parts.data_ptr(), out.data_ptr(),
                                            wide, stream)
     native.check(code, "psgd_grad_norm")
     if max_norm is not None:
