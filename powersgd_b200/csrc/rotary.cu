@@ -65,7 +65,7 @@ constexpr float RT_DOWN = 0x1p-70f;                            // for heads whos
 
 struct RtArgs {
   PsgdRotate c;
-  int lanes;                       // of a head: a power of two
+  int lanes;                       // of a head
   int parts[2];                    // warps that share a row's queries, and its keys (a gradient); its queries and keys (forward)
   float share;                     // 1 / size
   unsigned long long frequency[RT_MOST_ANGLES];
@@ -265,9 +265,10 @@ struct __align__(16) RtShared {
 static_assert(RT_MOST_HEADS / RT_STEPS + 2 <= RT_PART_BLOCKS * RT_WARPS, "a warp for each share of a row");
 static_assert(RT_THREADS >= RT_MOST_SIZE, "a thread for each element of a head");
 
-// Eight (or four) floats on a 16-byte boundary of shared memory.
+// Eight, four or two floats of shared memory, on a boundary of 16 bytes or of their size.
 template <int W>
 __device__ __forceinline__ void rt_get(const float* p, RtPair* f) {
+  if (W == 2) f[0] = *reinterpret_cast<const RtPair*>(p);
 #pragma unroll
   for (int i = 0; i < W / 4; ++i) {
     const ulonglong2 v = reinterpret_cast<const ulonglong2*>(p)[i];
@@ -275,31 +276,31 @@ __device__ __forceinline__ void rt_get(const float* p, RtPair* f) {
   }
 }
 
-// A thread's place in a head: W elements from `lo` on and W from `hi` on, which hold W pairs. LANES: of a head, 0: as the call says.
+// A thread's place in a head: W elements from `lo` on and W from `hi` on, which hold W pairs; each of the two lies beside its neighbours' in memory. LANES: of a
+// head, where that is known here, or 0: size / 2 W of them.
 template <int W, bool PAIRS, int LANES>
 struct RtPlace {
   int slot, heads;           // which of the heads that a warp takes at a time
-  int lo, hi, pair;          // and the first of its angles
+  int lo, hi, member;
   bool in, turned;
   RtPair cosine[W / 2], sine[W / 2];
   static __device__ __forceinline__ int lanes(const RtArgs& a) { return LANES ? LANES : a.lanes; }
   __device__ __forceinline__ RtPlace(const RtArgs& a) {
-    const int lane = threadIdx.x & 31, member = lane & (lanes(a) - 1), half = a.c.rotated / 2;
+    const int lane = threadIdx.x & 31, half = a.c.rotated / 2;
     slot = lane / lanes(a);
+    member = lane - slot * lanes(a);
     heads = 32 / lanes(a);
-    pair = member * W;
-    in = 2 * pair < a.c.size;
+    in = slot < heads;
+    lo = member * W;
+    turned = PAIRS || lo < half;
     if (PAIRS) {
-      lo = 2 * pair, hi = lo + W;
-      turned = true;
-    } else if (pair < half) {
-      lo = pair, hi = pair + half;
-      turned = true;
+      hi = lo + a.c.size / 2;
+    } else if (turned) {
+      hi = lo + half;
     } else {
-      lo = a.c.rotated + pair - half, hi = lo + (a.c.size - a.c.rotated) / 2;
-      turned = false;
+      lo += half;
+      hi = lo + (a.c.size - a.c.rotated) / 2;
     }
-    if (!in) lo = hi = pair = 0, turned = false;   // (a lane without elements: zeros, whose weights are not its own)
   }
   // Cosines and sines of a row's angles, by way of the warp's shared memory.
   __device__ __forceinline__ void angles(const RtArgs& a, unsigned long long position, RtShared& shared) {
@@ -310,12 +311,35 @@ struct RtPlace {
       shared.cosine[warp][i] = t.x, shared.sine[warp][i] = t.y;
     }
     __syncwarp();
+    if (PAIRS) {
+      rt_get<W / 2>(shared.cosine[warp] + lo / 2, cosine);
+      rt_get<W / 2>(shared.cosine[warp] + hi / 2, cosine + W / 4);
+      rt_get<W / 2>(shared.sine[warp] + lo / 2, sine);
+      rt_get<W / 2>(shared.sine[warp] + hi / 2, sine + W / 4);
+      return;
+    }
 #pragma unroll
     for (int e = 0; e < W / 2; ++e) cosine[e] = rt_both(1.f), sine[e] = rt_both(0.f);
     if (turned) {
-      rt_get<W>(shared.cosine[warp] + pair, cosine);
-      rt_get<W>(shared.sine[warp] + pair, sine);
+      rt_get<W>(shared.cosine[warp] + lo, cosine);
+      rt_get<W>(shared.sine[warp] + lo, sine);
     }
+  }
+  // Sum over the lanes of a head.
+  __device__ __forceinline__ float sum(float s, int lanes) const {
+    if (LANES && (LANES & (LANES - 1)) == 0) {
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      return s;
+    }
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < (LANES ? LANES : 32); o <<= 1) {      // (what lies `o` on, as long as that is the same head's)
+      if (!LANES && o >= lanes) break;
+      const float t = __shfl_sync(0xffffffffu, s, (lane + o) & 31);
+      s += member + o < lanes ? t : 0.f;
+    }
+    return __shfl_sync(0xffffffffu, s, lane - member);
   }
   // The 2 W elements turned, or turned back.
   template <bool BACK>
@@ -338,15 +362,6 @@ struct RtPlace {
   }
 };
 
-// Sums over the lanes of a head.
-template <int LANES>
-__device__ __forceinline__ void rt_sum(float& s, int lanes) {
-#pragma unroll
-  for (int o = 1; o < (LANES ? LANES : 32); o <<= 1) {
-    if (!LANES && o >= lanes) break;
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-  }
-}
 __device__ __forceinline__ float rt_two(RtPair p) {
   const float2 f = rt_floats(p);
   return f.x + f.y;
@@ -432,16 +447,14 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
     fetch();     // to where the step before this one was read
     const bool key = head >= a.c.heads;
     if (a.c.norm) {
-      float s = rt_two(rt_dot<W>(f, f)), eps = a.c.eps;
-      rt_sum<LANES>(s, lanes);
+      float s = place.sum(rt_two(rt_dot<W>(f, f)), lanes), eps = a.c.eps;
       if (RT_RANGE<T>) {
         const bool large = !(s < 0x1p126f);
         if (__any_sync(0xffffffffu, large)) {
           const RtPair down = rt_both(large ? RT_DOWN : 1.f);
 #pragma unroll
           for (int j = 0; j < W; ++j) f[j] = rt_mul(f[j], down);
-          float t = rt_two(rt_dot<W>(f, f));
-          rt_sum<LANES>(t, lanes);
+          const float t = place.sum(rt_two(rt_dot<W>(f, f)), lanes);
           if (large) s = t, eps *= RT_DOWN * RT_DOWN;
         }
       }
@@ -574,9 +587,8 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
               RtPair along = rt_mul(rt_mul(d[0], w[0]), f[0]);
 #pragma unroll
               for (int j = 1; j < W; ++j) along = rt_fma(rt_mul(d[j], w[j]), f[j], along);
-              s = rt_two(rt_dot<W>(f, f)), t = rt_two(along);
-              rt_sum<LANES>(s, lanes);
-              rt_sum<LANES>(t, lanes);
+              s = place.sum(rt_two(rt_dot<W>(f, f)), lanes);
+              t = place.sum(rt_two(along), lanes);
             };
             float s, t, eps = a.c.eps, down = 1.f;
             dots(s, t);
@@ -621,11 +633,20 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   for (int i = 0; i < W; ++i) {
     const float2 own = rt_floats(acc[i]);
     double2 v = make_double2(own.x, own.y);
-    for (int o = lanes; o < 32; o <<= 1) {
-      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
-      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+    if (LANES && (LANES & (LANES - 1)) == 0) {
+#pragma unroll
+      for (int o = LANES; o < 32; o <<= 1) {
+        v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+        v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+      }
+    } else {
+      const double2 first = v;
+      for (int k = 1; k < place.heads; ++k) {
+        v.x += __shfl_sync(0xffffffffu, first.x, (lane + k * lanes) & 31);
+        v.y += __shfl_sync(0xffffffffu, first.y, (lane + k * lanes) & 31);
+      }
     }
-    if (place.slot == 0 && place.in) *reinterpret_cast<double2*>(&s_sums[warp][(i < W / 2 ? place.lo : place.hi - W) + 2 * i]) = v;
+    if (place.slot == 0) *reinterpret_cast<double2*>(&s_sums[warp][(i < W / 2 ? place.lo : place.hi - W) + 2 * i]) = v;
   }
   if (lane == 0) s_kind[warp] = kind;
   __syncthreads();
@@ -700,17 +721,24 @@ int rt_launch(RtArgs& a, bool gradient, cudaStream_t stream) {
 }
 template <typename T, int W, bool PAIRS>
 int rt_lanes(RtArgs& a, bool gradient, cudaStream_t stream) {
-  a.lanes = 1;
-  while (a.lanes * 2 * W < a.c.size) a.lanes *= 2;
+  a.lanes = a.c.size / (2 * W);
   a.share = 1.f / (float)a.c.size;
+  // Lanes that are known at compile time where heads of 16-bit types are of the usual sizes (bfloat16, 16384 rows of 2048 elements and values, forward and backward:
+  // heads of 32 in 26 and 51 us, 29 and 66 otherwise; of 80 33 and 59, 34 and 71; of 256 28 and 59, 32 and 74; float32, which HBM bounds, takes as long).
   if constexpr (W == 8) {
+    if (a.lanes == 2) return rt_launch<T, W, PAIRS, 2>(a, gradient, stream);
     if (a.lanes == 4) return rt_launch<T, W, PAIRS, 4>(a, gradient, stream);
+    if (a.lanes == 5) return rt_launch<T, W, PAIRS, 5>(a, gradient, stream);
+    if (a.lanes == 6) return rt_launch<T, W, PAIRS, 6>(a, gradient, stream);
     if (a.lanes == 8) return rt_launch<T, W, PAIRS, 8>(a, gradient, stream);
+    if (a.lanes == 16) return rt_launch<T, W, PAIRS, 16>(a, gradient, stream);
   }
   return rt_launch<T, W, PAIRS, 0>(a, gradient, stream);
 }
 template <typename T>
 int rt_dispatch(RtArgs& a, bool gradient, cudaStream_t stream) {
+  // Eight elements on either side of the pairs where both fit into vectors of 16 bytes, else four (bfloat16 heads of 64, forward and backward, 8192 rows: 14 and 26 us,
+  // with four 18 and 40).
   if constexpr (sizeof(T) == 2) {
     if (a.c.size % 16 == 0 && (a.c.pairs || a.c.rotated % 16 == 0)) return a.c.pairs ? rt_lanes<T, 8, true>(a, gradient, stream) : rt_lanes<T, 8, false>(a, gradient, stream);
   }
