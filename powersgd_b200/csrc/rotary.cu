@@ -325,21 +325,37 @@ struct RtPlace {
       rt_get<W>(shared.sine[warp] + lo, sine);
     }
   }
-  // Sum over the lanes of a head.
-  __device__ __forceinline__ float sum(float s, int lanes) const {
+  // Sums over the lanes of a head, N of them side by side (one behind another each would wait for the one before).
+  template <int N>
+  __device__ __forceinline__ void sums(float (&s)[N], int lanes) const {
     if (LANES && (LANES & (LANES - 1)) == 0) {
 #pragma unroll
-      for (int o = 1; o < LANES; o <<= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-      return s;
+      for (int o = 1; o < LANES; o <<= 1) {
+        float t[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = __shfl_xor_sync(0xffffffffu, s[i], o);
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] += t[i];
+      }
+      return;
     }
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int o = 1; o < (LANES ? LANES : 32); o <<= 1) {      // (what lies `o` on, as long as that is the same head's)
       if (!LANES && o >= lanes) break;
-      const float t = __shfl_sync(0xffffffffu, s, (lane + o) & 31);
-      s += member + o < lanes ? t : 0.f;
+      float t[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) t[i] = __shfl_sync(0xffffffffu, s[i], (lane + o) & 31);
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i] += member + o < lanes ? t[i] : 0.f;
     }
-    return __shfl_sync(0xffffffffu, s, lane - member);
+#pragma unroll
+    for (int i = 0; i < N; ++i) s[i] = __shfl_sync(0xffffffffu, s[i], lane - member);
+  }
+  __device__ __forceinline__ float sum(float s, int lanes) const {
+    float one[1] = {s};
+    sums(one, lanes);
+    return one[0];
   }
   // The 2 W elements turned, or turned back.
   template <bool BACK>
@@ -587,8 +603,9 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
               RtPair along = rt_mul(rt_mul(d[0], w[0]), f[0]);
 #pragma unroll
               for (int j = 1; j < W; ++j) along = rt_fma(rt_mul(d[j], w[j]), f[j], along);
-              s = place.sum(rt_two(rt_dot<W>(f, f)), lanes);
-              t = place.sum(rt_two(along), lanes);
+              float two[2] = {rt_two(rt_dot<W>(f, f)), rt_two(along)};
+              place.sums(two, lanes);
+              s = two[0], t = two[1];
             };
             float s, t, eps = a.c.eps, down = 1.f;
             dots(s, t);
