@@ -316,13 +316,12 @@ struct RtPlace {
       rt_get<W / 2>(shared.cosine[warp] + hi / 2, cosine + W / 4);
       rt_get<W / 2>(shared.sine[warp] + lo / 2, sine);
       rt_get<W / 2>(shared.sine[warp] + hi / 2, sine + W / 4);
-      return;
-    }
-#pragma unroll
-    for (int e = 0; e < W / 2; ++e) cosine[e] = rt_both(1.f), sine[e] = rt_both(0.f);
-    if (turned) {
+    } else if (turned) {
       rt_get<W>(shared.cosine[warp] + lo, cosine);
       rt_get<W>(shared.sine[warp] + lo, sine);
+    } else {
+#pragma unroll
+      for (int e = 0; e < W / 2; ++e) cosine[e] = rt_both(1.f), sine[e] = rt_both(0.f);
     }
   }
   // Sums over the lanes of a head, N of them side by side (one behind another each would wait for the one before).
