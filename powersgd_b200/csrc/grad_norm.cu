@@ -42,7 +42,7 @@ constexpr int GN_PER_SM_LARGE = 4;                  // for more pieces than GN_L
 constexpr long long GN_LARGE = 32768;
 constexpr int GN_CLUSTER = 16, GN_HELD = 4;         // blocks of a short list's one launch, pieces that each holds
 constexpr int GN_SMALL_THREADS = GN_PIECE / 16;
-constexpr int GN_SHORT = 40, GN_LONG = 1200;        // tensors of a launch (28.8 KB of arguments; short lists are launched sooner)
+constexpr int GN_SHORT = 40, GN_MIDDLE = 320, GN_LONG = 1200;   // tensors of a launch (28.8 KB of arguments; shorter ones are launched sooner)
 
 template <int MOST>
 struct GnList {
@@ -541,6 +541,7 @@ template <int KIND>
 int gn_dispatch(const PsgdNormTensor* list, int count, int clip, double max_norm, void* parts_at, void* out, int wide, cudaStream_t stream) {
   typename GnPart<KIND>::type* parts = (typename GnPart<KIND>::type*)parts_at;
   if (count <= GN_SHORT) return gn_run<KIND, GN_SHORT>(list, count, clip, max_norm, parts, out, wide, stream);
+  if (count <= GN_MIDDLE) return gn_run<KIND, GN_MIDDLE>(list, count, clip, max_norm, parts, out, wide, stream);
   return gn_run<KIND, GN_LONG>(list, count, clip, max_norm, parts, out, wide, stream);
 }
 
@@ -554,7 +555,7 @@ PSGD_API long long psgd_grad_norm_parts(const void* list, int count) {
   long long pieces = 0;
   for (int i = 0; i < count && pieces <= GN_CLUSTER * GN_HELD; ++i) pieces += gn_pieces(t[i]);
   if (pieces <= GN_CLUSTER * GN_HELD) return 0;
-  return (GN_BLOCKS + 1ll) * (count <= GN_SHORT ? 1 : (count + GN_LONG - 1) / GN_LONG);
+  return (GN_BLOCKS + 1ll) * (count <= GN_LONG ? 1 : (count + GN_LONG - 1) / GN_LONG);
 }
 
 // `list`: host memory, read before the call returns. `largest`: the largest magnitude instead of the root of the sum of squares. `clip`: gradients are
