@@ -610,8 +610,8 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
       PyObject* object = PyList_GET_ITEM(list, i);
       if (!THPVariable_CheckExact(object)) Py_RETURN_NONE;
       const Tensor& p = THPVariable_Unpack(object);
-      if (!p.defined() || at::isTensorSubclassLike(p)) Py_RETURN_NONE;
-      const Tensor& g = p.grad();
+      if (!p.defined()) Py_RETURN_NONE;
+      const Tensor& g = p.unsafeGetTensorImpl()->grad();
       if (!g.defined()) continue;
       if (g.layout() != at::kStrided || !g.unsafeGetTensorImpl()->has_storage() || at::isTensorSubclassLike(g) || g._is_zerotensor() || !g.is_cuda() || has_tangent(g) ||
           !g.is_non_overlapping_and_dense() || (!grads.empty() && g.get_device() != grads[0]->get_device()))
