@@ -446,7 +446,7 @@ variable_list rotate_forward(const Tensor& x0, const Turn& turn, const Tensor& q
   variable_list out = {at::empty({rows, turn.heads, size}, x.options())};
   if (turn.keys > 0) {
     out.push_back(at::empty({rows, turn.keys, size}, x.options()));
-    out.push_back(x0.narrow(1, turn.heads + turn.keys, x0.size(1) - turn.heads - turn.keys));
+    out.push_back(x0.slice(1, turn.heads + turn.keys));
   }
   RotateCall c = rotate_call(x, turn, wq, wk, o, p);
   c.out[0] = out[0].data_ptr();
