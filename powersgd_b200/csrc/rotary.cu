@@ -739,9 +739,15 @@ template <typename T, int W, bool PAIRS>
 int rt_lanes(RtArgs& a, bool gradient, cudaStream_t stream) {
   a.lanes = a.c.size / (2 * W);
   a.share = 1.f / (float)a.c.size;
-  // Lanes that are known at compile time where heads of 16-bit types are of the usual sizes (bfloat16, 16384 rows of 2048 elements and values, forward and backward:
-  // heads of 32 in 26 and 51 us, 29 and 66 otherwise; of 80 33 and 59, 34 and 71; of 256 28 and 59, 32 and 74; float32, which HBM bounds, takes as long).
+  // Lanes that are known at compile time where heads are of the usual sizes (bfloat16, 16384 rows of 2048 elements and values, forward and backward: heads of 16 in 33
+  // and 67 us, 37 and 78 otherwise; of 32 26 and 51, 29 and 66; of 40 33 and 69, 35 and 76; of 72 39 and 84, 41 and 91; of 80 33 and 59, 34 and 71; of 256 28 and 59, 32 and
+  // 74. float32 gains 5 % with 40 and 72, and nothing elsewhere, where HBM bounds it).
+  if constexpr (W == 4) {
+    if (a.lanes == 5) return rt_launch<T, W, PAIRS, 5>(a, gradient, stream);
+    if (a.lanes == 9) return rt_launch<T, W, PAIRS, 9>(a, gradient, stream);
+  }
   if constexpr (W == 8) {
+    if (a.lanes == 1) return rt_launch<T, W, PAIRS, 1>(a, gradient, stream);
     if (a.lanes == 2) return rt_launch<T, W, PAIRS, 2>(a, gradient, stream);
     if (a.lanes == 4) return rt_launch<T, W, PAIRS, 4>(a, gradient, stream);
     if (a.lanes == 5) return rt_launch<T, W, PAIRS, 5>(a, gradient, stream);
