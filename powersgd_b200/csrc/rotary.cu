@@ -22,6 +22,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "psgd_common.cuh"
@@ -51,7 +52,7 @@ namespace {
 
 constexpr int RT_THREADS = 256, RT_WARPS = RT_THREADS / 32;
 constexpr int RT_MOST_SIZE = 256, RT_MOST_ANGLES = RT_MOST_SIZE / 2;
-constexpr int RT_MOST_HEADS = 4096;      // (so that no row is shared by more warps than RT_PART_BLOCKS have)
+constexpr int RT_MOST_HEADS = 4096;      // (so that the fewest warps that can share a row are no more than RT_PART_BLOCKS have)
 constexpr int RT_SMS = 148;
 constexpr int RT_FORWARD_BLOCKS = 4, RT_BACKWARD_BLOCKS = 2;      // of an SM at a time
 constexpr int RT_FORWARD_STAGES = 3;     // steps whose inputs are on their way or read
@@ -702,9 +703,13 @@ __global__ void __launch_bounds__(32 * RT_SLICES) psgd_rotate_weights_kernel(con
   else ((__half*)out)[e] = __float2half_rn((float)v);
 }
 
-// How many warps share `heads` of a row: as few as `most` steps to a warp allow, and more where there are few rows.
-inline int rt_parts(const RtArgs& a, int heads, int most, int warps) {
-  const int step = 32 / a.lanes, steps = (heads + step - 1) / step;
+// How many warps share `heads` of a row: as few as `most` steps to a warp allow, and more where there are few rows, as long as these are `warps` at most.
+inline int rt_steps(const RtArgs& a, int heads) {
+  const int step = 32 / a.lanes;
+  return (heads + step - 1) / step;
+}
+inline int rt_parts(const RtArgs& a, int heads, int most, long long warps) {
+  const int steps = rt_steps(a, heads);
   int parts = (steps + most - 1) / most;
   while (parts < steps && (long long)a.c.rows * (parts + 1) <= warps) ++parts;
   return parts;
@@ -718,8 +723,15 @@ int rt_forward(RtArgs& a, cudaStream_t stream) {
 }
 template <typename T, int W, bool PAIRS, int LANES>
 int rt_backward(RtArgs& a, cudaStream_t stream) {
-  a.parts[0] = rt_parts(a, a.c.heads, RT_STEPS, RT_PART_BLOCKS * RT_WARPS / 2);
-  a.parts[1] = a.c.keys > 0 ? rt_parts(a, a.c.keys, RT_STEPS, RT_PART_BLOCKS * RT_WARPS / 2) : 0;
+  // Half of the warps for either kind, and less where the other kind cannot do with half: every share of a row has a warp of the launch.
+  constexpr long long warps = RT_PART_BLOCKS * RT_WARPS;
+  const auto left = [&](long long others) { return std::min(warps / 2, warps - a.c.rows * others); };
+  a.parts[0] = rt_parts(a, a.c.heads, RT_STEPS, left((rt_steps(a, a.c.keys) + RT_STEPS - 1) / RT_STEPS));
+  a.parts[1] = a.c.keys > 0 ? rt_parts(a, a.c.keys, RT_STEPS, left(a.parts[0])) : 0;
+  if (a.parts[0] + a.parts[1] > warps) {
+    psgd_set_error("psgd_rotate_grad: a row of %d heads of %d wants %d warps", a.c.heads + a.c.keys, a.c.size, a.parts[0] + a.parts[1]);
+    return PSGD_BAD_ARGUMENT;
+  }
   const long long blocks = ((long long)a.c.rows * (a.parts[0] + a.parts[1]) + RT_WARPS - 1) / RT_WARPS;
   const int grid = (int)(blocks < RT_PART_BLOCKS ? blocks : RT_PART_BLOCKS);
   constexpr size_t ring = (size_t)RT_THREADS * (RT_STEPS * 4 * RtVec<T, W>::BYTES + RT_PASSING * 16);
