@@ -82,17 +82,27 @@ void check(int code, const char* what) { TORCH_CHECK(code == 0, what, " failed (
 
 int type_code(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
 
+// Was the memory of a tensor that has elements given back?
+bool without_memory(const Tensor& t) { return t.numel() > 0 && t.unsafeGetTensorImpl()->unsafe_storage().nbytes() == 0; }
+
 const Tensor* plain(PyObject* object) {
   if (!THPVariable_CheckExact(object)) return nullptr;
   const Tensor& t = THPVariable_Unpack(object);
-  if (!t.defined() || t.layout() != at::kStrided || !t.unsafeGetTensorImpl()->has_storage() || at::isTensorSubclassLike(t) || t.is_neg() || t.is_conj()) return nullptr;
+  if (!t.defined() || t.layout() != at::kStrided || !t.unsafeGetTensorImpl()->has_storage() || at::isTensorSubclassLike(t) || t.is_neg() || t.is_conj() || without_memory(t))
+    return nullptr;
   return &t;
 }
 
 // Does the tensor carry a tangent of forward-mode differentiation? Results here would lose it.
 bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
-void refuse_tangents(const variable_list& grads, const char* what) {
-  for (const Tensor& g : grads) TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(g), what, ": forward-mode differentiation is not supported");
+// What a backward pass is handed that its kernels cannot read.
+void refuse_gradients(const variable_list& grads, const char* what) {
+  for (const Tensor& g : grads) {
+    if (!g.defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(g), what, ": forward-mode differentiation is not supported");
+    TORCH_CHECK_TYPE(g._is_zerotensor() || (!at::isTensorSubclassLike(g) && g.unsafeGetTensorImpl()->has_storage()), what, ": a gradient has no memory of its own; plain tensors are supported");
+    TORCH_CHECK(g._is_zerotensor() || !without_memory(g), what, ": the memory of a gradient was given back");
+  }
 }
 
 void* current_stream(const Tensor& t) { return (void*)c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
@@ -179,7 +189,7 @@ struct TokenLogProbs : torch::autograd::Function<TokenLogProbs> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    refuse_tangents(grads, "token_log_probs");
+    refuse_gradients(grads, "token_log_probs");
     const auto saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &targets = saved[1], &stats = saved[2], &entropy = saved[3], &tokens = saved[4];
     Tensor grad;
@@ -337,7 +347,7 @@ struct PackedAttention : torch::autograd::Function<PackedAttention> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    refuse_tangents(grads, "packed_attention");
+    refuse_gradients(grads, "packed_attention");
     const auto saved = ctx->get_saved_variables();
     variable_list result(6);
     {
@@ -471,7 +481,7 @@ struct Rotate : torch::autograd::Function<Rotate> {
   }
 
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    refuse_tangents(grads, "rotate_heads");
+    refuse_gradients(grads, "rotate_heads");
     const auto saved = ctx->get_saved_variables();
     variable_list result(6);
     {
@@ -613,7 +623,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
       if (!p.defined()) Py_RETURN_NONE;
       const Tensor& g = p.unsafeGetTensorImpl()->grad();
       if (!g.defined()) continue;
-      if (g.layout() != at::kStrided || !g.unsafeGetTensorImpl()->has_storage() || at::isTensorSubclassLike(g) || g._is_zerotensor() || !g.is_cuda() || has_tangent(g) ||
+      if (g.layout() != at::kStrided || !g.unsafeGetTensorImpl()->has_storage() || at::isTensorSubclassLike(g) || g._is_zerotensor() || without_memory(g) || !g.is_cuda() || has_tangent(g) ||
           !g.is_non_overlapping_and_dense() || (!grads.empty() && g.get_device() != grads[0]->get_device()))
         Py_RETURN_NONE;
       const int type = g.scalar_type() == at::kDouble ? 3 : type_code(g.scalar_type());

@@ -80,6 +80,8 @@ def lay_like(state: dict, p: torch.Tensor) -> None:
 def check_lists(params, grads, moments, steps, bits: int) -> None:
     names = state_names(bits)
     for i, p in enumerate(params):
+        if p.is_cuda:
+            native.refuse_without_memory("AdamW", p, grads[i], steps[i], *(m[i] for m in moments))
         if p.dtype not in DTYPES:
             raise TypeError(f"AdamW: parameter {i} is {p.dtype}; float32, bfloat16 and float16 are supported")
         if not in_one_piece(p):

@@ -50,6 +50,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
 def check(q, k, v, offsets, scale) -> None:
     native.refuse_tracing("packed_attention", q)
+    if q.is_cuda:
+        native.refuse_without_memory("packed_attention", q, k, v, offsets)
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError(f"packed_attention: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together; [tokens, heads, size] is expected")
     heads, groups, size = q.shape[1], k.shape[1], q.shape[2]
@@ -182,6 +184,8 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        if grad.is_cuda:
+            native.refuse_without_memory("packed_attention", grad)
         native.refuse_tangents("packed_attention", grad)
         q, k, v, offsets, out, lse, rest = ctx.saved_tensors
         return (*_backward(q, k, v, offsets, out, lse, rest, grad, ctx.causal, ctx.scale), None, None, None)

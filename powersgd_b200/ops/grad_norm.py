@@ -33,7 +33,7 @@ def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_
     dimensions on their device, float32 (float64 where a gradient is), zero where there are none. As `torch.nn.utils.clip_grad_norm_`, in one launch or two for the
     whole list and without waiting for the GPU.
 
-    Gradients are dense, float32, bfloat16, float16 or float64, in one list if need be, of one device, and none lies in another's
+    Gradients are plain tensors (no DTensors), dense, float32, bfloat16, float16 or float64, in one list if need be, of one device, and none lies in another's
     memory (a parameter is listed once). Those that do not lie in one piece are copied to and fro. Squares are added in float64; a
     gradient is rounded once. Where the norm is no number all gradients become NaN, where it is infinite finite ones become zero:
     with `error_if_nonfinite` a RuntimeError is raised instead and nothing is changed; it waits for the GPU.
@@ -55,7 +55,7 @@ def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_
 
 def clip_for_step(parameters: Iterable[torch.Tensor], max_norm: float) -> torch.Tensor:
     """What a training loop of this package clips with: `clip_grad_norm` on the GPU. Gradients on the CPU, and lists that it refuses (complex
-    gradients, several devices), go to the library, which refuses sparse ones too."""
+    gradients, DTensors, several devices), go to the library, which refuses sparse ones too."""
     listed = _listed(parameters)
     if any(p.is_cuda for p in listed):
         try:
@@ -89,6 +89,8 @@ def _norm_checked(what: str, parameters: List[torch.Tensor], largest: bool, max_
     grads = [p.grad for p in parameters if p.grad is not None]
     if not grads:
         return torch.zeros((), device=parameters[0].device if parameters else None)
+    native.refuse_tracing(what, grads[0])
+    native.refuse_without_memory(what, *grads)
     for i, g in enumerate(grads):
         if g.layout != torch.strided:
             raise TypeError(f"{what}: gradient {i} is {g.layout}; dense gradients are supported")
@@ -97,7 +99,6 @@ def _norm_checked(what: str, parameters: List[torch.Tensor], largest: bool, max_
         if g.device != grads[0].device:
             raise ValueError(f"{what}: gradients on {grads[0].device} and {g.device}")
     native.refuse_tangents(what, *grads)
-    native.refuse_tracing(what, grads[0])
     if max_norm is not None:
         _refuse_overlaps(what, grads)
     if not (grads[0].is_cuda and native.use_for_cuda()):

@@ -89,6 +89,22 @@ def refuse_tracing(what: str, t: torch.Tensor) -> None:
         raise NotImplementedError(f"{what}: torch.jit.trace does not see native calls")
 
 
+def wrapper(t) -> bool:
+    """Does Python take this tensor's operations over (a DTensor, a FakeTensor)? What it stands for lies elsewhere, and its own address is zero."""
+    return type(t).__torch_dispatch__ is not torch.Tensor.__torch_dispatch__
+
+
+def refuse_without_memory(what: str, *tensors) -> None:
+    """Kernels read memory at a tensor's address: asked before any address is. (None, and tensors that only say that they are zero, pass.)"""
+    for t in tensors:
+        if t is None:
+            continue
+        if wrapper(t):
+            raise TypeError(f"{what}: a {type(t).__name__} has no memory of its own; plain tensors are supported")
+        if torch._C._has_storage(t) and t.layout == torch.strided and not t._is_zerotensor() and t.numel() > 0 and t.untyped_storage().nbytes() == 0:
+            raise RuntimeError(f"{what}: the memory of a tensor {tuple(t.shape)} was given back")
+
+
 def in_memory(t: torch.Tensor) -> torch.Tensor:
     """The numbers that a tensor stands for: some only say that what they refer to is to be negated (the imaginary part of a conjugate),
     or that all of it is zero. Kernels read memory."""

@@ -78,6 +78,7 @@ def _rotate(what, x, heads, keys, offsets, positions, q_weight, k_weight, eps, b
 
 def check(what, x, heads, keys, offsets, positions, q_weight, k_weight, eps, base, rotated) -> None:
     native.refuse_tracing(what, x)
+    native.refuse_without_memory(what, x, q_weight, k_weight, offsets, positions)
     if x.dim() != 3:
         raise ValueError(f"{what}: {tuple(x.shape)}; [rows, heads, size] is expected")
     rows, have, size = x.shape
@@ -206,6 +207,7 @@ class _Rotate(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, *grads):
+        native.refuse_without_memory("rotate_heads", *grads)
         native.refuse_tangents("rotate_heads", *grads)
         return (*_backward(*ctx.saved_tensors, grads, ctx.needs_input_grad, *ctx.arguments), *[None] * (2 + len(ctx.arguments)))
 

@@ -11,6 +11,7 @@ import torch
 
 from ..csrc.build import SCAN_LIB, scan_target
 from ..utils import is_dense, same_layout
+from .native import wrapper
 
 
 def _load(path: str = SCAN_LIB):
@@ -33,18 +34,26 @@ def _words(values) -> bytes:
     return np.array(list(values), dtype=np.uint64).tobytes()
 
 
+def _address(t: Optional[torch.Tensor]) -> int:
+    if t is None:
+        return 0
+    if t.is_cuda and wrapper(t):
+        raise TypeError(f"a {type(t).__name__} has no memory of its own; plain tensors are supported")
+    return t.data_ptr()
+
+
 def addresses(tensors: Optional[Sequence[Optional[torch.Tensor]]]) -> Optional[bytes]:
     """The addresses of a list, 8 bytes each (0 for None); None for no list."""
     if tensors is None:
         return None
     key = _native.addresses(tensors) if _native is not None else None
-    return _words(0 if t is None else t.data_ptr() for t in tensors) if key is None else key
+    return _words(_address(t) for t in tensors) if key is None else key
 
 
 def grad_addresses(params: Sequence[torch.Tensor]) -> bytes:
     """The addresses of the parameters' gradients."""
     key = _native.grad_addresses(params) if _native is not None else None
-    return _words(p.grad.data_ptr() for p in params) if key is None else key
+    return _words(_address(p.grad) for p in params) if key is None else key
 
 
 def sizes(tensors: Sequence[torch.Tensor]) -> bytes:

@@ -48,6 +48,8 @@ def token_log_probs(logits: torch.Tensor, targets: torch.Tensor, *, top: int = 0
 
 def check(logits, targets, top, ignore_index, temperature) -> None:
     native.refuse_tracing("token_log_probs", logits)
+    if logits.is_cuda:
+        native.refuse_without_memory("token_log_probs", logits, targets)
     if logits.dtype not in DTYPES and not (logits.dtype == torch.float64 and not logits.is_cuda):
         raise TypeError(f"token_log_probs: logits are {logits.dtype}; float32, bfloat16 and float16 are supported")
     if targets.dtype not in (torch.int64, torch.int32):
@@ -165,6 +167,8 @@ class _TokenLogProbs(torch.autograd.Function):
     def backward(ctx, g, g_entropy, g_top, _):
         native.refuse_tangents("token_log_probs", g, g_entropy, g_top)
         logits, targets, stats, entropy, tokens = ctx.saved_tensors
+        if logits.is_cuda:
+            native.refuse_without_memory("token_log_probs", g, g_entropy, g_top)
         if g is None and g_entropy is None and g_top is None:
             return (None,) * 6
         if g_entropy is None:
