@@ -612,6 +612,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
     const Py_ssize_t count = PyList_GET_SIZE(list);
     std::vector<NormItem> items;
     std::vector<const Tensor*> grads;
+    std::optional<c10::cuda::CUDAGuard> guard;
     items.reserve(count);
     grads.reserve(count);
     bool wide = false, sorted = true;
@@ -629,7 +630,9 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
       const int type = g.scalar_type() == at::kDouble ? 3 : type_code(g.scalar_type());
       if (type < 0) Py_RETURN_NONE;
       wide = wide || type == 3;
-      const uint64_t at = (uint64_t)g.const_data_ptr();
+      if (grads.empty()) guard.emplace(g.device());
+      // (where it is written, a tensor that shares its memory until then is given its own)
+      const uint64_t at = clip ? (uint64_t)g.mutable_data_ptr() : (uint64_t)g.const_data_ptr();
       if (g.numel() > 0) {
         sorted = sorted && at >= end;
         end = at + (uint64_t)g.numel() * g.element_size();
@@ -647,7 +650,6 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
       for (size_t i = 1; i < places.size(); ++i)
         if (places[i].first < places[i - 1].second) Py_RETURN_NONE;
     }
-    const c10::cuda::CUDAGuard guard(grads[0]->device());
     const at::NoGradGuard no_grad;
     const auto f64 = at::TensorOptions().device(grads[0]->device()).dtype(at::kDouble);
     const long long words = entry.grad_norm_parts(items.data(), (int)items.size());
