@@ -57,6 +57,7 @@ constexpr int RT_SMS = 148;
 constexpr int RT_FORWARD_BLOCKS = 4, RT_BACKWARD_BLOCKS = 2;      // of an SM at a time
 constexpr int RT_FORWARD_STAGES = 3;     // steps whose inputs are on their way or read
 constexpr int RT_STEPS = 2;              // of a warp, gradients
+constexpr int RT_SUMMED = 32;            // rows of a warp whose products, RT_STEPS to a row, a thread adds up in 32 bits
 constexpr int RT_PASSING = 2;            // vectors of values of a thread that pass by with them
 // Do the squares of a type leave the range of float32?
 template <typename T>
@@ -504,7 +505,6 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   constexpr int HALF = RT_THREADS * Vec::BYTES, STEP = 4 * HALF, N = 16 / (int)sizeof(T);
   extern __shared__ __align__(16) char ring[];
   __shared__ RtShared shared;
-  __shared__ __align__(16) double s_sums[RT_WARPS][RT_MOST_SIZE];
   __shared__ int s_kind[RT_WARPS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, size = a.c.size, lanes = LANES ? LANES : a.lanes;
   RtPlace<W, PAIRS, LANES> place(a);
@@ -522,6 +522,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   // values: 16 bytes at a time, RT_PASSING of them by way of shared memory as well
   const int all = a.c.heads + a.c.keys + a.c.values, vectors = size / N, passing = a.c.dx != nullptr ? a.c.values * vectors : 0;
   char* const values = ring + RT_STEPS * STEP + threadIdx.x * 16;
+  double2* const wide = reinterpret_cast<double2*>(ring + RT_STEPS * STEP + RT_PASSING * RT_THREADS * 16) + threadIdx.x;      // a thread's sums
   const bool valued = a.c.grad[2] != nullptr;
   const T* gv = valued ? (const T*)a.c.grad[2] + (long long)row * a.c.grad_row[2] : x;
   long long passed[RT_PASSING];
@@ -557,99 +558,115 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   const float* weight = shared.weight[kind] + place.lo;
   RtPair acc[W];
 #pragma unroll
-  for (int i = 0; i < W; ++i) acc[i] = 0;
+  for (int i = 0; i < W; ++i) {
+    acc[i] = 0;
+    wide[i * RT_THREADS] = make_double2(0.0, 0.0);
+  }
+  // A thread's sum of the products of RT_SUMMED rows at most is one of 32 bits, of any more of 64 (with 32 all the way a weight's gradient was 2e-7 off for 8192 rows,
+  // now 1e-7, and up to 5e-6 for 4 M of them; the sums of 64 wait in shared memory).
 #pragma unroll 1
-  for (; row < a.c.rows; row = ahead) {
-    ahead = stride < a.c.rows - row ? row + stride : a.c.rows;
-    x += x_stride;
-    g += g_stride;
-    gv += gv_stride;
-    unsigned long long position;
-    const bool held = positions.of(a.c, row, position);
-    if (a.c.rotated > 0) place.angles(a, position, shared);
+  do {
+#pragma unroll 1
+    for (int left = RT_SUMMED; left > 0 && row < a.c.rows; --left, row = ahead) {
+      ahead = stride < a.c.rows - row ? row + stride : a.c.rows;
+      x += x_stride;
+      g += g_stride;
+      gv += gv_stride;
+      unsigned long long position;
+      const bool held = positions.of(a.c, row, position);
+      if (a.c.rotated > 0) place.angles(a, position, shared);
 #pragma unroll
-    for (int i = 0; i < RT_STEPS; ++i) {
-      rt_await<RT_STEPS - 1>();
-      if (i == 0 && passing > 0) {     // values pass by
-        T* o = (T*)a.c.dx + ((long long)row * all + a.c.heads + a.c.keys) * size;
+      for (int i = 0; i < RT_STEPS; ++i) {
+        rt_await<RT_STEPS - 1>();
+        if (i == 0 && passing > 0) {     // values pass by
+          T* o = (T*)a.c.dx + ((long long)row * all + a.c.heads + a.c.keys) * size;
 #pragma unroll
-        for (int j = 0; j < RT_PASSING; ++j) {
-          const int e = (j * parts + part) * 32 + lane;
-          if (e < passing) *reinterpret_cast<uint4*>(o + e * N) = *reinterpret_cast<const uint4*>(values + j * RT_THREADS * 16);
+          for (int j = 0; j < RT_PASSING; ++j) {
+            const int e = (j * parts + part) * 32 + lane;
+            if (e < passing) *reinterpret_cast<uint4*>(o + e * N) = *reinterpret_cast<const uint4*>(values + j * RT_THREADS * 16);
+          }
+          for (int e = (RT_PASSING * parts + part) * 32 + lane; e < passing; e += 32 * parts) {
+            const int h = e / vectors;
+            *reinterpret_cast<uint4*>(o + e * N) =
+                valued ? __ldcs(reinterpret_cast<const uint4*>(gv - gv_stride + h * a.c.grad_head[2] + (e - h * vectors) * N)) : make_uint4(0, 0, 0, 0);
+          }
         }
-        for (int e = (RT_PASSING * parts + part) * 32 + lane; e < passing; e += 32 * parts) {
-          const int h = e / vectors;
-          *reinterpret_cast<uint4*>(o + e * N) =
-              valued ? __ldcs(reinterpret_cast<const uint4*>(gv - gv_stride + h * a.c.grad_head[2] + (e - h * vectors) * N)) : make_uint4(0, 0, 0, 0);
-        }
-      }
-      if (i < count) {
-        RtPair f[W], d[W];
-        {
-          Vec raw[4];
+        if (i < count) {
+          RtPair f[W], d[W];
+          {
+            Vec raw[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) raw[j].get(mine + i * STEP + j * HALF);
-          raw[0].unpack(f), raw[1].unpack(f + W / 2);
-          raw[2].unpack(d), raw[3].unpack(d + W / 2);
-        }
-        fetch(i);
-        if (held) {
-          if (a.c.rotated > 0) place.template turn<true>(d);
-          if (a.c.norm) {
-            RtPair w[W];
-            rt_get<W>(weight, w);
-            rt_get<W>(weight + apart, w + W / 2);
-            const auto dots = [&](float& s, float& t) {
-              RtPair along = rt_mul(rt_mul(d[0], w[0]), f[0]);
+            for (int j = 0; j < 4; ++j) raw[j].get(mine + i * STEP + j * HALF);
+            raw[0].unpack(f), raw[1].unpack(f + W / 2);
+            raw[2].unpack(d), raw[3].unpack(d + W / 2);
+          }
+          fetch(i);
+          if (held) {
+            if (a.c.rotated > 0) place.template turn<true>(d);
+            if (a.c.norm) {
+              RtPair w[W];
+              rt_get<W>(weight, w);
+              rt_get<W>(weight + apart, w + W / 2);
+              const auto dots = [&](float& s, float& t) {
+                RtPair along = rt_mul(rt_mul(d[0], w[0]), f[0]);
 #pragma unroll
-              for (int j = 1; j < W; ++j) along = rt_fma(rt_mul(d[j], w[j]), f[j], along);
-              float two[2] = {rt_two(rt_dot<W>(f, f)), rt_two(along)};
-              place.sums(two, lanes);
-              s = two[0], t = two[1];
-            };
-            float s, t, eps = a.c.eps, down = 1.f;
-            dots(s, t);
-            if (RT_RANGE<T>) {
-              const bool large = !(s < 0x1p126f);
-              if (__any_sync(0xffffffffu, large)) {
-                const RtPair less = rt_both(large ? RT_DOWN : 1.f);
+                for (int j = 1; j < W; ++j) along = rt_fma(rt_mul(d[j], w[j]), f[j], along);
+                float two[2] = {rt_two(rt_dot<W>(f, f)), rt_two(along)};
+                place.sums(two, lanes);
+                s = two[0], t = two[1];
+              };
+              float s, t, eps = a.c.eps, down = 1.f;
+              dots(s, t);
+              if (RT_RANGE<T>) {
+                const bool large = !(s < 0x1p126f);
+                if (__any_sync(0xffffffffu, large)) {
+                  const RtPair less = rt_both(large ? RT_DOWN : 1.f);
 #pragma unroll
-                for (int j = 0; j < W; ++j) f[j] = rt_mul(f[j], less);
-                dots(s, t);
-                if (large) eps *= RT_DOWN * RT_DOWN, down = RT_DOWN;
+                  for (int j = 0; j < W; ++j) f[j] = rt_mul(f[j], less);
+                  dots(s, t);
+                  if (large) eps *= RT_DOWN * RT_DOWN, down = RT_DOWN;
+                }
+              }
+              const float r = rsqrtf(fmaf(s, a.share, eps));
+              const RtPair r2 = rt_both(r), rd = rt_both(r * down), along = rt_both(-t * r * a.share);     // - mean(dn n)
+#pragma unroll
+              for (int j = 0; j < W; ++j) {
+                const RtPair n = rt_mul(f[j], r2);
+                acc[j] = rt_fma(d[j], n, acc[j]);
+                d[j] = rt_mul(rt_fma(n, along, rt_mul(d[j], w[j])), rd);
               }
             }
-            const float r = rsqrtf(fmaf(s, a.share, eps));
-            const RtPair r2 = rt_both(r), rd = rt_both(r * down), along = rt_both(-t * r * a.share);     // - mean(dn n)
+          } else {
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-              const RtPair n = rt_mul(f[j], r2);
-              acc[j] = rt_fma(d[j], n, acc[j]);
-              d[j] = rt_mul(rt_fma(n, along, rt_mul(d[j], w[j])), rd);
-            }
+            for (int j = 0; j < W; ++j) d[j] = 0;
+          }
+          if (place.in && a.c.dx != nullptr && head + i * step < have) {
+            T* o = dx + i * step * size;
+            Vec::store(o, d);
+            Vec::store(o + apart, d + W / 2);
           }
         } else {
-#pragma unroll
-          for (int j = 0; j < W; ++j) d[j] = 0;
+          rt_fetched();
         }
-        if (place.in && a.c.dx != nullptr && head + i * step < have) {
-          T* o = dx + i * step * size;
-          Vec::store(o, d);
-          Vec::store(o + apart, d + W / 2);
-        }
-      } else {
-        rt_fetched();
       }
+      dx += dx_stride;
     }
-    dx += dx_stride;
-  }
+    if (!sums) continue;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float2 own = rt_floats(acc[i]);
+      const double2 before = wide[i * RT_THREADS];
+      wide[i * RT_THREADS] = make_double2(before.x + own.x, before.y + own.y);
+      acc[i] = 0;
+    }
+  } while (row < a.c.rows);
   rt_await<0>();
   if (!sums) return;
-  // (a thread's sum of some tens of products is one of 32 bits; from here on 64: with 32 all the way a weight's gradient was 2e-7 off, now 1e-7)
+  __syncthreads();       // (the ring, where the warps' sums go, is free)
+  double(*const s_sums)[RT_MOST_SIZE] = reinterpret_cast<double(*)[RT_MOST_SIZE]>(ring);
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    const float2 own = rt_floats(acc[i]);
-    double2 v = make_double2(own.x, own.y);
+    double2 v = wide[i * RT_THREADS];
     if (LANES && (LANES & (LANES - 1)) == 0) {
 #pragma unroll
       for (int o = LANES; o < 32; o <<= 1) {
@@ -734,7 +751,8 @@ int rt_backward(RtArgs& a, cudaStream_t stream) {
   }
   const long long blocks = ((long long)a.c.rows * (a.parts[0] + a.parts[1]) + RT_WARPS - 1) / RT_WARPS;
   const int grid = (int)(blocks < RT_PART_BLOCKS ? blocks : RT_PART_BLOCKS);
-  constexpr size_t ring = (size_t)RT_THREADS * (RT_STEPS * 4 * RtVec<T, W>::BYTES + RT_PASSING * 16);
+  constexpr size_t ring = (size_t)RT_THREADS * (RT_STEPS * 4 * RtVec<T, W>::BYTES + RT_PASSING * 16 + W * sizeof(double2));
+  static_assert(RT_STEPS * 4 * RtVec<T, W>::BYTES >= RT_MOST_SIZE / 32 * (int)sizeof(double), "room for the warps' sums");
   static unsigned long long devices = 0;
   if (const int code = psgd_allow_shared((const void*)psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, ring, devices)) return code;
   if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, grid, RT_THREADS, ring, stream, 0, a)) return code;

@@ -1,4 +1,4 @@
-"""Rows that more warps would share than a launch of gradients has."""
+"""Rows that more warps would share than a launch of gradients has, weights' gradients of many rows."""
 import pytest
 import torch
 from test_rotary_cpu import check, values
@@ -24,3 +24,15 @@ def test_queries_and_keys_share_the_warps_of_a_launch(form, rows, heads, keys, v
     """Each kind alone may take half of the warps and more; both together have to find room."""
     torch.empty(rows, heads + keys + values_, size, device="cuda").fill_(float("nan"))     # (what an output that is not written may hold)
     check(values(rows, heads + keys + values_, size, torch.float32, "cuda"), heads, keys, lengths=[rows])
+
+
+@pytest.mark.parametrize("rows, heads", [(2**22, 1), (2**20, 4), (2**19, 40)])
+def test_weights_gradients_of_many_rows(form, rows, heads):
+    """Products that are all 1 + 2^-17: up to 64 of them add up exactly in 32 bits, and any number in 64, while a sum of 32 bits loses the 2^-17 from 128 on. What
+    is left of a bound is the reciprocal root of one, two steps of 2^-23, and the last rounding."""
+    x = torch.ones(rows, heads, 8, device="cuda")
+    w = torch.ones(8, device="cuda", requires_grad=True)
+    z = rotate_heads(x, weight=w, eps=2.0**-100, rotated=0)
+    got, = torch.autograd.grad(z, w, torch.full_like(z, 1 + 2.0**-17))
+    want = rows * heads * (1 + 2.0**-17)
+    assert ((got.double() - want).abs() <= want * (2 * 2.0**-23 + 2.0**-24)).all(), (got.double() / want - 1).abs().max().item()
