@@ -21,6 +21,7 @@
 // waiting for shuffles and shared memory: issue is 59 and 58 % busy in the first two.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <math_constants.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -617,8 +618,8 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
               };
               float s, t, eps = a.c.eps, down = 1.f;
               dots(s, t);
-              if (RT_RANGE<T>) {
-                const bool large = !(s < 0x1p126f);
+              if (RT_RANGE<T>) {     // (where only products with gradients leave the range, their heads are large enough to be made smaller)
+                const bool large = !(s < 0x1p126f && fabsf(t) < CUDART_INF_F);
                 if (__any_sync(0xffffffffu, large)) {
                   const RtPair less = rt_both(large ? RT_DOWN : 1.f);
 #pragma unroll

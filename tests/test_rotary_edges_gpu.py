@@ -36,3 +36,16 @@ def test_weights_gradients_of_many_rows(form, rows, heads):
     got, = torch.autograd.grad(z, w, torch.full_like(z, 1 + 2.0**-17))
     want = rows * heads * (1 + 2.0**-17)
     assert ((got.double() - want).abs() <= want * (2 * 2.0**-23 + 2.0**-24)).all(), (got.double() / want - 1).abs().max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_gradients_of_large_heads(form, dtype):
+    """Products of a gradient and a head leave the range of float32; what they are the mean of, over the head's norm, does not. The same numbers times powers of two
+    give the same but for numbers below 2^-126, which are far below a head's largest, and a rounding to the type: the bound leaves room for more."""
+    x, g = values(9, 4, 64, dtype, "cuda") * 2.0**50, values(9, 4, 64, dtype, "cuda", seed=1) * 2.0**100
+    one, two = ((x * s).requires_grad_() for s in (1.0, 2.0**-50))
+    at = torch.arange(9, device="cuda")
+    a, = torch.autograd.grad(rotate_heads(one, positions=at, eps=2.0**-100), one, g)
+    b, = torch.autograd.grad(rotate_heads(two, positions=at, eps=2.0**-100), two, g * 2.0**-100)
+    assert a.isfinite().all()
+    assert ((a.double() * 2.0**-50 - b.double()).abs() <= b.double().abs().amax(-1, keepdim=True) * (2.0**-18 + torch.finfo(dtype).eps)).all()
