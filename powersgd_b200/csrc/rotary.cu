@@ -8,7 +8,8 @@
 //   dw = sum over rows and heads of dy n        dx = r (dn - n mean(dn n)),  dn = dy w
 //
 // Everything is held in 32 bits; results are rounded to their type once. An angle is a fraction of a turn: the position times the frequency in turns,
-// a number of 64 bits behind the point, whose whole turns fall off by themselves. So it is as exact for far positions as for near ones.
+// a number of 64 bits behind the point, whose whole turns fall off by themselves. What is left of an angle is
+// off by |position| 2^-65 turns, which the rounding of its frequency leaves (less than a float32's rounding up to 2^38), and by 2^-32 that are cut off.
 //
 // Forward, a row is a warp's: its lanes find where the row's sequence begins (32 offsets at a time), compute one angle each, hand them round in
 // shared memory, and then take 2 W elements of a head each, W on either side of the pairs, so that a pair lies in one thread. Where there are few

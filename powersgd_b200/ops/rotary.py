@@ -43,8 +43,9 @@ def rotate_heads(x: torch.Tensor, *, offsets: Optional[torch.Tensor] = None, pos
     norm. `weight`: [size], float32 or of the type of x; None: ones.
 
     Positions come from `offsets` (int32, [sequences + 1], as `packed_attention` takes them: a sequence's rows are counted from zero; rows that
-    belong to no sequence give zeros, whatever they hold) or from `positions` (int32 or int64, [rows], below zero too). Both are read by the kernels and not by the host, and
-    as exact far out as near zero. Without a rotation neither is needed.
+    belong to no sequence give zeros, whatever they hold) or from `positions` (int32 or int64, [rows], below zero too). Both are read by the kernels and not by the host. Without a
+    rotation neither is needed. Angles are off by |position| * 2^-65 turns, in float32 and less by 2^-32 more: for positions up to 2^38 (some 2.7e11) less than a float32's rounding, 1.7e-4 radians at
+    10^15, and of no meaning from some 2^60 on.
 
     Differentiable (once, backwards) in x and weight. The result and the gradients are the same in every run. `x` may be a view; rows and
     heads that do not begin on 16-byte boundaries are copied first. A head that holds what is no number is spoiled, and with it the weight's gradient."""

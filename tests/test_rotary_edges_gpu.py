@@ -1,7 +1,8 @@
-"""Rows that more warps would share than a launch of gradients has, weights' gradients of many rows."""
+"""Rows that more warps would share than a launch of gradients has, weights' gradients of many rows, products that leave the range, far positions."""
 import pytest
 import torch
 from test_rotary_cpu import check, values
+from test_rotary_edges_cpu import check_far
 
 from powersgd_b200.ops import host, rotary
 from powersgd_b200.ops.rotary import rotate_heads
@@ -49,3 +50,9 @@ def test_large_gradients_of_large_heads(form, dtype):
     b, = torch.autograd.grad(rotate_heads(two, positions=at, eps=2.0**-100), two, g * 2.0**-100)
     assert a.isfinite().all()
     assert ((a.double() * 2.0**-50 - b.double()).abs() <= b.double().abs().amax(-1, keepdim=True) * (2.0**-18 + torch.finfo(dtype).eps)).all()
+
+
+@pytest.mark.parametrize("rotated, interleaved, base", [(16, False, 10000.0), (64, True, 10000.0), (128, False, 500000.0), (8, False, 1.0)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_far_positions(form, dtype, rotated, interleaved, base):
+    check_far(dtype, rotated, interleaved, base, "cuda")
