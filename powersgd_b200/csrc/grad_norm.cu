@@ -496,15 +496,36 @@ int gn_fill(GnList<MOST>& a, const PsgdNormTensor* list, int count, int& done, i
   return 0;
 }
 
-// Clusters of more than 8 blocks are asked for once per device (one bit each).
-inline int gn_allow_cluster(const void* kernel, unsigned long long& devices) {
+// Does the current device run a cluster of a short list's blocks? (16 of them on one group's SMs are more than every device, or every part of one, has.)
+template <int KIND, int MOST>
+bool gn_runs_cluster() {
+  const auto kernel = psgd_grad_small_kernel<KIND, MOST>;
+  cudaLaunchConfig_t cfg;
+  cudaLaunchAttribute attrs[2];
+  psgd_launch_config(cfg, attrs, GN_CLUSTER, GN_SMALL_THREADS, 0, nullptr, 0, GN_CLUSTER);
+  int clusters = 0;
+  const bool runs = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+                    cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters > 0;
+  if (!runs) (void)cudaGetLastError();
+  return runs;
+}
+// Asked once per device (one bit each).
+template <int MOST>
+bool gn_runs_short() {
+  static unsigned long long asked = 0, runs = 0;
   int device = 0;
-  PSGD_CUDA_OK(cudaGetDevice(&device));
+  if (cudaGetDevice(&device) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
   const unsigned long long bit = 1ull << (device & 63);
-  if (device < 64 && (__atomic_load_n(&devices, __ATOMIC_RELAXED) & bit) != 0) return 0;
-  PSGD_CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  if (device < 64) __atomic_fetch_or(&devices, bit, __ATOMIC_RELAXED);
-  return 0;
+  if (device < 64 && (__atomic_load_n(&asked, __ATOMIC_ACQUIRE) & bit) != 0) return (__atomic_load_n(&runs, __ATOMIC_RELAXED) & bit) != 0;
+  const bool both = gn_runs_cluster<GN_SQUARES, MOST>() && gn_runs_cluster<GN_LARGEST, MOST>();
+  if (device < 64) {
+    if (both) __atomic_fetch_or(&runs, bit, __ATOMIC_RELAXED);
+    __atomic_fetch_or(&asked, bit, __ATOMIC_RELEASE);
+  }
+  return both;
 }
 
 template <int KIND, int MOST>
@@ -517,9 +538,11 @@ int gn_run(const PsgdNormTensor* list, int count, int clip, double max_norm, typ
   for (int done = 0; done < count;) {
     if (const int code = gn_fill(a, list, count, done, grid)) return code;
     if (grid == 0) continue;
-    if (launches == 0 && done == count && a.t[a.count - 1].piece_end <= GN_CLUSTER * GN_HELD) {     // (`parts` is null)
-      static unsigned long long devices = 0;
-      if (const int code = gn_allow_cluster((const void*)psgd_grad_small_kernel<KIND, MOST>, devices)) return code;
+    if (parts == nullptr) {     // (psgd_grad_norm_parts has found that the device runs it)
+      if (launches != 0 || done != count || a.t[a.count - 1].piece_end > GN_CLUSTER * GN_HELD) {
+        psgd_set_error("psgd_grad_norm: a list of %d tensors without scratch", count);
+        return PSGD_BAD_ARGUMENT;
+      }
       return psgd_launch_clusters(psgd_grad_small_kernel<KIND, MOST>, GN_CLUSTER, GN_SMALL_THREADS, 0, stream, 0, GN_CLUSTER, a, clip, max_norm, out, wide);
     }
     if (const int code = psgd_launch(psgd_grad_norm_kernel<KIND, MOST>, grid, GN_THREADS, 0, stream, 0, a, parts + have, taken, clip && launches == 0 ? most : 0)) return code;
@@ -549,17 +572,18 @@ int gn_dispatch(const PsgdNormTensor* list, int count, int clip, double max_norm
 
 PSGD_API int psgd_grad_norm_item_bytes() { return (int)sizeof(PsgdNormTensor); }
 
-// Words of 8 bytes of scratch that a list asks for: none where one launch holds it.
+// Words of 8 bytes of scratch that a list asks for on the current device: none where one launch holds it. A list that is given scratch takes two launches.
 PSGD_API long long psgd_grad_norm_parts(const void* list, int count) {
   const PsgdNormTensor* t = (const PsgdNormTensor*)list;
   long long pieces = 0;
   for (int i = 0; i < count && pieces <= GN_CLUSTER * GN_HELD; ++i) pieces += gn_pieces(t[i]);
-  if (pieces <= GN_CLUSTER * GN_HELD) return 0;
+  if (pieces == 0) return 0;
+  if (pieces <= GN_CLUSTER * GN_HELD && (count <= GN_SHORT ? gn_runs_short<GN_SHORT>() : count <= GN_MIDDLE ? gn_runs_short<GN_MIDDLE>() : gn_runs_short<GN_LONG>())) return 0;
   return (GN_BLOCKS + 1ll) * (count <= GN_LONG ? 1 : (count + GN_LONG - 1) / GN_LONG);
 }
 
 // `list`: host memory, read before the call returns. `largest`: the largest magnitude instead of the root of the sum of squares. `clip`: gradients are
-// scaled where max_norm / (norm + 1e-6) is not at least one. `out`: the norm before that, float, or double where `wide`.
+// scaled where max_norm / (norm + 1e-6) is not at least one. `parts`: scratch, null where psgd_grad_norm_parts asked for none. `out`: the norm before that, float, or double where `wide`.
 PSGD_API int psgd_grad_norm(const void* list, int count, int largest, int clip, double max_norm, void* parts, void* out, int wide, cudaStream_t stream) {
   const PsgdNormTensor* t = (const PsgdNormTensor*)list;
   if (largest) return gn_dispatch<GN_LARGEST>(t, count, clip, max_norm, parts, out, wide, stream);

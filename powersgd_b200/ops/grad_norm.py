@@ -111,10 +111,11 @@ def _norm_checked(what: str, parameters: List[torch.Tensor], largest: bool, max_
     items["type"] = [DTYPES[g.dtype] for g in laid]
     device, wide, listed = grads[0].device, any(g.dtype == torch.float64 for g in grads), items.tobytes()
     out = torch.empty((), dtype=torch.float64 if wide else torch.float32, device=device)
-    parts = torch.empty(native.lib().psgd_grad_norm_parts(listed, len(laid)), dtype=torch.float64, device=device)
     with native.on_device(device) as stream:
-        code = native.lib().psgd_grad_norm(listed, len(laid), largest, max_norm is not None, 0.0 if max_norm is None else max_norm, parts.data_ptr(), out.data_ptr(),
-                                           wide, stream)
+        words = native.lib().psgd_grad_norm_parts(listed, len(laid))     # (asks what the device runs)
+        parts = torch.empty(words, dtype=torch.float64, device=device)
+        code = native.lib().psgd_grad_norm(listed, len(laid), largest, max_norm is not None, 0.0 if max_norm is None else max_norm, parts.data_ptr() if words else None,
+                                           out.data_ptr(), wide, stream)
     native.check(code, "psgd_grad_norm")
     if max_norm is not None:
         for g, t in zip(grads, laid):
