@@ -2,8 +2,8 @@
 //
 //   n = (sum_t sum_i g_ti^2)^(1/2)   or   max |g_ti|          c = max_norm / (n + 1e-6)          g <- c g   where not c >= 1
 //
-// Squares are added in 64 bits: no gradient of the types below is so large or so small that its square leaves the range, and the order of
-// the sums does not show in a norm of 32 bits. The product is rounded to the gradient's type once. A norm that is no number makes every
+// Squares are added in 64 bits: no gradient of 32 bits or less is so large or so small that its square leaves the range, and the order of
+// the sums does not show in a norm of 32 bits. (Squares of float64 gradients do from 1.3e154 on, whose norm is infinite, and vanish below 1e-162.) The product is rounded to the gradient's type once. A norm that is no number makes every
 // gradient one too; an infinite one makes zeros of the finite ones.
 //
 // Two launches: sums of blocks, which a second one adds up again in every block, always in the same order. (Lists of up to a megabyte: one, see below.) The list

@@ -30,12 +30,12 @@ def grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type
 def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
                    error_if_nonfinite: bool = False) -> torch.Tensor:
     """Scales the gradients of `parameters` by max_norm / (norm + 1e-6) where that is below one, and returns their norm before that: a tensor without
-    dimensions on their device, float32 (float64 where a gradient is), zero where there are none. As `torch.nn.utils.clip_grad_norm_`, in one launch or two for the
-    whole list and without waiting for the GPU.
+    dimensions on their device, float32 (float64 where a gradient is), zero where there are none. As `torch.nn.utils.clip_grad_norm_`, in one launch or two for
+    up to 1200 tensors (two more for each 1200 after them) and without waiting for the GPU.
 
     Gradients are plain tensors (no DTensors), dense, float32, bfloat16, float16 or float64, in one list if need be, of one device, and none lies in another's
-    memory (a parameter is listed once). Those that do not lie in one piece are copied to and fro. Squares are added in float64; a
-    gradient is rounded once. Where the norm is no number all gradients become NaN, where it is infinite finite ones become zero:
+    memory (a parameter is listed once). Those that do not lie in one piece are copied to and fro. Squares are added in float64 (those of float64
+    gradients leave its range from 1.3e154 on, and the norm is infinite, as the library's is; the largest magnitude has no such bound); a gradient is rounded once. Where the norm is no number all gradients become NaN, where it is infinite finite ones become zero:
     with `error_if_nonfinite` a RuntimeError is raised instead and nothing is changed; it waits for the GPU.
 
     May be recorded in a CUDA graph, which reads the gradients where they lay, and `max_norm` as it was, at every replay."""

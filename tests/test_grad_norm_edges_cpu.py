@@ -1,8 +1,11 @@
-"""What the native call for the gradients' norm asks of the device, without one."""
+"""Gradients whose squares leave the range of float64; what the native call for the gradients' norm asks of the device, without one."""
+import math
+
 import numpy as np
 import pytest
 import torch
 
+from powersgd_b200 import clip_grad_norm, grad_norm
 from powersgd_b200.ops import grad_norm as module
 from powersgd_b200.ops import native
 
@@ -25,3 +28,36 @@ def test_short_lists_ask_for_scratch_where_no_device_runs_their_cluster():
         assert words >= long
     for sizes in ([0], [0] * 50, [0] * 2000):
         assert native.lib().psgd_grad_norm_parts(*items(*sizes)) == 0     # (nothing to add up)
+
+
+def check_range_of_float64(device):
+    """As the library has it: beyond 1.3e154 the norm is infinite and clipping leaves zeros; below 1e-162 it is zero. Float32 gradients in the same list count by
+    their own size, and the largest magnitude has the range of its type."""
+    for value, norm, left in ((1e200, math.inf, 0.0), (1e-200, 0.0, 1e-200), (1e153, 1e153 * 10, 1.0 / 10)):
+        params = []
+        for _ in range(2):
+            p = torch.nn.Parameter(torch.zeros(50, dtype=torch.float64, device=device))
+            p.grad = torch.full((50,), value, dtype=torch.float64, device=device)
+            params.append(p)
+        theirs = [torch.nn.Parameter(p.detach().clone()) for p in params]
+        for p, t in zip(params, theirs):
+            t.grad = p.grad.clone()
+        got, want = clip_grad_norm(params, 1.0), torch.nn.utils.clip_grad_norm_(theirs, 1.0)
+        assert got.dtype == torch.float64
+        if math.isinf(norm):
+            assert got == norm and want == norm
+        else:
+            assert abs(got.item() - norm) <= norm * 2.0**-50
+        for p, t in zip(params, theirs):
+            assert ((p.grad - left).abs() <= left * 2.0**-49).all() and torch.allclose(p.grad, t.grad, rtol=2.0**-40, atol=0.0)
+        for p in params:
+            p.grad.fill_(value)
+        assert grad_norm(params, math.inf).item() == value
+    with pytest.raises(RuntimeError, match="nothing was scaled"):
+        params[0].grad.fill_(1e200)
+        clip_grad_norm(params, 1.0, error_if_nonfinite=True)
+    assert (params[0].grad == 1e200).all()
+
+
+def test_range_of_float64():
+    check_range_of_float64("cpu")

@@ -5,6 +5,7 @@ import numpy as np
 import pytest
 import torch
 from test_grad_norm_cpu import TYPES, check, make
+from test_grad_norm_edges_cpu import check_range_of_float64
 
 from powersgd_b200 import clip_grad_norm, grad_norm
 from powersgd_b200.ops import grad_norm as module
@@ -60,3 +61,7 @@ def test_short_lists_in_two_launches(monkeypatch, count, largest):
         check(make([(3,)] * held + [(0,)] * (count - 1 - held) + [(70, 9)], TYPES, "cuda"), max_norm, largest)
     check(make([(0,)] * (count - 1) + [(1,)], TYPES, "cuda"), 0.1, largest)
     assert asked and not any(asked)     # (this device runs it)
+
+
+def test_range_of_float64(form):
+    check_range_of_float64("cuda")
