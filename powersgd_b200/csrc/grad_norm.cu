@@ -161,6 +161,18 @@ struct GnWide<double> {
   typedef double type;
 };
 
+// What gradients are multiplied with. One below the normal numbers of 32 bits, for gradients near the end of their range, has few digits left there: two factors then, of
+// which the second is at most one, so that nothing vanishes on the way that does not vanish in the end.
+struct GnFactor {
+  double whole;
+  float first, second;
+  __device__ __forceinline__ explicit GnFactor(double factor) : whole(factor), first(1.f), second((float)factor) {
+    if (factor < 0x1p-126) first = 0x1p-126f, second = (float)(factor * 0x1p126);
+  }
+  __device__ __forceinline__ float times(float g) const { return g * first * second; }
+  __device__ __forceinline__ double times(double g) const { return g * whole; }
+};
+
 // Piece `piece` of a tensor: its vectors of 16 bytes lie on 16-byte boundaries, the first one from `base` on; elements [lo, hi) of
 // the piece belong to the tensor.
 template <typename T>
@@ -208,12 +220,11 @@ __device__ __forceinline__ void gn_read(const PsgdNormTensor& t, uint32_t piece,
 }
 
 template <typename T>
-__device__ __forceinline__ void gn_scale(const PsgdNormTensor& t, uint32_t piece, double factor) {
+__device__ __forceinline__ void gn_scale(const PsgdNormTensor& t, uint32_t piece, const GnFactor& c) {
   typedef GnType<T> V;
   typedef typename GnWide<T>::type F;
   constexpr int N = V::N, E = GN_PIECE / (int)sizeof(T);
   const GnPiece<T> p(t, piece);
-  const F c = (F)factor;
   if (p.lo == 0 && p.hi == E) {
     uint4 raw[GN_VECTORS];
 #pragma unroll
@@ -223,7 +234,7 @@ __device__ __forceinline__ void gn_scale(const PsgdNormTensor& t, uint32_t piece
       F f[N];
       V::unpack(raw[i], f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[j] *= c;
+      for (int j = 0; j < N; ++j) f[j] = c.times(f[j]);
       __stcs(reinterpret_cast<uint4*>(p.base + (i * GN_THREADS + threadIdx.x) * N), V::pack(f));
     }
     return;
@@ -233,10 +244,10 @@ __device__ __forceinline__ void gn_scale(const PsgdNormTensor& t, uint32_t piece
       F f[N];
       V::unpack(*reinterpret_cast<const uint4*>(p.base + i), f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[j] *= c;
+      for (int j = 0; j < N; ++j) f[j] = c.times(f[j]);
       *reinterpret_cast<uint4*>(p.base + i) = V::pack(f);
     } else {
-      for (int j = max(i, p.lo); j < min(i + N, p.hi); ++j) V::put(p.base + j, V::get(p.base + j) * c);
+      for (int j = max(i, p.lo); j < min(i + N, p.hi); ++j) V::put(p.base + j, c.times(V::get(p.base + j)));
     }
   }
 }
@@ -330,6 +341,7 @@ __global__ void __launch_bounds__(GN_THREADS, GN_PER_SM)
   if (blockIdx.x == 0 && threadIdx.x == 0 && out != nullptr) gn_write(out, wide, norm);
   const double factor = max_norm / (norm + 1e-6);
   if (factor >= 1.0) return;
+  const GnFactor c(factor);
   __shared__ uint32_t s_next;
   const uint32_t pieces = a.t[a.count - 1].piece_end;
   const bool more = pieces > gridDim.x;
@@ -345,10 +357,10 @@ __global__ void __launch_bounds__(GN_THREADS, GN_PER_SM)
       end = a.t[which].piece_end;
     }
     const PsgdNormTensor& t = a.t[which];
-    if (t.type == 0) gn_scale<float>(t, piece - first, factor);
-    else if (t.type == 1) gn_scale<__nv_bfloat16>(t, piece - first, factor);
-    else if (t.type == 2) gn_scale<__half>(t, piece - first, factor);
-    else gn_scale<double>(t, piece - first, factor);
+    if (t.type == 0) gn_scale<float>(t, piece - first, c);
+    else if (t.type == 1) gn_scale<__nv_bfloat16>(t, piece - first, c);
+    else if (t.type == 2) gn_scale<__half>(t, piece - first, c);
+    else gn_scale<double>(t, piece - first, c);
     if (!more) return;
     __syncthreads();
     back = s_next;
@@ -380,15 +392,14 @@ __device__ __forceinline__ void gn_take(const uint4& raw, GnSeen<KIND>& seen) {
   for (int j = 0; j < GnType<T>::N; ++j) seen.take(f[j]);
 }
 template <typename T>
-__device__ __forceinline__ void gn_put_back(const GnPiece<T>& p, const uint4& held, double factor) {
+__device__ __forceinline__ void gn_put_back(const GnPiece<T>& p, const uint4& held, const GnFactor& c) {
   typedef typename GnWide<T>::type F;
   constexpr int N = GnType<T>::N;
   const int i = threadIdx.x * N;
-  const F c = (F)factor;
   F f[N];
   GnType<T>::unpack(held, f);
 #pragma unroll
-  for (int j = 0; j < N; ++j) f[j] *= c;
+  for (int j = 0; j < N; ++j) f[j] = c.times(f[j]);
   union {
     uint4 v;
     T t[N];
@@ -456,16 +467,17 @@ __global__ void __launch_bounds__(GN_SMALL_THREADS, 1)
   if (rank == 0 && threadIdx.x == 0) gn_write(out, wide, norm);
   const double factor = max_norm / (norm + 1e-6);
   if (!clip || factor >= 1.0) return;
+  const GnFactor c(factor);
 #pragma unroll
   for (int i = 0; i < GN_HELD; ++i) {
     const int which = s_which[i];
     if (which < 0) continue;
     const PsgdNormTensor& t = a.t[which];
     const uint32_t at = rank + i * GN_CLUSTER - (which ? a.t[which - 1].piece_end : 0);
-    if (t.type == 0) gn_put_back(GnPiece<float>(t, at), raw[i], factor);
-    else if (t.type == 1) gn_put_back(GnPiece<__nv_bfloat16>(t, at), raw[i], factor);
-    else if (t.type == 2) gn_put_back(GnPiece<__half>(t, at), raw[i], factor);
-    else gn_put_back(GnPiece<double>(t, at), raw[i], factor);
+    if (t.type == 0) gn_put_back(GnPiece<float>(t, at), raw[i], c);
+    else if (t.type == 1) gn_put_back(GnPiece<__nv_bfloat16>(t, at), raw[i], c);
+    else if (t.type == 2) gn_put_back(GnPiece<__half>(t, at), raw[i], c);
+    else gn_put_back(GnPiece<double>(t, at), raw[i], c);
   }
 }
 

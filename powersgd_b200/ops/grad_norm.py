@@ -35,7 +35,8 @@ def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_
 
     Gradients are plain tensors (no DTensors), dense, float32, bfloat16, float16 or float64, in one list if need be, of one device, and none lies in another's
     memory (a parameter is listed once). Those that do not lie in one piece are copied to and fro. Squares are added in float64 (those of float64
-    gradients leave its range from 1.3e154 on, and the norm is infinite, as the library's is; the largest magnitude has no such bound); a gradient is rounded once. Where the norm is no number all gradients become NaN, where it is infinite finite ones become zero:
+    gradients leave its range from 1.3e154 on, and the norm is infinite, as the library's is; the largest magnitude has no such bound); a gradient is rounded once. Where the norm is no number all gradients become NaN, where it is infinite finite ones become zero
+    (a norm that only float32 does not hold is returned as infinity, and gradients are scaled by what it is):
     with `error_if_nonfinite` a RuntimeError is raised instead and nothing is changed; it waits for the GPU.
 
     May be recorded in a CUDA graph, which reads the gradients where they lay, and `max_norm` as it was, at every replay."""
@@ -148,7 +149,8 @@ def _norm_torch(grads: List[torch.Tensor], largest: bool, max_norm) -> torch.Ten
     if max_norm is not None:
         factor = max_norm / (norm + 1e-6)
         factor = torch.where(factor >= 1, torch.ones_like(factor), factor)
+        down = torch.where(factor < 2.0**-126, 2.0**-126, 1.0).to(factor.dtype)      # (below the normal numbers of 32 bits few digits would be left)
         for g in grads:
             if not g._is_zerotensor():
-                g.copy_(g * factor if g.dtype == torch.float64 else g.float() * factor.float())
+                g.copy_(g * factor if g.dtype == torch.float64 else g.float() * down.float() * (factor / down).float())
     return norm if any(g.dtype == torch.float64 for g in grads) else norm.float()

@@ -61,3 +61,24 @@ def check_range_of_float64(device):
 
 def test_range_of_float64():
     check_range_of_float64("cpu")
+
+
+def check_small_factors(numel, dtype, device):
+    """Gradients near the end of float32's range: what they are multiplied with is far below its normal numbers, and what comes of it is not. Bounds: the factor's
+    rounding to 32 bits, the product's, and half a step of the type."""
+    p, q = (torch.nn.Parameter(torch.zeros(n, dtype=t, device=device)) for n, t in ((numel, dtype), (77, torch.float32)))
+    for t, seed in ((p, 0), (q, 1)):
+        t.grad = ((1 + torch.rand(t.shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64)) * 2.0**126).to(t.dtype).to(device)
+    before = [t.grad.double() for t in (p, q)]
+    norm = math.sqrt(sum(b.square().sum().item() for b in before))
+    clip_grad_norm([p, q], 2.0**-10)
+    for t, b in zip((p, q), before):
+        want = b * (2.0**-10 / norm)
+        own = 2.0**-22.9 + (torch.finfo(t.dtype).eps / 2 if t.dtype.itemsize == 2 else 0)
+        assert ((t.grad.double() - want).abs() <= want * own).all(), ((t.grad.double() - want).abs() / want).max().item()
+
+
+@pytest.mark.parametrize("numel", [3, 30000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_factors_below_the_normal_numbers(numel, dtype):
+    check_small_factors(numel, dtype, "cpu")

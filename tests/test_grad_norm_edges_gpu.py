@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 from test_grad_norm_cpu import TYPES, check, make
-from test_grad_norm_edges_cpu import check_range_of_float64
+from test_grad_norm_edges_cpu import check_range_of_float64, check_small_factors
 
 from powersgd_b200 import clip_grad_norm, grad_norm
 from powersgd_b200.ops import grad_norm as module
@@ -65,3 +65,9 @@ def test_short_lists_in_two_launches(monkeypatch, count, largest):
 
 def test_range_of_float64(form):
     check_range_of_float64("cuda")
+
+
+@pytest.mark.parametrize("numel", [300, 3_000_000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_factors_below_the_normal_numbers(form, numel, dtype):
+    check_small_factors(numel, dtype, "cuda")
