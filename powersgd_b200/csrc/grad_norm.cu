@@ -27,7 +27,8 @@ typedef struct {
   long long n;
   uint32_t type;        // 0 float32, 1 bfloat16, 2 float16, 3 float64
   uint32_t piece_end;   // pieces of the list up to and with this tensor (filled in by the launch)
-} PsgdNormTensor;       // 24 bytes
+} PsgdNormTensor;
+static_assert(sizeof(PsgdNormTensor) == 24, "as ops/grad_norm.py and host/operators.cpp have it");
 
 namespace {
 
@@ -581,8 +582,6 @@ int gn_dispatch(const PsgdNormTensor* list, int count, int clip, double max_norm
 }
 
 }  // namespace
-
-PSGD_API int psgd_grad_norm_item_bytes() { return (int)sizeof(PsgdNormTensor); }
 
 // Words of 8 bytes of scratch that a list asks for on the current device: none where one launch holds it. A list that is given scratch takes two launches.
 PSGD_API long long psgd_grad_norm_parts(const void* list, int count) {

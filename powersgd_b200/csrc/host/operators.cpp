@@ -22,6 +22,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 #include <cstdint>
 #include <optional>
 #include <string>
@@ -52,6 +53,7 @@ struct RotateCall {   // PsgdRotate, csrc/rotary.cu
   float eps;
   int pad;
 };
+static_assert(sizeof(RotateCall) == 240 && offsetof(RotateCall, x_row) == 120 && offsetof(RotateCall, rows) == 184, "as csrc/rotary.cu has it");
 
 // ---- entry points of the native library ---------------------------------------------------------
 struct Entry {
@@ -597,6 +599,7 @@ struct NormItem {   // PsgdNormTensor, csrc/grad_norm.cu
   int64_t n;
   uint32_t type, piece_end;
 };
+static_assert(sizeof(NormItem) == 24, "as csrc/grad_norm.cu has it");
 
 // grad_norm(parameters, largest, clip, max_norm): the norm of their gradients, scaled where `clip`; or None.
 PyObject* grad_norm(PyObject*, PyObject* args) {

@@ -25,6 +25,7 @@
 #include <math_constants.h>
 
 #include <algorithm>
+#include <cstddef>
 #include <type_traits>
 
 #include "psgd_common.cuh"
@@ -48,7 +49,8 @@ typedef struct {
   int norm;
   float eps;
   int pad;
-} PsgdRotate;                      // 240 bytes
+} PsgdRotate;
+static_assert(sizeof(PsgdRotate) == 240 && offsetof(PsgdRotate, x_row) == 120 && offsetof(PsgdRotate, rows) == 184, "as ops/rotary.py and host/operators.cpp have it");
 
 namespace {
 
@@ -814,8 +816,6 @@ int rt_call(const PsgdRotate* call, bool gradient, cudaStream_t stream) {
 }
 
 }  // namespace
-
-PSGD_API int psgd_rotate_call_bytes() { return (int)sizeof(PsgdRotate); }
 
 // Numbers of 64 bits, scratch for the gradients of weights.
 PSGD_API long long psgd_rotate_parts(int size) { return (long long)RT_PART_BLOCKS * 2 * size; }

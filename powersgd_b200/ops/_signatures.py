@@ -77,10 +77,8 @@ f64 = C.c_double
 _OPTIONAL = {
     "psgd_adamw_item_bytes": (i32, []),
     "psgd_adamw_step": (i32, [C.c_char_p, i32, i32, i32, f64, vp, f64, f64, f64, f64, f64, f64, C.c_uint, vp, vp]),
-    "psgd_grad_norm_item_bytes": (i32, []),
     "psgd_grad_norm_parts": (i64, [C.c_char_p, i32]),
     "psgd_grad_norm": (i32, [C.c_char_p, i32, i32, i32, f64, vp, vp, i32, vp]),
-    "psgd_rotate_call_bytes": (i32, []),
     "psgd_rotate_parts": (i64, [i32]),
     "psgd_rotate": (i32, [vp, vp]),
     "psgd_rotate_grad": (i32, [vp, vp]),

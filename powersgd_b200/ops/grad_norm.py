@@ -19,6 +19,7 @@ DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 
 
 # one tensor of a list, see PsgdNormTensor
 ITEM = np.dtype([("g", "u8"), ("n", "i8"), ("type", "u4"), ("piece_end", "u4")])
+assert ITEM.itemsize == 24
 
 
 def grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], norm_type: float = 2.0) -> torch.Tensor:

@@ -33,6 +33,9 @@ class Call(ctypes.Structure):
                 ("eps", ctypes.c_float), ("pad", ctypes.c_int)]
 
 
+assert ctypes.sizeof(Call) == 240 and Call.x_row.offset == 120 and Call.rows.offset == 184
+
+
 def rotate_heads(x: torch.Tensor, *, offsets: Optional[torch.Tensor] = None, positions: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
                  eps: Optional[float] = 1e-6, base: float = 10000.0, rotated: Optional[int] = None, interleaved: bool = False) -> torch.Tensor:
     """Each head of `x` divided by the root of its mean square and multiplied with `weight`, and its first `rotated` elements turned pair by
