@@ -35,7 +35,7 @@ using at::Tensor;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-struct RotateCall {   // PsgdRotate, csrc/rotary.cu
+struct RotateCall {   // PsgdRotate, csrc/rotary.cuh
   const void* x;
   const void* grad[3];
   const void* weight[2];
@@ -53,7 +53,7 @@ struct RotateCall {   // PsgdRotate, csrc/rotary.cu
   float eps;
   int pad;
 };
-static_assert(sizeof(RotateCall) == 240 && offsetof(RotateCall, x_row) == 120 && offsetof(RotateCall, rows) == 184, "as csrc/rotary.cu has it");
+static_assert(sizeof(RotateCall) == 240 && offsetof(RotateCall, x_row) == 120 && offsetof(RotateCall, rows) == 184, "as csrc/rotary.cuh has it");
 
 // ---- entry points of the native library ---------------------------------------------------------
 struct Entry {

@@ -1,4 +1,4 @@
-"""Heads normed and turned by their row's position (csrc/rotary.cu): what a transformer does to its queries and keys between
+"""Heads normed and turned by their row's position (csrc/rotary.cuh): what a transformer does to its queries and keys between
 their projection and the attention.
 
 On the CPU (or on CUDA without the native library where PSGD_B200_ALLOW_FALLBACK=1 allows it) the same comes from torch
@@ -24,7 +24,7 @@ MOST_HEADS = 4096
 
 
 class Call(ctypes.Structure):
-    """PsgdRotate, see csrc/rotary.cu."""
+    """PsgdRotate, see csrc/rotary.cuh."""
 
     _fields_ = [("x", ctypes.c_void_p), ("grad", ctypes.c_void_p * 3), ("weight", ctypes.c_void_p * 2), ("offsets", ctypes.c_void_p), ("positions", ctypes.c_void_p),
                 ("out", ctypes.c_void_p * 2), ("dx", ctypes.c_void_p), ("dweight", ctypes.c_void_p * 2), ("parts", ctypes.c_void_p), ("frequencies", ctypes.c_void_p),
