@@ -506,6 +506,9 @@ __global__ void __launch_bounds__(RT_THREADS, RT_FORWARD_BLOCKS) psgd_rotate_ker
   rt_await<0>();
 }
 
+// Do warps that take every `stride`th row have sums of more than RT_SUMMED rows?
+__host__ __device__ __forceinline__ bool rt_many_rows(int rows, int stride) { return rows > RT_SUMMED * stride; }
+
 // Gradients: a warp has the same heads of every row that it comes to, RT_STEPS times what its lanes take at once, queries or keys, so that it adds up one weight's
 // gradient, and a share of the rows' values, which pass by. Each step has its place in shared memory, which, once read, is filled with the same
 // step of the warp's next row.
@@ -569,14 +572,15 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
   const float* weight = shared.weight[kind] + place.lo;
   RtPair acc[W];
 #pragma unroll
-  for (int i = 0; i < W; ++i) {
-    acc[i] = 0;
-    wide[i * RT_THREADS] = make_double2(0.0, 0.0);
+  for (int i = 0; i < W; ++i) acc[i] = 0;
+  if (sums && rt_many_rows(a.c.rows, stride)) {     // (there is room for these sums only then)
+#pragma unroll
+    for (int i = 0; i < W; ++i) wide[i * RT_THREADS] = make_double2(0.0, 0.0);
   }
   // A thread's sum of the products of RT_SUMMED rows at most is one of 32 bits, of any more of 64 (with 32 all the way a weight's gradient was 2e-7 off for 8192 rows,
   // now 1e-7, and up to 5e-6 for 4 M of them; the sums of 64 wait in shared memory).
 #pragma unroll 1
-  do {
+  for (;;) {
 #pragma unroll 1
     for (int left = RT_SUMMED; left > 0 && row < a.c.rows; --left, row = ahead) {
       ahead = stride < a.c.rows - row ? row + stride : a.c.rows;
@@ -662,6 +666,7 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
       }
       dx += dx_stride;
     }
+    if (row >= a.c.rows) break;
     if (!sums) continue;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
@@ -670,14 +675,16 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
       wide[i * RT_THREADS] = make_double2(before.x + own.x, before.y + own.y);
       acc[i] = 0;
     }
-  } while (row < a.c.rows);
+  }
   rt_await<0>();
   if (!sums) return;
   __syncthreads();       // (the ring, where the warps' sums go, is free)
   double(*const s_sums)[RT_MOST_SIZE] = reinterpret_cast<double(*)[RT_MOST_SIZE]>(ring);
 #pragma unroll
   for (int i = 0; i < W; ++i) {
-    double2 v = wide[i * RT_THREADS];
+    const float2 own = rt_floats(acc[i]);
+    double2 v = make_double2(own.x, own.y);
+    if (rt_many_rows(a.c.rows, stride)) v.x += wide[i * RT_THREADS].x, v.y += wide[i * RT_THREADS].y;
     if (LANES && (LANES & (LANES - 1)) == 0) {
 #pragma unroll
       for (int o = LANES; o < 32; o <<= 1) {
@@ -762,11 +769,12 @@ int rt_backward(RtArgs& a, cudaStream_t stream) {
   }
   const long long blocks = ((long long)a.c.rows * (a.parts[0] + a.parts[1]) + RT_WARPS - 1) / RT_WARPS;
   const int grid = (int)(blocks < RT_PART_BLOCKS ? blocks : RT_PART_BLOCKS);
-  constexpr size_t ring = (size_t)RT_THREADS * (RT_STEPS * 4 * RtVec<T, W>::BYTES + RT_PASSING * 16 + W * sizeof(double2));
+  constexpr size_t ring = (size_t)RT_THREADS * (RT_STEPS * 4 * RtVec<T, W>::BYTES + RT_PASSING * 16), wide = (size_t)RT_THREADS * W * sizeof(double2);
   static_assert(RT_STEPS * 4 * RtVec<T, W>::BYTES >= RT_MOST_SIZE / 32 * (int)sizeof(double), "room for the warps' sums");
   static unsigned long long devices = 0;
-  if (const int code = psgd_allow_shared((const void*)psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, ring, devices)) return code;
-  if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, grid, RT_THREADS, ring, stream, 0, a)) return code;
+  if (const int code = psgd_allow_shared((const void*)psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, ring + wide, devices)) return code;
+  const size_t shared = ring + (a.c.parts != nullptr && rt_many_rows(a.c.rows, grid * RT_WARPS / (a.parts[0] + a.parts[1])) ? wide : 0);
+  if (const int code = psgd_launch(psgd_rotate_grad_kernel<T, W, PAIRS, LANES>, grid, RT_THREADS, shared, stream, 0, a)) return code;
   if (a.c.parts == nullptr) return 0;
   return psgd_launch(psgd_rotate_weights_kernel, (2 * a.c.size + 31) / 32, 32 * RT_SLICES, 0, stream, 1, (const double*)a.c.parts, grid, a.c.size, a.c.weight_type, a.c.dweight[0],
                      a.c.dweight[1]);
