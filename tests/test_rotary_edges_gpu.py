@@ -58,10 +58,10 @@ def test_far_positions(form, dtype, rotated, interleaved, base):
     check_far(dtype, rotated, interleaved, base, "cuda")
 
 
-@pytest.mark.parametrize("size", [16, 40, 136])
+@pytest.mark.parametrize("size", [16, 40, 136, 256])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 def test_more_rows_than_are_added_up_at_a_time(form, dtype, size):
     """A warp comes to 84 rows; with and without gradients of weights."""
-    rows = 100_000 if size < 100 else 40_000
-    check(values(rows, 3, size, dtype, "cuda"), 1, 1, lengths=[rows // 3, rows // 2])
-    check(values(rows, 1, size, dtype, "cuda"), 1, 0, lengths=[rows], weights=False)
+    rows = 100_000
+    check(values(rows, 3, size, dtype, "cuda"), 1, 1, lengths=[rows // 3, rows // 2], rotated=0)
+    check(values(rows, 1, size, dtype, "cuda"), 1, 0, lengths=[rows], weights=False, rotated=0)
