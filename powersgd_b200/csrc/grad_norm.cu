@@ -10,8 +10,8 @@
 // travels in the launches' own arguments, so nothing is uploaded and a recorded graph keeps it. A block takes pieces of 16 KiB that begin on
 // 16-byte boundaries, wherever a tensor begins: only what a piece's first and last 16 bytes hold of other tensors is left out.
 //
-// What bounds it is HBM, two reads and a write of everything: 355 M float32 gradients take 203 us for the norm (7.0 TB/s) and 626 with clipping (6.8), as
-// bfloat16 113 and 325; 31.8 M float32 25 and 61, where the second read finds a third of them in L2. Squares of 32 bits instead of 64 would save 6 % of a norm of
+// What bounds it is HBM, two reads and a write of everything: 355 M float32 gradients take 204 us for the norm (7.0 TB/s) and 626 with clipping (6.8), as
+// bfloat16 118 and 309; 31.8 M float32 25 and 61, where the second read finds a third of them in L2. Squares of 32 bits instead of 64 would save 6 % of a norm of
 // 16-bit gradients, whose conversions to 64 bits are then felt, and nothing of float32 ones.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
@@ -39,7 +39,7 @@ constexpr int GN_PIECE = 16384;                     // bytes
 constexpr int GN_VECTORS = GN_PIECE / 16 / GN_THREADS;
 constexpr int GN_PER_SM = 6;                        // blocks that run at a time
 constexpr int GN_BLOCKS = 148 * GN_PER_SM;          // of a launch, at most
-constexpr int GN_PER_SM_LARGE = 4;                  // for more pieces than GN_LARGE (355 M float32: 633 us and 656 with six; 31.8 M: 65 and 63)
+constexpr int GN_PER_SM_LARGE = 4;                  // for more pieces than GN_LARGE, half a gigabyte (355 M float32: 626 us, 631 with six)
 constexpr long long GN_LARGE = 32768;
 constexpr int GN_CLUSTER = 16, GN_HELD = 4;         // blocks of a short list's one launch, pieces that each holds
 constexpr int GN_SMALL_THREADS = GN_PIECE / 16;
@@ -415,8 +415,8 @@ __device__ __forceinline__ void gn_put_back(const GnPiece<T>& p, const uint4& he
   }
 }
 
-// (A perceptron's 0.8 MB: 6.8 us to a program that calls it again and again, 8 with clusters of 8, 11.4 in two launches, which the host takes longer
-// to make. A megabyte: 6.8, 10 and 11. A few KB: 4.7.)
+// (A perceptron's 0.8 MB: 7.2 to 7.5 us to a program that calls it again and again, 9.3 with clusters of 8, 7.8 in two launches. A megabyte: 7.1, 10.3 and 7.7. A few KB: 4.7, 5.3 and
+// 7.7. Programs that do more between two calls: 7.6 to 8.2 for the 0.8 MB, by the host.)
 template <int KIND, int MOST>
 __global__ void __launch_bounds__(GN_SMALL_THREADS, 1)
     psgd_grad_small_kernel(const __grid_constant__ GnList<MOST> a, int clip, double max_norm, void* out, int wide) {

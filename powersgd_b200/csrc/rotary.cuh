@@ -17,9 +17,9 @@
 // has the same heads of every row that it comes to, queries or keys, whose weight's gradient it adds up. The sums go from threads to warps to blocks
 // to one more launch, always in the same order. Inputs come by asynchronous copies into a thread's own places in shared memory, some steps ahead.
 //
-// 8192 rows of 16 + 16 heads of 64, bfloat16: forward 14.1 us (67 MB, 4.8 TB/s); backward, with 16 heads of values, 26.5 us (134 MB, 5.1 TB/s) and 2 for the
+// 8192 rows of 16 + 16 heads of 64, bfloat16: forward 14.1 us (67 MB, 4.8 TB/s); backward, with 16 heads of values, 25.9 us (134 MB, 5.2 TB/s) and 2 for the
 // weights. 14336 rows of 32 + 8 heads of 128: forward 49 us (294 MB, 6.0 TB/s). Besides HBM it is the instructions, some 4 to an element and pass, and
-// waiting for shuffles and shared memory: issue is 59 and 58 % busy in the first two.
+// waiting for shuffles and shared memory: issue is 62 and 57 % busy in the first two.
 #pragma once
 
 #include <cuda_bf16.h>

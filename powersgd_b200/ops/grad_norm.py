@@ -35,10 +35,11 @@ def clip_grad_norm(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_
     up to 1200 tensors (two more for each 1200 after them) and without waiting for the GPU.
 
     Gradients are plain tensors (no DTensors), dense, float32, bfloat16, float16 or float64, in one list if need be, of one device, and none lies in another's
-    memory (a parameter is listed once). Those that do not lie in one piece are copied to and fro. Squares are added in float64 (those of float64
-    gradients leave its range from 1.3e154 on, and the norm is infinite, as the library's is; the largest magnitude has no such bound); a gradient is rounded once. Where the norm is no number all gradients become NaN, where it is infinite finite ones become zero
-    (a norm that only float32 does not hold is returned as infinity, and gradients are scaled by what it is):
-    with `error_if_nonfinite` a RuntimeError is raised instead and nothing is changed; it waits for the GPU.
+    memory (a parameter is listed once). Those that do not lie in one piece are copied to and fro. Squares are added in float64; a
+    gradient is rounded once. Where the norm is no number all gradients become NaN, where it is infinite finite ones become zero:
+    with `error_if_nonfinite` a RuntimeError is raised instead and nothing is changed; it waits for the GPU. A norm that float32 does not hold is
+    returned as infinity, and gradients are scaled by what it is. Squares of float64 gradients leave the range from 1.3e154 on: their norm is infinite, as
+    the library's is (the largest magnitude has no such bound).
 
     May be recorded in a CUDA graph, which reads the gradients where they lay, and `max_norm` as it was, at every replay."""
     largest = _largest("clip_grad_norm", norm_type)
