@@ -102,7 +102,9 @@ void refuse_gradients(const variable_list& grads, const char* what) {
   for (const Tensor& g : grads) {
     if (!g.defined()) continue;
     TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(g), what, ": forward-mode differentiation is not supported");
-    TORCH_CHECK_TYPE(g._is_zerotensor() || (!at::isTensorSubclassLike(g) && g.unsafeGetTensorImpl()->has_storage()), what, ": a gradient has no memory of its own; plain tensors are supported");
+    // (asked of the tensor alone: at::isTensorSubclassLike says yes of any while something watches the operations)
+    const at::TensorImpl* const impl = g.unsafeGetTensorImpl();
+    TORCH_CHECK_TYPE(g._is_zerotensor() || (!impl->is_python_dispatch() && impl->has_storage()), what, ": a gradient has no memory of its own; plain tensors are supported");
     TORCH_CHECK(g._is_zerotensor() || !without_memory(g), what, ": the memory of a gradient was given back");
   }
 }
