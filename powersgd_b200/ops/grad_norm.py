@@ -151,7 +151,7 @@ def _norm_torch(grads: List[torch.Tensor], largest: bool, max_norm) -> torch.Ten
     if max_norm is not None:
         factor = max_norm / (norm + 1e-6)
         factor = torch.where(factor >= 1, torch.ones_like(factor), factor)
-        down = torch.where(factor < 2.0**-126, 2.0**-126, 1.0).to(factor.dtype)      # (below the normal numbers of 32 bits few digits would be left)
+        down = torch.where(factor < 2.0**-126, torch.full_like(factor, 2.0**-126), torch.ones_like(factor))      # (below the normal numbers of 32 bits few digits would be left)
         for g in grads:
             if not g._is_zerotensor():
                 g.copy_(g * factor if g.dtype == torch.float64 else g.float() * down.float() * (factor / down).float())

@@ -82,3 +82,17 @@ def check_small_factors(numel, dtype, device):
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_factors_below_the_normal_numbers(numel, dtype):
     check_small_factors(numel, dtype, "cpu")
+
+
+@pytest.mark.parametrize("default", [torch.float16, torch.float64])
+def test_other_default_types(default):
+    before = torch.get_default_dtype()
+    torch.set_default_dtype(default)
+    try:
+        check_small_factors(300, torch.float32, "cpu")
+        p = torch.nn.Parameter(torch.zeros(100, dtype=torch.float32))
+        p.grad = torch.ones(100, dtype=torch.float32)
+        assert abs(clip_grad_norm([p], 5.0).item() - 10) <= 10 * 2.0**-23
+        assert ((p.grad - 0.5).abs() <= 2.0**-22).all()
+    finally:
+        torch.set_default_dtype(before)
