@@ -119,3 +119,15 @@ def test_tensors_that_are_not_refused():
     empty = torch.nn.Parameter(torch.zeros(0))
     empty.grad = torch.zeros(0)
     assert grad_norm([empty]) == 0
+
+
+@pytest.mark.parametrize("count", [1, 2])
+def test_clipping_of_a_step_hands_them_to_the_library(count, monkeypatch):
+    listed = [Far(3) for _ in range(count)]
+    for p in listed:
+        p.grad = Far(3)
+    assert listed[0].is_cuda
+    given = []
+    monkeypatch.setattr(torch.nn.utils, "clip_grad_norm_", lambda parameters, max_norm: given.append((parameters, max_norm)))
+    clip_for_step(iter(listed), 0.5)
+    assert len(given) == 1 and [id(p) for p in given[0][0]] == [id(p) for p in listed] and given[0][1] == 0.5
