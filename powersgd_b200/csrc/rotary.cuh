@@ -632,9 +632,10 @@ __global__ void __launch_bounds__(RT_THREADS, RT_BACKWARD_BLOCKS) psgd_rotate_gr
               };
               float s, t, eps = a.c.eps, down = 1.f;
               dots(s, t);
-              if (RT_RANGE<T>) {     // (where only products with gradients leave the range, their heads are large enough to be made smaller)
-                const bool large = !(s < 0x1p126f && fabsf(t) < CUDART_INF_F);
-                if (__any_sync(0xffffffffu, large)) {
+              if (RT_RANGE<T>) {     // (where only products with gradients leave the range, heads are made smaller that are large enough to stay in it themselves)
+                const bool far = !(s < 0x1p126f && fabsf(t) < CUDART_INF_F);
+                if (__any_sync(0xffffffffu, far)) {
+                  const bool large = far && !(s < 0x1p40f);
                   const RtPair less = rt_both(large ? RT_DOWN : 1.f);
 #pragma unroll
                   for (int j = 0; j < W; ++j) f[j] = rt_mul(f[j], less);

@@ -65,3 +65,23 @@ def test_more_rows_than_are_added_up_at_a_time(form, dtype, size):
     rows = 100_000
     check(values(rows, 3, size, dtype, "cuda"), 1, 1, lengths=[rows // 3, rows // 2], rotated=0)
     check(values(rows, 1, size, dtype, "cuda"), 1, 0, lengths=[rows], weights=False, rotated=0)
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0**-8, 2.0**18])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradients_near_the_end_of_the_range(form, dtype, scale):
+    """Where their products with a small head leave float32, or where one of them is infinite, the weights' gradients (products with normed elements, here of one row)
+    are what they are. Bounds: as for sums of one product (five roundings on the way to a normed element, one of the product, one at the end)."""
+    for spoiled in (False, True):
+        x = (values(1, 1, 64, dtype, "cuda").abs() + 0.5) * scale
+        g = (1 + values(1, 1, 64, dtype, "cuda", seed=1).abs().clamp(max=0.5)) * 2.0**124
+        if spoiled:
+            g[0, 0, 5] = float("inf")
+        w = torch.ones(64, device="cuda", requires_grad=True)
+        got, = torch.autograd.grad(rotate_heads(x, weight=w, eps=1e-6, rotated=0), w, g)
+        wide = x.double()[0, 0]
+        want = g.double()[0, 0] * wide / (wide.square().mean() + 1e-6).sqrt()
+        if spoiled:
+            assert got[5] == float("inf")
+            got, want = got[torch.arange(64) != 5], want[torch.arange(64) != 5]
+        assert ((got.double() - want).abs() <= want * 8 * 2.0**-24).all()
